@@ -26,7 +26,6 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -35,22 +34,9 @@
 #include <utility>
 
 #include "kda_abi.h"
+#include "torch_util.h"
 
 namespace {
-
-using NamedTensor = std::pair<const char *, const at::Tensor &>;
-
-void check_same_device(const at::Tensor &q, const char *name, const at::Tensor &t) {
-    TORCH_CHECK(t.device() == q.device(), name, " must be on the same device as q");
-}
-
-void check_ok(int status, const char *op) {
-    TORCH_CHECK(status == KDA_OK, op, ": ", kda_status_string(status), " (status ", status, ")");
-}
-
-void *stream_of(const at::Tensor &t) {
-    return static_cast<void *>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
-}
 
 // A launch's metadata (int32 or int64, checked before), made contiguous where it
 // is not, and which of its arrays are int64 (KDA_WIDE_*): the kernels read
@@ -155,13 +141,6 @@ void check_pool(const at::Tensor &pool, int64_t H, int64_t D) {
     TORCH_CHECK(pool.stride(2) == 1 && pool.stride(3) == D,
                 "state must be K-contiguous (stride(2)==1, stride(3)==", D, "), got strides (",
                 pool.stride(2), ", ", pool.stride(3), ")");
-}
-
-// The kernels run on a HIP device only; a host tensor is an error, never a
-// fallback. Checked after the shape/layout rules so those are testable on a
-// machine without a GPU.
-void check_on_gpu(const char *name, const at::Tensor &t) {
-    TORCH_CHECK(t.device().is_cuda(), name, " must be a CUDA (HIP) tensor");
 }
 
 struct PoolRef {

@@ -1,0 +1,1199 @@
+// paged_attention.hip -- attention of new tokens over a paged key/value cache, gfx950.
+//
+// The query heads of a key head share its keys, so a request's new tokens and
+// their G = heads / kv_heads query heads of one key head are the rows of one
+// matrix: row r is token r / G, head r % G. Both kernels form S^T = K Q^T and
+// O^T = V^T P^T, so that a lane owns a row of the softmax (a column of the
+// tiles): the running maximum and sum need no LDS, and the scores that a lane
+// holds after the first product are, in their order, the operand it must supply
+// to the second. V^T comes from the row-major V tile in LDS through the
+// transposing read (ds_read_b64_tr_b16).
+//
+//   decode_kernel   few rows a request (at most 32): HBM-bound on the keys and
+//                   values, split over the keys
+//   prefill_kernel  many rows: bound by the matrix cores and the softmax's
+//                   vector instructions
+//   *_combine       join the parts of rows whose keys were split
+//
+// Softmax in powers of two: c = |scale| log2(e) k_scale is one factor of the
+// score (its sign goes into q), the weights are 2^(c s - m). m is raised only when
+// a score passes it by 2^8: the weights then stay below 2^8, far inside fp32 and
+// bf16, and the accumulators are rescaled a few times a row instead of every
+// tile. Scores, m, the sums and O are fp32; the weights are rounded to bf16 for
+// the second product only (the sum takes them unrounded).
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "kda_abi.h"
+#include "kda_device.h"
+#include "paged_cache.h"
+
+namespace kda {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kCus = 256;  // of an MI355X: only the number of workgroups goes by it
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kRaise = 8.0f;  // log2 of the largest weight before m is raised
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+struct __attribute__((packed, aligned(2))) Bf16x8Any {
+    u32x4 w;
+};
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Sixteen e4m3 (16 bytes) as bf16, exactly (three mantissa bits): two operands of 8.
+__device__ __forceinline__ void fp8_to_bf16(u32x4 x, u32x4 &lo, u32x4 &hi) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        lo[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.0f, false));
+        lo[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.0f, true));
+        hi[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 + i], 1.0f, false));
+        hi[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 + i], 1.0f, true));
+    }
+}
+
+// The other half's value (lanes l and l ^ 32), and sums and maxima over both.
+__device__ __forceinline__ float other_half(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(__lane_id() < 32 ? r[1] : r[0]);
+}
+__device__ __forceinline__ float max_halves(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The same over the four groups of 16 lanes.
+__device__ __forceinline__ float max_groups(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// cap tanh(s / cap) in log2 units; x = 2 log2(e) s / cap. tanh = 1 - 2 / (e^(2s/cap) + 1):
+// infinities give +-1, NaN stays; the error is an ulp of the cap, absolute.
+__device__ __forceinline__ float capped(float x, float cap2) {
+    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(ex2(x) + 1.0f);
+}
+
+// Rows of zeros that stand for keys outside a request or pages outside the pool.
+__device__ const u32x4 g_zero_row[16] = {};
+
+struct Request {
+    int begin;   // first token in q
+    int tokens;  // new tokens
+    int keys;    // keys in the cache, the new tokens' among them
+};
+
+struct Params : KdaPagedAttentionArgs {
+    int group;  // query heads a key head
+
+    __device__ __forceinline__ int meta(const void *p, int64_t i, int bit) const {
+        // the low word of an int64 entry is what a conversion to int32 keeps
+        const int shift = (wide & bit) != 0 ? 1 : 0;
+        return static_cast<const int32_t *>(p)[i << shift];
+    }
+    // Token ranges and lengths cut to the tensors, whatever the metadata says.
+    __device__ __forceinline__ int cu(int n) const {
+        return min(max(meta(cu_seqlens, n, KDA_WIDE_CU_SEQLENS), 0), num_tokens);
+    }
+    __device__ __forceinline__ Request request(int n) const {
+        Request r;
+        r.begin = cu(n);
+        r.tokens = max(cu(n + 1) - r.begin, 0);
+        r.keys = min(max(meta(kv_lens, n, KDA_WIDE_KV_LENS), 0), max_pages * cache.page_size);
+        return r;
+    }
+    // Keys visible to the i-th new token: [x, y)
+    __device__ __forceinline__ int2 visible(const Request &r, int i) const {
+        const int end = max(r.keys - r.tokens + i + 1, 0);
+        return make_int2(window > 0 ? max(end - window, 0) : 0, end);
+    }
+    // Page of key j of request n, or -1 (a page outside the pool).
+    __device__ __forceinline__ int page_of(int n, int at) const {
+        return meta(page_table, n * page_table_stride + at, KDA_WIDE_PAGE_TABLE);
+    }
+};
+
+// Factor of the scores in log2 units, and what the capped form needs. The sign
+// of scale * k_scale goes into q, so the largest score is the largest product.
+struct Scores {
+    float c;     // of the products, not capped
+    float cap;   // cap log2(e), 0: none
+    float in;    // 2 log2(e) / cap times the score's factor
+    uint32_t flip;
+};
+__device__ __forceinline__ Scores scores_of(const Params &a, int head) {
+    const float ks = a.cache.k_scale != nullptr ? a.cache.k_scale[head] : 1.0f;
+    const float f = a.scale * ks;
+    Scores s;
+    s.flip = f < 0.0f ? 0x80008000u : 0u;
+    // never 0: a masked score is -inf and stays it
+    const float mag = fabsf(f) < 1e-30f ? 1e-30f : fabsf(f);
+    s.c = mag * kLog2e;
+    s.cap = a.logit_cap * kLog2e;
+    s.in = a.logit_cap > 0.0f ? 2.0f * kLog2e * mag / a.logit_cap : 0.0f;
+    return s;
+}
+
+// A row of the cache: D elements, 16-byte chunks.
+template <int D, bool FP8> struct Row {
+    static constexpr int kBytes = FP8 ? D : 2 * D;
+    static constexpr int kLanes = kBytes / 16;   // lanes that load a row
+    static constexpr int kRows = 64 / kLanes;    // rows a wave loads at a time
+    static constexpr int kShift = FP8 ? 0 : 1;   // bytes of an element, log2
+};
+
+// LDS tiles of bf16 rows of D, without padding. Chunks of 16 bytes are permuted
+// within 256 bytes (one row of 128 or two of 64) by the row, so that the reads of
+// one column over 16 rows touch all banks alike.
+// K: chunk reads. V: transposing reads of 32-byte pairs of chunks, which stay together.
+template <int D> __device__ __forceinline__ int k_at(int row, int chunk) {
+    if constexpr (D == 128) {
+        return row * 256 + ((chunk ^ (row & 15)) << 4);
+    } else {
+        return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
+    }
+}
+template <int D> __device__ __forceinline__ int v_at(int row, int chunk) {
+    if constexpr (D == 128) {
+        return row * 256 + ((chunk ^ ((row & 7) << 1)) << 4);
+    } else {
+        return row * 128 + ((chunk ^ (((row >> 1) & 3) << 1)) << 4);
+    }
+}
+// Transposing read of rows row .. row + 3 (16 lanes: lane 4m + c takes row m), columns
+// 16 pair .. 16 pair + 15: lane i of the 16 gets column i of the four rows.
+template <int D> __device__ __forceinline__ u32x2 read_tr(const char *tile, int row, int pair, int lane) {
+    const int r = row + ((lane >> 2) & 3);
+    const int c = lane & 3;
+    const char *p = tile + v_at<D>(r, 2 * pair + (c >> 1)) + (c & 1) * 8;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+}
+
+// A 16-byte chunk of a loaded row into a tile, 8-bit ones widened to two chunks.
+template <int D, bool FP8, class At>
+__device__ __forceinline__ void stage(char *tile, int row, int chunk, u32x4 x, At at) {
+    if constexpr (FP8) {
+        u32x4 lo, hi;
+        fp8_to_bf16(x, lo, hi);
+        *reinterpret_cast<u32x4 *>(tile + at(row, 2 * chunk)) = lo;
+        *reinterpret_cast<u32x4 *>(tile + at(row, 2 * chunk + 1)) = hi;
+    } else {
+        *reinterpret_cast<u32x4 *>(tile + at(row, chunk)) = x;
+    }
+}
+
+__device__ __forceinline__ u32x4 load_q(const Params &a, int64_t token, int head, int d, uint32_t flip) {
+    const uint16_t *p =
+        static_cast<const uint16_t *>(a.q) + token * a.q_stride_token + head * a.q_stride_head + d;
+    return reinterpret_cast<const Bf16x8Any *>(p)->w ^ flip;
+}
+
+// Tokens that no request covers: zeros, spread over the grid.
+template <int D> __device__ __forceinline__ void zero_uncovered(const Params &a, int64_t block, int64_t blocks) {
+    const int64_t begin = a.cu(0), end = max(a.cu(a.num_seqs), a.cu(0));
+    const int64_t count = begin + (a.num_tokens - end);
+    for (int64_t i = block; i < count; i += blocks) {
+        const int64_t t = i < begin ? i : end + (i - begin);
+        for (int e = threadIdx.x; e < a.num_heads * D; e += kThreads) {
+            static_cast<uint16_t *>(a.out)[t * a.out_stride_token + (e / D) * a.out_stride_head + e % D] = 0;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: decode and verify steps.
+//
+// An item is a (request, key head, tile of 16 NB rows); its keys are cut at
+// multiples of 128 (a unit: 32 keys a wave). The units of all items in order are
+// dealt out evenly to the workgroups, whatever the lengths are: each takes
+// one contiguous range, which may begin and end inside an item. Every
+// workgroup finds its range itself from the lengths (a prefix sum over the
+// requests), so the call needs no host knowledge of them. An item inside one
+// range is finished there; the parts of the others are joined by
+// decode_combine_kernel, always in the same order.
+//
+// The waves are independent within an item: each streams its own 32-key blocks,
+// the keys straight into the matrix operands' registers, the values through
+// registers into 32 rows of LDS. The next block's loads (16 KiB a wave in bf16
+// at D = 128) are in flight while one is computed, the page numbers one
+// block further ahead.
+// ---------------------------------------------------------------------------
+
+constexpr int kUnit = 128;
+constexpr int kBlock = 32;
+constexpr int kDecodeGroups = 2 * kCus;
+
+struct DecodeWs {
+    float *o;     // [2 groups][rows][D]: a workgroup's part that continues an item, its part that begins one
+    float2 *ml;   // [2 groups][rows]
+    int4 *desc;   // [groups]: the item that begins in a workgroup and does not end there: request (-1: none),
+                  // key head, tile, last workgroup
+};
+
+template <int D, bool FP8> struct KvBlock {
+    static constexpr int kK = FP8 ? D / 64 : D / 32;  // 16-byte chunks of a key a lane holds
+    static constexpr int kV = kBlock / Row<D, FP8>::kRows;
+    u32x4 k[2][kK];
+    u32x4 v[kV];
+};
+
+template <int D, int NB> struct DecodeShared {
+    char v[kWaves][kBlock * D * 2];  // values of a wave's block; 16 rows of O when waves join
+    float2 ml[kWaves][16 * NB];
+    long long scan[kWaves];
+    long long before;  // the first unit of request `first`
+    int first;
+};
+
+// Units of a tile of `rows` rows of a request: the most that any of its tiles has.
+__device__ __forceinline__ int tile_units(const Params &a, const Request &r, int rows) {
+    int units = (r.keys + kUnit - 1) / kUnit;
+    if (a.window > 0) {
+        const int64_t tokens = (rows + a.group - 2) / a.group + 1;  // that a tile may touch
+        const int64_t span = a.window + tokens - 1;                 // keys that they see
+        const int64_t most = (span + kUnit - 2) / kUnit + 1;
+        units = static_cast<int>(min(static_cast<int64_t>(units), most));
+    }
+    return max(units, 1);  // an item without keys still writes its zeros
+}
+
+template <int D, bool FP8, int NB>
+__global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, const DecodeWs ws) {
+    constexpr int kRows = 16 * NB;
+    using R = Row<D, FP8>;
+    using Kv = KvBlock<D, FP8>;
+    __shared__ __attribute__((aligned(16))) DecodeShared<D, NB> sm;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4;
+    const int col = lane & 15;
+    const int heads = a.cache.kv_heads;
+
+    zero_uncovered<D>(a, blockIdx.x, gridDim.x);
+
+    // ---- this workgroup's range of units
+    const int per = (a.num_seqs + kThreads - 1) / kThreads;
+    const int n0 = min(tid * per, a.num_seqs), n1 = min(n0 + per, a.num_seqs);
+    auto units_of = [&](int n) -> long long {
+        const Request r = a.request(n);
+        const long long rows = static_cast<long long>(r.tokens) * a.group;
+        return (rows + kRows - 1) / kRows * heads * tile_units(a, r, kRows);
+    };
+    long long mine = 0;
+    for (int n = n0; n < n1; ++n) {
+        mine += units_of(n);
+    }
+    long long scan = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long up = __shfl_up(scan, d);
+        scan += lane >= d ? up : 0;
+    }
+    if (lane == 63) {
+        sm.scan[wave] = scan;
+    }
+    __syncthreads();
+    long long total = 0, base = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        base += w < wave ? sm.scan[w] : 0;
+        total += sm.scan[w];
+    }
+    const long long groups = min(static_cast<long long>(gridDim.x), total);
+    const long long w = blockIdx.x;
+    if (w >= groups) {
+        if (tid == 0) {
+            ws.desc[w] = make_int4(-1, 0, 0, 0);
+        }
+        return;
+    }
+    const long long u0 = w * total / groups, u1 = (w + 1) * total / groups;
+    long long at = base + scan - mine;
+    if (u0 >= at && u0 < at + mine) {  // one thread's requests hold the first unit
+        int n = n0;
+        for (;; ++n) {
+            const long long u = units_of(n);
+            if (u0 < at + u) {
+                break;
+            }
+            at += u;
+        }
+        sm.first = n;
+        sm.before = at;
+    }
+    __syncthreads();
+    int n = __builtin_amdgcn_readfirstlane(sm.first);
+    long long start = sm.before;  // the first unit of request n
+    int4 desc = make_int4(-1, 0, 0, 0);
+
+    for (long long u = u0; u < u1;) {
+        const Request req = a.request(n);
+        const int rows_all = req.tokens * a.group;
+        const int tiles = (rows_all + kRows - 1) / kRows;
+        const int count = tile_units(a, req, kRows);
+        const long long units = static_cast<long long>(tiles) * heads * count;
+        if (u >= start + units) {
+            start += units;
+            ++n;
+            continue;
+        }
+        // ---- the item and the part of it that is in this range
+        const long long local = u - start;
+        const long long item = local / count;
+        const int part0 = static_cast<int>(local - item * count);
+        const int part1 = static_cast<int>(min(static_cast<long long>(count), part0 + (u1 - u)));
+        const int tile = static_cast<int>(item % tiles);
+        const int head = static_cast<int>(item / tiles);
+        const int row0 = tile * kRows;
+        const int rows = min(kRows, rows_all - row0);
+        const int2 first = a.visible(req, row0 / a.group);
+        const int2 last = a.visible(req, (row0 + rows - 1) / a.group);
+        const int unit0 = first.x / kUnit;
+        const int lo = max(first.x, (unit0 + part0) * kUnit);  // keys of this part: [lo, hi)
+        const int hi = min(last.y, (unit0 + part1) * kUnit);
+        const Scores sc = scores_of(a, head);
+
+        // ---- queries: 16 rows a block as the right operand
+        u32x4 q[NB][D / 32];
+        int2 see[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int r = min(b * 16 + col, rows - 1);
+            const int t = (row0 + r) / a.group;
+            const int h = head * a.group + (row0 + r) - t * a.group;
+            see[b] = a.visible(req, t);
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+                // 8-bit keys are loaded 16 columns at a time, two products' worth
+                const int d = FP8 ? (s / 2) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
+                q[b][s] = load_q(a, req.begin + t, h, d, sc.flip);
+            }
+        }
+        f32x4 o[NB][D / 16];
+        float m[NB], l[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            m[b] = kNegInf;
+            l[b] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                o[b][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+
+        // ---- this wave's blocks of 32 keys: key0 + 128 i
+        const int key0 = (unit0 + part0) * kUnit + wave * kBlock;
+        const int blocks = hi > key0 ? (hi - key0 + kUnit - 1) / kUnit : 0;
+        const char *kbase = static_cast<const char *>(a.cache.k) + ((head * a.cache.k_stride_head) << R::kShift);
+        const char *vbase = static_cast<const char *>(a.cache.v) + ((head * a.cache.v_stride_head) << R::kShift);
+        auto lookup = [&](int i) -> int {  // page of key lane % 32 of block i; any entry where it has none
+            const int key = key0 + i * kUnit + (lane & 31);
+            return a.page_of(n, min(max(key, 0) / a.cache.page_size, a.max_pages - 1));
+        };
+        auto load = [&](int i, int page, Kv &kv) {
+            const int key = key0 + i * kUnit + (lane & 31);
+            const int off = key - key / a.cache.page_size * a.cache.page_size;
+            const bool real = key >= lo && key < hi && page >= 0 && page < a.cache.num_pages;
+            const char *kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
+            const char *vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
+            const unsigned long long ka = reinterpret_cast<unsigned long long>(real ? kp : reinterpret_cast<const char *>(g_zero_row));
+            const unsigned long long va = reinterpret_cast<unsigned long long>(real ? vp : reinterpret_cast<const char *>(g_zero_row));
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const char *p = reinterpret_cast<const char *>(__shfl(ka, kt * 16 + col));
+#pragma unroll
+                for (int s = 0; s < Kv::kK; ++s) {
+                    kv.k[kt][s] = *reinterpret_cast<const u32x4 *>(p + s * 64 + g * 16);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < Kv::kV; ++s) {
+                const char *p = reinterpret_cast<const char *>(__shfl(va, s * R::kRows + lane / R::kLanes));
+                kv.v[s] = *reinterpret_cast<const u32x4 *>(p + lane % R::kLanes * 16);
+            }
+        };
+        auto compute = [&](int i, const Kv &kv) {
+            char *vt = sm.v[wave];
+            f32x4 s[NB][2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                u32x4 op[D / 32];
+                if constexpr (FP8) {
+#pragma unroll
+                    for (int x = 0; x < Kv::kK; ++x) {
+                        fp8_to_bf16(kv.k[kt][x], op[2 * x], op[2 * x + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < Kv::kK; ++x) {
+                        op[x] = kv.k[kt][x];
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    s[b][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x) {
+                        s[b][kt] = mfma16(op[x], q[b][x], s[b][kt]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < Kv::kV; ++x) {
+                stage<D, FP8>(vt, x * R::kRows + lane / R::kLanes, lane % R::kLanes, kv.v[x],
+                              [](int r, int c) { return v_at<D>(r, c); });
+            }
+            // a lane's scores: row `col`, keys 16 kt + 4 g + e
+            const int key = key0 + i * kUnit + 4 * g;
+            u32x4 p[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int from = max(see[b].x, lo), to = min(see[b].y, hi);
+                float top = kNegInf;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int k = key + 16 * kt + e;
+                        float x = s[b][kt][e];
+                        x = sc.cap > 0.0f ? capped(x * sc.in, sc.cap) : x * sc.c;
+                        x = k >= from && k < to ? x : kNegInf;
+                        s[b][kt][e] = x;
+                        top = fmaxf(top, x);
+                    }
+                }
+                top = max_groups(top);
+                if (__any(top > m[b] + kRaise)) {
+                    const float next = fmaxf(m[b], top);
+                    const float f = next == m[b] ? 1.0f : ex2(m[b] - next);
+                    m[b] = next;
+                    l[b] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        o[b][d] *= f;
+                    }
+                }
+                const float base = m[b] == kNegInf ? 0.0f : m[b];
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = ex2(s[b][e >> 2][e & 3] - base);
+                    l[b] += w[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[b][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                const u32x2 v0 = read_tr<D>(vt, 4 * g, d, lane);
+                const u32x2 v1 = read_tr<D>(vt, 16 + 4 * g, d, lane);
+                const u32x4 op = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    o[b][d] = mfma16(op, p[b], o[b][d]);
+                }
+            }
+        };
+        if (blocks > 0) {
+            // two register sets, so that no loaded value is copied before it has arrived; past the
+            // last block the rows of zeros are loaded
+            Kv even, odd;
+            int p0 = lookup(0), p1 = lookup(1);
+            load(0, p0, even);
+            for (int i = 0;; i += 2) {
+                p0 = lookup(i + 2);
+                load(i + 1, p1, odd);
+                compute(i, even);
+                if (i + 1 >= blocks) {
+                    break;
+                }
+                p1 = lookup(i + 3);
+                load(i + 2, p0, even);
+                compute(i + 1, odd);
+                if (i + 2 >= blocks) {
+                    break;
+                }
+            }
+        }
+
+        // ---- join the waves: their maxima, sums and 16 rows of O at a time through LDS
+        const bool begins = part0 == 0, ends = part1 == count;
+        const int64_t slot = 2 * w + (begins ? 1 : 0);
+        if (begins && !ends) {
+            const long long end = start + (item + 1) * count;  // its last unit + 1
+            desc = make_int4(n, head, tile, static_cast<int>((end * groups + total - 1) / total - 1));
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float sum = sum_groups(l[b]);
+            if (g == 0) {
+                sm.ml[wave][b * 16 + col] = make_float2(m[b], sum);
+            }
+        }
+        const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            // 16 rows of D floats take a wave's 32 rows of D bf16
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {  // 16-byte chunks, permuted by the row against bank conflicts
+                const int chunk = (4 * d + g) ^ (D == 128 ? col : col & 7);
+                *reinterpret_cast<f32x4 *>(sm.v[wave] + col * D * 4 + chunk * 16) = o[b][d];
+            }
+            __syncthreads();
+            const int r = tid >> 4;  // 16 threads a row
+            float2 ml[kWaves];
+            float top = kNegInf;
+#pragma unroll
+            for (int x = 0; x < kWaves; ++x) {
+                ml[x] = sm.ml[x][b * 16 + r];
+                top = fmaxf(top, ml[x].x);
+            }
+            float sum = 0.0f, f[kWaves];
+#pragma unroll
+            for (int x = 0; x < kWaves; ++x) {
+                f[x] = ml[x].x == top ? 1.0f : ex2(ml[x].x - top);
+                sum += ml[x].y * f[x];
+            }
+            const float norm = begins && ends ? (sum == 0.0f ? 0.0f : vs / sum) : 1.0f;
+            const int t = (row0 + b * 16 + r) / a.group;
+            const int h = head * a.group + (row0 + b * 16 + r) - t * a.group;
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) {
+                const int c = (tid & 15) + 16 * x;
+                const int chunk = c ^ (D == 128 ? r : r & 7);
+                f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < kWaves; ++k) {
+                    y += *reinterpret_cast<const f32x4 *>(sm.v[k] + r * D * 4 + chunk * 16) * f[k];
+                }
+                y *= norm;
+                if (b * 16 + r < rows) {
+                    if (begins && ends) {
+                        uint16_t *out = static_cast<uint16_t *>(a.out) + (req.begin + t) * a.out_stride_token +
+                                        h * a.out_stride_head + c * 4;
+                        struct __attribute__((packed, aligned(2))) Out {
+                            uint32_t w[2];
+                        };
+                        *reinterpret_cast<Out *>(out) = {{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}};
+                    } else {
+                        *reinterpret_cast<f32x4 *>(ws.o + (slot * kRows + b * 16 + r) * D + c * 4) = y;
+                    }
+                }
+            }
+            if (!(begins && ends) && (tid & 15) == 0) {
+                ws.ml[slot * kRows + b * 16 + r] = make_float2(top, sum);
+            }
+            __syncthreads();
+        }
+        u += part1 - part0;
+    }
+    if (tid == 0) {
+        ws.desc[w] = desc;
+    }
+}
+
+// One workgroup for each of decode_kernel's: joins the item that began there.
+template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const Params a, const DecodeWs ws) {
+    constexpr int kRows = 16 * NB;
+    const int w = blockIdx.x;
+    const int4 desc = ws.desc[w];
+    if (desc.x < 0) {
+        return;
+    }
+    const Request req = a.request(desc.x);
+    const int row0 = desc.z * kRows;
+    const int rows = min(kRows, req.tokens * a.group - row0);
+    const int last = desc.w;
+    const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[desc.y] : 1.0f;
+    // parts: the second slot of w, then the first ones of w + 1 .. last
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+        const int r = i / (D / 4);
+        const int c = i % (D / 4);
+        auto slot = [&](int x) -> int64_t { return x == w ? 2 * static_cast<int64_t>(w) + 1 : 2 * static_cast<int64_t>(x); };
+        float top = kNegInf;
+        for (int x = w; x <= last; ++x) {
+            top = fmaxf(top, ws.ml[slot(x) * kRows + r].x);
+        }
+        float sum = 0.0f;
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x = w; x <= last; ++x) {
+            const float2 ml = ws.ml[slot(x) * kRows + r];
+            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+            sum += ml.y * f;
+            y += *reinterpret_cast<const f32x4 *>(ws.o + (slot(x) * kRows + r) * D + c * 4) * f;
+        }
+        y *= sum == 0.0f ? 0.0f : vs / sum;
+        const int t = (row0 + r) / a.group;
+        const int h = desc.y * a.group + (row0 + r) - t * a.group;
+        uint16_t *out = static_cast<uint16_t *>(a.out) + (req.begin + t) * a.out_stride_token + h * a.out_stride_head + c * 4;
+        struct __attribute__((packed, aligned(2))) Out {
+            uint32_t w[2];
+        };
+        *reinterpret_cast<Out *>(out) = {{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}};
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: prefill chunks and long verify steps.
+//
+// A workgroup takes a tile of 128 RB rows of one (request, key head), 32 RB a
+// wave, and walks the visible keys in tiles of 64. The four waves share a key and
+// a value tile in LDS (bf16; 8-bit ones are widened when staged, once for all four),
+// two of each, so one barrier a tile is enough. The next tile's rows are loaded into
+// registers while this one is computed.
+//
+// Tiles of rows are found from cu_seqlens alone: request n gets the numbers
+// from floor(cu[n] G / rows) + n, at least as many as it needs, so a tile's
+// request is a count over the requests and no host copy of the lengths is needed.
+// The last tiles (the longest, under the causal mask) go first; the key head is the
+// fastest index, so that the workgroups of a head meet in one chiplet's L2.
+// ---------------------------------------------------------------------------
+
+constexpr int kTile = 64;
+
+struct PrefillWs {
+    float *o;    // [splits][key heads][tokens * group][D], not normalized
+    float2 *ml;  // [splits][key heads][tokens * group]
+};
+
+template <int D, bool FP8, int RB, bool UNIFORM>
+__global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(const Params a, const PrefillWs ws, int tiles,
+                                                                            int splits) {
+    constexpr int kRows = 128 * RB;
+    using R = Row<D, FP8>;
+    constexpr int kLoads = 16 / R::kRows;  // 16-byte loads a thread, of 16 rows a wave
+    constexpr int kBytes = kTile * D * 2;
+    __shared__ __attribute__((aligned(16))) char sm[2][2][kBytes];  // [parity][K, V]
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5;
+    const int col = lane & 31;
+
+    if (blockIdx.x < 64) {
+        zero_uncovered<D>(a, blockIdx.x, min(gridDim.x, 64u));
+    }
+
+    // ---- the tile: key head, split, request, rows
+    uint32_t id = blockIdx.x;
+    const int head = id % a.cache.kv_heads;
+    id /= a.cache.kv_heads;
+    const int split = id % splits;
+    const int tile = tiles - 1 - static_cast<int>(id / splits);
+    int below = 0;  // requests that begin at or before this tile
+    for (int n = 0; n < a.num_seqs; n += kThreads) {
+        const int x = n + tid;
+        const int first = x < a.num_seqs ? static_cast<int>(static_cast<int64_t>(a.cu(x)) * a.group / kRows) + x : INT32_MAX;
+        below += __syncthreads_count(first <= tile);
+    }
+    const int n = __builtin_amdgcn_readfirstlane(below) - 1;
+    if (n < 0) {
+        return;
+    }
+    const Request req = a.request(n);
+    const int first_tile = static_cast<int>(static_cast<int64_t>(req.begin) * a.group / kRows) + n;
+    const int64_t row0_wide = static_cast<int64_t>(tile - first_tile) * kRows;
+    const int rows_all = req.tokens * a.group;
+    if (row0_wide < 0 || row0_wide >= rows_all) {
+        return;
+    }
+    const int row0 = static_cast<int>(row0_wide);
+    const int rows = min(kRows, rows_all - row0);
+
+    // ---- visible keys: of the tile in tiles of 64, of the wave, of each lane's rows
+    const int2 see0 = a.visible(req, row0 / a.group);
+    const int2 see1 = a.visible(req, (row0 + rows - 1) / a.group);
+    const int all0 = see0.x / kTile, all1 = (see1.y + kTile - 1) / kTile;
+    const int share = (all1 - all0 + splits - 1) / splits;
+    const int t0 = all0 + split * share, t1 = min(all1, t0 + share);
+    const int wrow0 = min(row0 + wave * 32 * RB, row0 + rows - 1);
+    const int wrow1 = min(wrow0 + 32 * RB, row0 + rows) - 1;
+    const int2 wsee0 = a.visible(req, wrow0 / a.group);
+    const int2 wsee1 = a.visible(req, wrow1 / a.group);
+    const bool active = wave * 32 * RB < rows;  // the wave has rows
+    const Scores sc = scores_of(a, head);
+
+    u32x4 q[RB][D / 16];
+    int2 see[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int r = min(row0 + wave * 32 * RB + b * 32 + col, row0 + rows - 1);
+        const int t = r / a.group;
+        const int h = head * a.group + r - t * a.group;
+        see[b] = a.visible(req, t);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            q[b][s] = load_q(a, req.begin + t, h, s * 16 + half * 8, sc.flip);
+        }
+    }
+    f32x16 o[RB][D / 32];
+    float m[RB], l[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        m[b] = kNegInf;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[b][d][e] = 0.0f;
+            }
+        }
+    }
+
+    // ---- staging: a wave loads 16 of a tile's 64 rows
+    const char *kbase = static_cast<const char *>(a.cache.k) + ((head * a.cache.k_stride_head) << R::kShift);
+    const char *vbase = static_cast<const char *>(a.cache.v) + ((head * a.cache.v_stride_head) << R::kShift);
+    const int srow = wave * 16 + lane / R::kLanes;  // + kRows of Row for each further load
+    const int schunk = lane % R::kLanes;
+    struct Pages {
+        int p[kLoads];
+    };
+    // UNIFORM: pages hold a multiple of 16 tokens, so a wave's 16 rows are on one page
+    auto lookup = [&](int t) -> Pages {
+        Pages r;
+        if constexpr (UNIFORM) {
+            const int at = __builtin_amdgcn_readfirstlane((t * kTile + wave * 16) / a.cache.page_size);
+            r.p[0] = a.page_of(n, min(at, a.max_pages - 1));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                r.p[i] = a.page_of(n, min((t * kTile + srow + i * R::kRows) / a.cache.page_size, a.max_pages - 1));
+            }
+        }
+        return r;
+    };
+    u32x4 kreg[kLoads], vreg[kLoads];
+    auto load = [&](int t, const Pages &pages) {
+        const int key0 = t * kTile;
+        int page = 0, off0 = 0;
+        const char *kp0 = nullptr, *vp0 = nullptr;
+        if constexpr (UNIFORM) {
+            page = __builtin_amdgcn_readfirstlane(pages.p[0]);
+            const int k = key0 + wave * 16;
+            off0 = k - k / a.cache.page_size * a.cache.page_size;
+            kp0 = kbase + ((page * a.cache.k_stride_page + off0 * a.cache.k_stride_token) << R::kShift);
+            vp0 = vbase + ((page * a.cache.v_stride_page + off0 * a.cache.v_stride_token) << R::kShift);
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int key = key0 + srow + i * R::kRows;
+            const char *kp, *vp;
+            if constexpr (UNIFORM) {
+                const int r = lane / R::kLanes + i * R::kRows;
+                kp = kp0 + ((r * a.cache.k_stride_token) << R::kShift);
+                vp = vp0 + ((r * a.cache.v_stride_token) << R::kShift);
+            } else {
+                page = pages.p[i];
+                const int off = key - key / a.cache.page_size * a.cache.page_size;
+                kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
+                vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
+            }
+            const bool real = key >= see0.x && key < see1.y && page >= 0 && page < a.cache.num_pages;
+            const char *zero = reinterpret_cast<const char *>(g_zero_row);
+            kp = real ? kp : zero;
+            vp = real ? vp : zero;
+            kreg[i] = *reinterpret_cast<const u32x4 *>(kp + schunk * 16);
+            vreg[i] = *reinterpret_cast<const u32x4 *>(vp + schunk * 16);
+        }
+    };
+    auto write = [&](int parity) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            stage<D, FP8>(sm[parity][0], srow + i * R::kRows, schunk, kreg[i], [](int r, int c) { return k_at<D>(r, c); });
+            stage<D, FP8>(sm[parity][1], srow + i * R::kRows, schunk, vreg[i], [](int r, int c) { return v_at<D>(r, c); });
+        }
+    };
+    auto compute = [&](int t, int parity) {
+        const char *kt_ = sm[parity][0];
+        const char *vt = sm[parity][1];
+        f32x16 s[2][RB];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[kt][b][e] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                const u32x4 op = *reinterpret_cast<const u32x4 *>(kt_ + k_at<D>(kt * 32 + col, 2 * x + half));
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    s[kt][b] = mfma32(op, q[b][x], s[kt][b]);
+                }
+            }
+        }
+        const int key0 = t * kTile;
+        const bool whole = key0 >= wsee1.x && key0 + kTile <= wsee0.y;  // every row of the wave sees every key
+        u32x4 p[RB][4];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            float c = sc.c;
+            if (sc.cap > 0.0f) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[kt][b][e] = capped(s[kt][b][e] * sc.in, sc.cap);
+                    }
+                }
+                c = 1.0f;
+            }
+            if (!whole) {
+                // a lane's scores: row `col`, keys 32 kt + 8 (e / 4) + 4 half + e % 4
+                const int from = see[b].x - key0 - 4 * half, to = see[b].y - key0 - 4 * half;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int k = 32 * kt + 8 * (e >> 2) + (e & 3);
+                        s[kt][b][e] = k >= from && k < to ? s[kt][b][e] : kNegInf;
+                    }
+                }
+            }
+            float top = kNegInf;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    top = fmaxf(top, s[kt][b][e]);
+                }
+            }
+            top = max_halves(top) * c;
+            if (__any(top > m[b] + kRaise)) {
+                const float next = fmaxf(m[b], top);
+                const float f = next == m[b] ? 1.0f : ex2(m[b] - next);
+                m[b] = next;
+                l[b] *= f;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    o[b][d] *= f;
+                }
+            }
+            const float base = m[b] == kNegInf ? 0.0f : m[b];
+            float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {  // 16 keys: 8 of this half
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = ex2(s[x >> 1][b][8 * (x & 1) + e] * c - base);
+                }
+                sum0 += (w[0] + w[1]) + (w[2] + w[3]);
+                sum1 += (w[4] + w[5]) + (w[6] + w[7]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[b][x][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+                }
+            }
+            l[b] += sum0 + sum1;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const int pair = 2 * d + ((lane >> 4) & 1);
+                const u32x2 v0 = read_tr<D>(vt, 16 * x + 4 * half, pair, lane);
+                const u32x2 v1 = read_tr<D>(vt, 16 * x + 8 + 4 * half, pair, lane);
+                const u32x4 op = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    o[b][d] = mfma32(op, p[b][x], o[b][d]);
+                }
+            }
+        }
+    };
+
+    if (t0 < t1) {
+        Pages pages = lookup(t0);
+        load(t0, pages);
+        pages = lookup(t0 + 1);
+        write(0);
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            const int parity = (t - t0) & 1;
+            // past the last tile the rows of zeros are loaded and staged, and not read
+            load(t + 1, pages);
+            pages = lookup(t + 2);
+            if (active && t * kTile < wsee1.y && (t + 1) * kTile > wsee0.x) {
+                compute(t, parity);
+            }
+            write(parity ^ 1);
+            __syncthreads();
+        }
+    }
+
+    // ---- out, or this split's part: lane: row `col` of 32, columns 32 d + 8 (e / 4) + 4 half + e % 4
+    const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int r = wave * 32 * RB + b * 32 + col;
+        const float sum = sum_halves(l[b]);
+        if (r >= rows) {
+            continue;
+        }
+        if (splits == 1) {
+            const float f = sum == 0.0f ? 0.0f : vs / sum;
+            const int t = (row0 + r) / a.group;
+            const int h = head * a.group + (row0 + r) - t * a.group;
+            uint16_t *out = static_cast<uint16_t *>(a.out) + static_cast<int64_t>(req.begin + t) * a.out_stride_token +
+                            h * a.out_stride_head + half * 4;
+            struct __attribute__((packed, aligned(2))) Out {
+                uint32_t w[2];
+            };
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    *reinterpret_cast<Out *>(out + d * 32 + e * 8) = {
+                        {pack_bf16x2(o[b][d][4 * e] * f, o[b][d][4 * e + 1] * f),
+                         pack_bf16x2(o[b][d][4 * e + 2] * f, o[b][d][4 * e + 3] * f)}};
+                }
+            }
+        } else {
+            const int64_t all = static_cast<int64_t>(a.num_tokens) * a.group;
+            const int64_t at = (static_cast<int64_t>(split) * a.cache.kv_heads + head) * all +
+                               static_cast<int64_t>(req.begin) * a.group + row0 + r;
+            if (half == 0) {
+                ws.ml[at] = make_float2(m[b], sum);
+            }
+            if (sum != 0.0f) {  // the join reads no others
+                float *po = ws.o + at * D + half * 4;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        *reinterpret_cast<f32x4 *>(po + d * 32 + e * 8) =
+                            f32x4{o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]};
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Joins the splits of every (token, head): 16 or 32 threads a row, 4 columns each.
+template <int D> __global__ __launch_bounds__(kThreads) void prefill_combine_kernel(const Params a, const PrefillWs ws, int splits) {
+    constexpr int kPer = D / 4;
+    const int64_t all = static_cast<int64_t>(a.num_tokens) * a.group;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / kPer) + threadIdx.x / kPer;
+    if (i >= all * a.cache.kv_heads) {
+        return;
+    }
+    const int64_t row = i / a.cache.kv_heads;
+    const int head = static_cast<int>(i % a.cache.kv_heads);
+    const int64_t t = row / a.group;
+    if (t < a.cu(0) || t >= a.cu(a.num_seqs)) {
+        return;  // no request's token: zero already
+    }
+    const int c = threadIdx.x % kPer * 4;
+    const int64_t step = a.cache.kv_heads * all, at = head * all + row;
+    float top = kNegInf;
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = ws.ml[at + s * step];
+        top = ml.y == 0.0f ? top : fmaxf(top, ml.x);
+    }
+    float sum = 0.0f;
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = ws.ml[at + s * step];
+        if (ml.y != 0.0f) {
+            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+            sum += ml.y * f;
+            y += *reinterpret_cast<const f32x4 *>(ws.o + (at + s * step) * D + c) * f;
+        }
+    }
+    const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
+    y *= sum == 0.0f ? 0.0f : vs / sum;
+    uint16_t *out = static_cast<uint16_t *>(a.out) + t * a.out_stride_token +
+                    (head * a.group + row - t * a.group) * a.out_stride_head + c;
+    struct __attribute__((packed, aligned(2))) Out {
+        uint32_t w[2];
+    };
+    *reinterpret_cast<Out *>(out) = {{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}};
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+constexpr int kRowBlocks = 1;  // RB of the prefill kernel
+
+struct Plan {
+    bool decode;
+    int blocks;     // decode: NB
+    bool join;      // decode: items may be split
+    int64_t tiles;  // prefill
+    int splits;
+    size_t ml_at, desc_at, bytes;
+};
+
+size_t up256(size_t x) { return (x + 255) & ~size_t{255}; }
+
+Plan plan_of(const KdaPagedAttentionArgs &a) {
+    Plan p{};
+    const int64_t group = a.num_heads / a.cache.kv_heads;
+    const int64_t rows = std::max<int64_t>(a.max_query_len, 1) * group;
+    const int64_t keys = static_cast<int64_t>(a.max_pages) * a.cache.page_size;
+    const size_t d = a.cache.head_dim;
+    p.decode = rows <= 32 || a.num_seqs == 0;  // without requests it only writes the zeros
+    if (p.decode) {
+        p.blocks = rows <= 16 ? 1 : 2;
+        p.join = keys > kUnit;
+        const size_t parts = size_t{2} * kDecodeGroups * 16 * p.blocks;
+        p.ml_at = up256(p.join ? parts * d * 4 : 0);
+        p.desc_at = up256(p.ml_at + (p.join ? parts * 8 : 0));
+        p.bytes = p.desc_at + size_t{kDecodeGroups} * 16;
+        return p;
+    }
+    const int64_t tile_rows = 128 * kRowBlocks;
+    p.tiles = static_cast<int64_t>(a.num_tokens) * group / tile_rows + a.num_seqs;
+    // few tiles over many keys: cut the keys until two workgroups a CU have work, in
+    // parts of 512 keys at least
+    const int64_t units = p.tiles * a.cache.kv_heads;
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2 * kCus / units, keys / 512, 64})));
+    if (p.splits > 1) {
+        const size_t parts = static_cast<size_t>(p.splits) * a.num_tokens * a.num_heads;
+        p.ml_at = up256(parts * d * 4);
+        p.bytes = up256(p.ml_at + parts * 8);
+    }
+    return p;
+}
+
+int check(const KdaPagedAttentionArgs *args) {
+    if (args == nullptr) {
+        return KDA_ERR_INVALID_ARGUMENT;
+    }
+    const KdaPagedAttentionArgs &a = *args;
+    if (const int rc = check_cache(a.cache); rc != KDA_OK) {
+        return rc;
+    }
+    constexpr int32_t kWide = KDA_WIDE_PAGE_TABLE | KDA_WIDE_KV_LENS | KDA_WIDE_CU_SEQLENS;
+    if (a.num_seqs < 0 || a.num_tokens < 0 || a.num_heads <= 0 || a.max_pages < 0 || a.window < 0 ||
+        !(a.logit_cap >= 0.0f) || (a.wide & ~kWide) != 0 || a.num_heads % a.cache.kv_heads != 0) {
+        return KDA_ERR_INVALID_ARGUMENT;
+    }
+    const int64_t group = a.num_heads / a.cache.kv_heads;
+    // row and key numbers, and the roundings up of both, stay in 32 bits
+    if (a.num_tokens * group + 128 * static_cast<int64_t>(a.num_seqs) > INT32_MAX - 1024 ||
+        static_cast<int64_t>(a.max_pages) * a.cache.page_size > INT32_MAX - 1024) {
+        return KDA_ERR_TOO_LARGE;
+    }
+    return KDA_OK;
+}
+
+bool misaligned(const void *p, uintptr_t m) { return reinterpret_cast<uintptr_t>(p) % m != 0; }
+
+template <int D, bool FP8, int NB> void launch_decode(const Params &a, const Plan &p, char *ws, hipStream_t s) {
+    const DecodeWs w{reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.ml_at),
+                     reinterpret_cast<int4 *>(ws + p.desc_at)};
+    decode_kernel<D, FP8, NB><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
+    if (p.join) {
+        decode_combine_kernel<D, NB><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
+    }
+}
+
+template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p, char *ws, hipStream_t s) {
+    if (p.decode) {
+        p.blocks == 1 ? launch_decode<D, FP8, 1>(a, p, ws, s) : launch_decode<D, FP8, 2>(a, p, ws, s);
+        return;
+    }
+    const PrefillWs w{reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.ml_at)};
+    const unsigned grid = static_cast<unsigned>(p.tiles * a.cache.kv_heads * p.splits);
+    const int tiles = static_cast<int>(p.tiles);
+    if (a.cache.page_size % 16 == 0) {
+        prefill_kernel<D, FP8, kRowBlocks, true><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
+    } else {
+        prefill_kernel<D, FP8, kRowBlocks, false><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
+    }
+    if (p.splits > 1) {
+        const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.num_heads;
+        constexpr int kPer = kThreads / (D / 4);
+        prefill_combine_kernel<D><<<static_cast<unsigned>((rows + kPer - 1) / kPer), kThreads, 0, s>>>(a, w, p.splits);
+    }
+}
+
+}  // namespace
+}  // namespace kda
+
+extern "C" size_t kda_paged_attention_workspace_bytes(const KdaPagedAttentionArgs *args) {
+    using namespace kda;
+    if (check(args) != KDA_OK || args->num_tokens == 0) {
+        return 0;
+    }
+    return plan_of(*args).bytes;
+}
+
+extern "C" int kda_paged_attention_launch(const KdaPagedAttentionArgs *args, void *workspace, size_t workspace_bytes,
+                                          void *stream) {
+    using namespace kda;
+    if (const int rc = check(args); rc != KDA_OK) {
+        return rc;
+    }
+    Params a{*args, args->num_heads / args->cache.kv_heads};
+    if (a.num_tokens == 0) {
+        return KDA_OK;
+    }
+    if (a.q == nullptr || a.out == nullptr || misaligned(a.q, 2) || misaligned(a.out, 2) || a.cu_seqlens == nullptr ||
+        misaligned(a.cu_seqlens, (a.wide & KDA_WIDE_CU_SEQLENS) != 0 ? 8 : 4) ||
+        (a.num_seqs > 0 && (a.kv_lens == nullptr || misaligned(a.kv_lens, (a.wide & KDA_WIDE_KV_LENS) != 0 ? 8 : 4))) ||
+        (a.num_seqs > 0 && a.max_pages > 0 &&
+         (a.page_table == nullptr || misaligned(a.page_table, (a.wide & KDA_WIDE_PAGE_TABLE) != 0 ? 8 : 4)))) {
+        return KDA_ERR_INVALID_ARGUMENT;
+    }
+    const Plan p = plan_of(a);
+    // a grid counts its threads in 32 bits
+    if (!p.decode && (p.tiles * a.cache.kv_heads * p.splits > (INT64_C(1) << 24) - 1 ||
+                      (p.splits > 1 && static_cast<int64_t>(a.num_tokens) * a.num_heads > (INT64_C(1) << 26)))) {
+        return KDA_ERR_TOO_LARGE;
+    }
+    if (p.bytes > 0 && (workspace == nullptr || misaligned(workspace, 256) || workspace_bytes < p.bytes)) {
+        return KDA_ERR_WORKSPACE;
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char *ws = static_cast<char *>(workspace);
+    const bool fp8 = a.cache.dtype == KDA_FP8_E4M3;
+    (void)hipGetLastError();
+    if (a.cache.head_dim == 128) {
+        fp8 ? launch_attention<128, true>(a, p, ws, s) : launch_attention<128, false>(a, p, ws, s);
+    } else {
+        fp8 ? launch_attention<64, true>(a, p, ws, s) : launch_attention<64, false>(a, p, ws, s);
+    }
+    return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+}

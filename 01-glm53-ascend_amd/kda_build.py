@@ -31,9 +31,9 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = os.environ.get("KDA_OFFLOAD_ARCH", "gfx950")
 
-HIP_SOURCES = ["kda_recurrent.hip", "kda_chunk.hip"]
+HIP_SOURCES = ["kda_recurrent.hip", "kda_chunk.hip", "rms_norm.hip", "paged_store.hip", "paged_attention.hip"]
 ABI_SOURCES = ["kda_abi.cpp"]
-TORCH_SOURCES = ["kda_torch_ops.cpp"]
+TORCH_SOURCES = ["kda_torch_ops.cpp", "decoder_torch_ops.cpp"]
 
 # Packed-FP32 VALU forms are disabled for all device code: they are not
 # needed for throughput here and some of their forms have misbehaved on this

@@ -1,3 +1,4 @@
+from .decoder import add_rms_norm, add_rms_norm_fp8, paged_attention, paged_kv_store
 from .kda import (
     kda_prepared_varlen_chunk,
     kda_prepared_varlen_recurrent,
@@ -10,6 +11,8 @@ from .kda import (
 )
 
 __all__ = [
+    "add_rms_norm",
+    "add_rms_norm_fp8",
     "kda_prepared_varlen_chunk",
     "kda_prepared_varlen_recurrent",
     "kda_varlen_chunk",
@@ -17,5 +20,7 @@ __all__ = [
     "kda_varlen_chunk_with_state",
     "kda_varlen_recurrent",
     "kda_varlen_recurrent_v2",
+    "paged_attention",
+    "paged_kv_store",
     "prepared_recurrent",
 ]

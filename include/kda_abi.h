@@ -38,6 +38,10 @@
  * null: the requests still run, so a prefix tracked at length 0 receives the
  * request's initial state.
  *
+ * Beside the KDA entry points stand those of the other parts of a decoder that
+ * interleaves KDA layers with full attention (no counterpart in the reference):
+ * kda_rms_norm_launch, kda_paged_store_launch and kda_paged_attention_launch.
+ *
  * All launches are asynchronous on `stream` and never synchronize the host.
  * Every function returns a KdaStatus (0 = success).
  */
@@ -66,7 +70,8 @@ typedef enum KdaStatus {
 
 typedef enum KdaDType {
     KDA_BF16 = 0,
-    KDA_F32 = 1
+    KDA_F32 = 1,
+    KDA_FP8_E4M3 = 2 /* OCP e4m3 (no infinities); norm outputs and key/value caches only */
 } KdaDType;
 
 /* How the per-channel decay and beta arrive.
@@ -265,6 +270,115 @@ int kda_chunk_launch_wide(const KdaChunkArgs *args, int32_t wide, void *workspac
  * that overlap on one GPU -- concurrent streams, or host threads -- race, and
  * must be serialized by the caller. */
 int kda_chunk_launch_noalloc(const KdaChunkArgs *args, void *stream);
+
+/* Residual addition and root-mean-square norm of `rows` rows of `width`:
+ *   h = x + residual (fp32);  residual <- h;  y = h * weight / sqrt(mean(h^2) + eps)
+ * The norm reads h before it is rounded into the residual. `out` has x's type,
+ * or is KDA_FP8_E4M3 with y = out * scale: scale = max(max|y| / 448, 1e-12) over
+ * the row (group = 0) or over each 128 columns of it (group = 128, the last group
+ * shorter where width is no multiple). A NaN in a group makes its scale NaN. */
+typedef struct KdaRmsNormArgs {
+    const void *x;      /* [rows, width], columns contiguous */
+    void *residual;     /* [rows, width] or null, updated in place */
+    const void *weight; /* [width] */
+    void *out;          /* [rows, width] */
+    float *scale;       /* [rows, groups], fp8 output only */
+    int64_t x_stride;   /* elements between rows */
+    int64_t residual_stride;
+    int64_t out_stride;
+    int64_t rows;
+    int32_t width;
+    float eps;
+    int32_t x_dtype;        /* KDA_BF16 or KDA_F32, as the next two */
+    int32_t residual_dtype;
+    int32_t weight_dtype;
+    int32_t out_dtype; /* x_dtype, or KDA_FP8_E4M3 */
+    int32_t group;     /* columns of a scale: 0 (the row) or 128 */
+} KdaRmsNormArgs;
+
+/* Pointers need their element's alignment only; rows of out and of the residual
+ * must not overlap (stride >= width). */
+int kda_rms_norm_launch(const KdaRmsNormArgs *args, void *stream);
+
+/* A paged key/value cache: token `off` of page `p` and key head h are head_dim
+ * contiguous elements at base + p * stride_page + off * stride_token + h * stride_head
+ * (elements; bases 16-byte aligned, strides multiples of 16 bytes). */
+typedef struct KdaPagedCache {
+    void *k;
+    void *v;
+    int64_t k_stride_page, k_stride_token, k_stride_head;
+    int64_t v_stride_page, v_stride_token, v_stride_head;
+    const float *k_scale; /* [kv_heads], KDA_FP8_E4M3 only (null = 1): key = cache * scale */
+    const float *v_scale;
+    int64_t num_pages; /* num_pages * page_size < 2^31 */
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim; /* 64 or 128 */
+    int32_t dtype;    /* KDA_BF16 or KDA_FP8_E4M3 */
+} KdaPagedCache;
+
+/* Writes the keys and values of new tokens into a paged cache: token t goes to
+ * slot slots[t] = page * page_size + offset. A slot outside the pool (negative:
+ * a padding token) is skipped. An 8-bit cache keeps e4m3(clamp(x / scale, -448, 448)).
+ * Two tokens with one slot leave either's values there, element by element. */
+typedef struct KdaPagedStoreArgs {
+    const void *k; /* [tokens, kv_heads, head_dim] bf16, head_dim contiguous */
+    const void *v;
+    int64_t k_stride_token, k_stride_head; /* elements */
+    int64_t v_stride_token, v_stride_head;
+    const void *slots; /* [tokens] int32, or int64 */
+    int32_t slots_int64;
+    int32_t num_tokens;
+    KdaPagedCache cache;
+} KdaPagedStoreArgs;
+
+int kda_paged_store_launch(const KdaPagedStoreArgs *args, void *stream);
+
+/* More KDA_WIDE_* bits, of kda_paged_attention_launch's metadata (with KDA_WIDE_CU_SEQLENS). */
+#define KDA_WIDE_PAGE_TABLE 16
+#define KDA_WIDE_KV_LENS 32
+
+/* Attention of new tokens over a paged cache that already holds their keys and
+ * values. Request n has the tokens cu_seqlens[n] .. cu_seqlens[n + 1] of q; its
+ * cache holds kv_lens[n] tokens, the new ones last, on the pages page_table[n].
+ * The new token at position p of the request sees the keys j <= p, with a window
+ * only the last `window` of them (its own among them). Query head h reads key head
+ * h / (num_heads / kv_heads). Per token and head:
+ *   s_j = scale * (q . key_j);   logit_cap > 0: s_j = logit_cap * tanh(s_j / logit_cap)
+ *   out = sum_j softmax(s)_j value_j, and 0 where no key is visible.
+ * Scores, softmax and sums are fp32; the weights are rounded to bf16 for the
+ * product with the values. A page outside [0, num_pages) reads as zero keys and
+ * values (nothing outside the pool is addressed); kv_lens beyond the table are cut
+ * to it; tokens that no request covers get 0. */
+typedef struct KdaPagedAttentionArgs {
+    const void *q; /* [tokens, num_heads, head_dim] bf16, head_dim contiguous */
+    void *out;     /* the same shape, bf16 */
+    int64_t q_stride_token, q_stride_head; /* elements */
+    int64_t out_stride_token, out_stride_head;
+    const void *page_table; /* [num_seqs, max_pages] */
+    int64_t page_table_stride; /* entries between requests */
+    const void *kv_lens;    /* [num_seqs] */
+    const void *cu_seqlens; /* [num_seqs + 1], non-decreasing */
+    float scale;
+    float logit_cap; /* 0: none */
+    int32_t window;  /* 0: none */
+    int32_t wide;    /* which of the three are int64: KDA_WIDE_PAGE_TABLE, _KV_LENS, _CU_SEQLENS */
+    int32_t num_seqs;
+    int32_t num_tokens;
+    int32_t num_heads; /* a multiple of kv_heads */
+    int32_t max_pages;
+    int32_t max_query_len; /* most new tokens of a request: chooses the kernel, results hold for any value */
+    KdaPagedCache cache;
+} KdaPagedAttentionArgs;
+
+/* Bytes of device scratch that kda_paged_attention_launch needs for these sizes
+ * (host-only; the pointers, strides and contents do not matter). */
+size_t kda_paged_attention_workspace_bytes(const KdaPagedAttentionArgs *args);
+
+/* `workspace`: 256-byte aligned device memory of the bytes above (null if 0), no
+ * initialization needed. q and out need their element's alignment only. */
+int kda_paged_attention_launch(const KdaPagedAttentionArgs *args, void *workspace, size_t workspace_bytes,
+                               void *stream);
 
 /* Human-readable text of a KdaStatus. */
 const char *kda_status_string(int status);

@@ -49,6 +49,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
 
 struct __attribute__((packed, aligned(2))) Bf16x8Any {
     u32x4 w;
@@ -62,6 +63,10 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                    0);
 }
+// A 16-byte load that is known to be from global memory: through a selected or shuffled
+// pointer the compiler would issue a flat load, which also counts as an LDS access and is waited for as one.
+__device__ __forceinline__ u32x4 load16(const char *p) { return *(global_u32x4 *)p; }
+
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Sixteen e4m3 (16 bytes) as bf16, exactly (three mantissa bits): two operands of 8.
@@ -256,8 +261,8 @@ constexpr int kDecodeGroups = 2 * kCus;
 struct DecodeWs {
     float *o;     // [2 groups][rows][D]: a workgroup's part that continues an item, its part that begins one
     float2 *ml;   // [2 groups][rows]
-    int4 *desc;   // [groups]: the item that begins in a workgroup and does not end there: request (-1: none),
-                  // key head, tile, last workgroup
+    int4 *desc;   // [groups]: the item that begins in a workgroup and does not end there: its request's first
+                  // token, its first row of the request, rows (0: no such item) + 256 key head, last workgroup
 };
 
 template <int D, bool FP8> struct KvBlock {
@@ -270,9 +275,9 @@ template <int D, bool FP8> struct KvBlock {
 template <int D, int NB> struct DecodeShared {
     char v[kWaves][kBlock * D * 2];  // values of a wave's block; 16 rows of O when waves join
     float2 ml[kWaves][16 * NB];
-    long long scan[kWaves];
-    long long before;  // the first unit of request `first`
-    int first;
+    int scan[kWaves];
+    int first, before;  // the request of the range's first unit, and the first unit of that request
+    Request request;
 };
 
 // Units of a tile of `rows` rows of a request: the most that any of its tiles has.
@@ -305,76 +310,72 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
     // ---- this workgroup's range of units
     const int per = (a.num_seqs + kThreads - 1) / kThreads;
     const int n0 = min(tid * per, a.num_seqs), n1 = min(n0 + per, a.num_seqs);
-    auto units_of = [&](int n) -> long long {
-        const Request r = a.request(n);
-        const long long rows = static_cast<long long>(r.tokens) * a.group;
-        return (rows + kRows - 1) / kRows * heads * tile_units(a, r, kRows);
-    };
-    long long mine = 0;
+    auto units_of = [&](const Request &r) { return (r.tokens * a.group + kRows - 1) / kRows * heads * tile_units(a, r, kRows); };
+    int mine = 0;
     for (int n = n0; n < n1; ++n) {
-        mine += units_of(n);
+        mine += units_of(a.request(n));
     }
-    long long scan = mine;
+    int scan = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const long long up = __shfl_up(scan, d);
+        const int up = __shfl_up(scan, d);
         scan += lane >= d ? up : 0;
     }
     if (lane == 63) {
         sm.scan[wave] = scan;
     }
     __syncthreads();
-    long long total = 0, base = 0;
+    int total = 0, base = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         base += w < wave ? sm.scan[w] : 0;
         total += sm.scan[w];
     }
-    const long long groups = min(static_cast<long long>(gridDim.x), total);
-    const long long w = blockIdx.x;
+    total = __builtin_amdgcn_readfirstlane(total);
+    const int w = blockIdx.x;
+    const int groups = min(static_cast<int>(gridDim.x), total);
     if (w >= groups) {
         if (tid == 0) {
-            ws.desc[w] = make_int4(-1, 0, 0, 0);
+            ws.desc[w] = make_int4(0, 0, 0, 0);
         }
         return;
     }
-    const long long u0 = w * total / groups, u1 = (w + 1) * total / groups;
-    long long at = base + scan - mine;
+    const int share = total / groups, more = total - share * groups;  // the first `more` workgroups take one unit more
+    const int u0 = w * share + min(w, more), u1 = u0 + share + (w < more ? 1 : 0);
+    int at = base + scan - mine;
     if (u0 >= at && u0 < at + mine) {  // one thread's requests hold the first unit
         int n = n0;
-        for (;; ++n) {
-            const long long u = units_of(n);
-            if (u0 < at + u) {
-                break;
-            }
+        Request r = a.request(n);
+        for (int u = units_of(r); u0 >= at + u; u = units_of(r)) {
             at += u;
+            r = a.request(++n);
         }
         sm.first = n;
         sm.before = at;
+        sm.request = r;
     }
     __syncthreads();
     int n = __builtin_amdgcn_readfirstlane(sm.first);
-    long long start = sm.before;  // the first unit of request n
-    int4 desc = make_int4(-1, 0, 0, 0);
+    int start = __builtin_amdgcn_readfirstlane(sm.before);  // the first unit of request n
+    Request req = {__builtin_amdgcn_readfirstlane(sm.request.begin), __builtin_amdgcn_readfirstlane(sm.request.tokens),
+                   __builtin_amdgcn_readfirstlane(sm.request.keys)};
+    int4 desc = make_int4(0, 0, 0, 0);
 
-    for (long long u = u0; u < u1;) {
-        const Request req = a.request(n);
+    for (int u = u0; u < u1;) {
         const int rows_all = req.tokens * a.group;
         const int tiles = (rows_all + kRows - 1) / kRows;
         const int count = tile_units(a, req, kRows);
-        const long long units = static_cast<long long>(tiles) * heads * count;
-        if (u >= start + units) {
-            start += units;
-            ++n;
+        if (u >= start + tiles * heads * count) {
+            start += tiles * heads * count;
+            req = a.request(++n);
             continue;
         }
         // ---- the item and the part of it that is in this range
-        const long long local = u - start;
-        const long long item = local / count;
-        const int part0 = static_cast<int>(local - item * count);
-        const int part1 = static_cast<int>(min(static_cast<long long>(count), part0 + (u1 - u)));
-        const int tile = static_cast<int>(item % tiles);
-        const int head = static_cast<int>(item / tiles);
+        const int item = (u - start) / count;
+        const int part0 = u - start - item * count;
+        const int part1 = min(count, part0 + (u1 - u));
+        const int head = item / tiles;
+        const int tile = item - head * tiles;
         const int row0 = tile * kRows;
         const int rows = min(kRows, rows_all - row0);
         const int2 first = a.visible(req, row0 / a.group);
@@ -434,13 +435,13 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                 const char *p = reinterpret_cast<const char *>(__shfl(ka, kt * 16 + col));
 #pragma unroll
                 for (int s = 0; s < Kv::kK; ++s) {
-                    kv.k[kt][s] = *reinterpret_cast<const u32x4 *>(p + s * 64 + g * 16);
+                    kv.k[kt][s] = load16(p + s * 64 + g * 16);
                 }
             }
 #pragma unroll
             for (int s = 0; s < Kv::kV; ++s) {
                 const char *p = reinterpret_cast<const char *>(__shfl(va, s * R::kRows + lane / R::kLanes));
-                kv.v[s] = *reinterpret_cast<const u32x4 *>(p + lane % R::kLanes * 16);
+                kv.v[s] = load16(p + lane % R::kLanes * 16);
             }
         };
         auto compute = [&](int i, const Kv &kv) {
@@ -551,10 +552,11 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
 
         // ---- join the waves: their maxima, sums and 16 rows of O at a time through LDS
         const bool begins = part0 == 0, ends = part1 == count;
-        const int64_t slot = 2 * w + (begins ? 1 : 0);
+        const int64_t slot = 2 * static_cast<int64_t>(w) + (begins ? 1 : 0);
         if (begins && !ends) {
-            const long long end = start + (item + 1) * count;  // its last unit + 1
-            desc = make_int4(n, head, tile, static_cast<int>((end * groups + total - 1) / total - 1));
+            const int end = start + item * count + count - 1;  // its last unit, and that unit's workgroup
+            const int wide = more * (share + 1);
+            desc = make_int4(req.begin, row0, rows + 256 * head, end < wide ? end / (share + 1) : more + (end - wide) / share);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -625,44 +627,90 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
     }
 }
 
-// One workgroup for each of decode_kernel's: joins the item that began there.
+// Joins the items that began in a workgroup of decode_kernel and did not end there:
+// one workgroup each for every fourth row. Its threads take 4 columns each, and
+// the rows and the parts are spread over what is left of them, so that a
+// thread's loads are few and in flight together (32 parts of 4 rows: 20.8 us with
+// a thread to all parts of a row, one after another).
+constexpr int kJoinRows = 4;
+
 template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const Params a, const DecodeWs ws) {
     constexpr int kRows = 16 * NB;
+    constexpr int kCols = D / 4;
+    constexpr int kSlots = kThreads / kCols;
+    __shared__ f32x4 sum_o[kThreads];
+    __shared__ float2 sum_ml[kThreads];
     const int w = blockIdx.x;
     const int4 desc = ws.desc[w];
-    if (desc.x < 0) {
+    const int rows = ((desc.z & 255) - static_cast<int>(blockIdx.y) + kJoinRows - 1) / kJoinRows;  // of this workgroup
+    if (rows <= 0) {
         return;
     }
-    const Request req = a.request(desc.x);
-    const int row0 = desc.z * kRows;
-    const int rows = min(kRows, req.tokens * a.group - row0);
-    const int last = desc.w;
-    const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[desc.y] : 1.0f;
-    // parts: the second slot of w, then the first ones of w + 1 .. last
-    for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
-        const int r = i / (D / 4);
-        const int c = i % (D / 4);
-        auto slot = [&](int x) -> int64_t { return x == w ? 2 * static_cast<int64_t>(w) + 1 : 2 * static_cast<int64_t>(x); };
-        float top = kNegInf;
-        for (int x = w; x <= last; ++x) {
-            top = fmaxf(top, ws.ml[slot(x) * kRows + r].x);
-        }
-        float sum = 0.0f;
+    const int head = desc.z >> 8;
+    const int parts = desc.w - w + 1;  // the second slot of w, then the first ones of w + 1 .. last
+    // threads of a row: a power of two, at most the parts, such that all rows are taken at once
+    int lanes = 1;
+    while (2 * lanes <= parts && 2 * lanes * rows <= kSlots) {
+        lanes *= 2;
+    }
+    const int c = threadIdx.x % kCols;
+    const int slot = threadIdx.x / kCols;
+    const int lane = slot & (lanes - 1);
+    const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
+    for (int first = 0; first < rows; first += kSlots / lanes) {
+        const int i = first + slot / lanes;
+        const int r = min(i, rows - 1) * kJoinRows + blockIdx.y;
+        float top = kNegInf, sum = 0.0f;
         f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int x = w; x <= last; ++x) {
-            const float2 ml = ws.ml[slot(x) * kRows + r];
-            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
-            sum += ml.y * f;
-            y += *reinterpret_cast<const f32x4 *>(ws.o + (slot(x) * kRows + r) * D + c * 4) * f;
+        for (int x = lane; x < parts; x += 4 * lanes) {
+            float2 ml[4];
+            f32x4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int part = min(x + k * lanes, parts - 1);
+                const int64_t at = (2 * static_cast<int64_t>(w + part) + (part == 0 ? 1 : 0)) * kRows + r;
+                ml[k] = ws.ml[at];
+                o[k] = *reinterpret_cast<const f32x4 *>(ws.o + at * D + c * 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (x + k * lanes < parts) {
+                    const float next = fmaxf(top, ml[k].x);
+                    const float f0 = top == next ? 1.0f : ex2(top - next), f1 = ml[k].x == next ? 1.0f : ex2(ml[k].x - next);
+                    top = next;
+                    sum = sum * f0 + ml[k].y * f1;
+                    y = y * f0 + o[k] * f1;
+                }
+            }
         }
-        y *= sum == 0.0f ? 0.0f : vs / sum;
-        const int t = (row0 + r) / a.group;
-        const int h = desc.y * a.group + (row0 + r) - t * a.group;
-        uint16_t *out = static_cast<uint16_t *>(a.out) + (req.begin + t) * a.out_stride_token + h * a.out_stride_head + c * 4;
-        struct __attribute__((packed, aligned(2))) Out {
-            uint32_t w[2];
-        };
-        *reinterpret_cast<Out *>(out) = {{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}};
+        if (lanes > 1) {
+            __syncthreads();  // the last round's values are read
+            sum_o[threadIdx.x] = y;
+            sum_ml[threadIdx.x] = make_float2(top, sum);
+            __syncthreads();
+            if (lane == 0) {
+                for (int k = 1; k < lanes; ++k) {
+                    const float2 ml = sum_ml[threadIdx.x + k * kCols];
+                    const float next = fmaxf(top, ml.x);
+                    const float f0 = top == next ? 1.0f : ex2(top - next), f1 = ml.x == next ? 1.0f : ex2(ml.x - next);
+                    top = next;
+                    sum = sum * f0 + ml.y * f1;
+                    y = y * f0 + sum_o[threadIdx.x + k * kCols] * f1;
+                }
+            }
+        }
+        if (lane == 0 && i < rows) {
+            y *= sum == 0.0f ? 0.0f : vs / sum;
+            const int row = desc.y + r;
+            const int t = row / a.group;
+            const int h = head * a.group + row - t * a.group;
+            uint16_t *out = static_cast<uint16_t *>(a.out) + static_cast<int64_t>(desc.x + t) * a.out_stride_token +
+                            h * a.out_stride_head + c * 4;
+            struct __attribute__((packed, aligned(2))) Out {
+                uint32_t w[2];
+            };
+            *reinterpret_cast<Out *>(out) = {{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}};
+        }
     }
 }
 
@@ -779,15 +827,41 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
     const char *vbase = static_cast<const char *>(a.cache.v) + ((head * a.cache.v_stride_head) << R::kShift);
     const int srow = wave * 16 + lane / R::kLanes;  // + kRows of Row for each further load
     const int schunk = lane % R::kLanes;
+    const char *zero = reinterpret_cast<const char *>(g_zero_row);
+    u32x4 kreg[kLoads], vreg[kLoads];
+    // Pages of a tile's rows: of the lane's own rows, or, where pages hold a multiple of 16 tokens
+    // (UNIFORM), the one page of the wave's 16 rows, which is walked without divisions and
+    // leaves the lanes an offset each that is the same in every tile.
     struct Pages {
-        int p[kLoads];
+        int p[UNIFORM ? 1 : kLoads];
+        int off;  // UNIFORM: of the first row on its page
     };
-    // UNIFORM: pages hold a multiple of 16 tokens, so a wave's 16 rows are on one page
+    int walk_at = 0, walk_off = 0;  // the next tile to look up
+    uint32_t kpre[kLoads], vpre[kLoads];
+    if constexpr (UNIFORM) {
+        const int key = t0 * kTile + wave * 16;
+        walk_at = key / a.cache.page_size;
+        walk_off = key - walk_at * a.cache.page_size;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t r = lane / R::kLanes + i * R::kRows;
+            kpre[i] = ((r * static_cast<uint32_t>(a.cache.k_stride_token)) << R::kShift) + schunk * 16;
+            vpre[i] = ((r * static_cast<uint32_t>(a.cache.v_stride_token)) << R::kShift) + schunk * 16;
+        }
+    }
+    const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
     auto lookup = [&](int t) -> Pages {
         Pages r;
+        r.off = 0;
         if constexpr (UNIFORM) {
-            const int at = __builtin_amdgcn_readfirstlane((t * kTile + wave * 16) / a.cache.page_size);
-            r.p[0] = a.page_of(n, min(at, a.max_pages - 1));
+            r.p[0] = a.page_of(n, min(walk_at, a.max_pages - 1));
+            r.off = walk_off;
+            walk_at += step_at;
+            walk_off += step_off;
+            if (walk_off >= a.cache.page_size) {
+                walk_off -= a.cache.page_size;
+                ++walk_at;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
@@ -796,38 +870,49 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
         }
         return r;
     };
-    u32x4 kreg[kLoads], vreg[kLoads];
     auto load = [&](int t, const Pages &pages) {
-        const int key0 = t * kTile;
-        int page = 0, off0 = 0;
-        const char *kp0 = nullptr, *vp0 = nullptr;
         if constexpr (UNIFORM) {
-            page = __builtin_amdgcn_readfirstlane(pages.p[0]);
-            const int k = key0 + wave * 16;
-            off0 = k - k / a.cache.page_size * a.cache.page_size;
-            kp0 = kbase + ((page * a.cache.k_stride_page + off0 * a.cache.k_stride_token) << R::kShift);
-            vp0 = vbase + ((page * a.cache.v_stride_page + off0 * a.cache.v_stride_token) << R::kShift);
-        }
+            const int page = __builtin_amdgcn_readfirstlane(pages.p[0]);
+            const int key = t * kTile + wave * 16;
+            const bool any = key < see1.y && key + 16 > see0.x && page >= 0 && page < a.cache.num_pages;
+            const char *kp = any ? kbase + ((page * a.cache.k_stride_page + pages.off * a.cache.k_stride_token) << R::kShift) : zero;
+            const char *vp = any ? vbase + ((page * a.cache.v_stride_page + pages.off * a.cache.v_stride_token) << R::kShift) : zero;
+            uint32_t ko[kLoads], vo[kLoads];
+            if (any && key >= see0.x && key + 16 <= see1.y) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int key = key0 + srow + i * R::kRows;
-            const char *kp, *vp;
-            if constexpr (UNIFORM) {
-                const int r = lane / R::kLanes + i * R::kRows;
-                kp = kp0 + ((r * a.cache.k_stride_token) << R::kShift);
-                vp = vp0 + ((r * a.cache.v_stride_token) << R::kShift);
+                for (int i = 0; i < kLoads; ++i) {
+                    ko[i] = kpre[i];
+                    vo[i] = vpre[i];
+                }
             } else {
-                page = pages.p[i];
-                const int off = key - key / a.cache.page_size * a.cache.page_size;
-                kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
-                vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
+                // some rows have no key that the tile sees: the nearest that has stands in (its
+                // scores are masked), so nothing is read that no request wrote
+                const uint32_t ks = any ? static_cast<uint32_t>(a.cache.k_stride_token) : 0;
+                const uint32_t vs = any ? static_cast<uint32_t>(a.cache.v_stride_token) : 0;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = max(min(static_cast<int>(lane / R::kLanes + i * R::kRows), see1.y - 1 - key), see0.x - key);
+                    ko[i] = ((static_cast<uint32_t>(r) * ks) << R::kShift) + schunk * 16;
+                    vo[i] = ((static_cast<uint32_t>(r) * vs) << R::kShift) + schunk * 16;
+                }
             }
-            const bool real = key >= see0.x && key < see1.y && page >= 0 && page < a.cache.num_pages;
-            const char *zero = reinterpret_cast<const char *>(g_zero_row);
-            kp = real ? kp : zero;
-            vp = real ? vp : zero;
-            kreg[i] = *reinterpret_cast<const u32x4 *>(kp + schunk * 16);
-            vreg[i] = *reinterpret_cast<const u32x4 *>(vp + schunk * 16);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                kreg[i] = load16(kp + ko[i]);
+                vreg[i] = load16(vp + vo[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int key = t * kTile + srow + i * R::kRows;
+                const int page = pages.p[i];
+                const int off = key - key / a.cache.page_size * a.cache.page_size;
+                const bool real = key >= see0.x && key < see1.y && page >= 0 && page < a.cache.num_pages;
+                const char *kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
+                const char *vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
+                kreg[i] = load16((real ? kp : zero) + schunk * 16);
+                vreg[i] = load16((real ? vp : zero) + schunk * 16);
+            }
         }
     };
     auto write = [&](int parity) {
@@ -945,7 +1030,7 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
         load(t0, pages);
         pages = lookup(t0 + 1);
         write(0);
-        __syncthreads();
+        lds_barrier();
         for (int t = t0; t < t1; ++t) {
             const int parity = (t - t0) & 1;
             // past the last tile the rows of zeros are loaded and staged, and not read
@@ -955,7 +1040,7 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
                 compute(t, parity);
             }
             write(parity ^ 1);
-            __syncthreads();
+            lds_barrier();
         }
     }
 
@@ -1066,13 +1151,20 @@ struct Plan {
 
 size_t up256(size_t x) { return (x + 255) & ~size_t{255}; }
 
+int64_t most_rows(const KdaPagedAttentionArgs &a) {
+    return std::max<int64_t>(a.max_query_len, 1) * (a.num_heads / a.cache.kv_heads);
+}
+
+// At most 32 rows a request (without requests, the decode kernel only writes the zeros).
+bool decodes(const KdaPagedAttentionArgs &a) { return most_rows(a) <= 32 || a.num_seqs == 0; }
+
 Plan plan_of(const KdaPagedAttentionArgs &a) {
     Plan p{};
     const int64_t group = a.num_heads / a.cache.kv_heads;
-    const int64_t rows = std::max<int64_t>(a.max_query_len, 1) * group;
+    const int64_t rows = most_rows(a);
     const int64_t keys = static_cast<int64_t>(a.max_pages) * a.cache.page_size;
     const size_t d = a.cache.head_dim;
-    p.decode = rows <= 32 || a.num_seqs == 0;  // without requests it only writes the zeros
+    p.decode = decodes(a);
     if (p.decode) {
         p.blocks = rows <= 16 ? 1 : 2;
         p.join = keys > kUnit;
@@ -1110,9 +1202,12 @@ int check(const KdaPagedAttentionArgs *args) {
         return KDA_ERR_INVALID_ARGUMENT;
     }
     const int64_t group = a.num_heads / a.cache.kv_heads;
-    // row and key numbers, and the roundings up of both, stay in 32 bits
-    if (a.num_tokens * group + 128 * static_cast<int64_t>(a.num_seqs) > INT32_MAX - 1024 ||
-        static_cast<int64_t>(a.max_pages) * a.cache.page_size > INT32_MAX - 1024) {
+    // row and key numbers, the roundings up of both and the decode kernel's units stay in 32 bits
+    const int64_t rows = a.num_tokens * group, keys = static_cast<int64_t>(a.max_pages) * a.cache.page_size;
+    if (rows + 128 * static_cast<int64_t>(a.num_seqs) > INT32_MAX - 1024 || keys > INT32_MAX - 1024) {
+        return KDA_ERR_TOO_LARGE;
+    }
+    if (decodes(a) && (rows / 16 + a.num_seqs) * a.cache.kv_heads > INT32_MAX / (keys / kUnit + 1)) {
         return KDA_ERR_TOO_LARGE;
     }
     return KDA_OK;
@@ -1125,7 +1220,7 @@ template <int D, bool FP8, int NB> void launch_decode(const Params &a, const Pla
                      reinterpret_cast<int4 *>(ws + p.desc_at)};
     decode_kernel<D, FP8, NB><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
     if (p.join) {
-        decode_combine_kernel<D, NB><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
+        decode_combine_kernel<D, NB><<<dim3(kDecodeGroups, kJoinRows), kThreads, 0, s>>>(a, w);
     }
 }
 
@@ -1137,7 +1232,9 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
     const PrefillWs w{reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.ml_at)};
     const unsigned grid = static_cast<unsigned>(p.tiles * a.cache.kv_heads * p.splits);
     const int tiles = static_cast<int>(p.tiles);
-    if (a.cache.page_size % 16 == 0) {
+    // 16 rows of a page at offsets that fit 32 bits
+    const auto near = [](int64_t stride) { return stride >= 0 && stride < (1 << 26); };
+    if (a.cache.page_size % 16 == 0 && near(a.cache.k_stride_token) && near(a.cache.v_stride_token)) {
         prefill_kernel<D, FP8, kRowBlocks, true><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
     } else {
         prefill_kernel<D, FP8, kRowBlocks, false><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);

@@ -67,6 +67,22 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // pointer the compiler would issue a flat load, which also counts as an LDS access and is waited for as one.
 __device__ __forceinline__ u32x4 load16(const char *p) { return *(global_u32x4 *)p; }
 
+// 64 x 16 bytes from memory into 1 KiB of LDS in lane order (`to` is the wave's), without
+// registers. Written as assembly because the compiler makes every later LDS read wait for the builtin's loads,
+// of whichever buffer; here whoever reads them waits for vmcnt and the barrier first.
+// `from` + `at`: a base the wave shares and each lane's offset.
+__device__ __forceinline__ void load16_to_lds(const char *from, uint32_t at, char *to) {
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(at), "s"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void load16_to_lds(const char *from, char *to) {
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Sixteen e4m3 (16 bytes) as bf16, exactly (three mantissa bits): two operands of 8.
@@ -181,19 +197,18 @@ template <int D, bool FP8> struct Row {
 // within 256 bytes (one row of 128 or two of 64) by the row, so that the reads of
 // one column over 16 rows touch all banks alike.
 // K: chunk reads. V: transposing reads of 32-byte pairs of chunks, which stay together.
+// k_chunk, v_chunk: the slot of a chunk, and the chunk at a slot.
+template <int D> __device__ __forceinline__ int k_chunk(int row, int slot) {
+    return slot ^ (D == 128 ? row & 15 : (row >> 1) & 7);
+}
+template <int D> __device__ __forceinline__ int v_chunk(int row, int slot) {
+    return slot ^ (D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1);
+}
 template <int D> __device__ __forceinline__ int k_at(int row, int chunk) {
-    if constexpr (D == 128) {
-        return row * 256 + ((chunk ^ (row & 15)) << 4);
-    } else {
-        return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
-    }
+    return row * 2 * D + (k_chunk<D>(row, chunk) << 4);
 }
 template <int D> __device__ __forceinline__ int v_at(int row, int chunk) {
-    if constexpr (D == 128) {
-        return row * 256 + ((chunk ^ ((row & 7) << 1)) << 4);
-    } else {
-        return row * 128 + ((chunk ^ (((row >> 1) & 3) << 1)) << 4);
-    }
+    return row * 2 * D + (v_chunk<D>(row, chunk) << 4);
 }
 // Transposing read of rows row .. row + 3 (16 lanes: lane 4m + c takes row m), columns
 // 16 pair .. 16 pair + 15: lane i of the 16 gets column i of the four rows.
@@ -731,6 +746,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 // ---------------------------------------------------------------------------
 
 constexpr int kTile = 64;
+constexpr int kWaitMemory = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
 
 struct PrefillWs {
     float *o;    // [splits][key heads][tokens * group][D], not normalized
@@ -828,194 +844,237 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
     const int srow = wave * 16 + lane / R::kLanes;  // + kRows of Row for each further load
     const int schunk = lane % R::kLanes;
     const char *zero = reinterpret_cast<const char *>(g_zero_row);
-    u32x4 kreg[kLoads], vreg[kLoads];
+    u32x4 kreg[FP8 ? kLoads : 1], vreg[FP8 ? kLoads : 1];
     // Pages of a tile's rows: of the lane's own rows, or, where pages hold a multiple of 16 tokens
     // (UNIFORM), the one page of the wave's 16 rows, which is walked without divisions and
     // leaves the lanes an offset each that is the same in every tile.
     struct Pages {
+        int key;  // the wave's first row
         int p[UNIFORM ? 1 : kLoads];
         int off;  // UNIFORM: of the first row on its page
     };
-    int walk_at = 0, walk_off = 0;  // the next tile to look up
-    uint32_t kpre[kLoads], vpre[kLoads];
-    if constexpr (UNIFORM) {
-        const int key = t0 * kTile + wave * 16;
-        walk_at = key / a.cache.page_size;
-        walk_off = key - walk_at * a.cache.page_size;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t r = lane / R::kLanes + i * R::kRows;
-            kpre[i] = ((r * static_cast<uint32_t>(a.cache.k_stride_token)) << R::kShift) + schunk * 16;
-            vpre[i] = ((r * static_cast<uint32_t>(a.cache.v_stride_token)) << R::kShift) + schunk * 16;
-        }
-    }
+    struct Walk {
+        int key, at, off;
+    };
     const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
-    auto lookup = [&](int t) -> Pages {
+    auto walk_from = [&](int key) -> Walk {
+        const int at = max(key, 0) / a.cache.page_size;
+        return Walk{key, at, max(key, 0) - at * a.cache.page_size};
+    };
+    auto lookup = [&](Walk &w) -> Pages {  // and on to the next tile
         Pages r;
-        r.off = 0;
+        r.key = w.key;
+        r.off = w.off;
         if constexpr (UNIFORM) {
-            r.p[0] = a.page_of(n, min(walk_at, a.max_pages - 1));
-            r.off = walk_off;
-            walk_at += step_at;
-            walk_off += step_off;
-            if (walk_off >= a.cache.page_size) {
-                walk_off -= a.cache.page_size;
-                ++walk_at;
+            r.p[0] = a.page_of(n, min(w.at, a.max_pages - 1));
+            w.at += step_at;
+            w.off += step_off;
+            if (w.off >= a.cache.page_size) {
+                w.off -= a.cache.page_size;
+                ++w.at;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                r.p[i] = a.page_of(n, min((t * kTile + srow + i * R::kRows) / a.cache.page_size, a.max_pages - 1));
+                const int key = max(w.key + static_cast<int>(lane / R::kLanes) + i * R::kRows, 0);
+                r.p[i] = a.page_of(n, min(key / a.cache.page_size, a.max_pages - 1));
             }
         }
+        w.key += kTile;
         return r;
     };
-    auto load = [&](int t, const Pages &pages) {
+    // A lane's rows of a tile and its bytes of them. bf16 rows go from memory into LDS directly, where a
+    // wave's 64 x 16 bytes land in order: a lane fetches the chunk that belongs at its place. 8-bit ones
+    // go through registers, where they are widened.
+    uint32_t krow[kLoads], vrow[kLoads], kcol[kLoads], vcol[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const uint32_t r = lane / R::kLanes + i * R::kRows;
+        kcol[i] = (FP8 ? schunk : k_chunk<D>(r, schunk)) * 16;
+        vcol[i] = (FP8 ? schunk : v_chunk<D>(r, schunk)) * 16;
+        krow[i] = ((r * static_cast<uint32_t>(a.cache.k_stride_token)) << R::kShift) + kcol[i];
+        vrow[i] = ((r * static_cast<uint32_t>(a.cache.v_stride_token)) << R::kShift) + vcol[i];
+    }
+    // The looked-up rows, of K or of V, into their buffer or (8 bits) into registers.
+    auto load = [&](const Pages &pages, const char *head_base, int64_t stride_page, int64_t stride_token,
+                    const uint32_t (&row)[kLoads], const uint32_t (&column)[kLoads], auto &reg, char *tile) {
         if constexpr (UNIFORM) {
             const int page = __builtin_amdgcn_readfirstlane(pages.p[0]);
-            const int key = t * kTile + wave * 16;
+            const int key = pages.key;
             const bool any = key < see1.y && key + 16 > see0.x && page >= 0 && page < a.cache.num_pages;
-            const char *kp = any ? kbase + ((page * a.cache.k_stride_page + pages.off * a.cache.k_stride_token) << R::kShift) : zero;
-            const char *vp = any ? vbase + ((page * a.cache.v_stride_page + pages.off * a.cache.v_stride_token) << R::kShift) : zero;
-            uint32_t ko[kLoads], vo[kLoads];
+            const char *first = any ? head_base + ((page * stride_page + pages.off * stride_token) << R::kShift) : zero;
+            uint32_t at[kLoads];
             if (any && key >= see0.x && key + 16 <= see1.y) {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    ko[i] = kpre[i];
-                    vo[i] = vpre[i];
+                    at[i] = row[i];
                 }
             } else {
                 // some rows have no key that the tile sees: the nearest that has stands in (its
                 // scores are masked), so nothing is read that no request wrote
-                const uint32_t ks = any ? static_cast<uint32_t>(a.cache.k_stride_token) : 0;
-                const uint32_t vs = any ? static_cast<uint32_t>(a.cache.v_stride_token) : 0;
+                const uint32_t step = any ? static_cast<uint32_t>(stride_token) : 0;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
                     const int r = max(min(static_cast<int>(lane / R::kLanes + i * R::kRows), see1.y - 1 - key), see0.x - key);
-                    ko[i] = ((static_cast<uint32_t>(r) * ks) << R::kShift) + schunk * 16;
-                    vo[i] = ((static_cast<uint32_t>(r) * vs) << R::kShift) + schunk * 16;
+                    at[i] = ((static_cast<uint32_t>(r) * step) << R::kShift) + column[i];
                 }
             }
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                kreg[i] = load16(kp + ko[i]);
-                vreg[i] = load16(vp + vo[i]);
+                if constexpr (FP8) {
+                    reg[i] = load16(first + at[i]);
+                } else {
+                    load16_to_lds(first, at[i], tile + wave * (16 * 2 * D) + i * 1024);
+                }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int key = t * kTile + srow + i * R::kRows;
+                const int key = pages.key + lane / R::kLanes + i * R::kRows;
                 const int page = pages.p[i];
                 const int off = key - key / a.cache.page_size * a.cache.page_size;
                 const bool real = key >= see0.x && key < see1.y && page >= 0 && page < a.cache.num_pages;
-                const char *kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
-                const char *vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
-                kreg[i] = load16((real ? kp : zero) + schunk * 16);
-                vreg[i] = load16((real ? vp : zero) + schunk * 16);
+                const char *first = head_base + ((page * stride_page + off * stride_token) << R::kShift);
+                if constexpr (FP8) {
+                    reg[i] = load16((real ? first : zero) + column[i]);
+                } else {
+                    load16_to_lds((real ? first : zero) + column[i], tile + wave * (16 * 2 * D) + i * 1024);
+                }
             }
         }
     };
-    auto write = [&](int parity) {
+    auto load_k = [&](const Pages &pages, int parity) {
+        load(pages, kbase, a.cache.k_stride_page, a.cache.k_stride_token, krow, kcol, kreg, sm[parity][0]);
+    };
+    auto load_v = [&](const Pages &pages, int parity) {
+        load(pages, vbase, a.cache.v_stride_page, a.cache.v_stride_token, vrow, vcol, vreg, sm[parity][1]);
+    };
+    auto write_k = [&](int parity) {
+        if constexpr (FP8) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            stage<D, FP8>(sm[parity][0], srow + i * R::kRows, schunk, kreg[i], [](int r, int c) { return k_at<D>(r, c); });
-            stage<D, FP8>(sm[parity][1], srow + i * R::kRows, schunk, vreg[i], [](int r, int c) { return v_at<D>(r, c); });
+            for (int i = 0; i < kLoads; ++i) {
+                stage<D, FP8>(sm[parity][0], srow + i * R::kRows, schunk, kreg[i], [](int r, int c) { return k_at<D>(r, c); });
+            }
         }
     };
-    auto compute = [&](int t, int parity) {
-        const char *kt_ = sm[parity][0];
-        const char *vt = sm[parity][1];
-        f32x16 s[2][RB];
+    auto write_v = [&](int parity) {
+        if constexpr (FP8) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+            for (int i = 0; i < kLoads; ++i) {
+                stage<D, FP8>(sm[parity][1], srow + i * R::kRows, schunk, vreg[i], [](int r, int c) { return v_at<D>(r, c); });
+            }
+        }
+    };
+    // All rows of the buffers are there, and the reads of the others have ended, for every wave.
+    auto staged = [&] {
+        if constexpr (FP8) {
+            lds_barrier();
+        } else {
+            // as a builtin, so that the compiler counts its own loads as done too
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(kWaitMemory);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
+    };
+    // Scores of 32 keys: a lane's are of row `col`, keys 8 (e / 4) + 4 half + e % 4.
+    typedef f32x16 Half[RB];
+    auto products = [&](int parity, int kt, Half &s) {
+        const char *tile = sm[parity][0];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[b][e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+            const u32x4 op = *reinterpret_cast<const u32x4 *>(tile + k_at<D>(kt * 32 + col, 2 * x + half));
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                s[b] = mfma32(op, q[b][x], s[b]);
+            }
+        }
+    };
+    const float c = sc.cap > 0.0f ? 1.0f : sc.c;
+    float top[RB];  // largest of the scores that are next, in log2 units
+    // cap, mask and largest score of the keys from key0
+    auto finish = [&](int key0, Half &s) {
+        if (sc.cap > 0.0f) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    s[kt][b][e] = 0.0f;
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
-                const u32x4 op = *reinterpret_cast<const u32x4 *>(kt_ + k_at<D>(kt * 32 + col, 2 * x + half));
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    s[kt][b] = mfma32(op, q[b][x], s[kt][b]);
+                    s[b][e] = capped(s[b][e] * sc.in, sc.cap);
                 }
             }
         }
-        const int key0 = t * kTile;
-        const bool whole = key0 >= wsee1.x && key0 + kTile <= wsee0.y;  // every row of the wave sees every key
-        u32x4 p[RB][4];
+        if (!(key0 >= wsee1.x && key0 + 32 <= wsee0.y)) {  // some row of the wave does not see some key
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            float c = sc.c;
-            if (sc.cap > 0.0f) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        s[kt][b][e] = capped(s[kt][b][e] * sc.in, sc.cap);
-                    }
-                }
-                c = 1.0f;
-            }
-            if (!whole) {
-                // a lane's scores: row `col`, keys 32 kt + 8 (e / 4) + 4 half + e % 4
+            for (int b = 0; b < RB; ++b) {
                 const int from = see[b].x - key0 - 4 * half, to = see[b].y - key0 - 4 * half;
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int k = 32 * kt + 8 * (e >> 2) + (e & 3);
-                        s[kt][b][e] = k >= from && k < to ? s[kt][b][e] : kNegInf;
-                    }
-                }
-            }
-            float top = kNegInf;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    top = fmaxf(top, s[kt][b][e]);
+                    const int k = 8 * (e >> 2) + (e & 3);
+                    s[b][e] = k >= from && k < to ? s[b][e] : kNegInf;
                 }
             }
-            top = max_halves(top) * c;
-            if (__any(top > m[b] + kRaise)) {
-                const float next = fmaxf(m[b], top);
-                const float f = next == m[b] ? 1.0f : ex2(m[b] - next);
-                m[b] = next;
+        }
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            float x = kNegInf;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x = fmaxf(x, s[b][e]);
+            }
+            top[b] = max_halves(x) * c;
+        }
+    };
+    // weights of the scores s and their products with rows 32 kt .. of the values in buffer `parity`; the
+    // next 32 keys' scores are formed meanwhile
+    auto step = [&](int parity, int kt, const Half &s, int next_kt, Half &next) {
+        const char *vt = sm[parity][1];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            if (__any(top[b] > m[b] + kRaise)) {
+                const float up = fmaxf(m[b], top[b]);
+                const float f = up == m[b] ? 1.0f : ex2(m[b] - up);
+                m[b] = up;
                 l[b] *= f;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) {
                     o[b][d] *= f;
                 }
             }
-            const float base = m[b] == kNegInf ? 0.0f : m[b];
-            float sum0 = 0.0f, sum1 = 0.0f;
+        }
+        products(parity, next_kt, next);
+        u32x4 p[RB][2];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {  // 16 keys: 8 of this half
+        for (int b = 0; b < RB; ++b) {
+            const float base = m[b] == kNegInf ? 0.0f : m[b];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // 16 keys: 8 of this half of the wave
                 float w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    w[e] = ex2(s[x >> 1][b][8 * (x & 1) + e] * c - base);
+                    w[e] = ex2(s[b][8 * x + e] * c - base);
                 }
-                sum0 += (w[0] + w[1]) + (w[2] + w[3]);
-                sum1 += (w[4] + w[5]) + (w[6] + w[7]);
+                l[b] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     p[b][x][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
                 }
             }
-            l[b] += sum0 + sum1;
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
                 const int pair = 2 * d + ((lane >> 4) & 1);
-                const u32x2 v0 = read_tr<D>(vt, 16 * x + 4 * half, pair, lane);
-                const u32x2 v1 = read_tr<D>(vt, 16 * x + 8 + 4 * half, pair, lane);
+                const int row = 32 * kt + 16 * x + 4 * half;
+                const u32x2 v0 = read_tr<D>(vt, row, pair, lane);
+                const u32x2 v1 = read_tr<D>(vt, row + 8, pair, lane);
                 const u32x4 op = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
@@ -1026,21 +1085,54 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
     };
 
     if (t0 < t1) {
-        Pages pages = lookup(t0);
-        load(t0, pages);
-        pages = lookup(t0 + 1);
-        write(0);
-        lds_barrier();
-        for (int t = t0; t < t1; ++t) {
-            const int parity = (t - t0) & 1;
-            // past the last tile the rows of zeros are loaded and staged, and not read
-            load(t + 1, pages);
-            pages = lookup(t + 2);
-            if (active && t * kTile < wsee1.y && (t + 1) * kTile > wsee0.x) {
-                compute(t, parity);
+        // tiles that the wave sees: [w0, w1)
+        const int w0 = active ? max(t0, wsee0.x / kTile) : t1, w1 = active ? min(t1, (wsee1.y + kTile - 1) / kTile) : t1;
+        Walk kwalk = walk_from(t0 * kTile + wave * 16 + 32), vwalk = walk_from(t0 * kTile + wave * 16);
+        // the first tile's first keys, as the second half of the tile before
+        Walk before = walk_from(t0 * kTile + wave * 16 - 32);
+        Pages kp = lookup(before);
+        load_k(kp, 1);
+        write_k(1);
+        Pages vp = lookup(vwalk);
+        kp = lookup(kwalk);
+        load_k(kp, 0);
+        load_v(vp, 0);
+        vp = lookup(vwalk);
+        kp = lookup(kwalk);
+        write_k(0);
+        write_v(0);
+        staged();
+        Half even, odd;
+        if (t0 == w0) {
+            products(1, 1, even);
+            finish(t0 * kTile, even);
+        }
+        lds_barrier();  // before the first turn stages over these keys
+        // K's tiles are 32 keys ahead of V's, as the scores are. Past the last tile rows of zeros
+        // are loaded and staged, whose scores nobody uses.
+        auto turn = [&](int t, int parity) {
+            load_k(kp, parity ^ 1);
+            load_v(vp, parity ^ 1);
+            kp = lookup(kwalk);
+            vp = lookup(vwalk);
+            if (t >= w0 && t < w1) {
+                step(parity, 0, even, 0, odd);
+                finish(t * kTile + 32, odd);
+                step(parity, 1, odd, 1, even);
+                finish(t * kTile + kTile, even);
+            } else if (t + 1 == w0) {
+                products(parity, 1, even);
+                finish(t * kTile + kTile, even);
             }
-            write(parity ^ 1);
-            lds_barrier();
+            write_k(parity ^ 1);
+            write_v(parity ^ 1);
+            staged();
+        };
+        for (int t = t0; t < t1; t += 2) {
+            turn(t, 0);
+            if (t + 1 < t1) {
+                turn(t + 1, 1);
+            }
         }
     }
 

@@ -202,7 +202,9 @@ template <int D> __device__ __forceinline__ int k_chunk(int row, int slot) {
     return slot ^ (D == 128 ? row & 15 : (row >> 1) & 7);
 }
 template <int D> __device__ __forceinline__ int v_chunk(int row, int slot) {
-    return slot ^ (D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1);
+    // 32 lanes of a transposing read take 4 neighbouring rows and two neighbouring pairs, or 8 rows and one
+    // pair: eight different 32-byte places of the 256 bytes either way
+    return slot ^ (D == 128 ? (row & 3) << 2 | (row & 4) >> 1 : (row & 2) << 1 | (row & 4) >> 1);
 }
 template <int D> __device__ __forceinline__ int k_at(int row, int chunk) {
     return row * 2 * D + (k_chunk<D>(row, chunk) << 4);

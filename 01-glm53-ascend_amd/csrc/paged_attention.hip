@@ -34,6 +34,9 @@
 namespace kda {
 namespace {
 
+// The kernels' lambdas belong into them: called, the arrays they work on would go through memory.
+#define KDA_INLINE __attribute__((always_inline))
+
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kCus = 256;  // of an MI355X: only the number of workgroups goes by it
@@ -70,17 +73,34 @@ __device__ __forceinline__ u32x4 load16(const char *p) { return *(global_u32x4 *
 // 64 x 16 bytes from memory into 1 KiB of LDS in lane order (`to` is the wave's), without
 // registers. Written as assembly because the compiler makes every later LDS read wait for the builtin's loads,
 // of whichever buffer; here whoever reads them waits for vmcnt and the barrier first.
-// `from` + `at`: a base the wave shares and each lane's offset.
-__device__ __forceinline__ void load16_to_lds(const char *from, uint32_t at, char *to) {
+// Several KiB: a base the wave shares, each lane's offsets, and for the i-th KiB i * 1024 on both addresses.
+template <int N> __device__ __forceinline__ void load16_to_lds(const char *from, const uint32_t (&at)[N], char *to) {
+    static_assert(N == 2 || N == 4);
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds), "v"(at), "s"(from)
-                 : "memory");
+    if constexpr (N == 4) {
+        asm volatile(
+            "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+            "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072"
+            :
+            : "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(from)
+            : "memory");
+    } else {
+        asm volatile(
+            "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024"
+            :
+            : "s"(lds), "v"(at[0]), "v"(at[1]), "s"(from)
+            : "memory");
+    }
 }
 __device__ __forceinline__ void load16_to_lds(const char *from, char *to) {
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "memory");
+}
+
+// sum + both bf16 of a pair, in fp32
+__device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
+    constexpr uint32_t kOnes = 0x3f803f80u;
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, kOnes), sum, false);
 }
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -734,7 +754,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 // ---------------------------------------------------------------------------
 // Many rows: prefill chunks and long verify steps.
 //
-// A workgroup takes a tile of 128 RB rows of one (request, key head), 32 RB a
+// A workgroup takes a tile of 128 rows of one (request, key head), 32 a
 // wave, and walks the visible keys in tiles of 64. The four waves share a key and
 // a value tile in LDS (bf16; 8-bit ones are widened when staged, once for all four),
 // two of each, so one barrier a tile is enough. The next tile's rows are loaded into
@@ -748,6 +768,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 // ---------------------------------------------------------------------------
 
 constexpr int kTile = 64;
+constexpr int kTileRows = 128;
 constexpr int kWaitMemory = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
 
 struct PrefillWs {
@@ -755,10 +776,10 @@ struct PrefillWs {
     float2 *ml;  // [splits][key heads][tokens * group]
 };
 
-template <int D, bool FP8, int RB, bool UNIFORM>
-__global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(const Params a, const PrefillWs ws, int tiles,
+template <int D, bool FP8, bool UNIFORM>
+__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, const PrefillWs ws, int tiles,
                                                                             int splits) {
-    constexpr int kRows = 128 * RB;
+    constexpr int kRows = kTileRows;
     using R = Row<D, FP8>;
     constexpr int kLoads = 16 / R::kRows;  // 16-byte loads a thread, of 16 rows a wave
     constexpr int kBytes = kTile * D * 2;
@@ -805,170 +826,175 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
     const int all0 = see0.x / kTile, all1 = (see1.y + kTile - 1) / kTile;
     const int share = (all1 - all0 + splits - 1) / splits;
     const int t0 = all0 + split * share, t1 = min(all1, t0 + share);
-    const int wrow0 = min(row0 + wave * 32 * RB, row0 + rows - 1);
-    const int wrow1 = min(wrow0 + 32 * RB, row0 + rows) - 1;
+    const int wrow0 = min(row0 + wave * 32, row0 + rows - 1);
+    const int wrow1 = min(wrow0 + 32, row0 + rows) - 1;
     const int2 wsee0 = a.visible(req, wrow0 / a.group);
     const int2 wsee1 = a.visible(req, wrow1 / a.group);
-    const bool active = wave * 32 * RB < rows;  // the wave has rows
+    const bool active = wave * 32 < rows;  // the wave has rows
     const Scores sc = scores_of(a, head);
 
-    u32x4 q[RB][D / 16];
-    int2 see[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const int r = min(row0 + wave * 32 * RB + b * 32 + col, row0 + rows - 1);
+    u32x4 q[D / 16];
+    int2 see;
+    {
+        const int r = min(row0 + wave * 32 + col, row0 + rows - 1);
         const int t = r / a.group;
         const int h = head * a.group + r - t * a.group;
-        see[b] = a.visible(req, t);
+        see = a.visible(req, t);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-            q[b][s] = load_q(a, req.begin + t, h, s * 16 + half * 8, sc.flip);
+            q[s] = load_q(a, req.begin + t, h, s * 16 + half * 8, sc.flip);
         }
     }
-    f32x16 o[RB][D / 32];
-    float m[RB], l[RB];
+    f32x16 o[D / 32];
+    float m = kNegInf, l = 0.0f;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        m[b] = kNegInf;
-        l[b] = 0.0f;
+    for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                o[b][d][e] = 0.0f;
-            }
+        for (int e = 0; e < 16; ++e) {
+            o[d][e] = 0.0f;
         }
     }
 
-    // ---- staging: a wave loads 16 of a tile's 64 rows
+    // ---- staging. Of every 64 keys a wave loads 16, a group: keys 64 j + 16 wave, j = t0, t0 + 1, ...
     const char *kbase = static_cast<const char *>(a.cache.k) + ((head * a.cache.k_stride_head) << R::kShift);
     const char *vbase = static_cast<const char *>(a.cache.v) + ((head * a.cache.v_stride_head) << R::kShift);
-    const int srow = wave * 16 + lane / R::kLanes;  // + kRows of Row for each further load
-    const int schunk = lane % R::kLanes;
+    const int64_t kpage = a.cache.k_stride_page << R::kShift, vpage = a.cache.v_stride_page << R::kShift;
+    const int64_t ktoken = a.cache.k_stride_token << R::kShift, vtoken = a.cache.v_stride_token << R::kShift;
     const char *zero = reinterpret_cast<const char *>(g_zero_row);
-    u32x4 kreg[FP8 ? kLoads : 1], vreg[FP8 ? kLoads : 1];
-    // Pages of a tile's rows: of the lane's own rows, or, where pages hold a multiple of 16 tokens
-    // (UNIFORM), the one page of the wave's 16 rows, which is walked without divisions and
-    // leaves the lanes an offset each that is the same in every tile.
-    struct Pages {
-        int key;  // the wave's first row
-        int p[UNIFORM ? 1 : kLoads];
-        int off;  // UNIFORM: of the first row on its page
+    const int srow = lane / R::kLanes, schunk = lane % R::kLanes;  // of a load; kRows of Row further for each next
+    const int pool = static_cast<int>(a.cache.num_pages);
+    // A group's page numbers: of the lane's own rows, or, where pages hold a multiple of 16 tokens
+    // (UNIFORM), of all 16 rows. Those are walked without divisions.
+    struct Group {
+        int key;                       // its first
+        int page[UNIFORM ? 1 : kLoads];
+        int64_t koff, voff;  // UNIFORM: bytes of its first row on the page
     };
-    struct Walk {
-        int key, at, off;
-    };
+    Group ahead;  // the walk's next
+    int at = 0, off = 0;
+    ahead.key = t0 * kTile + wave * 16;
     const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
-    auto walk_from = [&](int key) -> Walk {
-        const int at = max(key, 0) / a.cache.page_size;
-        return Walk{key, at, max(key, 0) - at * a.cache.page_size};
-    };
-    auto lookup = [&](Walk &w) -> Pages {  // and on to the next tile
-        Pages r;
-        r.key = w.key;
-        r.off = w.off;
+    if constexpr (UNIFORM) {
+        at = ahead.key / a.cache.page_size;
+        off = ahead.key - at * a.cache.page_size;
+        ahead.koff = off * ktoken;
+        ahead.voff = off * vtoken;
+    }
+    auto walk = [&]() KDA_INLINE -> Group {
+        Group r = ahead;
         if constexpr (UNIFORM) {
-            r.p[0] = a.page_of(n, min(w.at, a.max_pages - 1));
-            w.at += step_at;
-            w.off += step_off;
-            if (w.off >= a.cache.page_size) {
-                w.off -= a.cache.page_size;
-                ++w.at;
+            r.page[0] = a.page_of(n, min(at, a.max_pages - 1));
+            at += step_at;
+            off += step_off;
+            int wrap = 0;
+            if (off >= a.cache.page_size) {
+                off -= a.cache.page_size;
+                ++at;
+                wrap = a.cache.page_size;
             }
+            ahead.koff += (step_off - wrap) * ktoken;
+            ahead.voff += (step_off - wrap) * vtoken;
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int key = max(w.key + static_cast<int>(lane / R::kLanes) + i * R::kRows, 0);
-                r.p[i] = a.page_of(n, min(key / a.cache.page_size, a.max_pages - 1));
+                r.page[i] = a.page_of(n, min((r.key + srow + i * R::kRows) / a.cache.page_size, a.max_pages - 1));
             }
         }
-        w.key += kTile;
+        ahead.key += kTile;
         return r;
     };
-    // A lane's rows of a tile and its bytes of them. bf16 rows go from memory into LDS directly, where a
-    // wave's 64 x 16 bytes land in order: a lane fetches the chunk that belongs at its place. 8-bit ones
-    // go through registers, where they are widened.
-    uint32_t krow[kLoads], vrow[kLoads], kcol[kLoads], vcol[kLoads];
+    // A lane's bytes of a group. bf16 rows go from memory into LDS directly, where a wave's 64 x 16
+    // bytes land in order: a lane fetches the chunk that belongs at its place. 8-bit ones go through
+    // registers, where they are widened. The loads' immediate offsets (1 KiB each) move both addresses.
+    constexpr int kKib = FP8 ? 0 : 1024;
+    uint32_t krow[kLoads], vrow[kLoads];
+    auto kcol = [&](int i) KDA_INLINE { return (FP8 ? schunk : k_chunk<D>(srow + i * R::kRows, schunk)) * 16; };
+    auto vcol = [&](int i) KDA_INLINE { return (FP8 ? schunk : v_chunk<D>(srow + i * R::kRows, schunk)) * 16; };
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-        const uint32_t r = lane / R::kLanes + i * R::kRows;
-        kcol[i] = (FP8 ? schunk : k_chunk<D>(r, schunk)) * 16;
-        vcol[i] = (FP8 ? schunk : v_chunk<D>(r, schunk)) * 16;
-        krow[i] = ((r * static_cast<uint32_t>(a.cache.k_stride_token)) << R::kShift) + kcol[i];
-        vrow[i] = ((r * static_cast<uint32_t>(a.cache.v_stride_token)) << R::kShift) + vcol[i];
+        const uint32_t r = srow + i * R::kRows;
+        krow[i] = r * static_cast<uint32_t>(ktoken) + kcol(i) + (kLoads - 1 - i) * kKib;
+        vrow[i] = r * static_cast<uint32_t>(vtoken) + vcol(i) + (kLoads - 1 - i) * kKib;
     }
-    // The looked-up rows, of K or of V, into their buffer or (8 bits) into registers.
-    auto load = [&](const Pages &pages, const char *head_base, int64_t stride_page, int64_t stride_token,
-                    const uint32_t (&row)[kLoads], const uint32_t (&column)[kLoads], auto &reg, char *tile) {
+    u32x4 kreg[FP8 ? kLoads : 1], vreg[FP8 ? kLoads : 1];
+    auto load = [&](const Group &group, const char *base, int64_t page_bytes, int64_t in_page, int64_t token_bytes,
+                    const uint32_t (&row)[kLoads], auto column, auto &reg, char *rows_at) KDA_INLINE {
         if constexpr (UNIFORM) {
-            const int page = __builtin_amdgcn_readfirstlane(pages.p[0]);
-            const int key = pages.key;
-            const bool any = key < see1.y && key + 16 > see0.x && page >= 0 && page < a.cache.num_pages;
-            const char *first = any ? head_base + ((page * stride_page + pages.off * stride_token) << R::kShift) : zero;
-            uint32_t at[kLoads];
+            const int page = __builtin_amdgcn_readfirstlane(group.page[0]);
+            const int key = group.key;
+            const bool any = static_cast<uint32_t>(page) < static_cast<uint32_t>(pool) && key < see1.y && key + 16 > see0.x;
+            uint32_t lane_at[kLoads];
+            const char *first = zero;
             if (any && key >= see0.x && key + 16 <= see1.y) {
+                first = base + page * page_bytes + in_page;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    at[i] = row[i];
+                    lane_at[i] = row[i];
                 }
             } else {
                 // some rows have no key that the tile sees: the nearest that has stands in (its
                 // scores are masked), so nothing is read that no request wrote
-                const uint32_t step = any ? static_cast<uint32_t>(stride_token) : 0;
+                uint32_t token = 0;
+                if (any) {
+                    first = base + page * page_bytes + in_page;
+                    token = static_cast<uint32_t>(token_bytes);
+                }
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int r = max(min(static_cast<int>(lane / R::kLanes + i * R::kRows), see1.y - 1 - key), see0.x - key);
-                    at[i] = ((static_cast<uint32_t>(r) * step) << R::kShift) + column[i];
+                    const int r = max(min(srow + i * R::kRows, see1.y - 1 - key), see0.x - key);
+                    lane_at[i] = static_cast<uint32_t>(r) * token + column(i) + (kLoads - 1 - i) * kKib;
                 }
             }
+            if constexpr (FP8) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                if constexpr (FP8) {
-                    reg[i] = load16(first + at[i]);
-                } else {
-                    load16_to_lds(first, at[i], tile + wave * (16 * 2 * D) + i * 1024);
+                for (int i = 0; i < kLoads; ++i) {
+                    reg[i] = load16(first + lane_at[i]);
                 }
+            } else {
+                load16_to_lds(first - (kLoads - 1) * kKib, lane_at, rows_at);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int key = pages.key + lane / R::kLanes + i * R::kRows;
-                const int page = pages.p[i];
-                const int off = key - key / a.cache.page_size * a.cache.page_size;
-                const bool real = key >= see0.x && key < see1.y && page >= 0 && page < a.cache.num_pages;
-                const char *first = head_base + ((page * stride_page + off * stride_token) << R::kShift);
+                const int key = group.key + srow + i * R::kRows;
+                const int page = group.page[i];
+                const int in = key - key / a.cache.page_size * a.cache.page_size;
+                const bool real = key >= see0.x && key < see1.y && static_cast<uint32_t>(page) < static_cast<uint32_t>(pool);
+                const char *first = (real ? base + page * page_bytes + in * token_bytes : zero) + column(i);
                 if constexpr (FP8) {
-                    reg[i] = load16((real ? first : zero) + column[i]);
+                    reg[i] = load16(first);
                 } else {
-                    load16_to_lds((real ? first : zero) + column[i], tile + wave * (16 * 2 * D) + i * 1024);
+                    load16_to_lds(first, rows_at + i * 1024);
                 }
             }
         }
     };
-    auto load_k = [&](const Pages &pages, int parity) {
-        load(pages, kbase, a.cache.k_stride_page, a.cache.k_stride_token, krow, kcol, kreg, sm[parity][0]);
+    // K's buffer is filled 32 keys ahead of V's: its rows are the groups' of waves 2, 3, then 0, 1
+    const int kslot = 16 * ((wave + 2) & 3), vslot = 16 * wave;
+    auto load_k = [&](const Group &group, int parity) KDA_INLINE {
+        load(group, kbase, kpage, group.koff, ktoken, krow, kcol, kreg, sm[parity][0] + kslot * 2 * D);
     };
-    auto load_v = [&](const Pages &pages, int parity) {
-        load(pages, vbase, a.cache.v_stride_page, a.cache.v_stride_token, vrow, vcol, vreg, sm[parity][1]);
+    auto load_v = [&](const Group &group, int parity) KDA_INLINE {
+        load(group, vbase, vpage, group.voff, vtoken, vrow, vcol, vreg, sm[parity][1] + vslot * 2 * D);
     };
-    auto write_k = [&](int parity) {
+    auto write_k = [&](int parity) KDA_INLINE {
         if constexpr (FP8) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                stage<D, FP8>(sm[parity][0], srow + i * R::kRows, schunk, kreg[i], [](int r, int c) { return k_at<D>(r, c); });
+                stage<D, FP8>(sm[parity][0], kslot + srow + i * R::kRows, schunk, kreg[i], [](int r, int c) { return k_at<D>(r, c); });
             }
         }
     };
-    auto write_v = [&](int parity) {
+    auto write_v = [&](int parity) KDA_INLINE {
         if constexpr (FP8) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                stage<D, FP8>(sm[parity][1], srow + i * R::kRows, schunk, vreg[i], [](int r, int c) { return v_at<D>(r, c); });
+                stage<D, FP8>(sm[parity][1], vslot + srow + i * R::kRows, schunk, vreg[i], [](int r, int c) { return v_at<D>(r, c); });
             }
         }
     };
     // All rows of the buffers are there, and the reads of the others have ended, for every wave.
-    auto staged = [&] {
+    auto staged = [&]() KDA_INLINE {
         if constexpr (FP8) {
             lds_barrier();
         } else {
@@ -979,96 +1005,81 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
             asm volatile("" ::: "memory");
         }
     };
-    // Scores of 32 keys: a lane's are of row `col`, keys 8 (e / 4) + 4 half + e % 4.
-    typedef f32x16 Half[RB];
-    auto products = [&](int parity, int kt, Half &s) {
+
+    // ---- the chain, 32 keys a step: a lane's scores are of row `col`, keys 8 (e / 4) + 4 half + e % 4
+    auto products = [&](int parity, int kt, f32x16 &s) KDA_INLINE {
         const char *tile = sm[parity][0];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[b][e] = 0.0f;
-            }
+        for (int e = 0; e < 16; ++e) {
+            s[e] = 0.0f;
         }
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
-            const u32x4 op = *reinterpret_cast<const u32x4 *>(tile + k_at<D>(kt * 32 + col, 2 * x + half));
-#pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                s[b] = mfma32(op, q[b][x], s[b]);
-            }
+            s = mfma32(*reinterpret_cast<const u32x4 *>(tile + k_at<D>(kt * 32 + col, 2 * x + half)), q[x], s);
         }
     };
     const float c = sc.cap > 0.0f ? 1.0f : sc.c;
-    float top[RB];  // largest of the scores that are next, in log2 units
+    float top = kNegInf;  // largest of the scores that are next, in log2 units
     // cap, mask and largest score of the keys from key0
-    auto finish = [&](int key0, Half &s) {
+    auto finish = [&](int key0, f32x16 &s) KDA_INLINE {
         if (sc.cap > 0.0f) {
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[b][e] = capped(s[b][e] * sc.in, sc.cap);
-                }
+            for (int e = 0; e < 16; ++e) {
+                s[e] = capped(s[e] * sc.in, sc.cap);
             }
         }
         if (!(key0 >= wsee1.x && key0 + 32 <= wsee0.y)) {  // some row of the wave does not see some key
-#pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                const int from = see[b].x - key0 - 4 * half, to = see[b].y - key0 - 4 * half;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int k = 8 * (e >> 2) + (e & 3);
-                    s[b][e] = k >= from && k < to ? s[b][e] : kNegInf;
-                }
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            float x = kNegInf;
+            const int from = see.x - key0 - 4 * half, to = see.y - key0 - 4 * half;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                x = fmaxf(x, s[b][e]);
+                const int k = 8 * (e >> 2) + (e & 3);
+                s[e] = k >= from && k < to ? s[e] : kNegInf;
             }
-            top[b] = max_halves(x) * c;
         }
+        float x = kNegInf;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x = fmaxf(x, s[e]);
+        }
+        top = max_halves(x) * c;
     };
     // weights of the scores s and their products with rows 32 kt .. of the values in buffer `parity`; the
     // next 32 keys' scores are formed meanwhile
-    auto step = [&](int parity, int kt, const Half &s, int next_kt, Half &next) {
+    auto step = [&](int parity, int kt, const f32x16 &s, f32x16 &next) KDA_INLINE {
+        if (__any(top > m + kRaise)) {
+            const float up = fmaxf(m, top);
+            const float f = up == m ? 1.0f : ex2(m - up);
+            m = up;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                o[d] *= f;
+            }
+        }
+        products(parity, kt, next);
+        const float base = m == kNegInf ? 0.0f : m;
+        u32x4 p[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // 16 keys: 8 of this half of the wave
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = ex2(s[8 * x + e] * c - base);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[x][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+            }
+#ifdef NODOT
+            l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                l = add_pair(p[x][e], l);
+            }
+#endif
+        }
         const char *vt = sm[parity][1];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            if (__any(top[b] > m[b] + kRaise)) {
-                const float up = fmaxf(m[b], top[b]);
-                const float f = up == m[b] ? 1.0f : ex2(m[b] - up);
-                m[b] = up;
-                l[b] *= f;
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    o[b][d] *= f;
-                }
-            }
-        }
-        products(parity, next_kt, next);
-        u32x4 p[RB][2];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            const float base = m[b] == kNegInf ? 0.0f : m[b];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {  // 16 keys: 8 of this half of the wave
-                float w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[e] = ex2(s[b][8 * x + e] * c - base);
-                }
-                l[b] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[b][x][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
-                }
-            }
-        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
 #pragma unroll
@@ -1077,11 +1088,7 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
                 const int row = 32 * kt + 16 * x + 4 * half;
                 const u32x2 v0 = read_tr<D>(vt, row, pair, lane);
                 const u32x2 v1 = read_tr<D>(vt, row + 8, pair, lane);
-                const u32x4 op = {v0[0], v0[1], v1[0], v1[1]};
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    o[b][d] = mfma32(op, p[b][x], o[b][d]);
-                }
+                o[d] = mfma32(u32x4{v0[0], v0[1], v1[0], v1[1]}, p[x], o[d]);
             }
         }
     };
@@ -1089,38 +1096,39 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
     if (t0 < t1) {
         // tiles that the wave sees: [w0, w1)
         const int w0 = active ? max(t0, wsee0.x / kTile) : t1, w1 = active ? min(t1, (wsee1.y + kTile - 1) / kTile) : t1;
-        Walk kwalk = walk_from(t0 * kTile + wave * 16 + 32), vwalk = walk_from(t0 * kTile + wave * 16);
-        // the first tile's first keys, as the second half of the tile before
-        Walk before = walk_from(t0 * kTile + wave * 16 - 32);
-        Pages kp = lookup(before);
-        load_k(kp, 1);
+        // In turn t V's buffer holds the keys 64 t .., K's the keys 64 t + 32 ..: the first 32 keys'
+        // scores are formed before, from the second half of the other buffer.
+        Group now = walk(), next = walk(), after = walk();
+        const bool early = wave < 2;  // K's next rows are of the group after V's next rows
+        if (early) {
+            load_k(now, 1);
+        }
+        load_v(now, 0);
         write_k(1);
-        Pages vp = lookup(vwalk);
-        kp = lookup(kwalk);
-        load_k(kp, 0);
-        load_v(vp, 0);
-        vp = lookup(vwalk);
-        kp = lookup(kwalk);
+        load_k(early ? next : now, 0);
         write_k(0);
         write_v(0);
+        now = next;
+        next = after;
+        after = walk();
         staged();
-        Half even, odd;
+        f32x16 even, odd;
         if (t0 == w0) {
             products(1, 1, even);
             finish(t0 * kTile, even);
         }
         lds_barrier();  // before the first turn stages over these keys
-        // K's tiles are 32 keys ahead of V's, as the scores are. Past the last tile rows of zeros
-        // are loaded and staged, whose scores nobody uses.
-        auto turn = [&](int t, int parity) {
-            load_k(kp, parity ^ 1);
-            load_v(vp, parity ^ 1);
-            kp = lookup(kwalk);
-            vp = lookup(vwalk);
+        auto turn = [&](int t, int parity) KDA_INLINE {
+            // past the last tile rows of zeros are loaded and staged, whose scores nobody uses
+            load_k(early ? next : now, parity ^ 1);
+            load_v(now, parity ^ 1);
+            now = next;
+            next = after;
+            after = walk();
             if (t >= w0 && t < w1) {
-                step(parity, 0, even, 0, odd);
+                step(parity, 0, even, odd);
                 finish(t * kTile + 32, odd);
-                step(parity, 1, odd, 1, even);
+                step(parity, 1, odd, even);
                 finish(t * kTile + kTile, even);
             } else if (t + 1 == w0) {
                 products(parity, 1, even);
@@ -1140,47 +1148,44 @@ __global__ __launch_bounds__(kThreads, RB == 1 ? 2 : 1) void prefill_kernel(cons
 
     // ---- out, or this split's part: lane: row `col` of 32, columns 32 d + 8 (e / 4) + 4 half + e % 4
     const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
+    const int r = wave * 32 + col;
+    const float sum = sum_halves(l);
+    if (r >= rows) {
+        return;
+    }
+    if (splits == 1) {
+        const float f = sum == 0.0f ? 0.0f : vs / sum;
+        const int t = (row0 + r) / a.group;
+        const int h = head * a.group + (row0 + r) - t * a.group;
+        uint16_t *out = static_cast<uint16_t *>(a.out) + static_cast<int64_t>(req.begin + t) * a.out_stride_token +
+                        h * a.out_stride_head + half * 4;
+        struct __attribute__((packed, aligned(2))) Out {
+            uint32_t w[2];
+        };
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const int r = wave * 32 * RB + b * 32 + col;
-        const float sum = sum_halves(l[b]);
-        if (r >= rows) {
-            continue;
+        for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                *reinterpret_cast<Out *>(out + d * 32 + e * 8) = {
+                    {pack_bf16x2(o[d][4 * e] * f, o[d][4 * e + 1] * f),
+                     pack_bf16x2(o[d][4 * e + 2] * f, o[d][4 * e + 3] * f)}};
+            }
         }
-        if (splits == 1) {
-            const float f = sum == 0.0f ? 0.0f : vs / sum;
-            const int t = (row0 + r) / a.group;
-            const int h = head * a.group + (row0 + r) - t * a.group;
-            uint16_t *out = static_cast<uint16_t *>(a.out) + static_cast<int64_t>(req.begin + t) * a.out_stride_token +
-                            h * a.out_stride_head + half * 4;
-            struct __attribute__((packed, aligned(2))) Out {
-                uint32_t w[2];
-            };
+    } else {
+        const int64_t all = static_cast<int64_t>(a.num_tokens) * a.group;
+        const int64_t at = (static_cast<int64_t>(split) * a.cache.kv_heads + head) * all +
+                           static_cast<int64_t>(req.begin) * a.group + row0 + r;
+        if (half == 0) {
+            ws.ml[at] = make_float2(m, sum);
+        }
+        if (sum != 0.0f) {  // the join reads no others
+            float *po = ws.o + at * D + half * 4;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    *reinterpret_cast<Out *>(out + d * 32 + e * 8) = {
-                        {pack_bf16x2(o[b][d][4 * e] * f, o[b][d][4 * e + 1] * f),
-                         pack_bf16x2(o[b][d][4 * e + 2] * f, o[b][d][4 * e + 3] * f)}};
-                }
-            }
-        } else {
-            const int64_t all = static_cast<int64_t>(a.num_tokens) * a.group;
-            const int64_t at = (static_cast<int64_t>(split) * a.cache.kv_heads + head) * all +
-                               static_cast<int64_t>(req.begin) * a.group + row0 + r;
-            if (half == 0) {
-                ws.ml[at] = make_float2(m[b], sum);
-            }
-            if (sum != 0.0f) {  // the join reads no others
-                float *po = ws.o + at * D + half * 4;
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        *reinterpret_cast<f32x4 *>(po + d * 32 + e * 8) =
-                            f32x4{o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]};
-                    }
+                    *reinterpret_cast<f32x4 *>(po + d * 32 + e * 8) =
+                        f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
                 }
             }
         }
@@ -1232,8 +1237,6 @@ template <int D> __global__ __launch_bounds__(kThreads) void prefill_combine_ker
 // Host
 // ---------------------------------------------------------------------------
 
-constexpr int kRowBlocks = 1;  // RB of the prefill kernel
-
 struct Plan {
     bool decode;
     int blocks;     // decode: NB
@@ -1268,8 +1271,7 @@ Plan plan_of(const KdaPagedAttentionArgs &a) {
         p.bytes = p.desc_at + size_t{kDecodeGroups} * 16;
         return p;
     }
-    const int64_t tile_rows = 128 * kRowBlocks;
-    p.tiles = static_cast<int64_t>(a.num_tokens) * group / tile_rows + a.num_seqs;
+    p.tiles = static_cast<int64_t>(a.num_tokens) * group / kTileRows + a.num_seqs;
     // few tiles over many keys: cut the keys until two workgroups a CU have work, in
     // parts of 512 keys at least
     const int64_t units = p.tiles * a.cache.kv_heads;
@@ -1329,9 +1331,9 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
     // 16 rows of a page at offsets that fit 32 bits
     const auto near = [](int64_t stride) { return stride >= 0 && stride < (1 << 26); };
     if (a.cache.page_size % 16 == 0 && near(a.cache.k_stride_token) && near(a.cache.v_stride_token)) {
-        prefill_kernel<D, FP8, kRowBlocks, true><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
+        prefill_kernel<D, FP8, true><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
     } else {
-        prefill_kernel<D, FP8, kRowBlocks, false><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
+        prefill_kernel<D, FP8, false><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
     }
     if (p.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.num_heads;

@@ -10,7 +10,7 @@
 // pass that sums the squares, and a row takes one reduction, not two.
 //
 // Bound by HBM: a row stays in registers between its one read and its one
-// write. A lane holds 8 neighbouring columns at a time (16 or 32 bytes), so 16
+// write. A lane holds 16 bytes of the input at a time (8 or 4 columns), so 16 or 32
 // lanes hold a group of 128. Loads and stores are typed as unaligned vectors
 // (gfx950 serves them at any element address): rows of odd widths take the same
 // path, and only the last, partial chunk of a row goes element by element.
@@ -26,55 +26,87 @@
 namespace kda {
 namespace {
 
-constexpr int kVec = 8;          // columns a lane holds at a time
 constexpr int kGroup = 128;      // columns of a scale group
 constexpr float kFp8Max = 448.0f;
 constexpr float kMinScale = 1e-12f;
 
-struct __attribute__((packed, aligned(2))) Bf16x8 {
-    uint32_t w[4];
+// Vectors at any element address.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int BYTES> struct Any;
+template <> struct Any<16> {
+    typedef u32x4 T __attribute__((aligned(1)));
 };
-struct __attribute__((packed, aligned(4))) F32x4 {
-    float w[4];
+template <> struct Any<8> {
+    typedef u32x2 T __attribute__((aligned(1)));
 };
-struct __attribute__((packed, aligned(1))) Fp8x8 {
-    uint32_t w[2];
+template <> struct Any<4> {
+    typedef uint32_t T __attribute__((aligned(1)));
 };
+// STREAM: data read or written once. (A template argument: of a choice at run time the compiler
+// makes one access, without the hint.)
+template <class A, bool STREAM, class T> __device__ __forceinline__ auto load_as(const T *p) {
+    const typename A::T *q = reinterpret_cast<const typename A::T *>(p);
+    if constexpr (STREAM) {
+        return __builtin_nontemporal_load(q);
+    } else {
+        return *q;
+    }
+}
+template <class A, bool STREAM, class T, class R> __device__ __forceinline__ void store_as(T *p, R r) {
+    if constexpr (STREAM) {
+        __builtin_nontemporal_store(r, reinterpret_cast<typename A::T *>(p));
+    } else {
+        *reinterpret_cast<typename A::T *>(p) = r;
+    }
+}
 
-__device__ __forceinline__ void load8(const uint16_t *p, float (&f)[kVec]) {
-    const Bf16x8 r = *reinterpret_cast<const Bf16x8 *>(p);
+// Columns a lane holds at a time: 16 bytes of the input, so that the lanes of a load are neighbours.
+template <class T> constexpr int kVec = 16 / sizeof(T);
+
+// V (4 or 8) consecutive elements as they stand in memory, and as fp32.
+template <class T, int V> struct Raw {
+    static constexpr int kBytes = V * sizeof(T);
+    uint32_t w[kBytes / 4];
+    template <bool STREAM> __device__ __forceinline__ void load(const T *p) {
+        if constexpr (kBytes == 8) {
+            const u32x2 r = load_as<Any<8>, STREAM>(p);
+            w[0] = r[0];
+            w[1] = r[1];
+        } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(r.w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+            for (int j = 0; j < kBytes / 16; ++j) {
+                const u32x4 r = load_as<Any<16>, STREAM>(reinterpret_cast<const char *>(p) + 16 * j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[4 * j + i] = r[i];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                f[i] = __uint_as_float(w[i]);
+            } else {
+                f[i] = __uint_as_float(i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xffff0000u);
+            }
+        }
+    }
+};
+template <int V, bool STREAM> __device__ __forceinline__ void store(uint16_t *p, const float (&f)[V]) {
+    if constexpr (V == 8) {
+        store_as<Any<16>, STREAM>(p, u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])});
+    } else {
+        store_as<Any<8>, STREAM>(p, u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])});
     }
 }
-__device__ __forceinline__ void load8(const float *p, float (&f)[kVec]) {
-    const F32x4 a = *reinterpret_cast<const F32x4 *>(p);
-    const F32x4 b = *reinterpret_cast<const F32x4 *>(p + 4);
+template <int V, bool STREAM> __device__ __forceinline__ void store(float *p, const float (&f)[V]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[i] = a.w[i];
-        f[4 + i] = b.w[i];
+    for (int j = 0; j < V; j += 4) {
+        store_as<Any<16>, STREAM>(p + j, u32x4{__float_as_uint(f[j]), __float_as_uint(f[j + 1]), __float_as_uint(f[j + 2]), __float_as_uint(f[j + 3])});
     }
-}
-__device__ __forceinline__ void store8(uint16_t *p, const float (&f)[kVec]) {
-    Bf16x8 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r.w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-    }
-    *reinterpret_cast<Bf16x8 *>(p) = r;
-}
-__device__ __forceinline__ void store8(float *p, const float (&f)[kVec]) {
-    F32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        a.w[i] = f[i];
-        b.w[i] = f[4 + i];
-    }
-    *reinterpret_cast<F32x4 *>(p) = a;
-    *reinterpret_cast<F32x4 *>(p + 4) = b;
 }
 
 // Four fp32 to four e4m3 bytes, round to nearest even. |y / s| is at most
@@ -83,45 +115,60 @@ __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float 
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
-__device__ __forceinline__ void store8(uint8_t *p, const float (&f)[kVec]) {
-    Fp8x8 r;
-    r.w[0] = pack_fp8x4(f[0], f[1], f[2], f[3]);
-    r.w[1] = pack_fp8x4(f[4], f[5], f[6], f[7]);
-    *reinterpret_cast<Fp8x8 *>(p) = r;
+template <int V, bool STREAM> __device__ __forceinline__ void store(uint8_t *p, const float (&f)[V]) {
+    if constexpr (V == 8) {
+        store_as<Any<8>, STREAM>(p, u32x2{pack_fp8x4(f[0], f[1], f[2], f[3]), pack_fp8x4(f[4], f[5], f[6], f[7])});
+    } else {
+        store_as<Any<4>, STREAM>(p, pack_fp8x4(f[0], f[1], f[2], f[3]));
+    }
 }
 using kda::store1;
 __device__ __forceinline__ void store1(uint8_t *p, float x) {
     *p = static_cast<uint8_t>(pack_fp8x4(x, 0.0f, 0.0f, 0.0f));
 }
 
-// A chunk of a row: whole, or its first n columns (the others read as 0).
-template <class T> __device__ __forceinline__ void load_chunk(const T *p, int n, float (&f)[kVec]) {
-    if (n >= kVec) {
-        load8(p, f);
-    } else {
+// Chunk c of a lane: V columns from `col`. Where the row ends inside it or before it, the row's last V
+// columns are loaded instead and moved down, zeros after them: loads that no branch holds back, which a
+// lane by lane choice of a shorter one would (every load is then waited for before the next is issued).
+struct Place {
+    int col;    // may lie past the row's end
+    int at;     // the load's first column
+    bool any;   // the wave has columns of the row in this chunk
+    bool tail;  // and some lane's end before its chunk does
+};
+template <int V> __device__ __forceinline__ Place place(int index, int wave_first, int width) {
+    Place p;
+    p.col = index * V;
+    p.at = min(p.col, width - V);
+    p.any = wave_first * V < width;
+    p.tail = (wave_first + 64) * V > width;
+    return p;
+}
+template <int V> __device__ __forceinline__ void move_down(const Place &p, float (&f)[V]) {
+    const int by = p.col - p.at;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            f[i] = i < n ? load1(p + i) : 0.0f;
+    for (int s = V / 2; s > 0; s /= 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float from = i + s < V ? f[i + s] : 0.0f;
+            f[i] = (by & s) != 0 ? from : f[i];
         }
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        f[i] = by >= V ? 0.0f : f[i];
+    }
 }
-template <class T> __device__ __forceinline__ void store_chunk(T *p, int n, const float (&f)[kVec]) {
-    if (n >= kVec) {
-        store8(p, f);
+template <int V, bool STREAM, class T> __device__ __forceinline__ void store_chunk(T *p, int n, const float (&f)[V]) {
+    if (n >= V) {
+        store<V, STREAM>(p, f);
     } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+        for (int i = 0; i < V; ++i) {
             if (i < n) {
                 store1(p + i, f[i]);
             }
         }
-    }
-}
-__device__ __forceinline__ void load_chunk(const void *p, int dtype, int64_t at, int n, float (&f)[kVec]) {
-    if (dtype == KDA_F32) {
-        load_chunk(static_cast<const float *>(p) + at, n, f);
-    } else {
-        load_chunk(static_cast<const uint16_t *>(p) + at, n, f);
     }
 }
 
@@ -132,15 +179,15 @@ __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > 
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
     return larger(x, __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ uint32_t group_max16(uint32_t x) {
+template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t x) {  // of 16 or 32 lanes
     x = dpp_max<kDppQuadXor1>(x);
     x = dpp_max<kDppQuadXor2>(x);
     x = dpp_max<kDppRowHalfMirror>(x);
-    return dpp_max<kDppRowMirror>(x);
+    x = dpp_max<kDppRowMirror>(x);
+    return LANES == 16 ? x : larger(x, __shfl_xor(x, 16));
 }
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    x = group_max16(x);
-    x = larger(x, __shfl_xor(x, 16));
+    x = group_max<32>(x);
     return larger(x, __shfl_xor(x, 32));
 }
 __device__ __forceinline__ float wave_sum(float x) {
@@ -177,137 +224,208 @@ __device__ __forceinline__ float scale_of(uint32_t top, float rsqrt) {
 }
 
 // y of a chunk from h w, its 8-bit scale's group already reduced in `top` (the
-// whole row's) or reduced here over 16 lanes, and the chunk's store.
-template <class TO>
+// whole row's) or reduced here over the group's lanes, and the chunk's store.
+template <class TO, int V>
 __device__ __forceinline__ void finish(const KdaRmsNormArgs &a, int64_t row, int col, float rsqrt, uint32_t top,
-                                       float (&hw)[kVec]) {
+                                       float (&hw)[V]) {
     TO *out = static_cast<TO *>(a.out) + row * a.out_stride + col;
     const int n = a.width - col;  // may be <= 0: the lane only takes part in the group's maximum
     if constexpr (sizeof(TO) == 1) {
         if (a.group != 0) {
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
+            for (int i = 0; i < V; ++i) {
                 m = larger(m, magnitude(hw[i]));
             }
-            top = group_max16(m);
+            top = group_max<kGroup / V>(m);
         }
         const float s = scale_of(top, rsqrt);
         const float inv = rsqrt / s;
         // a zero sum of squares with eps = 0 gives an infinite factor: y is NaN there as 0 * inf is
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+        for (int i = 0; i < V; ++i) {
             hw[i] = hw[i] * inv;
         }
-        if (a.group != 0 && threadIdx.x % 16 == 0 && n > 0) {
+        if (a.group != 0 && threadIdx.x % (kGroup / V) == 0 && n > 0) {
             a.scale[row * ((a.width + kGroup - 1) / kGroup) + col / kGroup] = s;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+        for (int i = 0; i < V; ++i) {
             hw[i] *= rsqrt;
         }
     }
     if (n > 0) {
-        store_chunk(out, n, hw);
+        store_chunk<V, false>(out, n, hw);
     }
 }
 
-// x + r of a chunk.
-template <class TX>
-__device__ __forceinline__ void load_sum(const KdaRmsNormArgs &a, int64_t row, int col, int n, float (&h)[kVec]) {
-    load_chunk(static_cast<const TX *>(a.x) + row * a.x_stride + col, n, h);
-    if (a.residual != nullptr) {
-        float r[kVec];
-        load_chunk(a.residual, a.residual_dtype, row * a.residual_stride + col, n, r);
+// A row's columns in registers: CHUNKS chunks of V a thread, THREADS threads a row.
+template <int V, int THREADS, int CHUNKS> struct Columns {
+    __device__ __forceinline__ static Place at(int c, int width) {
+        const int lane = threadIdx.x % THREADS;
+        return place<V>(c * THREADS + lane, c * THREADS + __builtin_amdgcn_readfirstlane(lane & ~63), width);
+    }
+    // f(chunk, place, columns) for every chunk of an array that the wave has columns in; all loads first
+    template <bool STREAM, class T, class F> __device__ __forceinline__ static void each(const T *row, int width, F f) {
+        Raw<T, V> raw[CHUNKS];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            h[i] += r[i];
+        for (int c = 0; c < CHUNKS; ++c) {
+            const Place p = at(c, width);
+            if (p.any) {
+                raw[c].template load<STREAM>(row + p.at);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const Place p = at(c, width);
+            if (p.any) {
+                float x[V];
+                raw[c].get(x);
+                if (p.tail) {
+                    move_down<V>(p, x);
+                }
+                f(c, p, x);
+            }
         }
     }
-}
-__device__ __forceinline__ void store_residual(const KdaRmsNormArgs &a, int64_t row, int col, int n,
-                                               const float (&h)[kVec]) {
-    if (a.residual != nullptr) {
-        const int64_t at = row * a.residual_stride + col;
-        if (a.residual_dtype == KDA_F32) {
-            store_chunk(static_cast<float *>(a.residual) + at, n, h);
+    template <bool STREAM, class F> __device__ __forceinline__ static void each(const void *row, int dtype, int64_t at, int width, F f) {
+        if (dtype == KDA_F32) {
+            each<STREAM>(static_cast<const float *>(row) + at, width, f);
         } else {
-            store_chunk(static_cast<uint16_t *>(a.residual) + at, n, h);
+            each<STREAM>(static_cast<const uint16_t *>(row) + at, width, f);
         }
     }
-}
+};
 
-// THREADS threads a row (64: four rows a workgroup), CHUNKS chunks of 8 columns
-// a thread in registers.
+// THREADS threads a row (64: four rows a workgroup); width >= V.
 template <int THREADS, int CHUNKS, class TX, class TO>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel(const KdaRmsNormArgs a) {
+    constexpr int V = kVec<TX>;
+    using Row = Columns<V, THREADS, CHUNKS>;
     constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
-    const int lane = threadIdx.x % THREADS;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / THREADS;
     if (row >= a.rows) {
         return;  // whole waves: only rows of one wave share a workgroup
     }
-    float h[CHUNKS][kVec];
+    float h[CHUNKS][V];
     float sum = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-        const int col = (c * THREADS + lane) * kVec;
-        if (col < a.width) {
-            load_sum<TX>(a, row, col, a.width - col, h[c]);
-        } else {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                h[c][i] = 0.0f;
-            }
+        for (int i = 0; i < V; ++i) {
+            h[c][i] = 0.0f;
         }
     }
+    const TX *x = static_cast<const TX *>(a.x) + row * a.x_stride;
+    Raw<TX, V> raw[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-        const int col = (c * THREADS + lane) * kVec;
-        if (col < a.width) {
-            float w[kVec];
-            load_chunk(a.weight, a.weight_dtype, col, a.width - col, w);
-            store_residual(a, row, col, a.width - col, h[c]);
+        const Place p = Row::at(c, a.width);
+        if (p.any) {
+            raw[c].template load<true>(x + p.at);
+        }
+    }
+    const auto take_x = [&](int c, const Place &p) {
+        raw[c].get(h[c]);
+        if (p.tail) {
+            move_down<V>(p, h[c]);
+        }
+    };
+    if (a.residual != nullptr) {
+        const int64_t at = row * a.residual_stride;
+        Row::template each<true>(a.residual, a.residual_dtype, at, a.width, [&](int c, const Place &p, const float (&r)[V]) {
+            take_x(c, p);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                sum += h[c][i] * h[c][i];
-                h[c][i] *= w[i];
-                if constexpr (sizeof(TO) == 1) {
-                    top = larger(top, magnitude(h[c][i]));
-                }
+            for (int i = 0; i < V; ++i) {
+                h[c][i] += r[i];
+            }
+            // read again only a layer later
+            if (a.residual_dtype == KDA_F32) {
+                store_chunk<V, true>(static_cast<float *>(a.residual) + at + p.col, a.width - p.col, h[c]);
+            } else {
+                store_chunk<V, true>(static_cast<uint16_t *>(a.residual) + at + p.col, a.width - p.col, h[c]);
+            }
+        });
+    } else {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const Place p = Row::at(c, a.width);
+            if (p.any) {
+                take_x(c, p);
             }
         }
     }
+    Row::template each<false>(a.weight, a.weight_dtype, 0, a.width, [&](int c, const Place &, const float (&w)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            sum += h[c][i] * h[c][i];
+            h[c][i] *= w[i];
+            if constexpr (sizeof(TO) == 1) {
+                top = larger(top, magnitude(h[c][i]));
+            }
+        }
+    });
     row_reduce<THREADS / 64>(sum, top);
     const float rsqrt = 1.0f / sqrtf(sum / static_cast<float>(a.width) + a.eps);
-    if (sizeof(TO) == 1 && a.group == 0 && lane == 0) {
+    if (sizeof(TO) == 1 && a.group == 0 && threadIdx.x % THREADS == 0) {
         a.scale[row] = scale_of(top, rsqrt);
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-        // a chunk's 16 lanes leave the row's end together or not at all
-        const int col = (c * THREADS + lane) * kVec;
-        if (col / kGroup * kGroup < a.width) {
-            finish<TO>(a, row, col, rsqrt, top, h[c]);
+        const Place p = Row::at(c, a.width);
+        if (p.any) {
+            finish<TO, V>(a, row, p.col, rsqrt, top, h[c]);
         }
     }
 }
 
-// A row wider than the registers hold: read twice, its second read mostly from
-// the L2 cache. The residual is written in the second pass, which still reads
-// the old one.
+// A row wider than the registers hold: read twice, its second read mostly from the caches. The residual
+// is written in the second pass, which still reads the old one. Rows of less than 8 columns come here too:
+// no vector fits them.
 template <class TX, class TO> __global__ __launch_bounds__(1024) void rms_norm_wide_kernel(const KdaRmsNormArgs a) {
+    constexpr int V = kVec<TX>;
     const int64_t row = blockIdx.x;
+    const auto columns = [&](const void *p, int dtype, int64_t at, int n, float (&f)[V]) {
+        if (n >= V) {
+            if (dtype == KDA_F32) {
+                Raw<float, V> r;
+                r.template load<false>(static_cast<const float *>(p) + at);
+                r.get(f);
+            } else {
+                Raw<uint16_t, V> r;
+                r.template load<false>(static_cast<const uint16_t *>(p) + at);
+                r.get(f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                f[i] = i >= n ? 0.0f
+                              : dtype == KDA_F32 ? load1(static_cast<const float *>(p) + at + i)
+                                                 : load1(static_cast<const uint16_t *>(p) + at + i);
+            }
+        }
+    };
+    const auto sum_of = [&](int col, int n, float (&h)[V]) {
+        columns(a.x, a.x_dtype, row * a.x_stride + col, n, h);
+        if (a.residual != nullptr) {
+            float r[V];
+            columns(a.residual, a.residual_dtype, row * a.residual_stride + col, n, r);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                h[i] += r[i];
+            }
+        }
+    };
     float sum = 0.0f;
     uint32_t top = 0;
-    for (int col = threadIdx.x * kVec; col < a.width; col += 1024 * kVec) {
-        float h[kVec], w[kVec];
-        load_sum<TX>(a, row, col, a.width - col, h);
-        load_chunk(a.weight, a.weight_dtype, col, a.width - col, w);
+    for (int col = threadIdx.x * V; col < a.width; col += 1024 * V) {
+        float h[V], w[V];
+        sum_of(col, a.width - col, h);
+        columns(a.weight, a.weight_dtype, col, a.width - col, w);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+        for (int i = 0; i < V; ++i) {
             sum += h[i] * h[i];
             if constexpr (sizeof(TO) == 1) {
                 top = larger(top, magnitude(h[i] * w[i]));
@@ -319,33 +437,46 @@ template <class TX, class TO> __global__ __launch_bounds__(1024) void rms_norm_w
     if (sizeof(TO) == 1 && a.group == 0 && threadIdx.x == 0) {
         a.scale[row] = scale_of(top, rsqrt);
     }
-    for (int col = threadIdx.x * kVec; col / kGroup * kGroup < a.width; col += 1024 * kVec) {
-        float h[kVec] = {}, w[kVec];
-        if (col < a.width) {
-            load_sum<TX>(a, row, col, a.width - col, h);
-            load_chunk(a.weight, a.weight_dtype, col, a.width - col, w);
-            store_residual(a, row, col, a.width - col, h);
+    for (int col = threadIdx.x * V; col / kGroup * kGroup < a.width; col += 1024 * V) {
+        float h[V] = {}, w[V];
+        const int n = a.width - col;
+        if (n > 0) {
+            sum_of(col, n, h);
+            columns(a.weight, a.weight_dtype, col, n, w);
+            if (a.residual != nullptr) {
+                const int64_t at = row * a.residual_stride + col;
+                if (a.residual_dtype == KDA_F32) {
+                    store_chunk<V, false>(static_cast<float *>(a.residual) + at, n, h);
+                } else {
+                    store_chunk<V, false>(static_cast<uint16_t *>(a.residual) + at, n, h);
+                }
+            }
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
+            for (int i = 0; i < V; ++i) {
                 h[i] *= w[i];
             }
         }
-        finish<TO>(a, row, col, rsqrt, top, h);
+        finish<TO, V>(a, row, col, rsqrt, top, h);
     }
 }
 
+// Chunks of V columns a thread, by the row's width: a row of up to 512 is one wave's, longer ones take
+// a workgroup of 256 (up to 8192) or 1024 threads.
 template <class TX, class TO> void launch(const KdaRmsNormArgs &a, hipStream_t stream) {
+    constexpr int C = 8 / kVec<TX>;  // chunks in 8 columns
     const unsigned rows = static_cast<unsigned>(a.rows);
-    if (a.width <= 512) {
-        rms_norm_kernel<64, 1, TX, TO><<<(rows + 3) / 4, 256, 0, stream>>>(a);
+    if (a.width < 8) {
+        rms_norm_wide_kernel<TX, TO><<<rows, 1024, 0, stream>>>(a);
+    } else if (a.width <= 512) {
+        rms_norm_kernel<64, C, TX, TO><<<(rows + 3) / 4, 256, 0, stream>>>(a);
     } else if (a.width <= 2048) {
-        rms_norm_kernel<256, 1, TX, TO><<<rows, 256, 0, stream>>>(a);
+        rms_norm_kernel<256, C, TX, TO><<<rows, 256, 0, stream>>>(a);
     } else if (a.width <= 4096) {
-        rms_norm_kernel<256, 2, TX, TO><<<rows, 256, 0, stream>>>(a);
+        rms_norm_kernel<256, 2 * C, TX, TO><<<rows, 256, 0, stream>>>(a);
     } else if (a.width <= 8192) {
-        rms_norm_kernel<256, 4, TX, TO><<<rows, 256, 0, stream>>>(a);
+        rms_norm_kernel<256, 4 * C, TX, TO><<<rows, 256, 0, stream>>>(a);
     } else if (a.width <= 32768) {
-        rms_norm_kernel<1024, 4, TX, TO><<<rows, 1024, 0, stream>>>(a);
+        rms_norm_kernel<1024, 4 * C, TX, TO><<<rows, 1024, 0, stream>>>(a);
     } else {
         rms_norm_wide_kernel<TX, TO><<<rows, 1024, 0, stream>>>(a);
     }

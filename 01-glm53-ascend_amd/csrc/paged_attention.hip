@@ -26,6 +26,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kda_abi.h"
 #include "kda_device.h"
@@ -107,6 +108,39 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Infinite or NaN values that some rows of a tile do not see must not reach those, but in the matrix
+// product their weight of 0 makes a NaN. The steps do not look for them. A tile whose O is not finite at its end,
+// and whose rows do not all see the same keys, is formed again from values with 0 in those places, and
+// then they are added to the rows that see them.
+__device__ __forceinline__ u32x4 finite_only(u32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // the sign bit's place of each bf16 whose exponent is all ones
+        const uint32_t t = ((v[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        v[i] &= ~((t - (t >> 15)) | t);
+    }
+    return v;
+}
+template <bool FP8> __device__ __forceinline__ bool any_not_finite(u32x4 v) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        t |= FP8 ? ((v[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((v[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    }
+    return t != 0;
+}
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < __builtin_inff(); }
+// Column c of a row of values where it is infinite or NaN, else 0.
+template <bool FP8> __device__ __forceinline__ float not_finite(const char *row, int c) {
+    float x;
+    if constexpr (FP8) {
+        x = (reinterpret_cast<const uint8_t *>(row)[c] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.0f;
+    } else {
+        x = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row)[c]) << 16);
+    }
+    return is_finite(x) ? 0.0f : x;
+}
+
 // Sixteen e4m3 (16 bytes) as bf16, exactly (three mantissa bits): two operands of 8.
 __device__ __forceinline__ void fp8_to_bf16(u32x4 x, u32x4 &lo, u32x4 &hi) {
 #pragma unroll
@@ -118,11 +152,7 @@ __device__ __forceinline__ void fp8_to_bf16(u32x4 x, u32x4 &lo, u32x4 &hi) {
     }
 }
 
-// The other half's value (lanes l and l ^ 32), and sums and maxima over both.
-__device__ __forceinline__ float other_half(float x) {
-    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(__lane_id() < 32 ? r[1] : r[0]);
-}
+// Maxima and sums over lanes l and l ^ 32.
 __device__ __forceinline__ float max_halves(float x) {
     const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -184,7 +214,23 @@ struct Params : KdaPagedAttentionArgs {
     __device__ __forceinline__ int page_of(int n, int at) const {
         return meta(page_table, n * page_table_stride + at, KDA_WIDE_PAGE_TABLE);
     }
+    // The row of values of one of request n's keys, null on a page outside the pool.
+    template <bool FP8> __device__ __forceinline__ const char *value_row(int n, int head, int key) const {
+        const int page = page_of(n, key / cache.page_size);
+        const int64_t at = page * cache.v_stride_page + key % cache.page_size * cache.v_stride_token + head * cache.v_stride_head;
+        return static_cast<uint32_t>(page) < static_cast<uint32_t>(cache.num_pages)
+                   ? static_cast<const char *>(cache.v) + (FP8 ? at : 2 * at)
+                   : nullptr;
+    }
 };
+
+// A kernel's only argument, read again: what is needed only after a long loop would otherwise be kept in
+// scalar registers through it, of which the loop has none to spare.
+template <class T> __device__ __forceinline__ const T &arguments_again(const T &) {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const T *)p;
+}
 
 // Factor of the scores in log2 units, and what the capped form needs. The sign
 // of scale * k_scale goes into q, so the largest score is the largest product.
@@ -260,6 +306,37 @@ __device__ __forceinline__ u32x4 load_q(const Params &a, int64_t token, int head
     const uint16_t *p =
         static_cast<const uint16_t *>(a.q) + token * a.q_stride_token + head * a.q_stride_head + d;
     return reinterpret_cast<const Bf16x8Any *>(p)->w ^ flip;
+}
+
+// The first request after n that has new tokens, or num_seqs: 64 at a time, in every lane of a wave.
+__device__ __forceinline__ int next_request(const Params &a, int n) {
+    for (int first = n + 1; first < a.num_seqs; first += 64) {
+        const int x = min(first + static_cast<int>(__lane_id()), a.num_seqs - 1);
+        const unsigned long long some = __ballot(a.cu(x + 1) > a.cu(x));
+        if (some != 0) {
+            return __builtin_amdgcn_readfirstlane(first + __ffsll(some) - 1);
+        }
+    }
+    return a.num_seqs;
+}
+
+// f(key, row of values) for the keys in [lo, hi) of a request whose values are not all finite; by a whole wave.
+template <int D, bool FP8, class F>
+__device__ __forceinline__ void each_not_finite(const Params &a, int n, int head, int lo, int hi, F f) {
+    for (int key0 = lo; key0 < hi; key0 += 64) {
+        const int key = key0 + static_cast<int>(__lane_id());
+        const char *row = key < hi ? a.value_row<FP8>(n, head, key) : nullptr;
+        bool some = false;
+        if (row != nullptr) {
+            for (int c = 0; c < Row<D, FP8>::kBytes; c += 16) {
+                some |= any_not_finite<FP8>(load16(row + c));
+            }
+        }
+        for (unsigned long long left = __ballot(some); left != 0; left &= left - 1) {
+            const int found = key0 + __ffsll(left) - 1;
+            f(found, a.value_row<FP8>(n, head, found));
+        }
+    }
 }
 
 // Tokens that no request covers: zeros, spread over the grid.
@@ -345,8 +422,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
     const int n0 = min(tid * per, a.num_seqs), n1 = min(n0 + per, a.num_seqs);
     auto units_of = [&](const Request &r) { return (r.tokens * a.group + kRows - 1) / kRows * heads * tile_units(a, r, kRows); };
     int mine = 0;
+    bool bad = false;  // token offsets that decrease: requests overlap, and their units may not fit 32 bits
     for (int n = n0; n < n1; ++n) {
         mine += units_of(a.request(n));
+        bad |= a.cu(n) > a.cu(n + 1);
     }
     int scan = mine;
 #pragma unroll
@@ -357,14 +436,18 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
     if (lane == 63) {
         sm.scan[wave] = scan;
     }
+    if (__any(bad)) {
+        sm.scan[wave] = -1;
+    }
     __syncthreads();
     int total = 0, base = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         base += w < wave ? sm.scan[w] : 0;
         total += sm.scan[w];
+        bad |= sm.scan[w] < 0;
     }
-    total = __builtin_amdgcn_readfirstlane(total);
+    total = __builtin_amdgcn_readfirstlane(bad ? 0 : total);
     const int w = blockIdx.x;
     const int groups = min(static_cast<int>(gridDim.x), total);
     if (w >= groups) {
@@ -400,7 +483,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         const int count = tile_units(a, req, kRows);
         if (u >= start + tiles * heads * count) {
             start += tiles * heads * count;
-            req = a.request(++n);
+            n = next_request(a, n);
+            req = a.request(n);
             continue;
         }
         // ---- the item and the part of it that is in this range
@@ -434,15 +518,6 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         }
         f32x4 o[NB][D / 16];
         float m[NB], l[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            m[b] = kNegInf;
-            l[b] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                o[b][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-        }
 
         // ---- this wave's blocks of 32 keys: key0 + 128 i
         const int key0 = (unit0 + part0) * kUnit + wave * kBlock;
@@ -476,14 +551,27 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                 v[s] = load16_stream(reinterpret_cast<const char *>(__shfl(rows.v, from)) + lane % R::kLanes * 16);
             }
         };
+        bool again = false;
         // block i, whose rows are in k and v; the next one's are asked for as soon as these are in LDS
         auto compute = [&](int i, const Rows &next) KDA_INLINE {
             char *kt_ = sm.k[wave], *vt = sm.v[wave];
+            int lane = static_cast<int>(__lane_id());
+            if constexpr (NB > 1) {  // addresses in LDS formed anew for each block: kept, they do not all fit the registers
+                asm volatile("" : "+v"(lane));
+            }
+            const int col = lane & 15, g = lane >> 4;
 #pragma unroll
             for (int x = 0; x < kLoads; ++x) {
                 const int r = x * R::kRows + lane / R::kLanes;
                 stage<D, FP8>(kt_, r, lane % R::kLanes, k[x], [](int r, int c) { return k_at<D>(r, c); });
                 stage<D, FP8>(vt, r, lane % R::kLanes, v[x], [](int r, int c) { return v_at<D>(r, c); });
+            }
+            if (again) {
+#pragma unroll
+                for (int x = 0; x < kBlock * 2 * D / 1024; ++x) {
+                    u32x4 *p = reinterpret_cast<u32x4 *>(vt + x * 1024 + lane * 16);
+                    *p = finite_only(*p);
+                }
             }
             load(next);
             __builtin_amdgcn_sched_barrier(0);
@@ -561,18 +649,61 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                 }
             }
         };
-        if (blocks > 0) {
-            // past the last block rows of zeros are loaded
-            Rows rows = rows_of(0, lookup(0));
-            int page = lookup(1);
-            load(rows);
-            for (int i = 0; i < blocks; ++i) {
-                rows = rows_of(i + 1, page);
-                page = lookup(i + 2);
-                compute(i, rows);
+        for (;; again = true) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                m[b] = kNegInf;
+                l[b] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    o[b][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
+            if (blocks > 0) {
+                // past the last block rows of zeros are loaded
+                Rows rows = rows_of(0, lookup(0));
+                int page = lookup(1);
+                load(rows);
+                for (int i = 0; i < blocks; ++i) {
+                    rows = rows_of(i + 1, page);
+                    page = lookup(i + 2);
+                    compute(i, rows);
+                }
+            }
+            if (again || (first.x == last.x && first.y == last.y)) {
+                break;
+            }
+            bool fine = true;  // where a score is NaN the whole row is
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        fine &= is_finite(o[b][d][e]) || l[b] != l[b];
+                    }
+                }
+            }
+            if (__all(fine)) {
+                break;
             }
         }
-
+        if (again) {
+            each_not_finite<D, FP8>(a, n, head, lo, hi, [&](int key, const char *row) KDA_INLINE {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (key % kUnit / kBlock == wave && key >= see[b].x && key < see[b].y) {
+#pragma unroll
+                        for (int d = 0; d < D / 16; ++d) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                o[b][d][e] += not_finite<FP8>(row, 16 * d + 4 * g + e);
+                            }
+                        }
+                    }
+                }
+            });
+        }
         // ---- join the waves: their maxima, sums and 16 rows of O at a time through LDS
         const bool begins = part0 == 0, ends = part1 == count;
         const int64_t slot = 2 * static_cast<int64_t>(w) + (begins ? 1 : 0);
@@ -762,9 +893,16 @@ struct PrefillWs {
     float2 *ml;  // [splits][key heads][tokens * group]
 };
 
+struct PrefillArgs {
+    Params params;
+    PrefillWs ws;
+    int tiles, splits;
+};
+
 template <int D, bool FP8, bool UNIFORM>
-__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, const PrefillWs ws, int tiles,
-                                                                            int splits) {
+__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs args) {
+    const Params &a = args.params;
+    const int splits = args.splits;
     constexpr int kRows = kTileRows;
     using R = Row<D, FP8>;
     constexpr int kLoads = 16 / R::kRows;  // 16-byte loads a thread, of 16 rows a wave
@@ -785,7 +923,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
     const int head = id % a.cache.kv_heads;
     id /= a.cache.kv_heads;
     const int split = id % splits;
-    const int tile = tiles - 1 - static_cast<int>(id / splits);
+    const int tile = args.tiles - 1 - static_cast<int>(id / splits);
     int below = 0;  // requests that begin at or before this tile
     for (int n = 0; n < a.num_seqs; n += kThreads) {
         const int x = n + tid;
@@ -832,14 +970,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
         }
     }
     f32x16 o[D / 32];
-    float m = kNegInf, l = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            o[d][e] = 0.0f;
-        }
-    }
+    float m, l;
 
     // ---- staging. Of every 64 keys a wave loads 16, a group: keys 64 j + 16 wave, j = t0, t0 + 1, ...
     const char *kbase = static_cast<const char *>(a.cache.k) + ((head * a.cache.k_stride_head) << R::kShift);
@@ -858,14 +989,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
     };
     Group ahead;  // the walk's next
     int at = 0, off = 0;
-    ahead.key = t0 * kTile + wave * 16;
     const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
-    if constexpr (UNIFORM) {
-        at = ahead.key / a.cache.page_size;
-        off = ahead.key - at * a.cache.page_size;
-        ahead.koff = off * ktoken;
-        ahead.voff = off * vtoken;
-    }
+    auto begin_walk = [&]() KDA_INLINE {
+        ahead.key = t0 * kTile + wave * 16;
+        if constexpr (UNIFORM) {
+            at = ahead.key / a.cache.page_size;
+            off = ahead.key - at * a.cache.page_size;
+            ahead.koff = off * ktoken;
+            ahead.voff = off * vtoken;
+        }
+    };
     auto walk = [&]() KDA_INLINE -> Group {
         Group r = ahead;
         if constexpr (UNIFORM) {
@@ -979,6 +1112,19 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
             }
         }
     };
+    // In the second pass: the wave's rows of values without what is not finite.
+    auto finite_v = [&](auto again, int parity) KDA_INLINE {
+        if constexpr (again) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(kWaitMemory);  // the wave's own rows have landed
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int x = 0; x < 16 * 2 * D / 1024; ++x) {
+                u32x4 *p = reinterpret_cast<u32x4 *>(sm[parity][1] + vslot * 2 * D + x * 1024 + lane * 16);
+                *p = finite_only(*p);
+            }
+        }
+    };
     // All rows of the buffers are there, and the reads of the others have ended, for every wave.
     auto staged = [&]() KDA_INLINE {
         if constexpr (FP8) {
@@ -1005,7 +1151,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
         }
     };
     const float c = sc.cap > 0.0f ? 1.0f : sc.c;
-    float top = kNegInf;  // largest of the scores that are next, in log2 units
+    float top;  // largest of the scores that are next, in log2 units
     // cap, mask and largest score of the keys from key0
     auto finish = [&](int key0, f32x16 &s) KDA_INLINE {
         if (sc.cap > 0.0f) {
@@ -1056,14 +1202,10 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
             for (int e = 0; e < 4; ++e) {
                 p[x][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
             }
-#ifdef NODOT
-            l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-#else
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 l = add_pair(p[x][e], l);
             }
-#endif
         }
         const char *vt = sm[parity][1];
 #pragma unroll
@@ -1079,72 +1221,111 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
         }
     };
 
-    if (t0 < t1) {
-        // tiles that the wave sees: [w0, w1)
-        const int w0 = active ? max(t0, wsee0.x / kTile) : t1, w1 = active ? min(t1, (wsee1.y + kTile - 1) / kTile) : t1;
-        // In turn t V's buffer holds the keys 64 t .., K's the keys 64 t + 32 ..: the first 32 keys'
-        // scores are formed before, from the second half of the other buffer.
-        Group now = walk(), next = walk(), after = walk();
-        const bool early = wave < 2;  // K's next rows are of the group after V's next rows
-        if (early) {
-            load_k(now, 1);
+    auto pass = [&](auto again) KDA_INLINE {
+        m = kNegInf;
+        l = 0.0f;
+        top = kNegInf;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[d][e] = 0.0f;
+            }
         }
-        load_v(now, 0);
-        write_k(1);
-        load_k(early ? next : now, 0);
-        write_k(0);
-        write_v(0);
-        now = next;
-        next = after;
-        after = walk();
-        staged();
-        f32x16 even, odd;
-        if (t0 == w0) {
-            products(1, 1, even);
-            finish(t0 * kTile, even);
-        }
-        lds_barrier();  // before the first turn stages over these keys
-        auto turn = [&](int t, int parity) KDA_INLINE {
-            // past the last tile rows of zeros are loaded and staged, whose scores nobody uses
-            load_k(early ? next : now, parity ^ 1);
-            load_v(now, parity ^ 1);
+        if (t0 < t1) {
+            // tiles that the wave sees: [w0, w1)
+            const int w0 = active ? max(t0, wsee0.x / kTile) : t1, w1 = active ? min(t1, (wsee1.y + kTile - 1) / kTile) : t1;
+            // In turn t V's buffer holds the keys 64 t .., K's the keys 64 t + 32 ..: the first 32 keys'
+            // scores are formed before, from the second half of the other buffer.
+            begin_walk();
+            Group now = walk(), next = walk(), after = walk();
+            const bool early = wave < 2;  // K's next rows are of the group after V's next rows
+            if (early) {
+                load_k(now, 1);
+            }
+            load_v(now, 0);
+            write_k(1);
+            load_k(early ? next : now, 0);
+            write_k(0);
+            write_v(0);
+            finite_v(again, 0);
             now = next;
             next = after;
             after = walk();
-            if (t >= w0 && t < w1) {
-                step(parity, 0, even, odd);
-                finish(t * kTile + 32, odd);
-                step(parity, 1, odd, even);
-                finish(t * kTile + kTile, even);
-            } else if (t + 1 == w0) {
-                products(parity, 1, even);
-                finish(t * kTile + kTile, even);
-            }
-            write_k(parity ^ 1);
-            write_v(parity ^ 1);
             staged();
-        };
-        for (int t = t0; t < t1; t += 2) {
-            turn(t, 0);
-            if (t + 1 < t1) {
-                turn(t + 1, 1);
+            f32x16 even, odd;
+            if (t0 == w0) {
+                products(1, 1, even);
+                finish(t0 * kTile, even);
+            }
+            lds_barrier();  // before the first turn stages over these keys
+            auto turn = [&](int t, int parity) KDA_INLINE {
+                // past the last tile rows of zeros are loaded and staged, whose scores nobody uses
+                load_k(early ? next : now, parity ^ 1);
+                load_v(now, parity ^ 1);
+                now = next;
+                next = after;
+                after = walk();
+                if (t >= w0 && t < w1) {
+                    step(parity, 0, even, odd);
+                    finish(t * kTile + 32, odd);
+                    step(parity, 1, odd, even);
+                    finish(t * kTile + kTile, even);
+                } else if (t + 1 == w0) {
+                    products(parity, 1, even);
+                    finish(t * kTile + kTile, even);
+                }
+                write_k(parity ^ 1);
+                write_v(parity ^ 1);
+                finite_v(again, parity ^ 1);
+                staged();
+            };
+            for (int t = t0; t < t1; t += 2) {
+                turn(t, 0);
+                if (t + 1 < t1) {
+                    turn(t + 1, 1);
+                }
             }
         }
+    };
+    pass(std::false_type{});
+    bool fine = true;  // where a score is NaN the whole row is
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            fine &= is_finite(o[d][e]) || l != l;
+        }
+    }
+    if (!__syncthreads_and(fine)) {
+        pass(std::true_type{});
+        each_not_finite<D, FP8>(arguments_again(args).params, n, head, max(t0 * kTile, wsee0.x), min(t1 * kTile, wsee1.y), [&](int key, const char *row) KDA_INLINE {
+            if (key >= see.x && key < see.y) {
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        o[d][e] += not_finite<FP8>(row, d * 32 + 8 * (e >> 2) + 4 * half + (e & 3));
+                    }
+                }
+            }
+        });
     }
 
     // ---- out, or this split's part: lane: row `col` of 32, columns 32 d + 8 (e / 4) + 4 half + e % 4
-    const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
+    const PrefillArgs &last = arguments_again(args);
+    const float vs = last.params.cache.v_scale != nullptr ? last.params.cache.v_scale[head] : 1.0f;
     const int r = wave * 32 + col;
     const float sum = sum_halves(l);
     if (r >= rows) {
         return;
     }
-    if (splits == 1) {
+    if (last.splits == 1) {
         const float f = sum == 0.0f ? 0.0f : vs / sum;
-        const int t = (row0 + r) / a.group;
-        const int h = head * a.group + (row0 + r) - t * a.group;
-        uint16_t *out = static_cast<uint16_t *>(a.out) + static_cast<int64_t>(req.begin + t) * a.out_stride_token +
-                        h * a.out_stride_head + half * 4;
+        const int t = (row0 + r) / last.params.group;
+        const int h = head * last.params.group + (row0 + r) - t * last.params.group;
+        uint16_t *out = static_cast<uint16_t *>(last.params.out) + static_cast<int64_t>(req.begin + t) * last.params.out_stride_token +
+                        h * last.params.out_stride_head + half * 4;
         struct __attribute__((packed, aligned(2))) Out {
             uint32_t w[2];
         };
@@ -1158,14 +1339,14 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const Params a, co
             }
         }
     } else {
-        const int64_t all = static_cast<int64_t>(a.num_tokens) * a.group;
-        const int64_t at = (static_cast<int64_t>(split) * a.cache.kv_heads + head) * all +
-                           static_cast<int64_t>(req.begin) * a.group + row0 + r;
+        const int64_t all = static_cast<int64_t>(last.params.num_tokens) * last.params.group;
+        const int64_t at = (static_cast<int64_t>(split) * last.params.cache.kv_heads + head) * all +
+                           static_cast<int64_t>(req.begin) * last.params.group + row0 + r;
         if (half == 0) {
-            ws.ml[at] = make_float2(m, sum);
+            last.ws.ml[at] = make_float2(m, sum);
         }
         if (sum != 0.0f) {  // the join reads no others
-            float *po = ws.o + at * D + half * 4;
+            float *po = last.ws.o + at * D + half * 4;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
@@ -1280,7 +1461,7 @@ int check(const KdaPagedAttentionArgs *args) {
     }
     constexpr int32_t kWide = KDA_WIDE_PAGE_TABLE | KDA_WIDE_KV_LENS | KDA_WIDE_CU_SEQLENS;
     if (a.num_seqs < 0 || a.num_tokens < 0 || a.num_heads <= 0 || a.max_pages < 0 || a.window < 0 ||
-        !(a.logit_cap >= 0.0f) || (a.wide & ~kWide) != 0 || a.num_heads % a.cache.kv_heads != 0) {
+        !(a.logit_cap >= 0.0f) || a.num_heads > INT32_MAX / 128 || (a.wide & ~kWide) != 0 || a.num_heads % a.cache.kv_heads != 0) {
         return KDA_ERR_INVALID_ARGUMENT;
     }
     const int64_t group = a.num_heads / a.cache.kv_heads;
@@ -1313,13 +1494,13 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
     }
     const PrefillWs w{reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.ml_at)};
     const unsigned grid = static_cast<unsigned>(p.tiles * a.cache.kv_heads * p.splits);
-    const int tiles = static_cast<int>(p.tiles);
+    const PrefillArgs args{a, w, static_cast<int>(p.tiles), p.splits};
     // 16 rows of a page at offsets that fit 32 bits
     const auto near = [](int64_t stride) { return stride >= 0 && stride < (1 << 26); };
     if (a.cache.page_size % 16 == 0 && near(a.cache.k_stride_token) && near(a.cache.v_stride_token)) {
-        prefill_kernel<D, FP8, true><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
+        prefill_kernel<D, FP8, true><<<grid, kThreads, 0, s>>>(args);
     } else {
-        prefill_kernel<D, FP8, false><<<grid, kThreads, 0, s>>>(a, w, tiles, p.splits);
+        prefill_kernel<D, FP8, false><<<grid, kThreads, 0, s>>>(args);
     }
     if (p.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.num_heads;

@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "kda_abi.h"
 #include "kda_device.h"
 #include "paged_cache.h"
@@ -43,9 +45,11 @@ __device__ __forceinline__ uint2 to_fp8(const Bf16x8 &x, float inv) {
 
 // shift: 2^shift threads a token (its 16-byte chunks, rounded up to a power of
 // two, at most a workgroup); the rest of the workgroup takes further tokens.
-template <bool FP8> __global__ __launch_bounds__(kThreads) void paged_store_kernel(const KdaPagedStoreArgs a, int shift) {
+// first: the launch's first token.
+template <bool FP8>
+__global__ __launch_bounds__(kThreads) void paged_store_kernel(const KdaPagedStoreArgs a, int shift, int64_t first) {
     const KdaPagedCache &c = a.cache;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift);
+    const int64_t t = first + static_cast<int64_t>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift);
     if (t >= a.num_tokens) {
         return;
     }
@@ -107,13 +111,17 @@ extern "C" int kda_paged_store_launch(const KdaPagedStoreArgs *args, void *strea
         ++shift;
     }
     const int tokens = kThreads >> shift;
-    const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.num_tokens) + tokens - 1) / tokens);
     hipStream_t s = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    if (a.cache.dtype == KDA_FP8_E4M3) {
-        paged_store_kernel<true><<<grid, kThreads, 0, s>>>(a, shift);
-    } else {
-        paged_store_kernel<false><<<grid, kThreads, 0, s>>>(a, shift);
+    // a grid counts its threads in 32 bits
+    constexpr int64_t kMostGroups = (INT64_C(1) << 24) - 1;
+    for (int64_t first = 0; first < a.num_tokens; first += kMostGroups * tokens) {
+        const unsigned grid = static_cast<unsigned>(std::min((a.num_tokens - first + tokens - 1) / tokens, kMostGroups));
+        if (a.cache.dtype == KDA_FP8_E4M3) {
+            paged_store_kernel<true><<<grid, kThreads, 0, s>>>(a, shift, first);
+        } else {
+            paged_store_kernel<false><<<grid, kThreads, 0, s>>>(a, shift, first);
+        }
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }

@@ -462,7 +462,7 @@ template <class TX, class TO> __global__ __launch_bounds__(1024) void rms_norm_w
 
 // Chunks of V columns a thread, by the row's width: a row of up to 512 is one wave's, longer ones take
 // a workgroup of 256 (up to 8192) or 1024 threads.
-template <class TX, class TO> void launch(const KdaRmsNormArgs &a, hipStream_t stream) {
+template <class TX, class TO> void launch_rows(const KdaRmsNormArgs &a, hipStream_t stream) {
     constexpr int C = 8 / kVec<TX>;  // chunks in 8 columns
     const unsigned rows = static_cast<unsigned>(a.rows);
     if (a.width < 8) {
@@ -479,6 +479,24 @@ template <class TX, class TO> void launch(const KdaRmsNormArgs &a, hipStream_t s
         rms_norm_kernel<1024, 4 * C, TX, TO><<<rows, 1024, 0, stream>>>(a);
     } else {
         rms_norm_wide_kernel<TX, TO><<<rows, 1024, 0, stream>>>(a);
+    }
+}
+
+// A grid counts its threads in 32 bits: kMostRows rows of at most 1024 a launch.
+template <class TX, class TO> void launch(KdaRmsNormArgs a, hipStream_t stream) {
+    constexpr int64_t kMostRows = (INT64_C(1) << 22) - 1;
+    const int64_t scales = a.group == 0 ? 1 : (static_cast<int64_t>(a.width) + kGroup - 1) / kGroup;
+    for (int64_t left = a.rows; left > 0; left -= a.rows) {
+        a.rows = left < kMostRows ? left : kMostRows;
+        launch_rows<TX, TO>(a, stream);
+        a.x = static_cast<const TX *>(a.x) + a.rows * a.x_stride;
+        a.out = static_cast<TO *>(a.out) + a.rows * a.out_stride;
+        if (a.residual != nullptr) {
+            a.residual = static_cast<char *>(a.residual) + a.rows * a.residual_stride * (a.residual_dtype == KDA_F32 ? 4 : 2);
+        }
+        if (a.scale != nullptr) {
+            a.scale += a.rows * scales;
+        }
     }
 }
 

@@ -119,6 +119,23 @@ def test_norm_special_rows(ops, width):
         assert (scale[3] > 0).all() and torch.isfinite(out[3].float()).all()
 
 
+def test_norm_more_rows_than_a_launch_takes(ops):
+    rows = (1 << 22) + 5
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(rows, 4, device=DEV, generator=gen).bfloat16()
+    r = torch.randn(rows, 4, device=DEV, generator=gen)
+    w = torch.randn(4, device=DEV, generator=gen)
+    want, h = r.clone(), None
+    out = ops.add_rms_norm(x, w, EPS, residual=r)
+    h, y = C.norm_exact(x, w, EPS, want)
+    C.assert_within(out, y, y.abs() * (2.0 ** -8 * 1.01 + 4e-6), "out")
+    C.assert_within(r, h, h.abs() * 2.0 ** -24 * 1.01, "residual")
+    _, scale = ops.add_rms_norm_fp8(x, w, EPS)
+    _, y = C.norm_exact(x, w, EPS)
+    scales, _ = C.norm_scales(y, 0)
+    C.assert_within(scale, scales, scales * 4e-6, "scale")
+
+
 # ---------------------------------------------------------------------------
 # store
 # ---------------------------------------------------------------------------
@@ -183,6 +200,19 @@ def test_store_special_values_and_int64_slots(ops):
     assert row[0].isnan() and row[1:4].tolist() == [448.0, -448.0, 448.0] and (row[4:] == 0).all()
     cache[1, 1] = 1.0
     assert (cache.float() == 1).all()
+
+
+def test_store_more_tokens_than_a_launch_takes(ops):
+    tokens = (1 << 24) + 5
+    k = torch.randn(1, 1, 16, 128, device=DEV).bfloat16()
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device=DEV)
+    slots[0], slots[-7], slots[-1] = 3, 1, 0
+    cache = torch.zeros(2, 2, 16, 128, dtype=torch.bfloat16, device=DEV)
+    other = torch.zeros_like(cache)
+    ops.paged_kv_store(k.expand(1, tokens, 16, 128), (-k).expand(1, tokens, 16, 128), k_cache=cache, v_cache=other,
+                       slot_indices=slots)
+    for at, want in ((0, k[0, 0]), (1, k[0, 0]), (2, torch.zeros_like(k[0, 0])), (3, k[0, 0])):
+        assert torch.equal(cache.view(4, 16, 128)[at], want) and torch.equal(other.view(4, 16, 128)[at], -want)
 
 
 # ---------------------------------------------------------------------------
@@ -375,6 +405,64 @@ def test_attention_many_requests(ops):
     case = C.Attention(10, new, keys, 4, 2, 64, 16)
     _check_attention(ops, case)
     _check_attention(ops, case, max_query_len=1000)
+
+
+def test_attention_batches_padded_with_empty_requests(ops):
+    new = [0] * 70 + [1] + [0] * 3000 + [2, 1] + [0] * 129 + [1] + [0] * 900
+    keys = [m and 150 + 40 * m for m in new]
+    case = C.Attention(12, new, keys, 4, 2, 64, 16)
+    _check_attention(ops, case)
+    _check_attention(ops, case, max_query_len=1000)
+
+
+def test_attention_decreasing_offsets_address_nothing_outside(ops):
+    """Such metadata has no meaning, and its requests' units may pass 32 bits; a good call after it is right."""
+    case = C.Attention(13, [10, 20, 1], [40, 64, 30], 4, 2, 64, 16)
+    for hint in (1, 100):
+        kw = case.kwargs(DEV, max_query_len=hint)
+        kw["cu_seqlens"] = torch.tensor([0, 30, 10, 31], dtype=torch.int32, device=DEV)
+        assert ops.paged_attention(case.q.to(DEV), **kw).shape == case.q.shape
+        _check_attention(ops, case, max_query_len=hint)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("new,heads,hint", [([1, 3], 2, 3), ([8, 1], 4, 8), ([2, 150], 4, 150), ([400], 2, 400)])
+def test_attention_what_a_row_does_not_see_cannot_reach_it(ops, fp8, dim, window, new, heads, hint):
+    """Infinite and NaN keys and values of one token: rows that do not see it keep their bits, and of
+    those that do only its columns change."""
+    keys = [m + 333 for m in new]
+    case = C.Attention(14, new, keys, heads, 2, dim, 16, fp8=fp8, window=window)
+    clean = _check_attention(ops, case, max_query_len=hint).cpu()
+    G, n = heads // 2, max(range(len(new)), key=lambda i: new[i])
+    page, off = case.slots_of(n)
+    nan, inf = float("nan"), float("inf")
+    for back in {0, 1, new[n] // 2, new[n] - 1}:
+        j = keys[n] - 1 - back
+        sees = torch.zeros(case.q.shape[1], dtype=torch.bool)
+        start = int(case.cu_seqlens[n])
+        sees[start + new[n] - 1 - back:start + new[n]] = True
+        if window:
+            sees[start + new[n] - 1 - back + window:] = False
+        for which in ("v", "k"):
+            cache = case.v_cache if which == "v" else case.k_cache
+            held = cache[page[j], off[j], 1].clone()
+            bad = held.float()
+            if which == "v":
+                bad[3], bad[dim - 2] = nan, nan if fp8 else -inf
+            else:
+                bad[5] = nan
+            cache[page[j], off[j], 1] = bad.to(cache.dtype)
+            out = ops.paged_attention(case.q.to(DEV), **case.kwargs(DEV, max_query_len=hint)).cpu()
+            cache[page[j], off[j], 1] = held
+            hit = torch.zeros(out.shape, dtype=torch.bool)
+            if which == "v":
+                hit[:, sees, G:, 3] = hit[:, sees, G:, dim - 2] = True
+            else:
+                hit[:, sees, G:] = True
+            assert torch.equal(out[~hit], clean[~hit]), (which, back)
+            assert not torch.isfinite(out[hit]).any(), (which, back)
 
 
 def test_attention_nothing_to_do(ops):

@@ -11,11 +11,16 @@
 //
 // Bound by HBM: a row stays in registers between its one read and its one
 // write. A lane holds 16 bytes of the input at a time (8 or 4 columns), so 16 or 32
-// lanes hold a group of 128. Loads and stores are typed as unaligned vectors
-// (gfx950 serves them at any element address): rows of odd widths take the same
-// path, and only the last, partial chunk of a row goes element by element.
-// One row after another of an odd width costs little: 1001 x 5003 fp32 with
-// residual, see the table of kernels below.
+// lanes hold a group of 128, and all of a row's loads are issued before the
+// first is waited for. x and the residual are streamed (read or written once); the
+// weight and the output, which the next kernel reads, stay in the caches. Loads and
+// stores are typed as unaligned vectors (gfx950 serves them at any element
+// address), so rows of odd widths take the same path; the last, partial chunk of a row is loaded as the
+// row's last whole vector and moved down in registers, and stored element by element.
+//
+// Measured, residual read and written: 8192 x 8192 bf16 to 8 bits with a scale per 128
+// columns 77 us = 6.1 TB/s (reading alone reaches 6.1 to 6.4 on this card, a copy 4.9);
+// 1001 x 5003 fp32 16.5 us = 4.9 TB/s; one row 3 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -133,15 +138,15 @@ __device__ __forceinline__ void store1(uint8_t *p, float x) {
 struct Place {
     int col;    // may lie past the row's end
     int at;     // the load's first column
-    bool any;   // the wave has columns of the row in this chunk
+    bool any;   // the lanes that share the row in a wave have columns of it in this chunk
     bool tail;  // and some lane's end before its chunk does
 };
-template <int V> __device__ __forceinline__ Place place(int index, int wave_first, int width) {
+template <int V, int LANES> __device__ __forceinline__ Place place(int index, int wave_first, int width) {
     Place p;
     p.col = index * V;
     p.at = min(p.col, width - V);
     p.any = wave_first * V < width;
-    p.tail = (wave_first + 64) * V > width;
+    p.tail = (wave_first + LANES) * V > width;
     return p;
 }
 template <int V> __device__ __forceinline__ void move_down(const Place &p, float (&f)[V]) {
@@ -186,19 +191,21 @@ template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t x) {
     x = dpp_max<kDppRowMirror>(x);
     return LANES == 16 ? x : larger(x, __shfl_xor(x, 16));
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    x = group_max<32>(x);
-    return larger(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float wave_sum(float x) {
-    x = group_sum32(x);
-    return x + __shfl_xor(x, 32);
-}
 
-// Sum of squares and largest magnitude of a row, in all its threads.
-template <int WAVES> __device__ __forceinline__ void row_reduce(float &sum, uint32_t &top) {
-    sum = wave_sum(sum);
-    top = wave_max(top);
+// Sum of squares and largest magnitude of a row, in all its threads (16, 32, 64 or more).
+template <int THREADS> __device__ __forceinline__ void row_reduce(float &sum, uint32_t &top) {
+    constexpr int WAVES = THREADS / 64;
+    if constexpr (THREADS == 16) {
+        sum = group_sum16(sum);
+        top = group_max<16>(top);
+    } else {
+        sum = group_sum32(sum);
+        top = group_max<32>(top);
+    }
+    if constexpr (THREADS >= 64) {
+        sum += __shfl_xor(sum, 32);
+        top = larger(top, __shfl_xor(top, 32));
+    }
     if constexpr (WAVES > 1) {
         __shared__ float sums[WAVES];
         __shared__ uint32_t tops[WAVES];
@@ -264,7 +271,9 @@ __device__ __forceinline__ void finish(const KdaRmsNormArgs &a, int64_t row, int
 template <int V, int THREADS, int CHUNKS> struct Columns {
     __device__ __forceinline__ static Place at(int c, int width) {
         const int lane = threadIdx.x % THREADS;
-        return place<V>(c * THREADS + lane, c * THREADS + __builtin_amdgcn_readfirstlane(lane & ~63), width);
+        constexpr int kTogether = THREADS < 64 ? THREADS : 64;  // lanes of one row in a wave
+        const int first = THREADS <= 64 ? 0 : __builtin_amdgcn_readfirstlane(lane & ~63);
+        return place<V, kTogether>(c * THREADS + lane, c * THREADS + first, width);
     }
     // f(chunk, place, columns) for every chunk of an array that the wave has columns in; all loads first
     template <bool STREAM, class T, class F> __device__ __forceinline__ static void each(const T *row, int width, F f) {
@@ -298,7 +307,7 @@ template <int V, int THREADS, int CHUNKS> struct Columns {
     }
 };
 
-// THREADS threads a row (64: four rows a workgroup); width >= V.
+// THREADS threads a row (fewer than 256: several rows a workgroup); width >= V.
 template <int THREADS, int CHUNKS, class TX, class TO>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel(const KdaRmsNormArgs a) {
     constexpr int V = kVec<TX>;
@@ -306,7 +315,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
     constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / THREADS;
     if (row >= a.rows) {
-        return;  // whole waves: only rows of one wave share a workgroup
+        return;  // all threads of a row, and no barrier follows where rows share a workgroup
     }
     float h[CHUNKS][V];
     float sum = 0.0f;
@@ -367,7 +376,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
             }
         }
     });
-    row_reduce<THREADS / 64>(sum, top);
+    row_reduce<THREADS>(sum, top);
     const float rsqrt = 1.0f / sqrtf(sum / static_cast<float>(a.width) + a.eps);
     if (sizeof(TO) == 1 && a.group == 0 && threadIdx.x % THREADS == 0) {
         a.scale[row] = scale_of(top, rsqrt);
@@ -432,7 +441,7 @@ template <class TX, class TO> __global__ __launch_bounds__(1024) void rms_norm_w
             }
         }
     }
-    row_reduce<16>(sum, top);
+    row_reduce<1024>(sum, top);
     const float rsqrt = 1.0f / sqrtf(sum / static_cast<float>(a.width) + a.eps);
     if (sizeof(TO) == 1 && a.group == 0 && threadIdx.x == 0) {
         a.scale[row] = scale_of(top, rsqrt);
@@ -460,17 +469,30 @@ template <class TX, class TO> __global__ __launch_bounds__(1024) void rms_norm_w
     }
 }
 
-// Chunks of V columns a thread, by the row's width: a row of up to 512 is one wave's, longer ones take
-// a workgroup of 256 (up to 8192) or 1024 threads.
+// Threads a row, by its width: few enough that each has columns, more where a row would not fit their
+// registers. TB/s of 0.27 GB, bf16 with residual, and with the neighbouring choice:
+//   <= 128    16 lanes (fp32: 32)   262144 x 128   6.0   3.7 with 32 lanes
+//   <= 256    32 lanes (fp32: 64)   131072 x 256   6.0   3.5 with a wave
+//   <= 2048   a wave                32768 x 1024   6.25  4.8 with 256 threads;  16384 x 2048  6.25, 5.7
+//   <= 8192   256 threads           8192 x 4096    5.9   5.6 with a wave, 5.2 with 1024 threads
+//   <= 32768  1024 threads          2048 x 16384   5.6   4.6 read twice;        1024 x 32768  5.35, 4.1
 template <class TX, class TO> void launch_rows(const KdaRmsNormArgs &a, hipStream_t stream) {
     constexpr int C = 8 / kVec<TX>;  // chunks in 8 columns
     const unsigned rows = static_cast<unsigned>(a.rows);
     if (a.width < 8) {
         rms_norm_wide_kernel<TX, TO><<<rows, 1024, 0, stream>>>(a);
+    } else if (a.width <= 128) {
+        constexpr int kThreads = 128 / kVec<TX>, kRows = 256 / kThreads;
+        rms_norm_kernel<kThreads, 1, TX, TO><<<(rows + kRows - 1) / kRows, 256, 0, stream>>>(a);
+    } else if (a.width <= 256) {
+        constexpr int kThreads = 256 / kVec<TX>, kRows = 256 / kThreads;
+        rms_norm_kernel<kThreads, 1, TX, TO><<<(rows + kRows - 1) / kRows, 256, 0, stream>>>(a);
     } else if (a.width <= 512) {
         rms_norm_kernel<64, C, TX, TO><<<(rows + 3) / 4, 256, 0, stream>>>(a);
+    } else if (a.width <= 1024) {
+        rms_norm_kernel<64, 2 * C, TX, TO><<<(rows + 3) / 4, 256, 0, stream>>>(a);
     } else if (a.width <= 2048) {
-        rms_norm_kernel<256, C, TX, TO><<<rows, 256, 0, stream>>>(a);
+        rms_norm_kernel<64, 4 * C, TX, TO><<<(rows + 3) / 4, 256, 0, stream>>>(a);
     } else if (a.width <= 4096) {
         rms_norm_kernel<256, 2 * C, TX, TO><<<rows, 256, 0, stream>>>(a);
     } else if (a.width <= 8192) {

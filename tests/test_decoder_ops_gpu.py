@@ -119,6 +119,14 @@ def test_norm_special_rows(ops, width):
         assert (scale[3] > 0).all() and torch.isfinite(out[3].float()).all()
 
 
+@pytest.mark.parametrize("width", [9, 60, 128, 129, 200, 255, 256, 257, 500, 1023, 1024, 1025, 2047])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group", [None, 0, 128])
+def test_norm_rows_that_share_a_workgroup(ops, width, dtype, group):
+    x, r, w = _norm_inputs(37, width, dtype, torch.float32, torch.bfloat16, seed=width)
+    _check_norm(ops, x, r, w, group)
+
+
 def test_norm_more_rows_than_a_launch_takes(ops):
     rows = (1 << 22) + 5
     gen = torch.Generator(device=DEV).manual_seed(0)

@@ -19,8 +19,9 @@
 // score (its sign goes into q), the weights are 2^(c s - m). m is raised only when
 // a score passes it by 2^8: the weights then stay below 2^8, far inside fp32 and
 // bf16, and the accumulators are rescaled a few times a row instead of every
-// tile. Scores, m, the sums and O are fp32; the weights are rounded to bf16 for
-// the second product only (the sum takes them unrounded).
+// tile. Scores, m, the sums and O are fp32. The weights are rounded to bf16 for the
+// second product, and the sum takes them rounded too: numerator and denominator
+// then err alike, and a dot product sums two at a time.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -363,11 +364,19 @@ template <int D> __device__ __forceinline__ void zero_uncovered(const Params &a,
 // range is finished there; the parts of the others are joined by
 // decode_combine_kernel, always in the same order.
 //
-// The waves are independent within an item: each streams its own 32-key blocks,
-// the keys straight into the matrix operands' registers, the values through
-// registers into 32 rows of LDS. The next block's loads (16 KiB a wave in bf16
-// at D = 128) are in flight while one is computed, the page numbers one
-// block further ahead.
+// The waves are independent within an item: each streams its own 32-key blocks
+// through registers into 32 rows of keys and 32 of values in LDS, whole rows at a time and
+// past the caches (they are read once). The next block's loads (16 KiB a wave in
+// bf16 at D = 128) are in flight while one is computed, the page numbers one block
+// further ahead. Keys loaded straight into the operands' registers would skip LDS, but
+// a lane's 16 bytes of 16 different rows waste the memory's bursts: 64 ragged
+// requests of up to 32 K keys took 565 us so, 552 now.
+//
+// Bound by HBM: those 64 requests (64 heads on 8 key heads, D = 128) read 3.4 GB in
+// 552 us = 6.1 TB/s, what a kernel that only reads reaches. 256 requests in 8 bits:
+// 172 us = 5.5 TB/s, 7 us of it for joining parts. A single short request is bound by its
+// latencies: 9 us for the kernel (lengths, page numbers, keys, the waves' join one after another) and 4 to
+// 5 us for the second one.
 // ---------------------------------------------------------------------------
 
 constexpr int kUnit = 128;
@@ -782,11 +791,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
 }
 
 // Joins the items that began in a workgroup of decode_kernel and did not end there:
-// one workgroup each for every fourth row. Its threads take 4 columns each, and
+// gridDim.y workgroups each take every gridDim.y-th row. A workgroup's threads take 4 columns each, and
 // the rows and the parts are spread over what is left of them, so that a
 // thread's loads are few and in flight together (32 parts of 4 rows: 20.8 us with
 // a thread to all parts of a row, one after another).
-constexpr int kJoinRows = 4;
 
 template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const Params a, const DecodeWs ws) {
     constexpr int kRows = 16 * NB;
@@ -796,7 +804,8 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
     __shared__ float2 sum_ml[kThreads];
     const int w = blockIdx.x;
     const int4 desc = ws.desc[w];
-    const int rows = ((desc.z & 255) - static_cast<int>(blockIdx.y) + kJoinRows - 1) / kJoinRows;  // of this workgroup
+    const int step = gridDim.y;
+    const int rows = ((desc.z & 255) - static_cast<int>(blockIdx.y) + step - 1) / step;  // of this workgroup
     if (rows <= 0) {
         return;
     }
@@ -813,7 +822,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
     const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
     for (int first = 0; first < rows; first += kSlots / lanes) {
         const int i = first + slot / lanes;
-        const int r = min(i, rows - 1) * kJoinRows + blockIdx.y;
+        const int r = min(i, rows - 1) * step + blockIdx.y;
         float top = kNegInf, sum = 0.0f;
         f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int x = lane; x < parts; x += 4 * lanes) {
@@ -873,9 +882,21 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 //
 // A workgroup takes a tile of 128 rows of one (request, key head), 32 a
 // wave, and walks the visible keys in tiles of 64. The four waves share a key and
-// a value tile in LDS (bf16; 8-bit ones are widened when staged, once for all four),
-// two of each, so one barrier a tile is enough. The next tile's rows are loaded into
-// registers while this one is computed.
+// a value tile in LDS, two of each, so one barrier a tile is enough. While one is
+// computed the next one's rows go from memory straight into the other (8-bit ones through
+// registers, and widened once for all four waves).
+//
+// A wave's matrix instructions and its softmax take turns on the same SIMD, so the
+// loop is a chain of two stages: the scores of the next 32 keys are formed
+// between the instructions that turn this step's scores into weights. K's
+// buffer therefore runs 32 keys ahead of V's. Two workgroups a CU (64 KiB of LDS each at D = 128)
+// fill each other's waits.
+//
+// Bound by the matrix cores together with the softmax's vector instructions: 8192
+// tokens, 32 heads on 8, D = 128, causal: 550 us = 1.0 PFLOP/s (the skipped half
+// not counted). The library's bf16 product reaches 1.1 (4096 cubed) to 1.29 (8192); this
+// loop without its softmax and LDS reads 1.27, at the clock the card holds under such
+// load. Six chunks against up to 30 K keys: 925 us = 850 TFLOP/s.
 //
 // Tiles of rows are found from cu_seqlens alone: request n gets the numbers
 // from floor(cu[n] G / rows) + n, at least as many as it needs, so a tile's
@@ -1419,7 +1440,11 @@ int64_t most_rows(const KdaPagedAttentionArgs &a) {
     return std::max<int64_t>(a.max_query_len, 1) * (a.num_heads / a.cache.kv_heads);
 }
 
-// At most 32 rows a request (without requests, the decode kernel only writes the zeros).
+// At most 32 rows a request (without requests, the decode kernel only writes the zeros). 32 requests of 4096
+// keys, 32 heads on 4, D = 128, us:           rows   8   16   32   40   64
+//   decode kernel, tiles of 16 rows (NB = 1)        55   56   97  142  176
+//   decode kernel, tiles of 32 rows (NB = 2)        57   59   63  103  105
+//   prefill kernel                                  63   63   65   67   76
 bool decodes(const KdaPagedAttentionArgs &a) { return most_rows(a) <= 32 || a.num_seqs == 0; }
 
 Plan plan_of(const KdaPagedAttentionArgs &a) {
@@ -1439,8 +1464,9 @@ Plan plan_of(const KdaPagedAttentionArgs &a) {
         return p;
     }
     p.tiles = static_cast<int64_t>(a.num_tokens) * group / kTileRows + a.num_seqs;
-    // few tiles over many keys: cut the keys until two workgroups a CU have work, in
-    // parts of 512 keys at least
+    // few tiles over many keys: cut the keys until two workgroups a CU have work (512 tokens over 32 K keys:
+    // 325 us; 665 with one a CU, 339 with four), in parts of 512 keys at least (64 tokens over 8 K keys: 40 us;
+    // 47 with 256, 44 with 1024)
     const int64_t units = p.tiles * a.cache.kv_heads;
     p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2 * kCus / units, keys / 512, 64})));
     if (p.splits > 1) {
@@ -1483,7 +1509,13 @@ template <int D, bool FP8, int NB> void launch_decode(const Params &a, const Pla
                      reinterpret_cast<int4 *>(ws + p.desc_at)};
     decode_kernel<D, FP8, NB><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
     if (p.join) {
-        decode_combine_kernel<D, NB><<<dim3(kDecodeGroups, kJoinRows), kThreads, 0, s>>>(a, w);
+        // Few items are cut into many parts: more workgroups an item then (one request of 32 K keys and one
+        // key head: 26 us for 16 rows, 52 with 4 workgroups; 34 us for 32 rows, 95 with 4). Of many items most
+        // are whole, and the workgroups without one cost more than they give (256 requests in 8 bits: 172 us,
+        // 177 with 16).
+        const int64_t items = static_cast<int64_t>(a.num_seqs) * a.cache.kv_heads;
+        const unsigned joins = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(64 / std::max<int64_t>(items, 1), 4), 16 * NB));
+        decode_combine_kernel<D, NB><<<dim3(kDecodeGroups, joins), kThreads, 0, s>>>(a, w);
     }
 }
 
@@ -1495,7 +1527,8 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
     const PrefillWs w{reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.ml_at)};
     const unsigned grid = static_cast<unsigned>(p.tiles * a.cache.kv_heads * p.splits);
     const PrefillArgs args{a, w, static_cast<int>(p.tiles), p.splits};
-    // 16 rows of a page at offsets that fit 32 bits
+    // 16 rows of a page at offsets that fit 32 bits: one page number and one address for the wave's 16
+    // rows (8192 tokens 540 us, chunks over 30 K keys 925 us; each row's page looked up: 720 and 1342)
     const auto near = [](int64_t stride) { return stride >= 0 && stride < (1 << 26); };
     if (a.cache.page_size % 16 == 0 && near(a.cache.k_stride_token) && near(a.cache.v_stride_token)) {
         prefill_kernel<D, FP8, true><<<grid, kThreads, 0, s>>>(args);

@@ -415,6 +415,14 @@ def test_attention_many_requests(ops):
     _check_attention(ops, case, max_query_len=1000)
 
 
+@pytest.mark.parametrize("n", [16, 17, 128, 129])
+def test_attention_chunks_of_many_requests(ops, n):
+    rng = random.Random(n)
+    new = [rng.choice([0, 1, 20, 33, 64, 129]) for _ in range(n)]
+    case = C.Attention(15, new, [m and m + rng.choice([0, 0, 100, 300]) for m in new], 8, 2, 64, 16, before=1, after=2)
+    _check_attention(ops, case, max_query_len=129)
+
+
 def test_attention_batches_padded_with_empty_requests(ops):
     new = [0] * 70 + [1] + [0] * 3000 + [2, 1] + [0] * 129 + [1] + [0] * 900
     keys = [m and 150 + 40 * m for m in new]

@@ -27,6 +27,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "kda_abi.h"
@@ -911,6 +912,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 
 constexpr int kTile = 64;
 constexpr int kTileRows = 128;
+constexpr int kMinPart = 256;  // keys of a split, at least: the host knows the table's width only
 constexpr int kOrdered = 128;  // requests whose tiles go by length
 constexpr int kWaitMemory = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
 
@@ -1011,7 +1013,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     const int2 see0 = a.visible(req, row0 / a.group);
     const int2 see1 = a.visible(req, (row0 + rows - 1) / a.group);
     const int all0 = see0.x / kTile, all1 = (see1.y + kTile - 1) / kTile;
-    const int share = (all1 - all0 + splits - 1) / splits;
+    const int share = max((all1 - all0 + splits - 1) / splits, kMinPart / kTile);
     const int t0 = all0 + split * share, t1 = min(all1, t0 + share);
     const int wrow0 = min(row0 + wave * 32, row0 + rows - 1);
     const int wrow1 = min(wrow0 + 32, row0 + rows) - 1;
@@ -1422,8 +1424,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     }
 }
 
-// Joins the splits of every (token, head): 16 or 32 threads a row, 4 columns each.
-template <int D> __global__ __launch_bounds__(kThreads) void prefill_combine_kernel(const Params a, const PrefillWs ws, int splits) {
+// Joins the splits of every (token, head): 16 or 32 threads a row, 4 columns each. kAtOnce parts' loads
+// are in flight together: as many as there are, up to 8 (16 tokens over 30 K keys 77 us with one after
+// another, 58 with 4, 49 so; two splits of 1000 tokens 37 us, 43 with room for 8).
+template <int D, int kAtOnce>
+__global__ __launch_bounds__(kThreads) void prefill_combine_kernel(const Params a, const PrefillWs ws, int splits) {
     constexpr int kPer = D / 4;
     const int64_t all = static_cast<int64_t>(a.num_tokens) * a.group;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / kPer) + threadIdx.x / kPer;
@@ -1438,19 +1443,42 @@ template <int D> __global__ __launch_bounds__(kThreads) void prefill_combine_ker
     }
     const int c = threadIdx.x % kPer * 4;
     const int64_t step = a.cache.kv_heads * all, at = head * all + row;
+    // parts that saw no key (the table's width, not the request's keys, sets the number) have a sum of 0 and no O
     float top = kNegInf;
-    for (int s = 0; s < splits; ++s) {
-        const float2 ml = ws.ml[at + s * step];
-        top = ml.y == 0.0f ? top : fmaxf(top, ml.x);
+    for (int s = 0; s < splits; s += kAtOnce) {
+        float2 ml[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            ml[k] = ws.ml[at + min(s + k, splits - 1) * step];
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            top = ml[k].y == 0.0f ? top : fmaxf(top, ml[k].x);
+        }
     }
     float sum = 0.0f;
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; ++s) {
-        const float2 ml = ws.ml[at + s * step];
-        if (ml.y != 0.0f) {
-            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
-            sum += ml.y * f;
-            y += *reinterpret_cast<const f32x4 *>(ws.o + (at + s * step) * D + c) * f;
+    for (int s = 0; s < splits; s += kAtOnce) {
+        float2 ml[kAtOnce];
+        f32x4 o[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            ml[k] = ws.ml[at + min(s + k, splits - 1) * step];
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            o[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (s + k < splits && ml[k].y != 0.0f) {
+                o[k] = *reinterpret_cast<const f32x4 *>(ws.o + (at + (s + k) * step) * D + c);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (s + k < splits && ml[k].y != 0.0f) {
+                const float f = ml[k].x == top ? 1.0f : ex2(ml[k].x - top);
+                sum += ml[k].y * f;
+                y += o[k] * f;
+            }
         }
     }
     const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
@@ -1507,10 +1535,13 @@ Plan plan_of(const KdaPagedAttentionArgs &a) {
     }
     p.tiles = static_cast<int64_t>(a.num_tokens) * group / kTileRows + a.num_seqs;
     // few tiles over many keys: cut the keys until two workgroups a CU have work (512 tokens over 32 K keys:
-    // 325 us; 665 with one a CU, 339 with four), in parts of 512 keys at least (64 tokens over 8 K keys: 40 us;
-    // 47 with 256, 44 with 1024)
+    // 325 us; 665 with one a CU, 339 with four), in parts of 256 keys at least (64 tokens over 1008 keys 22 us,
+    // with 512 30 us). The join's time grows with the parts and the loop's falls with them, so the best number
+    // goes with the keys' root. 16 tokens over 30 K keys, us: 53 with at most 16 parts, 41 with 32, 50 with 64, 42 so;
+    // 64 tokens over 8 K: 31, 31, 35 and 31.
     const int64_t units = p.tiles * a.cache.kv_heads;
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2 * kCus / units, keys / 512, 64})));
+    const int64_t best = static_cast<int64_t>(std::sqrt(static_cast<double>(keys) / 32.0));
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2 * kCus / units, keys / 256, best})));
     if (p.splits > 1) {
         const size_t parts = static_cast<size_t>(p.splits) * a.num_tokens * a.num_heads;
         p.ml_at = up256(parts * d * 4);
@@ -1580,7 +1611,14 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
     if (p.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.num_heads;
         constexpr int kPer = kThreads / (D / 4);
-        prefill_combine_kernel<D><<<static_cast<unsigned>((rows + kPer - 1) / kPer), kThreads, 0, s>>>(a, w, p.splits);
+        const unsigned groups = static_cast<unsigned>((rows + kPer - 1) / kPer);
+        if (p.splits == 2) {
+            prefill_combine_kernel<D, 2><<<groups, kThreads, 0, s>>>(a, w, p.splits);
+        } else if (p.splits <= 4) {
+            prefill_combine_kernel<D, 4><<<groups, kThreads, 0, s>>>(a, w, p.splits);
+        } else {
+            prefill_combine_kernel<D, 8><<<groups, kThreads, 0, s>>>(a, w, p.splits);
+        }
     }
 }
 

@@ -236,7 +236,8 @@ at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const
     TORCH_CHECK(N < INT32_MAX && page_table.size(1) <= INT32_MAX && max_query_len >= 0 && max_query_len <= INT32_MAX, op,
                 " supports at most 2^31-1 requests, pages and new tokens of a request");
     TORCH_CHECK(window >= 0 && window <= INT32_MAX, op, ": window must be 0 (all keys) or a number of keys, got ", window);
-    TORCH_CHECK(logit_cap >= 0, op, ": logit_cap must be 0 (none) or positive, got ", logit_cap);
+    TORCH_CHECK(logit_cap == 0 || (logit_cap >= 1e-30 && logit_cap <= 1e30), op,
+                ": logit_cap must be 0 (none) or within 1e-30 and 1e30, got ", logit_cap);
     check_on_gpu("q", q);
     const c10::DeviceGuard device_guard(q.device());
     at::Tensor out = at::empty(q.sizes(), q.options());

@@ -173,10 +173,14 @@ __device__ __forceinline__ float sum_groups(float x) {
     return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// cap tanh(s / cap) in log2 units; x = 2 log2(e) s / cap. tanh = 1 - 2 / (e^(2s/cap) + 1):
-// infinities give +-1, NaN stays; the error is an ulp of the cap, absolute.
+// cap tanh(s / cap) in log2 units; x = 2 log2(e) s / cap, cap2 = cap log2(e). tanh = 1 - 2 / (e^(2s/cap) + 1):
+// infinities give +-1, NaN stays. Its error is an ulp of the cap, too much where the cap is far above the
+// scores: below a tenth of it the series t - t^3/3 + 2t^5/15, whose next term is under 6e-8 of it. (3% of a
+// capped verify step's time; a branch for large caps only would cost every prefill 3%.)
 __device__ __forceinline__ float capped(float x, float cap2) {
-    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(ex2(x) + 1.0f);
+    const float t = x * (0.5f / kLog2e), t2 = t * t;
+    const float low = cap2 * t * (1.0f - t2 * (1.0f / 3.0f - t2 * (2.0f / 15.0f)));
+    return t2 < 0.01f ? low : cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(ex2(x) + 1.0f);
 }
 
 // Rows of zeros that stand for keys outside a request or pages outside the pool.
@@ -251,7 +255,7 @@ __device__ __forceinline__ Scores scores_of(const Params &a, int head) {
     const float mag = fabsf(f) < 1e-30f ? 1e-30f : fabsf(f);
     s.c = mag * kLog2e;
     s.cap = a.logit_cap * kLog2e;
-    s.in = a.logit_cap > 0.0f ? 2.0f * kLog2e * mag / a.logit_cap : 0.0f;
+    s.in = a.logit_cap > 0.0f ? fminf(2.0f * kLog2e * mag / a.logit_cap, 3e38f) : 0.0f;  // a score of 0 stays 0
     return s;
 }
 
@@ -1560,7 +1564,7 @@ int check(const KdaPagedAttentionArgs *args) {
     }
     constexpr int32_t kWide = KDA_WIDE_PAGE_TABLE | KDA_WIDE_KV_LENS | KDA_WIDE_CU_SEQLENS;
     if (a.num_seqs < 0 || a.num_tokens < 0 || a.num_heads <= 0 || a.max_pages < 0 || a.window < 0 ||
-        !(a.logit_cap >= 0.0f) || a.num_heads > INT32_MAX / 128 || (a.wide & ~kWide) != 0 || a.num_heads % a.cache.kv_heads != 0) {
+        !(a.logit_cap == 0.0f || (a.logit_cap >= 0.9e-30f && a.logit_cap <= 1.1e30f)) || a.num_heads > INT32_MAX / 128 || (a.wide & ~kWide) != 0 || a.num_heads % a.cache.kv_heads != 0) {
         return KDA_ERR_INVALID_ARGUMENT;
     }
     const int64_t group = a.num_heads / a.cache.kv_heads;

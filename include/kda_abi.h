@@ -360,7 +360,7 @@ typedef struct KdaPagedAttentionArgs {
     const void *kv_lens;    /* [num_seqs] */
     const void *cu_seqlens; /* [num_seqs + 1], non-decreasing */
     float scale;
-    float logit_cap; /* 0: none */
+    float logit_cap; /* 0: none, else 1e-30 to 1e30 */
     int32_t window;  /* 0: none */
     int32_t wide;    /* which of the three are int64: KDA_WIDE_PAGE_TABLE, _KV_LENS, _CU_SEQLENS */
     int32_t num_seqs;

@@ -289,6 +289,48 @@ def test_attention_cap(ops, cap, new):
     _check_attention(ops, C.Attention(3, new, [400, 150], 8, 2, 128, 16, cap=cap, spread=20.0))
 
 
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e30])
+@pytest.mark.parametrize("new", [[1, 1], [90, 20]])
+def test_attention_cap_far_above_the_scores(ops, cap, new):
+    """There the capped scores are the scores (off by s^3 / 3 cap^2 < 1e-6 here) and no accuracy is lost."""
+    case = C.Attention(3, new, [n + 100 for n in new], 4, 2, 64, 16, cap=cap)
+    out = ops.paged_attention(case.q.to(DEV), **case.kwargs(DEV))
+    case.cap = 0.0
+    want, bound = case.exact()
+    C.assert_within(out, want, bound, "out")
+
+
+@pytest.mark.parametrize("cap", [4.0, 200.0])
+@pytest.mark.parametrize("hint", [1, 100])
+def test_attention_cap_on_both_sides_of_the_series(ops, cap, hint):
+    """Scores of up to four times the cap: the series, its end at a tenth, and saturation, in one request."""
+    case = C.Attention(5, [2, 40], [70, 90], 4, 2, 64, 16, cap=cap, spread=cap)
+    _check_attention(ops, case, max_query_len=hint)
+
+
+@pytest.mark.parametrize("cap", [1e-30, 1e-3])
+@pytest.mark.parametrize("hint", [1, 100])
+def test_attention_cap_far_below_the_scores(ops, cap, hint):
+    case = C.Attention(4, [1, 40], [50, 90], 4, 2, 64, 16, cap=cap)
+    case.q[0, 0] = 0  # scores of 0
+    _check_attention(ops, case, max_query_len=hint)
+
+
+@pytest.mark.parametrize("hint", [1, 100])
+@pytest.mark.parametrize("page", [16, 5])
+def test_attention_wide_tables_of_few_keys(ops, hint, page):
+    """Entries past a request's pages are any numbers; the table's width cuts the keys in many parts."""
+    case = C.Attention(16, [1, 60, 3], [70, 2000, 3], 8, 2, 64, page)
+    wide = torch.full((3, 9000), -7, dtype=torch.int32)
+    wide[:, ::3] = 1 << 30
+    wide[:, 1::3] = torch.tensor(case.unused[0], dtype=torch.int32)
+    for n, k in enumerate(case.keys):
+        used = -(-k // page)
+        wide[n, :used] = case.page_table[n, :used]
+    case.page_table = wide
+    _check_attention(ops, case, max_query_len=hint)
+
+
 @pytest.mark.parametrize("scale", [-0.125, 0.0, 3.0])
 @pytest.mark.parametrize("new", [[1, 2], [90, 20]])
 def test_attention_scales(ops, scale, new):

@@ -121,6 +121,8 @@ def test_cache_refusals(match, change):
     ("window must be", dict(window=-1)),
     ("logit_cap must be", dict(logit_cap=-1.0)),
     ("logit_cap must be", dict(logit_cap=float("nan"))),
+    ("logit_cap must be", dict(logit_cap=float("inf"))),
+    ("logit_cap must be", dict(logit_cap=1e-40)),
     ("at most 2\\^31-1", dict(max_query_len=-1)),
 ])
 def test_attention_refusals(match, over):

@@ -379,9 +379,9 @@ template <int D> __device__ __forceinline__ void zero_uncovered(const Params &a,
 //
 // Bound by HBM: those 64 requests (64 heads on 8 key heads, D = 128) read 3.4 GB in
 // 552 us = 6.1 TB/s, what a kernel that only reads reaches. 256 requests in 8 bits:
-// 172 us = 5.5 TB/s, 7 us of it for joining parts. A single short request is bound by its
-// latencies: 9 us for the kernel (lengths, page numbers, keys, the waves' join one after another) and 4 to
-// 5 us for the second one.
+// 167 us = 5.65 TB/s, 5 us of it for joining parts. A single short request is bound by its
+// latencies: 9 to 10 us for the kernel (lengths, page numbers, keys, the waves' join one after another) and
+// 4 us for the second one.
 // ---------------------------------------------------------------------------
 
 constexpr int kUnit = 128;
@@ -901,7 +901,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 // tokens, 32 heads on 8, D = 128, causal: 550 us = 1.0 PFLOP/s (the skipped half
 // not counted). The library's bf16 product reaches 1.1 (4096 cubed) to 1.29 (8192); this
 // loop without its softmax and LDS reads 1.27, at the clock the card holds under such
-// load. Six chunks against up to 30 K keys: 925 us = 850 TFLOP/s.
+// load. Six chunks against up to 30 K keys: 845 us = 930 TFLOP/s.
 //
 // Every workgroup finds its tile itself, from the lengths on the device. The longest
 // request's tiles go first, its last ones (the longest, under the causal mask) before the

@@ -48,6 +48,30 @@ int64_t row_stride(const char *op, const char *name, const at::Tensor &t) {
     return stride.value_or(t.size(-1));
 }
 
+// The same of x, whose rows may lie in groups at a second stride.
+void x_strides(const char *op, const at::Tensor &x, KdaRmsNormArgs &a) {
+    TORCH_CHECK(x.size(-1) <= 1 || x.stride(-1) == 1, op, ": x must be contiguous in its last dimension");
+    int64_t size[2] = {1, 1}, stride[2] = {x.size(-1), 0};
+    int levels = 0;
+    for (int64_t d = x.dim() - 2; d >= 0 && x.numel() > 0; --d) {
+        if (x.size(d) == 1) {
+            continue;
+        }
+        if (levels > 0 && x.stride(d) == stride[levels - 1] * size[levels - 1]) {
+            size[levels - 1] *= x.size(d);
+            continue;
+        }
+        TORCH_CHECK(levels < 2, op, ": x must have rows at one stride, or groups of rows at two, got strides ", x.strides());
+        size[levels] = x.size(d);
+        stride[levels] = x.stride(d);
+        ++levels;
+    }
+    TORCH_CHECK(levels < 2 || size[0] < (1 << 22), op, " supports fewer than 2^22 rows in a group");
+    a.x_stride = stride[0];
+    a.x_inner = levels < 2 ? 0 : static_cast<int32_t>(size[0]);
+    a.x_outer_stride = stride[1];
+}
+
 KdaRmsNormArgs norm_args(const char *op, const at::Tensor &x, const at::Tensor &weight, double eps,
                          const std::optional<at::Tensor> &residual) {
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, op, " expects x as [..., width]");
@@ -63,7 +87,7 @@ KdaRmsNormArgs norm_args(const char *op, const at::Tensor &x, const at::Tensor &
     KdaRmsNormArgs a{};
     a.x = x.data_ptr();
     a.weight = weight.data_ptr();
-    a.x_stride = row_stride(op, "x", x);
+    x_strides(op, x, a);
     a.out_stride = width;
     a.rows = rows;
     a.width = static_cast<int32_t>(width);

@@ -19,8 +19,8 @@
 // row's last whole vector and moved down in registers, and stored element by element.
 //
 // Measured, residual read and written: 8192 x 8192 bf16 to 8 bits with a scale per 128
-// columns 77 us = 6.1 TB/s (reading alone reaches 6.1 to 6.4 on this card, a copy 4.9);
-// 1001 x 5003 fp32 16.5 us = 4.9 TB/s; one row 3 us.
+// columns 75 us = 6.3 TB/s (reading alone reaches 6.1 to 6.4 on this card, a copy 4.9);
+// 1001 x 5003 fp32 16 us = 5.0 TB/s; one row 3 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -64,6 +64,15 @@ template <class A, bool STREAM, class T, class R> __device__ __forceinline__ voi
     } else {
         *reinterpret_cast<typename A::T *>(p) = r;
     }
+}
+
+// A row's first element in x; rows of a launch are counted in 32 bits.
+__device__ __forceinline__ int64_t x_at(const KdaRmsNormArgs &a, int64_t row) {
+    if (a.x_inner > 1) {
+        const uint32_t r = static_cast<uint32_t>(row), outer = r / static_cast<uint32_t>(a.x_inner);
+        return outer * a.x_outer_stride + static_cast<int64_t>(r - outer * a.x_inner) * a.x_stride;
+    }
+    return row * a.x_stride;
 }
 
 // Columns a lane holds at a time: 16 bytes of the input, so that the lanes of a load are neighbours.
@@ -327,7 +336,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
             h[c][i] = 0.0f;
         }
     }
-    const TX *x = static_cast<const TX *>(a.x) + row * a.x_stride;
+    const TX *x = static_cast<const TX *>(a.x) + x_at(a, row);
     Raw<TX, V> raw[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
@@ -417,7 +426,7 @@ template <class TX, class TO> __global__ __launch_bounds__(1024) void rms_norm_w
         }
     };
     const auto sum_of = [&](int col, int n, float (&h)[V]) {
-        columns(a.x, a.x_dtype, row * a.x_stride + col, n, h);
+        columns(a.x, a.x_dtype, x_at(a, row) + col, n, h);
         if (a.residual != nullptr) {
             float r[V];
             columns(a.residual, a.residual_dtype, row * a.residual_stride + col, n, r);
@@ -504,14 +513,15 @@ template <class TX, class TO> void launch_rows(const KdaRmsNormArgs &a, hipStrea
     }
 }
 
-// A grid counts its threads in 32 bits: kMostRows rows of at most 1024 a launch.
+// A grid counts its threads in 32 bits: kMostRows rows of at most 1024 a launch (whole groups of x_inner).
+constexpr int64_t kMostRows = (INT64_C(1) << 22) - 1;
 template <class TX, class TO> void launch(KdaRmsNormArgs a, hipStream_t stream) {
-    constexpr int64_t kMostRows = (INT64_C(1) << 22) - 1;
+    const int64_t inner = a.x_inner > 1 ? a.x_inner : 1, most = kMostRows / inner * inner;
     const int64_t scales = a.group == 0 ? 1 : (static_cast<int64_t>(a.width) + kGroup - 1) / kGroup;
     for (int64_t left = a.rows; left > 0; left -= a.rows) {
-        a.rows = left < kMostRows ? left : kMostRows;
+        a.rows = left < most ? left : most;
         launch_rows<TX, TO>(a, stream);
-        a.x = static_cast<const TX *>(a.x) + a.rows * a.x_stride;
+        a.x = static_cast<const TX *>(a.x) + (inner > 1 ? a.rows / inner * a.x_outer_stride : a.rows * a.x_stride);
         a.out = static_cast<TO *>(a.out) + a.rows * a.out_stride;
         if (a.residual != nullptr) {
             a.residual = static_cast<char *>(a.residual) + a.rows * a.residual_stride * (a.residual_dtype == KDA_F32 ? 4 : 2);
@@ -539,6 +549,12 @@ extern "C" int kda_rms_norm_launch(const KdaRmsNormArgs *args, void *stream) {
     if (!is_float(a.x_dtype) || !is_float(a.weight_dtype) || (a.residual != nullptr && !is_float(a.residual_dtype)) ||
         (!fp8 && (a.out_dtype != a.x_dtype || a.group != 0)) || (a.group != 0 && a.group != kGroup)) {
         return KDA_ERR_UNSUPPORTED;
+    }
+    if (a.x_inner > kMostRows) {
+        return KDA_ERR_TOO_LARGE;
+    }
+    if (a.x_inner < 0 || (a.x_inner > 1 && a.rows % a.x_inner != 0)) {
+        return KDA_ERR_INVALID_ARGUMENT;
     }
     if (a.rows == 0) {
         return KDA_OK;

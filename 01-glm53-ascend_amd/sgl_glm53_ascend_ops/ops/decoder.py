@@ -27,8 +27,9 @@ def add_rms_norm(
 ) -> torch.Tensor:
     """``h = x + residual``, normed: ``h * weight / sqrt(mean(h^2) + eps)`` in x's dtype.
 
-    ``x`` is ``[..., width]`` in bf16 or fp32 with rows at one stride; ``weight``
-    and ``residual`` may each be bf16 or fp32. ``residual`` (None: ``h = x``) is
+    ``x`` is ``[..., width]`` in bf16 or fp32 with rows at one stride, or at two (the
+    heads of a fused projection, ``qkv[:, :, :heads]``); ``weight`` and ``residual``
+    (rows at one stride) may each be bf16 or fp32. ``residual`` (None: ``h = x``) is
     updated in place to ``h``; the norm reads ``h`` in fp32, before that rounding.
     """
     return _OPS.add_rms_norm(x, weight, eps, residual=residual)

@@ -148,8 +148,8 @@ class HybridDecoder:
             qkv = ops.add_rms_norm(x, layer["norm"], EPS, residual=residual) @ layer["first"]
         qkv = qkv.view(1, T, H + 2 * KH, D)
         q, k, v = qkv[:, :, :H], qkv[:, :, H:H + KH], qkv[:, :, H + KH:]
-        k = ops.add_rms_norm(k.contiguous(), layer["head_norm"], EPS)
-        q = ops.add_rms_norm(q.contiguous(), layer["head_norm"], EPS)
+        k = ops.add_rms_norm(k, layer["head_norm"], EPS)  # slices as they are
+        q = ops.add_rms_norm(q, layer["head_norm"], EPS)
         ops.paged_kv_store(k, v, k_cache=layer["k_cache"], v_cache=layer["v_cache"], slot_indices=step.slots,
                            **layer["scales"])
         out = ops.paged_attention(

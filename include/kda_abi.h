@@ -294,6 +294,10 @@ typedef struct KdaRmsNormArgs {
     int32_t weight_dtype;
     int32_t out_dtype; /* x_dtype, or KDA_FP8_E4M3 */
     int32_t group;     /* columns of a scale: 0 (the row) or 128 */
+    /* x only: x_inner > 1 rows at x_stride, then the next ones x_outer_stride further (the heads of a
+     * fused projection); rows is a multiple of x_inner, at most 2^22 - 1. Else x_stride holds for all. */
+    int32_t x_inner;
+    int64_t x_outer_stride;
 } KdaRmsNormArgs;
 
 /* Pointers need their element's alignment only; rows of out and of the residual

@@ -127,6 +127,33 @@ def test_norm_rows_that_share_a_workgroup(ops, width, dtype, group):
     _check_norm(ops, x, r, w, group)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group", [None, 128])
+@pytest.mark.parametrize("tokens,heads,width", [(1, 3, 128), (19, 5, 128), (33, 2, 200), (7, 3, 5), (3, 2, 40000)])
+def test_norm_heads_of_a_fused_projection(ops, tokens, heads, width, dtype, group):
+    x, r, w = _norm_inputs(tokens * heads, width, dtype, torch.float32, torch.float32, seed=heads)
+    x, r = x.view(1, tokens, heads, width), r.view(1, tokens, heads, width)
+    fused = torch.randn(1, tokens, heads + 3, width + 1, device=DEV).to(dtype)
+    part = fused[:, :, 1:heads + 1, :width]
+    part.copy_(x)
+    _check_norm(ops, x, r, w, group, x_dev=part)
+
+
+def test_norm_broadcast_groups(ops):
+    x, _, w = _norm_inputs(4, 64, torch.bfloat16, None, torch.bfloat16)
+    _check_norm(ops, x.view(4, 1, 64).expand(4, 3, 64), None, w, None, x_dev=x.to(DEV).view(4, 1, 64).expand(4, 3, 64))
+    _check_norm(ops, x.view(1, 4, 64).expand(3, 4, 64), None, w, None, x_dev=x.to(DEV).view(1, 4, 64).expand(3, 4, 64))
+
+
+def test_norm_groups_over_several_launches(ops):
+    heads = 5
+    tokens = ((1 << 22) + 40) // heads
+    fused = torch.randn(tokens, heads + 1, 4, device=DEV).bfloat16()
+    x, w = fused[:, :heads], torch.randn(4, device=DEV)
+    _, y = C.norm_exact(x, w, EPS)
+    C.assert_within(ops.add_rms_norm(x, w, EPS), y, y.abs() * (2.0 ** -8 * 1.01 + 4e-6), "out")
+
+
 def test_norm_more_rows_than_a_launch_takes(ops):
     rows = (1 << 22) + 5
     gen = torch.Generator(device=DEV).manual_seed(0)

@@ -47,8 +47,9 @@ def test_norm_refusals():
         _refused("contiguous weight of the width", call, x, torch.ones(32)[::2], 1e-6)
         _refused("expects x as", call, torch.zeros(4, 0), torch.ones(0), 1e-6)
         _refused("contiguous in its last dimension", call, torch.zeros(16, 4).t(), w, 1e-6)
-        _refused("rows at one stride", call, torch.zeros(2, 3, 2, 16)[:, :2], w, 1e-6)
-        _refused("rows at one stride", call, torch.zeros(2, 1, 16).expand(2, 3, 16), w, 1e-6)
+        _refused("rows at one stride", call, torch.zeros(2, 3, 3, 2, 16)[:, :2, :2, :1], w, 1e-6)
+        _refused("rows at one stride", call, torch.zeros(2, 2, 16), w, 1e-6, residual=torch.zeros(2, 3, 16)[:, :2])
+        _refused("rows at one stride", call, torch.zeros(2, 3, 16), w, 1e-6, residual=torch.zeros(2, 1, 16).expand(2, 3, 16))
         _refused("residual in x's shape", call, x, w, 1e-6, residual=torch.zeros(3, 16))
         _refused("residual must be bf16 or fp32", call, x, w, 1e-6, residual=x.half())
         _refused("must not overlap", call, x, w, 1e-6, residual=torch.zeros(1, 16).expand(4, 16))
@@ -143,7 +144,8 @@ P, I64, I32, F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
 class NormArgs(ctypes.Structure):
     _fields_ = [("x", P), ("residual", P), ("weight", P), ("out", P), ("scale", P), ("x_stride", I64),
                 ("residual_stride", I64), ("out_stride", I64), ("rows", I64), ("width", I32), ("eps", F),
-                ("x_dtype", I32), ("residual_dtype", I32), ("weight_dtype", I32), ("out_dtype", I32), ("group", I32)]
+                ("x_dtype", I32), ("residual_dtype", I32), ("weight_dtype", I32), ("out_dtype", I32), ("group", I32),
+                ("x_inner", I32), ("x_outer_stride", I64)]
 
 
 class Cache(ctypes.Structure):

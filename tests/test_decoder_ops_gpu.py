@@ -515,9 +515,19 @@ def test_attention_decreasing_offsets_address_nothing_outside(ops):
 @pytest.mark.parametrize("window", [0, 70])
 @pytest.mark.parametrize("new,heads,hint", [([1, 3], 2, 3), ([8, 1], 4, 8), ([2, 150], 4, 150), ([400], 2, 400)])
 def test_attention_what_a_row_does_not_see_cannot_reach_it(ops, fp8, dim, window, new, heads, hint):
+    _check_isolation(ops, fp8, dim, window, new, heads, hint, 333)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("window", [0, 700])
+def test_attention_what_a_row_does_not_see_cannot_reach_it_over_splits(ops, fp8, window):
+    _check_isolation(ops, fp8, 128, window, [70], 4, 70, 2500)
+
+
+def _check_isolation(ops, fp8, dim, window, new, heads, hint, earlier):
     """Infinite and NaN keys and values of one token: rows that do not see it keep their bits, and of
     those that do only its columns change."""
-    keys = [m + 333 for m in new]
+    keys = [m + earlier for m in new]
     case = C.Attention(14, new, keys, heads, 2, dim, 16, fp8=fp8, window=window)
     clean = _check_attention(ops, case, max_query_len=hint).cpu()
     G, n = heads // 2, max(range(len(new)), key=lambda i: new[i])
@@ -611,3 +621,26 @@ def test_streams_and_graph_replay(ops):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("new,keys", [([70], [2570]), ([60, 1, 33], [60, 400, 200])])
+def test_prefill_graph_replay(ops, new, keys):
+    """Chunks, with their keys in parts and whole, captured and replayed on changed inputs and lengths."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    case = C.Attention(17, new, keys, 8, 2, 128, 16)
+    kw = case.kwargs(DEV)
+    q = case.q.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.paged_attention(q, **kw)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops.paged_attention(q, **kw)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device=DEV, generator=gen))
+        kw["kv_lens"].sub_(3)
+        graph.replay()
+        assert torch.equal(captured, ops.paged_attention(q, **kw)), i
+        torch.cuda.synchronize()

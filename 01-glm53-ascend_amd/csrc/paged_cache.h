@@ -17,7 +17,7 @@ inline int check_cache(const KdaPagedCache &c) {
     if (c.dtype != KDA_BF16 && c.dtype != KDA_FP8_E4M3) {
         return KDA_ERR_UNSUPPORTED;
     }
-    // kv_heads: a head's number times its row, and the grid's second dimension, stay in range
+    // kv_heads: a head's number times its row stays in range
     if (c.kv_heads <= 0 || c.kv_heads > 65535 || c.page_size <= 0 || c.num_pages < 0 ||
         c.num_pages > INT32_MAX / c.page_size) {
         return KDA_ERR_INVALID_ARGUMENT;

@@ -4,7 +4,7 @@
 // key head's row and the same 16 of its value, so two loads are in flight before
 // either store; a token's threads are neighbours, so its rows are read and
 // written in whole cache lines whatever its slot is. 8192 tokens of 8 heads of 128 to
-// 8 bits: 10 us for 50 MB, half of it written to scattered rows (a plain copy of as much takes 10.2 us);
+// 8 bits: 11 to 12 us for 50 MB, a third of it written to scattered rows (a plain copy of as much takes 10.2 us);
 // 256 tokens: 3 us, the time of an empty launch.
 
 #include <hip/hip_runtime.h>

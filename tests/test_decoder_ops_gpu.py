@@ -560,6 +560,34 @@ def _check_isolation(ops, fp8, dim, window, new, heads, hint, earlier):
             assert not torch.isfinite(out[hit]).any(), (which, back)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,heads,requests,earlier,hint", [
+    (4, 4, 300, 300, 4),     # decode, 16-row tiles: more units than workgroups, so that a wave has several blocks
+    (4, 16, 300, 300, 4),    # 32-row tiles
+    (40, 4, 2, 333, 40),     # prefill
+    (70, 4, 1, 2500, 70)])   # prefill over split keys
+def test_attention_rows_keep_their_bits_beside_large_hidden_scores(ops, fp8, dim, new, heads, requests, earlier, hint):
+    """The last key, which only the last token sees, gets a score far above the running maximum there: the other
+    rows of the tile keep theirs, and so their weights' roundings."""
+    L = new + earlier
+    case = C.Attention(18, [new] * requests, [L] * requests, heads, 2, dim, 16, fp8=fp8)
+    q, kw = case.q.to(DEV), case.kwargs(DEV, max_query_len=hint)
+    clean = ops.paged_attention(q, **kw)
+    ends = case.cu_seqlens[1:].long() - 1
+    page = torch.tensor([int(case.page_table[n, (L - 1) // 16]) for n in range(requests)], device=DEV)
+    loud = q[0, ends.to(DEV)][:, [0, heads // 2]].float() * 4  # each key head's first query head, times 4
+    if fp8:
+        loud = (loud / kw["k_scale"][:, None]).clamp(-448, 448)
+    kw["k_cache"].view(torch.uint8 if fp8 else torch.int16)[page, (L - 1) % 16] = \
+        loud.to(kw["k_cache"].dtype).view(torch.uint8 if fp8 else torch.int16)
+    out = ops.paged_attention(q, **kw)
+    sees = torch.zeros(q.shape[1], dtype=torch.bool, device=DEV)
+    sees[ends.to(DEV)] = True
+    assert torch.equal(out[0, ~sees], clean[0, ~sees])
+    assert (out[0, sees][:, [0, heads // 2]] != clean[0, sees][:, [0, heads // 2]]).any(-1).all()
+
+
 def test_attention_nothing_to_do(ops):
     case = C.Attention(1, [0, 0], [5, 0], 4, 2, 64, 16)
     assert ops.paged_attention(case.q.to(DEV), **case.kwargs(DEV)).shape == (1, 0, 4, 64)

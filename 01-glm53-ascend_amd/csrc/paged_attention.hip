@@ -1558,17 +1558,17 @@ Plan plan_of(const KdaPagedAttentionArgs &a) {
     return p;
 }
 
-int check(const KdaPagedAttentionArgs *args) {
+// What the plan and the workspace follow from; no pointer, stride or option of the softmax.
+int check_sizes(const KdaPagedAttentionArgs *args) {
     if (args == nullptr) {
         return KDA_ERR_INVALID_ARGUMENT;
     }
     const KdaPagedAttentionArgs &a = *args;
-    if (const int rc = check_cache(a.cache); rc != KDA_OK) {
+    if (const int rc = check_cache_sizes(a.cache); rc != KDA_OK) {
         return rc;
     }
-    constexpr int32_t kWide = KDA_WIDE_PAGE_TABLE | KDA_WIDE_KV_LENS | KDA_WIDE_CU_SEQLENS;
-    if (a.num_seqs < 0 || a.num_tokens < 0 || a.num_heads <= 0 || a.max_pages < 0 || a.window < 0 ||
-        !(a.logit_cap == 0.0f || (a.logit_cap >= 0.9e-30f && a.logit_cap <= 1.1e30f)) || a.num_heads > INT32_MAX / 128 || (a.wide & ~kWide) != 0 || a.num_heads % a.cache.kv_heads != 0) {
+    if (a.num_seqs < 0 || a.num_tokens < 0 || a.num_heads <= 0 || a.max_pages < 0 || a.num_heads > INT32_MAX / 128 ||
+        a.num_heads % a.cache.kv_heads != 0) {
         return KDA_ERR_INVALID_ARGUMENT;
     }
     const int64_t group = a.num_heads / a.cache.kv_heads;
@@ -1579,6 +1579,22 @@ int check(const KdaPagedAttentionArgs *args) {
     }
     if (decodes(a) && (rows / 16 + a.num_seqs) * a.cache.kv_heads > INT32_MAX / (keys / kUnit + 1)) {
         return KDA_ERR_TOO_LARGE;
+    }
+    return KDA_OK;
+}
+
+int check(const KdaPagedAttentionArgs *args) {
+    if (const int rc = check_sizes(args); rc != KDA_OK) {
+        return rc;
+    }
+    const KdaPagedAttentionArgs &a = *args;
+    if (const int rc = check_cache(a.cache); rc != KDA_OK) {
+        return rc;
+    }
+    constexpr int32_t kWide = KDA_WIDE_PAGE_TABLE | KDA_WIDE_KV_LENS | KDA_WIDE_CU_SEQLENS;
+    if (a.window < 0 || !(a.logit_cap == 0.0f || (a.logit_cap >= 0.9e-30f && a.logit_cap <= 1.1e30f)) ||
+        (a.wide & ~kWide) != 0) {
+        return KDA_ERR_INVALID_ARGUMENT;
     }
     return KDA_OK;
 }
@@ -1635,7 +1651,7 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
 
 extern "C" size_t kda_paged_attention_workspace_bytes(const KdaPagedAttentionArgs *args) {
     using namespace kda;
-    if (check(args) != KDA_OK || args->num_tokens == 0) {
+    if (check_sizes(args) != KDA_OK || args->num_tokens == 0) {
         return 0;
     }
     return plan_of(*args).bytes;

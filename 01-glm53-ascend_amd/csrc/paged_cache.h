@@ -8,9 +8,9 @@
 
 namespace kda {
 
-// Shapes, strides and alignment that the kernels assume. An empty pool
-// (num_pages = 0) is valid: nothing is addressed in it.
-inline int check_cache(const KdaPagedCache &c) {
+// Types and sizes that the kernels assume. An empty pool (num_pages = 0) is valid: nothing is
+// addressed in it.
+inline int check_cache_sizes(const KdaPagedCache &c) {
     if (c.head_dim != 64 && c.head_dim != 128) {
         return KDA_ERR_UNSUPPORTED;
     }
@@ -21,6 +21,14 @@ inline int check_cache(const KdaPagedCache &c) {
     if (c.kv_heads <= 0 || c.kv_heads > 65535 || c.page_size <= 0 || c.num_pages < 0 ||
         c.num_pages > INT32_MAX / c.page_size) {
         return KDA_ERR_INVALID_ARGUMENT;
+    }
+    return KDA_OK;
+}
+
+// The same, and the pointers, strides and alignment.
+inline int check_cache(const KdaPagedCache &c) {
+    if (const int rc = check_cache_sizes(c); rc != KDA_OK) {
+        return rc;
     }
     if (c.num_pages == 0) {
         return KDA_OK;

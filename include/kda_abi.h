@@ -376,7 +376,8 @@ typedef struct KdaPagedAttentionArgs {
 } KdaPagedAttentionArgs;
 
 /* Bytes of device scratch that kda_paged_attention_launch needs for these sizes
- * (host-only; the pointers, strides and contents do not matter). */
+ * (host-only; the pointers, strides and contents do not matter). 0 where it needs
+ * none, and for sizes that the launch refuses. */
 size_t kda_paged_attention_workspace_bytes(const KdaPagedAttentionArgs *args);
 
 /* `workspace`: 256-byte aligned device memory of the bytes above (null if 0), no

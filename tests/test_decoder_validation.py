@@ -255,3 +255,22 @@ def test_attention_launch_refusals(lib):
     assert need > 0
     for ws, size in ((None, need), (BASE, need - 1), (BASE + 128, need)):
         assert lib.kda_paged_attention_launch(args(), ws, size, None) == WORKSPACE
+
+
+@pytest.mark.parametrize("max_query_len,num_tokens", [(1, 7), (300, 300)])
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_attention_workspace_follows_from_the_sizes_alone(lib, max_query_len, num_tokens, dtype):
+    """The query may come before there is anything to point at."""
+    sizes = dict(num_seqs=7, num_tokens=num_tokens, num_heads=4, max_pages=640, max_query_len=max_query_len)
+    pool = dict(num_pages=999, page_size=16, kv_heads=2, head_dim=64, dtype=dtype)
+    bare = lib.kda_paged_attention_workspace_bytes(ctypes.byref(AttentionArgs(cache=Cache(**pool), **sizes)))
+    full = AttentionArgs(q=BASE, out=BASE, page_table=BASE, kv_lens=BASE, cu_seqlens=BASE, window=5, logit_cap=2.0, wide=48,
+                         cache=_cache(**pool), **sizes)
+    assert bare == lib.kda_paged_attention_workspace_bytes(ctypes.byref(full)) > 0
+    odd = AttentionArgs(q=BASE + 1, window=-1, logit_cap=-1.0, wide=1,
+                        cache=_cache(k=BASE + 1, v=None, k_stride_token=3, v_stride_page=1, k_scale=1, **pool), **sizes)
+    assert bare == lib.kda_paged_attention_workspace_bytes(ctypes.byref(odd))
+    assert lib.kda_paged_attention_launch(ctypes.byref(odd), BASE, bare, None) == INVALID
+    for wrong in (dict(num_heads=5), dict(num_tokens=0), dict(num_seqs=-1)):
+        args = AttentionArgs(cache=Cache(**pool), **dict(sizes, **wrong))
+        assert lib.kda_paged_attention_workspace_bytes(ctypes.byref(args)) == 0

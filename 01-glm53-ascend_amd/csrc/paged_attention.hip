@@ -58,6 +58,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
+typedef const __attribute__((address_space(1))) int global_int;
 
 struct __attribute__((packed, aligned(2))) Bf16x8Any {
     u32x4 w;
@@ -185,6 +186,8 @@ __device__ __forceinline__ float capped(float x, float cap2) {
     return t2 < 0.01f ? low : cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(ex2(x) + 1.0f);
 }
 
+constexpr int kDppQuadEven = 0xA0, kDppQuadOdd = 0xF5;  // quad_perm [0,0,2,2] and [1,1,3,3]
+
 // Rows of zeros that stand for keys outside a request or pages outside the pool.
 __device__ const u32x4 g_zero_row[16] = {};
 
@@ -194,40 +197,59 @@ struct Request {
     int keys;    // keys in the cache, the new tokens' among them
 };
 
+struct PageWords {
+    const char *row;
+    uint32_t step;  // bytes
+    __device__ __forceinline__ int of(int at) const {
+        return *(global_int *)(row + static_cast<uint64_t>(static_cast<uint32_t>(at)) * step);
+    }
+};
+// The page of an entry of these words: any number, which callers compare with the pool. -1 for one beyond 32 bits.
+__device__ __forceinline__ int page_of(int first, int last) { return last != 0 ? -1 : first; }
+
 struct Params : KdaPagedAttentionArgs {
     int group;  // query heads a key head
 
-    __device__ __forceinline__ int meta(const void *p, int64_t i, int bit) const {
-        // the low word of an int64 entry is what a conversion to int32 keeps
-        const int shift = (wide & bit) != 0 ? 1 : 0;
-        return static_cast<const int32_t *>(p)[i << shift];
+    // Token ranges and lengths cut to the tensors, whatever the metadata says: int64 entries as they are, not
+    // their low words.
+    __device__ __forceinline__ int cut(const void *p, int64_t i, int bit, int most) const {
+        if ((wide & bit) == 0) {
+            return min(max(static_cast<const int32_t *>(p)[i], 0), most);
+        }
+        return static_cast<int>(min(max(static_cast<const int64_t *>(p)[i], INT64_C(0)), static_cast<int64_t>(most)));
     }
-    // Token ranges and lengths cut to the tensors, whatever the metadata says.
-    __device__ __forceinline__ int cu(int n) const {
-        return min(max(meta(cu_seqlens, n, KDA_WIDE_CU_SEQLENS), 0), num_tokens);
-    }
+    __device__ __forceinline__ int cu(int n) const { return cut(cu_seqlens, n, KDA_WIDE_CU_SEQLENS, num_tokens); }
     __device__ __forceinline__ Request request(int n) const {
-        Request r;
-        r.begin = cu(n);
-        r.tokens = max(cu(n + 1) - r.begin, 0);
-        r.keys = min(max(meta(kv_lens, n, KDA_WIDE_KV_LENS), 0), max_pages * cache.page_size);
-        return r;
+        const int keys = max_pages * cache.page_size;
+        if ((wide & (KDA_WIDE_CU_SEQLENS | KDA_WIDE_KV_LENS)) == 0) {  // one branch for three loads in flight together
+            const int32_t *c = static_cast<const int32_t *>(cu_seqlens) + n;
+            const int begin = min(max(c[0], 0), num_tokens), end = min(max(c[1], 0), num_tokens);
+            return Request{begin, max(end - begin, 0), min(max(static_cast<const int32_t *>(kv_lens)[n], 0), keys)};
+        }
+        const int begin = cu(n);
+        return Request{begin, max(cu(n + 1) - begin, 0), cut(kv_lens, n, KDA_WIDE_KV_LENS, keys)};
     }
     // Keys visible to the i-th new token: [x, y)
     __device__ __forceinline__ int2 visible(const Request &r, int i) const {
         const int end = max(r.keys - r.tokens + i + 1, 0);
         return make_int2(window > 0 ? max(end - window, 0) : 0, end);
     }
-    // Page of key j of request n, or -1 (a page outside the pool).
-    __device__ __forceinline__ int page_of(int n, int at) const {
-        return meta(page_table, n * page_table_stride + at, KDA_WIDE_PAGE_TABLE);
+    // Request n's page table as a lane reads it: the entries' first words, or (`last`) the second ones of int64
+    // entries, 0 for int32 ones. Looked up ahead by lanes that share an entry, one word each: one register a
+    // lane, nothing waits for the load, and page_of puts them together.
+    __device__ __forceinline__ PageWords page_words(int n, bool last) const {
+        const bool both = (wide & KDA_WIDE_PAGE_TABLE) != 0;
+        const char *row = static_cast<const char *>(page_table) + ((n * page_table_stride) << (both ? 3 : 2));
+        return PageWords{last && !both ? reinterpret_cast<const char *>(g_zero_row) : row + (last ? 4 : 0),
+                         both ? 8u : last ? 0u : 4u};
     }
     // The row of values of one of request n's keys, null on a page outside the pool.
     template <bool FP8> __device__ __forceinline__ const char *value_row(int n, int head, int key) const {
-        const int page = page_of(n, key / cache.page_size);
-        const int64_t at = page * cache.v_stride_page + key % cache.page_size * cache.v_stride_token + head * cache.v_stride_head;
+        const int at = key / cache.page_size;
+        const int page = page_of(page_words(n, false).of(at), page_words(n, true).of(at));
+        const int64_t offset = page * cache.v_stride_page + key % cache.page_size * cache.v_stride_token + head * cache.v_stride_head;
         return static_cast<uint32_t>(page) < static_cast<uint32_t>(cache.num_pages)
-                   ? static_cast<const char *>(cache.v) + (FP8 ? at : 2 * at)
+                   ? static_cast<const char *>(cache.v) + (FP8 ? offset : 2 * offset)
                    : nullptr;
     }
 };
@@ -541,15 +563,21 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         const char *kbase = static_cast<const char *>(a.cache.k) + ((head * a.cache.k_stride_head) << R::kShift);
         const char *vbase = static_cast<const char *>(a.cache.v) + ((head * a.cache.v_stride_head) << R::kShift);
         auto lookup = [&](int i) KDA_INLINE -> int {  // page of key lane % 32 of block i; any entry where it has none
+            int lane = static_cast<int>(__lane_id());
+            if constexpr (NB > 1) {  // as in compute: the entry's word in no register of its own
+                asm volatile("" : "+v"(lane));
+            }
             const int key = key0 + i * kUnit + (lane & 31);
-            return a.page_of(n, min(max(key, 0) / a.cache.page_size, a.max_pages - 1));
+            return a.page_words(n, lane >= 32).of(min(max(key, 0) / a.cache.page_size, a.max_pages - 1));
         };
         // keys of a block that every row of the tile sees: [seen0, seen1)
         const int seen0 = max(lo, last.x), seen1 = min(hi, first.y);
         struct Rows {
             unsigned long long k, v;  // the rows of key lane % 32 of a block
         };
-        auto rows_of = [&](int i, int page) KDA_INLINE -> Rows {
+        auto rows_of = [&](int i, int word) KDA_INLINE -> Rows {
+            const u32x2 words = __builtin_amdgcn_permlane32_swap(word, word, false, false);
+            const int page = page_of(words[0], words[1]);
             const int key = key0 + i * kUnit + (lane & 31);
             const int off = key - key / a.cache.page_size * a.cache.page_size;
             const bool real = key >= lo && key < hi && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.cache.num_pages);
@@ -679,11 +707,11 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
             if (blocks > 0) {
                 // past the last block rows of zeros are loaded
                 Rows rows = rows_of(0, lookup(0));
-                int page = lookup(1);
+                int word = lookup(1);
                 load(rows);
                 for (int i = 0; i < blocks; ++i) {
-                    rows = rows_of(i + 1, page);
-                    page = lookup(i + 2);
+                    rows = rows_of(i + 1, word);
+                    word = lookup(i + 2);
                     compute(i, rows);
                 }
             }
@@ -1052,13 +1080,14 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     const char *zero = reinterpret_cast<const char *>(g_zero_row);
     const int srow = lane / R::kLanes, schunk = lane % R::kLanes;  // of a load; kRows of Row further for each next
     const int pool = static_cast<int>(a.cache.num_pages);
-    // A group's page numbers: of the lane's own rows, or, where pages hold a multiple of 16 tokens
+    // A group's page entries: of the lane's own rows, or, where pages hold a multiple of 16 tokens
     // (UNIFORM), of all 16 rows. Those are walked without divisions.
     struct Group {
         int key;                       // its first
-        int page[UNIFORM ? 1 : kLoads];
+        int page[UNIFORM ? 1 : kLoads];  // as looked up: the entry's first word in even lanes, its last in odd ones
         int64_t koff, voff;  // UNIFORM: bytes of its first row on the page
     };
+    const PageWords words = a.page_words(n, (lane & 1) != 0);
     Group ahead;  // the walk's next
     int at = 0, off = 0;
     const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
@@ -1074,7 +1103,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     auto walk = [&]() KDA_INLINE -> Group {
         Group r = ahead;
         if constexpr (UNIFORM) {
-            r.page[0] = a.page_of(n, min(at, a.max_pages - 1));
+            r.page[0] = words.of(min(at, a.max_pages - 1));
             at += step_at;
             off += step_off;
             int wrap = 0;
@@ -1088,10 +1117,21 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                r.page[i] = a.page_of(n, min((r.key + srow + i * R::kRows) / a.cache.page_size, a.max_pages - 1));
+                r.page[i] = words.of(min((r.key + srow + i * R::kRows) / a.cache.page_size, a.max_pages - 1));
             }
         }
         ahead.key += kTile;
+        return r;
+    };
+    // The entries have come: their pages, in every lane. (UNIFORM: when they are used, by scalar instructions.)
+    auto looked_up = [&](Group r) KDA_INLINE -> Group {
+        if constexpr (!UNIFORM) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                r.page[i] = page_of(__builtin_amdgcn_update_dpp(0, r.page[i], kDppQuadEven, 0xf, 0xf, false),
+                                    __builtin_amdgcn_update_dpp(0, r.page[i], kDppQuadOdd, 0xf, 0xf, false));
+            }
+        }
         return r;
     };
     // A lane's bytes of a group. bf16 rows go from memory into LDS directly, where a wave's 64 x 16
@@ -1111,7 +1151,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     auto load = [&](const Group &group, const char *base, int64_t page_bytes, int64_t in_page, int64_t token_bytes,
                     const uint32_t (&row)[kLoads], auto column, auto &reg, char *rows_at) KDA_INLINE {
         if constexpr (UNIFORM) {
-            const int page = __builtin_amdgcn_readfirstlane(group.page[0]);
+            const int page = page_of(__builtin_amdgcn_readlane(group.page[0], 0), __builtin_amdgcn_readlane(group.page[0], 1));
             const int key = group.key;
             const bool any = static_cast<uint32_t>(page) < static_cast<uint32_t>(pool) && key < see1.y && key + 16 > see0.x;
             uint32_t lane_at[kLoads];
@@ -1312,6 +1352,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
             // scores are formed before, from the second half of the other buffer.
             begin_walk();
             Group now = walk(), next = walk(), after = walk();
+            now = looked_up(now);
+            next = looked_up(next);
             const bool early = wave < 2;  // K's next rows are of the group after V's next rows
             if (early) {
                 load_k(now, 1);
@@ -1323,7 +1365,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
             write_v(0);
             finite_v(again, 0);
             now = next;
-            next = after;
+            next = looked_up(after);
             after = walk();
             staged();
             f32x16 even, odd;
@@ -1337,7 +1379,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 load_k(early ? next : now, parity ^ 1);
                 load_v(now, parity ^ 1);
                 now = next;
-                next = after;
+                next = looked_up(after);
                 after = walk();
                 if (t >= w0 && t < w1) {
                     step(parity, 0, even, odd);

@@ -353,7 +353,8 @@ int kda_paged_store_launch(const KdaPagedStoreArgs *args, void *stream);
  * Scores, softmax and sums are fp32; the weights are rounded to bf16 for the
  * product with the values. A page outside [0, num_pages) reads as zero keys and
  * values (nothing outside the pool is addressed); kv_lens beyond the table are cut
- * to it; tokens that no request covers get 0. */
+ * to it, cu_seqlens to the tokens; tokens that no request covers get 0. int64
+ * entries count whole: one beyond 32 bits is outside, not its low word. */
 typedef struct KdaPagedAttentionArgs {
     const void *q; /* [tokens, num_heads, head_dim] bf16, head_dim contiguous */
     void *out;     /* the same shape, bf16 */

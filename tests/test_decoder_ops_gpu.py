@@ -433,6 +433,33 @@ def test_attention_metadata_is_cut_to_the_tensors(ops):
 
 @pytest.mark.parametrize("hint", [1, 100])
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("page", [16, 5])
+def test_attention_int64_entries_beyond_32_bits(ops, hint, fp8, page):
+    """They are outside the pool, the table or the batch, as they are for the store: not their low words."""
+    case = C.Attention(19, [2, 40], [90, 100], 4, 2, 64, page, fp8=fp8, index64=True)
+    case.page_table[0, 1] += 1 << 32
+    case.page_table[0, 3] -= 1 << 32
+    case.page_table[1, 0] = (1 << 63) - 1
+    case.page_table[1, 2] += 1 << 62
+    kw = case.kwargs(DEV, max_query_len=hint)
+    exact = C.Attention(19, [2, 40], [90, 100], 4, 2, 64, page, fp8=fp8, index64=True)
+    for n, at in ((0, 1), (0, 3), (1, 0), (1, 2)):
+        exact.page_table[n, at] = -1
+    want, bound = exact.exact()
+    C.assert_within(ops.paged_attention(case.q.to(DEV), **kw), want, bound, "pages")
+
+    case = C.Attention(20, [1, 30], [64, 100], 4, 2, 64, page, fp8=fp8, index64=True)
+    kw = case.kwargs(DEV, max_query_len=hint)
+    kw["page_table"] = kw["page_table"][:, :80 // page].contiguous()
+    kw["kv_lens"] = torch.tensor([-(1 << 32) + 9, (1 << 32) + 9], device=DEV)
+    kw["cu_seqlens"] = torch.tensor([-(1 << 40) + 1, 1, (1 << 33) + 2], device=DEV)
+    case.keys = [0, 80]
+    want, bound = case.exact()
+    C.assert_within(ops.paged_attention(case.q.to(DEV), **kw), want, bound, "lengths and offsets")
+
+
+@pytest.mark.parametrize("hint", [1, 100])
+@pytest.mark.parametrize("fp8", [False, True])
 def test_attention_strides(ops, hint, fp8):
     """q a misaligned slice of a fused projection; keys and values interleaved in one allocation, heads outermost."""
     case = C.Attention(8, [1, 40], [77, 90], 6, 2, 64, 16, fp8=fp8)

@@ -91,18 +91,18 @@ template <int N> __device__ __forceinline__ void load16_to_lds(const char *from,
             "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072"
             :
             : "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(from)
-            : "memory");
+            : "m0", "memory");
     } else {
         asm volatile(
             "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024"
             :
             : "s"(lds), "v"(at[0]), "v"(at[1]), "s"(from)
-            : "memory");
+            : "m0", "memory");
     }
 }
 __device__ __forceinline__ void load16_to_lds(const char *from, char *to) {
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "m0", "memory");
 }
 
 // sum + both bf16 of a pair, in fp32

@@ -7,6 +7,8 @@ dereferenced).
 """
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -274,3 +276,20 @@ def test_attention_workspace_follows_from_the_sizes_alone(lib, max_query_len, nu
     for wrong in (dict(num_heads=5), dict(num_tokens=0), dict(num_seqs=-1)):
         args = AttentionArgs(cache=Cache(**pool), **dict(sizes, **wrong))
         assert lib.kda_paged_attention_workspace_bytes(ctypes.byref(args)) == 0
+
+
+# ---------------------------------------------------------------------------
+# kernel sources
+# ---------------------------------------------------------------------------
+
+def test_asm_that_writes_m0_says_so():
+    """A register that an asm statement writes and does not name is one the compiler may keep a value in across it."""
+    csrc = Path(__file__).resolve().parent.parent / "01-glm53-ascend_amd" / "csrc"
+    found = 0
+    for source in sorted(csrc.glob("*.h*")):
+        for statement in re.findall(r"\basm\b[^;]*?\((.*?)\);", source.read_text(), re.S):
+            if re.search(r"\bs_mov_b32 m0\b", statement):
+                found += 1
+                clobbers = statement.rsplit(":", 1)[1]
+                assert '"m0"' in clobbers and '"memory"' in clobbers, (source.name, statement)
+    assert found > 0

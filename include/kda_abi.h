@@ -65,7 +65,8 @@ typedef enum KdaStatus {
     KDA_ERR_UNSUPPORTED = 2,      /* a shape / dtype / mode with no kernel */
     KDA_ERR_LAUNCH = 3,           /* the HIP runtime refused the launch */
     KDA_ERR_WORKSPACE = 4,        /* workspace missing or too small */
-    KDA_ERR_TOO_LARGE = 5         /* needs more scratch than kda_chunk_launch_noalloc holds */
+    KDA_ERR_TOO_LARGE = 5         /* more rows, keys or workgroups than the call counts, or more scratch
+                                   * than kda_chunk_launch_noalloc holds */
 } KdaStatus;
 
 typedef enum KdaDType {

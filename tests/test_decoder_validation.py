@@ -278,6 +278,14 @@ def test_attention_workspace_follows_from_the_sizes_alone(lib, max_query_len, nu
         assert lib.kda_paged_attention_workspace_bytes(ctypes.byref(args)) == 0
 
 
+def test_too_large_names_every_reason(lib):
+    """The norms and the attention refuse sizes past their counts with the status that the static buffer has."""
+    lib.kda_status_string.restype = ctypes.c_char_p
+    text = lib.kda_status_string(TOO_LARGE)
+    for reason in (b"sizes", b"rows", b"keys", b"workgroups", b"kda_chunk_launch_noalloc"):
+        assert reason in text, text
+
+
 # ---------------------------------------------------------------------------
 # kernel sources
 # ---------------------------------------------------------------------------

@@ -36,7 +36,7 @@ int64_t row_stride(const char *op, const char *name, const at::Tensor &t) {
     TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, op, ": ", name, " must be contiguous in its last dimension");
     std::optional<int64_t> stride;  // of a row
     int64_t next = 0;               // stride of the next outer dimension
-    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    for (int64_t d = t.dim() - 2; d >= 0 && t.numel() > 0; --d) {
         if (t.size(d) == 1) {
             continue;
         }

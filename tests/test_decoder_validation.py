@@ -58,6 +58,15 @@ def test_norm_refusals():
     _refused("group_size 0", add_rms_norm_fp8, x, w, 1e-6, group_size=64)
 
 
+@pytest.mark.parametrize("shape", [(2, 0, 64), (0, 3, 64), (0, 64), (3, 2, 0, 64)])
+def test_norm_takes_an_empty_residual(shape):
+    """No rows, whatever strides torch gives their dimensions: the call gets as far as the device check."""
+    x, w = torch.zeros(shape), torch.ones(64)
+    for call in (add_rms_norm, add_rms_norm_fp8):
+        _refused("must be a CUDA", call, x, w, 1e-6)
+        _refused("must be a CUDA", call, x, w, 1e-6, residual=x.clone())
+
+
 def _store(**over):
     a = dict(k=torch.zeros(1, 3, 2, 64, dtype=BF16), v=torch.zeros(1, 3, 2, 64, dtype=BF16),
              k_cache=torch.zeros(4, 8, 2, 64, dtype=BF16), v_cache=torch.zeros(4, 8, 2, 64, dtype=BF16),

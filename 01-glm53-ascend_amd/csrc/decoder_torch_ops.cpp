@@ -143,6 +143,9 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm_fp8(const at::Tensor &x, const a
 // paged_kv_store, paged_attention
 // ---------------------------------------------------------------------------
 
+// The stride of a dimension, 0 where it has a single entry (torch leaves such strides at any number).
+int64_t stride_of(const at::Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 KdaPagedCache cache_of(const char *op, const char *of, const at::Tensor &x, const at::Tensor &k_cache,
                        const at::Tensor &v_cache, const std::optional<at::Tensor> &k_scale,
                        const std::optional<at::Tensor> &v_scale) {
@@ -161,8 +164,8 @@ KdaPagedCache cache_of(const char *op, const char *of, const at::Tensor &x, cons
         const at::Tensor &t = named.second;
         check_device_of(x, of, named.first, t);
         TORCH_CHECK(t.stride(3) == 1, op, ": ", named.first, " must be contiguous in D");
-        TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % unit == 0 &&
-                        t.stride(1) % unit == 0 && t.stride(2) % unit == 0,
+        TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && stride_of(t, 0) % unit == 0 &&
+                        stride_of(t, 1) % unit == 0 && stride_of(t, 2) % unit == 0,
                     op, ": rows of ", named.first, " must be 16-byte aligned");
     }
     for (const auto &named : {std::pair<const char *, const std::optional<at::Tensor> &>{"k_scale", k_scale},
@@ -178,12 +181,12 @@ KdaPagedCache cache_of(const char *op, const char *of, const at::Tensor &x, cons
     KdaPagedCache c{};
     c.k = k_cache.data_ptr();
     c.v = v_cache.data_ptr();
-    c.k_stride_page = k_cache.stride(0);
-    c.k_stride_token = k_cache.stride(1);
-    c.k_stride_head = k_cache.stride(2);
-    c.v_stride_page = v_cache.stride(0);
-    c.v_stride_token = v_cache.stride(1);
-    c.v_stride_head = v_cache.stride(2);
+    c.k_stride_page = stride_of(k_cache, 0);
+    c.k_stride_token = stride_of(k_cache, 1);
+    c.k_stride_head = stride_of(k_cache, 2);
+    c.v_stride_page = stride_of(v_cache, 0);
+    c.v_stride_token = stride_of(v_cache, 1);
+    c.v_stride_head = stride_of(v_cache, 2);
     c.k_scale = k_scale.has_value() ? k_scale->data_ptr<float>() : nullptr;
     c.v_scale = v_scale.has_value() ? v_scale->data_ptr<float>() : nullptr;
     c.num_pages = k_cache.size(0);

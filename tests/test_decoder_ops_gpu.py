@@ -482,6 +482,18 @@ def test_attention_strides(ops, hint, fp8):
 
 
 @pytest.mark.parametrize("hint", [1, 100])
+def test_attention_single_head_at_any_stride(ops, hint):
+    case = C.Attention(21, [1, 40], [40, 64], 4, 1, 64, 16)
+    kw = case.kwargs(DEV, max_query_len=hint)
+    for name in ("k_cache", "v_cache"):
+        t = kw[name]
+        kw[name] = t.as_strided(t.shape, (t.stride(0), t.stride(1), 3, 1))
+        assert torch.equal(kw[name], t)
+    want, bound = case.exact()
+    C.assert_within(ops.paged_attention(case.q.to(DEV), **kw), want, bound, "out")
+
+
+@pytest.mark.parametrize("hint", [1, 100])
 def test_attention_offsets_past_32_bits(ops, hint):
     """Pages more than 2^32 elements apart, written by the store and read back."""
     case = C.Attention(9, [1, 40], [40, 64], 4, 2, 64, 16)

@@ -121,6 +121,19 @@ def test_cache_refusals(match, change):
     _refused(match, paged_attention, case.q, **kw)
 
 
+@pytest.mark.parametrize("pages,page_size,kv_heads", [(4, 16, 1), (4, 1, 2), (1, 16, 2), (1, 1, 1)])
+def test_strides_of_single_pages_tokens_and_heads_do_not_matter(pages, page_size, kv_heads):
+    """A stride that nothing is multiplied by is any number: torch calls such a cache contiguous."""
+    sizes = (pages, page_size, kv_heads, 64)
+    whole = torch.zeros(sizes, dtype=BF16)
+    cache = whole.as_strided(sizes, [s if n > 1 else 3 for n, s in zip(sizes, whole.stride())])
+    assert cache.is_contiguous() and 3 in cache.stride()
+    k = torch.zeros(1, 2, kv_heads, 64, dtype=BF16)
+    _refused("must be a CUDA", paged_kv_store, k, k, k_cache=cache, v_cache=cache, slot_indices=torch.zeros(2, dtype=torch.int32))
+    case = C.Attention(0, [1, 1], [1, 1], 2, kv_heads, 64, page_size)
+    _refused("must be a CUDA", paged_attention, case.q, **case.kwargs("cpu", k_cache=cache, v_cache=cache))
+
+
 @pytest.mark.parametrize("match,over", [
     ("multiple of kv_heads", dict(q=torch.zeros(1, 4, 3, 64, dtype=BF16))),
     ("as one packed token batch", dict(q=torch.zeros(4, 4, 64, dtype=BF16))),

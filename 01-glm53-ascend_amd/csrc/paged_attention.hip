@@ -48,6 +48,10 @@ constexpr int kCus = 256;  // of an MI355X: only the number of workgroups goes b
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kRaise = 8.0f;  // log2 of the largest weight before m is raised
+// m of a row that sees keys, all with a score of -inf: below every other score's, so that parts of the row are
+// joined as ever, and told from -inf, m of a row that sees none. The first row's result is 0 / 0 = NaN as the
+// softmax's is, the second one's 0.
+constexpr float kLowest = -3e38f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -749,6 +753,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                 }
             });
         }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            m[b] = see[b].x < see[b].y ? fmaxf(m[b], kLowest) : m[b];
+        }
         // ---- join the waves: their maxima, sums and 16 rows of O at a time through LDS
         const bool begins = part0 == 0, ends = part1 == count;
         const int64_t slot = 2 * static_cast<int64_t>(w) + (begins ? 1 : 0);
@@ -788,7 +796,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                 f[x] = ml[x].x == top ? 1.0f : ex2(ml[x].x - top);
                 sum += ml[x].y * f[x];
             }
-            const float norm = begins && ends ? (sum == 0.0f ? 0.0f : vs / sum) : 1.0f;
+            const float norm = begins && ends ? (top == kNegInf ? 0.0f : vs / sum) : 1.0f;
             const int t = (row0 + b * 16 + r) / a.group;
             const int h = head * a.group + (row0 + b * 16 + r) - t * a.group;
 #pragma unroll
@@ -899,7 +907,7 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
             }
         }
         if (lane == 0 && i < rows) {
-            y *= sum == 0.0f ? 0.0f : vs / sum;
+            y *= top == kNegInf ? 0.0f : vs / sum;
             const int row = desc.y + r;
             const int t = row / a.group;
             const int h = head * a.group + row - t * a.group;
@@ -1432,11 +1440,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     const float vs = last.params.cache.v_scale != nullptr ? last.params.cache.v_scale[head] : 1.0f;
     const int r = wave * 32 + col;
     const float sum = sum_halves(l);
+    m = see.x < see.y ? fmaxf(m, kLowest) : m;
     if (r >= rows) {
         return;
     }
     if (last.splits == 1) {
-        const float f = sum == 0.0f ? 0.0f : vs / sum;
+        const float f = m == kNegInf ? 0.0f : vs / sum;
         const int t = (row0 + r) / last.params.group;
         const int h = head * last.params.group + (row0 + r) - t * last.params.group;
         uint16_t *out = static_cast<uint16_t *>(last.params.out) + static_cast<int64_t>(req.begin + t) * last.params.out_stride_token +
@@ -1503,7 +1512,7 @@ __global__ __launch_bounds__(kThreads) void prefill_combine_kernel(const Params 
         }
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
-            top = ml[k].y == 0.0f ? top : fmaxf(top, ml[k].x);
+            top = fmaxf(top, ml[k].x);
         }
     }
     float sum = 0.0f;
@@ -1532,7 +1541,7 @@ __global__ __launch_bounds__(kThreads) void prefill_combine_kernel(const Params 
         }
     }
     const float vs = a.cache.v_scale != nullptr ? a.cache.v_scale[head] : 1.0f;
-    y *= sum == 0.0f ? 0.0f : vs / sum;
+    y *= top == kNegInf ? 0.0f : vs / sum;
     uint16_t *out = static_cast<uint16_t *>(a.out) + t * a.out_stride_token +
                     (head * a.group + row - t * a.group) * a.out_stride_head + c;
     struct __attribute__((packed, aligned(2))) Out {

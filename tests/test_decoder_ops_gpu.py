@@ -382,6 +382,38 @@ def test_attention_rows_without_keys_and_uncovered_tokens(ops, hint):
     assert (out[0, :6] == 0).all() and (out[0, -6:] == 0).all() and (out[0, 8:11] == 0).all()
 
 
+@pytest.mark.parametrize("new,keys,hint", [
+    ([1, 3, 2, 1, 2], [5, 300, 1, 0, 600], 1), ([1], [9001], 1),             # decode, whole and over many workgroups
+    ([1, 40, 50, 3], [5, 70, 44, 0], 50), ([70], [2570], 70)])               # prefill, whole and over split keys
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_rows_whose_scores_are_all_minus_infinity(ops, dim, new, keys, hint):
+    """The softmax of such a row is 0 / 0, unlike that of a row that sees no key; one finite score is enough to make it
+    that key's value."""
+    case = C.Attention(22, new, keys, 4, 2, dim, 16)
+    case.q[..., 0] = 1
+    sees, last = [], []  # of each token: sees a key; the request's last key
+    for m, L in zip(new, keys):
+        sees += [L - m + i >= 0 for i in range(m)]
+        last += [L - m + i == L - 1 and L > 0 for i in range(m)]
+    sees, last = torch.tensor(sees), torch.tensor(last)
+    clean = ops.paged_attention(case.q.to(DEV), **case.kwargs(DEV, max_query_len=hint)).cpu()
+    held = case.k_cache.clone()
+    case.k_cache[:, :, 1, 0] = -float("inf")
+    out = ops.paged_attention(case.q.to(DEV), **case.kwargs(DEV, max_query_len=hint)).cpu()
+    assert torch.equal(out[:, :, :2], clean[:, :, :2])
+    assert out[0, sees, 2:].isnan().all() and (out[0, ~sees, 2:] == 0).all()
+    for n, L in enumerate(keys):
+        if L:
+            page, off = (x[L - 1] for x in case.slots_of(n))
+            case.k_cache[page, off] = held[page, off]
+            value = case.v_cache[page, off, 1]
+            out = ops.paged_attention(case.q.to(DEV), **case.kwargs(DEV, max_query_len=hint)).cpu()
+            row = int(case.cu_seqlens[n + 1]) - 1
+            assert torch.equal(out[0, row, 2:], value.expand(2, dim))
+            last[row] = False
+            assert out[0, last & sees, 2:].isnan().all()
+
+
 @pytest.mark.parametrize("hint", [1, 100])
 @pytest.mark.parametrize("page", [16, 5])
 def test_attention_unwritten_slots_hold_nan(ops, hint, page):

@@ -283,7 +283,8 @@ __device__ __forceinline__ Scores scores_of(const Params &a, int head) {
     const float mag = fabsf(f) < 1e-30f ? 1e-30f : fabsf(f);
     s.c = mag * kLog2e;
     s.cap = a.logit_cap * kLog2e;
-    s.in = a.logit_cap > 0.0f ? fminf(2.0f * kLog2e * mag / a.logit_cap, 3e38f) : 0.0f;  // a score of 0 stays 0
+    const float in = 2.0f * kLog2e * mag / a.logit_cap;
+    s.in = a.logit_cap > 0.0f ? (in > 3e38f ? 3e38f : in) : 0.0f;  // finite: a score of 0 stays 0; but a NaN stays one
     return s;
 }
 

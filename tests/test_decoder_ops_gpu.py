@@ -335,6 +335,21 @@ def test_attention_cap_on_both_sides_of_the_series(ops, cap, hint):
     _check_attention(ops, case, max_query_len=hint)
 
 
+@pytest.mark.parametrize("cap", [0.0, 1e-30, 30.0])
+@pytest.mark.parametrize("hint", [1, 100])
+def test_attention_nan_scales_stay(ops, cap, hint):
+    """A NaN scale of one head's keys or values is that head's result, capped or not; other heads keep their bits."""
+    case = C.Attention(23, [1, 40], [50, 90], 4, 2, 64, 16, fp8=True, cap=cap)
+    kw = case.kwargs(DEV, max_query_len=hint)
+    clean = ops.paged_attention(case.q.to(DEV), **kw)
+    for name in ("k_scale", "v_scale"):
+        scale = kw[name].clone()
+        scale[1] = float("nan")
+        out = ops.paged_attention(case.q.to(DEV), **dict(kw, **{name: scale}))
+        assert torch.equal(out[:, :, :2], clean[:, :, :2]) and out[:, :, 2:].isnan().all(), name
+    assert ops.paged_attention(case.q.to(DEV), **dict(kw, scale=float("nan"))).isnan().all()
+
+
 @pytest.mark.parametrize("cap", [1e-30, 1e-3])
 @pytest.mark.parametrize("hint", [1, 100])
 def test_attention_cap_far_below_the_scores(ops, cap, hint):

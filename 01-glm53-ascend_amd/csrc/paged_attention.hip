@@ -1727,9 +1727,8 @@ extern "C" int kda_paged_attention_launch(const KdaPagedAttentionArgs *args, voi
         return KDA_ERR_INVALID_ARGUMENT;
     }
     const Plan p = plan_of(a);
-    // a grid counts its threads in 32 bits
-    if (!p.decode && (p.tiles * a.cache.kv_heads * p.splits > (INT64_C(1) << 24) - 1 ||
-                      (p.splits > 1 && static_cast<int64_t>(a.num_tokens) * a.num_heads > (INT64_C(1) << 26)))) {
+    // a grid counts its threads in 32 bits (splits are made where units are few, so the join's grid is small)
+    if (!p.decode && p.tiles * a.cache.kv_heads * p.splits > (INT64_C(1) << 24) - 1) {
         return KDA_ERR_TOO_LARGE;
     }
     if (p.bytes > 0 && (workspace == nullptr || misaligned(workspace, 256) || workspace_bytes < p.bytes)) {

@@ -19,10 +19,6 @@
 
 namespace {
 
-void check_device_of(const at::Tensor &x, const char *of, const char *name, const at::Tensor &t) {
-    TORCH_CHECK(t.device() == x.device(), name, " must be on the same device as ", of);
-}
-
 // ---------------------------------------------------------------------------
 // add_rms_norm, add_rms_norm_fp8
 // ---------------------------------------------------------------------------
@@ -83,7 +79,7 @@ KdaRmsNormArgs norm_args(const char *op, const at::Tensor &x, const at::Tensor &
     TORCH_CHECK(bf16_or_fp32(weight), op, ": weight must be bf16 or fp32");
     TORCH_CHECK(weight.dim() == 1 && weight.size(0) == width && weight.is_contiguous(), op,
                 " expects a contiguous weight of the width ", width);
-    check_device_of(x, "x", "weight", weight);
+    check_same_device(x, "weight", weight, "x");
     KdaRmsNormArgs a{};
     a.x = x.data_ptr();
     a.weight = weight.data_ptr();
@@ -98,7 +94,7 @@ KdaRmsNormArgs norm_args(const char *op, const at::Tensor &x, const at::Tensor &
     if (residual.has_value()) {
         TORCH_CHECK(bf16_or_fp32(*residual), op, ": residual must be bf16 or fp32");
         TORCH_CHECK(residual->sizes() == x.sizes(), op, " expects residual in x's shape");
-        check_device_of(x, "x", "residual", *residual);
+        check_same_device(x, "residual", *residual, "x");
         a.residual = residual->data_ptr();
         a.residual_stride = row_stride(op, "residual", *residual);
         a.residual_dtype = dtype_of(*residual);
@@ -162,7 +158,7 @@ KdaPagedCache cache_of(const char *op, const char *of, const at::Tensor &x, cons
     const int64_t unit = fp8 ? 16 : 8;
     for (const auto &named : {NamedTensor{"k_cache", k_cache}, NamedTensor{"v_cache", v_cache}}) {
         const at::Tensor &t = named.second;
-        check_device_of(x, of, named.first, t);
+        check_same_device(x, named.first, t, of);
         TORCH_CHECK(t.stride(3) == 1, op, ": ", named.first, " must be contiguous in D");
         TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && stride_of(t, 0) % unit == 0 &&
                         stride_of(t, 1) % unit == 0 && stride_of(t, 2) % unit == 0,
@@ -175,7 +171,7 @@ KdaPagedCache cache_of(const char *op, const char *of, const at::Tensor &x, cons
             TORCH_CHECK(fp8, op, ": ", named.first, " belongs to a float8_e4m3fn cache");
             TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == k_cache.size(2) && t.is_contiguous(), op, ": ",
                         named.first, " must be contiguous fp32 with an entry per kv head");
-            check_device_of(x, of, named.first, t);
+            check_same_device(x, named.first, t, of);
         }
     }
     KdaPagedCache c{};
@@ -211,7 +207,7 @@ void check_index(const char *op, const char *name, const char *of, const at::Ten
     TORCH_CHECK(t.dim() == dim, op, " expects ", name, " with ", dim, " dimensions, got ", t.dim());
     TORCH_CHECK(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, op, ": ", name,
                 " must be contiguous in its last dimension");
-    check_device_of(x, of, name, t);
+    check_same_device(x, name, t, of);
 }
 
 void paged_kv_store(const at::Tensor &k, const at::Tensor &v, at::Tensor &k_cache, at::Tensor &v_cache,
@@ -224,7 +220,7 @@ void paged_kv_store(const at::Tensor &k, const at::Tensor &v, at::Tensor &k_cach
     check_tokens(op, "v", v, a.cache.head_dim);
     TORCH_CHECK(k.sizes() == v.sizes() && k.size(2) == a.cache.kv_heads, op,
                 " expects k and v as [1, T, kv_heads, D] with the cache's kv_heads");
-    check_device_of(k, "k", "v", v);
+    check_same_device(k, "v", v, "k");
     check_index(op, "slot_indices", "k", k, slot_indices, 1);
     TORCH_CHECK(slot_indices.numel() == k.size(1), op, ": slot_indices must have an entry per token, got ",
                 slot_indices.numel(), " for ", k.size(1), " tokens");

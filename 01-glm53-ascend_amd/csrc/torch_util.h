@@ -12,8 +12,8 @@ namespace {
 
 using NamedTensor = std::pair<const char *, const at::Tensor &>;
 
-inline void check_same_device(const at::Tensor &q, const char *name, const at::Tensor &t) {
-    TORCH_CHECK(t.device() == q.device(), name, " must be on the same device as q");
+inline void check_same_device(const at::Tensor &x, const char *name, const at::Tensor &t, const char *x_name = "q") {
+    TORCH_CHECK(t.device() == x.device(), name, " must be on the same device as ", x_name);
 }
 
 inline void check_ok(int status, const char *op) {

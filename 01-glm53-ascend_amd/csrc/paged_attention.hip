@@ -407,8 +407,9 @@ template <int D> __device__ __forceinline__ void zero_uncovered(const Params &a,
 // requests of up to 32 K keys took 565 us so, 552 now.
 //
 // Bound by HBM: those 64 requests (64 heads on 8 key heads, D = 128) read 3.4 GB in
-// 552 us = 6.1 TB/s, what a kernel that only reads reaches. 256 requests in 8 bits:
-// 167 us = 5.65 TB/s, 5 us of it for joining parts. A single short request is bound by its
+// 552 us = 6.1 TB/s, what a kernel that only reads reaches (other cards: up to 577 us).
+// D = 64: 311 us for half of it, 5.4 TB/s. 256 requests in 8 bits:
+// 169 us = 5.6 TB/s, 5 us of it for joining parts. A single short request is bound by its
 // latencies: 9 to 10 us for the kernel (lengths, page numbers, keys, the waves' join one after another) and
 // 4 us for the second one.
 // ---------------------------------------------------------------------------
@@ -938,10 +939,11 @@ template <int D, int NB> __global__ __launch_bounds__(kThreads) void decode_comb
 // fill each other's waits.
 //
 // Bound by the matrix cores together with the softmax's vector instructions: 8192
-// tokens, 32 heads on 8, D = 128, causal: 550 us = 1.0 PFLOP/s (the skipped half
-// not counted). The library's bf16 product reaches 1.1 (4096 cubed) to 1.29 (8192); this
+// tokens, 32 heads on 8, D = 128, causal: 550 to 565 us by the card = 1.0 PFLOP/s (the skipped half
+// not counted); with 8-bit keys and values 580. D = 64: 338 us = 810 TFLOP/s, as many
+// exponentials, maxima and conversions beside half the products. The library's bf16 product reaches 1.1 (4096 cubed) to 1.29 (8192); this
 // loop without its softmax and LDS reads 1.27, at the clock the card holds under such
-// load. Six chunks against up to 30 K keys: 845 us = 930 TFLOP/s.
+// load. Six chunks against up to 30 K keys: 865 us = 910 TFLOP/s.
 //
 // Every workgroup finds its tile itself, from the lengths on the device. The longest
 // request's tiles go first, its last ones (the longest, under the causal mask) before the
@@ -1573,11 +1575,13 @@ int64_t most_rows(const KdaPagedAttentionArgs &a) {
     return std::max<int64_t>(a.max_query_len, 1) * (a.num_heads / a.cache.kv_heads);
 }
 
-// At most 32 rows a request (without requests, the decode kernel only writes the zeros). 32 requests of 4096
-// keys, 32 heads on 4, D = 128, us:           rows   8   16   32   40   64
-//   decode kernel, tiles of 16 rows (NB = 1)        55   56   97  142  176
-//   decode kernel, tiles of 32 rows (NB = 2)        57   59   63  103  105
-//   prefill kernel                                  63   63   65   67   76
+// At most 32 rows a request (without requests, the decode kernel only writes the zeros). The largest request
+// decides for the whole call. us, in tiles of 16 rows (NB = 1), of 32 rows (NB = 2), by the prefill kernel:
+//   rows of each request                    8          16            32            40            64
+//   32 x 4096 keys, 32 heads on 4, D 128  56 58 63   57 60 64    98  64  67   142 103  68   176 106  69
+//   64 x 4096 keys, 32 heads on 4, D 64   53 55 74   53 55 75    92  56  76   135  96  78   175  95  78
+//   64 x 4096 keys, 8 on 1, D 128, 8 bit  26 29 33   28 33 33    36  38  35    48  43  40    58  43  44
+//   1 x 8192 keys, 32 heads on 4, D 128   18 20 25   23 24 25    31  30  26    31  36  27    34  41  27
 bool decodes(const KdaPagedAttentionArgs &a) { return most_rows(a) <= 32 || a.num_seqs == 0; }
 
 Plan plan_of(const KdaPagedAttentionArgs &a) {

@@ -7,7 +7,9 @@
 // h, the sum of squares and y are fp32; the norm reads h before it is rounded
 // into the residual. y is formed as (h w) rsqrt, so the largest |y| is the
 // largest |h w| times the same factor, rounded alike: it is known from the
-// pass that sums the squares, and a row takes one reduction, not two.
+// pass that sums the squares, and a row takes one reduction, not two. An 8-bit output is
+// (h w)(rsqrt / s) accordingly, a few fp32 roundings from y / s: a value beside a tie
+// may take the neighbouring 8-bit step, with the same error against exact arithmetic.
 //
 // Bound by HBM: a row stays in registers between its one read and its one
 // write. A lane holds 16 bytes of the input at a time (8 or 4 columns), so 16 or 32
@@ -19,7 +21,8 @@
 // row's last whole vector and moved down in registers, and stored element by element.
 //
 // Measured, residual read and written: 8192 x 8192 bf16 to 8 bits with a scale per 128
-// columns 75 us = 6.3 TB/s (reading alone reaches 6.1 to 6.4 on this card, a copy 4.9);
+// columns 75 us = 6.3 TB/s (reading alone reaches 6.1 to 6.4 on this card, a copy 4.9), with one
+// per row 75.5;
 // 1001 x 5003 fp32 16 us = 5.0 TB/s; one row 3 us.
 
 #include <hip/hip_runtime.h>

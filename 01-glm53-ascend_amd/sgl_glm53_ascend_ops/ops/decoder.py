@@ -47,7 +47,8 @@ def add_rms_norm_fp8(
 
     ``out`` is ``float8_e4m3fn``; ``scale`` is fp32, ``[..., 1]`` (``group_size``
     0: one a row) or ``[..., ceil(width / 128)]`` (``group_size`` 128):
-    ``max(max|y| / 448, 1e-12)`` of the group. ``y`` is not rounded in between.
+    ``max(max|y| / 448, 1e-12)`` of the group. ``y`` is not rounded in between; a value
+    within a few fp32 roundings of a tie may take either 8-bit neighbour.
     """
     return _OPS.add_rms_norm_fp8(x, weight, eps, residual=residual, group_size=group_size)
 
@@ -102,9 +103,10 @@ def paged_attention(
     them; ``logit_cap`` > 0 turns a score ``s`` into ``logit_cap * tanh(s /
     logit_cap)``. ``k_scale, v_scale`` as in :func:`paged_kv_store`. A token that
     sees no key, or that no request covers, gets zeros; pages outside the pool
-    read as zero keys and values. ``max_query_len``, the most new tokens of a
-    request, chooses the kernel (results hold for any value). Returns ``[1, T,
-    heads, D]`` in bf16.
+    read as zero keys and values. Scores, softmax and sums are fp32; the softmax
+    weights are rounded to bf16 for the product with the values. ``max_query_len``,
+    the most new tokens of a request, chooses the kernel (results hold for any
+    value). Returns ``[1, T, heads, D]`` in bf16.
     """
     return _OPS.paged_attention(
         q, k_cache=k_cache, v_cache=v_cache, page_table=page_table, kv_lens=kv_lens,

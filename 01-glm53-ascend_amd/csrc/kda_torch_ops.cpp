@@ -74,16 +74,6 @@ struct Metadata {
     static const int32_t *ptr(const at::Tensor &t) { return static_cast<const int32_t *>(t.data_ptr()); }
 };
 
-// One packed token batch [1, T, H, D] (the sglang contract; a leading batch
-// above one would otherwise be ignored), with T and the request count in the
-// kernels' int32 range.
-void check_packed(const char *op, const at::Tensor &q, const at::Tensor &indices) {
-    TORCH_CHECK(q.size(0) == 1, op, " expects one packed token batch [1, T, H, D], got batch ",
-                q.size(0));
-    TORCH_CHECK(q.size(1) <= INT32_MAX && indices.numel() < INT32_MAX, op,
-                " supports at most 2^31-1 tokens and requests");
-}
-
 void check_gate_params(const at::Tensor &q, const at::Tensor &A_log, const at::Tensor &dt_bias,
                        int64_t HV, int64_t D) {
     TORCH_CHECK(A_log.scalar_type() == at::kFloat && A_log.numel() == HV,
@@ -94,64 +84,6 @@ void check_gate_params(const at::Tensor &q, const at::Tensor &A_log, const at::T
                 "A_log and dt_bias must be contiguous");
     check_same_device(q, "A_log", A_log);
     check_same_device(q, "dt_bias", dt_bias);
-}
-
-void check_index_tensors(const char *op, const at::Tensor &q, const at::Tensor &indices,
-                         const at::Tensor &cu_seqlens) {
-    for (const auto &named : {NamedTensor{"initial_state_indices", indices},
-                              NamedTensor{"cu_seqlens", cu_seqlens}}) {
-        TORCH_CHECK(named.second.scalar_type() == at::kInt ||
-                        named.second.scalar_type() == at::kLong,
-                    named.first, " must be int32 or int64");
-        TORCH_CHECK(named.second.is_contiguous(), named.first, " must be contiguous");
-        TORCH_CHECK(named.second.device() == q.device(), named.first,
-                    " must be on the same device as q");
-    }
-    TORCH_CHECK(cu_seqlens.numel() == indices.numel() + 1, op,
-                ": cu_seqlens must have numReq+1 entries, got ", cu_seqlens.numel(), " for ",
-                indices.numel(), " requests");
-}
-
-void check_track(const at::Tensor &q, const at::Tensor &indices,
-                 const std::optional<at::Tensor> &track_indices,
-                 const std::optional<at::Tensor> &track_lens) {
-    if (!track_indices.has_value()) {
-        return;
-    }
-    TORCH_CHECK(track_lens.has_value(), "track_state_indices requires track_state_lens");
-    for (const auto &named : {NamedTensor{"track_state_indices", *track_indices},
-                              NamedTensor{"track_state_lens", *track_lens}}) {
-        TORCH_CHECK(named.second.scalar_type() == at::kInt ||
-                        named.second.scalar_type() == at::kLong,
-                    named.first, " must be int32 or int64");
-        TORCH_CHECK(named.second.numel() == indices.numel(), named.first,
-                    " must have one entry per request");
-        TORCH_CHECK(named.second.device() == q.device(), named.first,
-                    " must be on the same device as q");
-    }
-}
-
-// The state pool: 4-D fp32 [slots, H, K, V] with K contiguous
-// (kda_varlen_recurrent.cpp:60-74).
-void check_pool(const at::Tensor &pool, int64_t H, int64_t D) {
-    TORCH_CHECK(pool.dim() == 4 && pool.scalar_type() == at::kFloat,
-                "state must be a 4-D fp32 [slots,HV,K,V] pool");
-    TORCH_CHECK(pool.size(1) == H && pool.size(2) == D && pool.size(3) == D,
-                "state must be [slots,HV,K,V] matching the head and feature dims");
-    TORCH_CHECK(pool.stride(2) == 1 && pool.stride(3) == D,
-                "state must be K-contiguous (stride(2)==1, stride(3)==", D, "), got strides (",
-                pool.stride(2), ", ", pool.stride(3), ")");
-}
-
-struct PoolRef {
-    float *base;
-    int64_t stride_slot;
-    int64_t stride_head;
-    int64_t num_slots;
-};
-
-PoolRef pool_ref(at::Tensor &pool) {
-    return PoolRef{pool.data_ptr<float>(), pool.stride(0), pool.stride(1), pool.size(0)};
 }
 
 // A prefill of K = V = 128 whose requests average at least this many tokens

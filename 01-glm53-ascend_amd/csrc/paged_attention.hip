@@ -34,6 +34,7 @@
 
 #include "kda_abi.h"
 #include "kda_device.h"
+#include "matrix_device.h"
 #include "paged_cache.h"
 
 namespace kda {
@@ -53,14 +54,6 @@ constexpr float kRaise = 8.0f;  // log2 of the largest weight before m is raised
 // softmax's is, the second one's 0.
 constexpr float kLowest = -3e38f;
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
 typedef const __attribute__((address_space(1))) int global_int;
 
@@ -68,14 +61,6 @@ struct __attribute__((packed, aligned(2))) Bf16x8Any {
     u32x4 w;
 };
 
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                   0);
-}
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                   0);
-}
 // A 16-byte load that is known to be from global memory: through a selected or shuffled
 // pointer the compiler would issue a flat load, which also counts as an LDS access and is waited for as one.
 __device__ __forceinline__ u32x4 load16(const char *p) { return *(global_u32x4 *)p; }
@@ -114,8 +99,6 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
     constexpr uint32_t kOnes = 0x3f803f80u;
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, kOnes), sum, false);
 }
-
-__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Infinite or NaN values that some rows of a tile do not see must not reach those, but in the matrix
 // product their weight of 0 makes a NaN. The steps do not look for them. A tile whose O is not finite at its end,
@@ -321,7 +304,7 @@ template <int D> __device__ __forceinline__ u32x2 read_tr(const char *tile, int 
     const int r = row + ((lane >> 2) & 3);
     const int c = lane & 3;
     const char *p = tile + v_at<D>(r, 2 * pair + (c >> 1)) + (c & 1) * 8;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+    return lds_read_tr(p);
 }
 
 // A 16-byte chunk of a loaded row into a tile, 8-bit ones widened to two chunks.

@@ -9,6 +9,7 @@ from .kda import (
     kda_varlen_recurrent_v2,
     prepared_recurrent,
 )
+from .linear import linear_varlen_chunk, linear_varlen_recurrent
 
 __all__ = [
     "add_rms_norm",
@@ -20,6 +21,8 @@ __all__ = [
     "kda_varlen_chunk_with_state",
     "kda_varlen_recurrent",
     "kda_varlen_recurrent_v2",
+    "linear_varlen_chunk",
+    "linear_varlen_recurrent",
     "paged_attention",
     "paged_kv_store",
     "prepared_recurrent",

@@ -39,8 +39,10 @@
  * request's initial state.
  *
  * Beside the KDA entry points stand those of the other parts of a decoder that
- * interleaves KDA layers with full attention (no counterpart in the reference):
- * kda_rms_norm_launch, kda_paged_store_launch and kda_paged_attention_launch.
+ * interleaves KDA layers with others (no counterpart in the reference): linear
+ * attention with a decay for each head (kda_linear_recurrent_launch,
+ * kda_linear_chunk_launch), kda_rms_norm_launch, kda_paged_store_launch and
+ * kda_paged_attention_launch.
  *
  * All launches are asynchronous on `stream` and never synchronize the host.
  * Every function returns a KdaStatus (0 = success).
@@ -271,6 +273,71 @@ int kda_chunk_launch_wide(const KdaChunkArgs *args, int32_t wide, void *workspac
  * that overlap on one GPU -- concurrent streams, or host threads -- race, and
  * must be serialized by the caller. */
 int kda_chunk_launch_noalloc(const KdaChunkArgs *args, void *stream);
+
+/* Linear attention with a decay for each head over packed varlen sequences, on the
+ * slot-indexed state pool of the KDA entry points. Per request and head, with the
+ * state S [K, V] and for its tokens t in turn:
+ *   S <- exp(g_t) S + k_t v_t^T;   out_t = scale * S^T q_t
+ * The pool's layout and its slot 0 are those above, and so are checkpoints and tracked
+ * prefixes; a request with slot 0 starts from zeros and leaves no state. Metadata may be
+ * int64 (`wide`), and int64 entries count whole: one beyond 32 bits is outside the pool or
+ * past the tokens, not its low word. Every token of out is written, 0 where no request
+ * covers it. Requests of one call must not share a slot other than 0 or a tracked one. */
+typedef struct KdaLinearArgs {
+    const void *q; /* [tokens, heads, D], `dtype`, D contiguous; element strides of tokens and heads */
+    const void *k;
+    const void *v;
+    int64_t q_stride_token, q_stride_head;
+    int64_t k_stride_token, k_stride_head;
+    int64_t v_stride_token, v_stride_head;
+    const float *g; /* log decay of token t, head h: g[t * g_stride_token + h * g_stride_head] */
+    int64_t g_stride_token; /* 0: one decay for each head */
+    int64_t g_stride_head;
+
+    float *state;
+    int64_t state_stride_slot; /* elements */
+    int64_t state_stride_head;
+    int64_t num_slots;
+
+    const void *state_indices; /* [num_seqs] */
+    const void *cu_seqlens;    /* [num_seqs + 1], non-decreasing */
+    void *out;                 /* [tokens, heads, D] contiguous, `dtype` */
+
+    /* As in KdaRecurrentArgs; the recurrent form only. */
+    float *intermediate;
+    int64_t mid_stride_req;
+    int64_t mid_stride_step;
+    int64_t mid_stride_head;
+    int64_t mid_rows;
+    int64_t mid_steps;
+
+    const void *track_indices; /* [num_seqs] or null: as in KdaRecurrentArgs */
+    const void *track_lens;
+
+    float scale;
+    int32_t num_seqs;
+    int32_t num_tokens;
+    int32_t num_heads;
+    int32_t head_dim; /* K == V; 64 or 128 */
+    int32_t dtype;    /* KDA_BF16, or (recurrent) KDA_F32: q, k, v and out */
+    int32_t wide;     /* which metadata is int64: a sum of KDA_WIDE_CU_SEQLENS, _STATE_INDICES, _TRACK_INDICES, _TRACK_LENS */
+} KdaLinearArgs;
+
+/* Token by token: decode and verify steps, short prompts. Alignment
+ * (KDA_ERR_INVALID_ARGUMENT otherwise): q, k, v, out, state and intermediate 16 bytes, with
+ * strides in multiples of 16 bytes. */
+int kda_linear_recurrent_launch(const KdaLinearArgs *args, void *stream);
+
+/* Bytes of device scratch that kda_linear_chunk_launch needs for these sizes
+ * (host-only; pointers, strides and contents do not matter), 0 where it needs none. */
+size_t kda_linear_chunk_workspace_bytes(const KdaLinearArgs *args);
+
+/* In chunks of 64 tokens on the matrix cores: prompts. bf16 only, no checkpoints; alignment as
+ * above. Log decays are at most 0 in earnest (positive ones work while exp(sum) stays finite over 64
+ * tokens), down to -infinity; below -10000 they count as -10000, whose exponential is 0. An
+ * infinite or NaN value reaches its own token and later ones of its request only.
+ * `workspace`: 256-byte aligned device memory of the bytes above, no initialization needed. */
+int kda_linear_chunk_launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Residual addition and root-mean-square norm of `rows` rows of `width`:
  *   h = x + residual (fp32);  residual <- h;  y = h * weight / sqrt(mean(h^2) + eps)

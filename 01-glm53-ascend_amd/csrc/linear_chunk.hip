@@ -14,10 +14,10 @@
 // (a request of one segment needs the last only). L goes by the call's tokens and heads, so that two
 // workgroups a CU have work whatever the number of heads is.
 //
-// A wave owns 16 or 32 of the state's columns (values) and keeps them as accumulators, in fp32, through its segment:
+// A wave owns 16 of the state's columns (values) and keeps them as accumulators, in fp32, through its segment:
 // as they lie there they are, split into bf16 parts, the left operand of S^T q. The values, read transposed from
 // LDS, serve both the outputs (left operand) and the update (right operand, times their decays). The
-// scores of 16 tokens are formed by each wave for all of them. q, k and v are exact in bf16; what is rounded
+// scores are formed once, by all waves for all, and go through LDS. q, k and v are exact in bf16; what is rounded
 // is split: scores and S into two parts (17 bits), the decayed values into three (25 bits, all of fp32: these errors
 // would stay in the state). The sums of log decays are formed in 64 bits, so that neighbours' differences are exact
 // behind a steep decay.
@@ -37,9 +37,10 @@ namespace {
 
 #define KDA_INLINE __attribute__((always_inline))
 
-constexpr int kThreads = 256;
-constexpr int kWaves = 4;
 constexpr int kChunk = 64;
+template <int D> constexpr int kWaves = D / 16;
+template <int D> constexpr int kThreads = 64 * kWaves<D>;
+constexpr int kStartThreads = 64;
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kSteepest = -1e4f;  // of a log decay: its exponential is 0 long before
 
@@ -49,6 +50,11 @@ struct ChunkParams : LinearParams {
     int segment;    // tokens, a multiple of 64
 };
 
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
+    return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32))) << 32 | low;
+}
+
 // A workgroup's segment of a request.
 struct Segment {
     int n, index, count;
@@ -56,24 +62,29 @@ struct Segment {
     int64_t slot;  // in the workspace, for requests of several segments
 };
 
-// Segment number `tile` of all: request n gets the numbers from floor(cu[n] / L) + n, at least as many as it has
-// segments. By a whole workgroup; n < 0: none.
-__device__ __forceinline__ Segment segment_of(const ChunkParams &a, int tile) {
+// A workgroup's segment, by all its threads; n < 0: none. The numbers up to tokens / L are those of segments that
+// others of their request follow: request n has those from floor(cu[n] / L), at least as many as it needs. Then one
+// for each request: its last segment. Long ones so go first.
+template <int THREADS> __device__ __forceinline__ Segment segment_of(const ChunkParams &a, int tile) {
+    const int whole = a.num_tokens / a.segment;
     Segment s;
-    int below = 0;  // requests that begin at or before this tile
-    for (int first = 0; first < a.num_seqs; first += kThreads) {
-        const int x = first + static_cast<int>(threadIdx.x);
-        below += __syncthreads_count(x < a.num_seqs && a.cu(x) / a.segment + x <= tile);
+    s.n = tile - whole;
+    if (tile < whole) {
+        int below = 0;  // requests that begin at or before this tile
+        for (int first = 0; first < a.num_seqs; first += THREADS) {
+            const int x = first + static_cast<int>(threadIdx.x);
+            below += __syncthreads_count(x < a.num_seqs && a.cu(x) / a.segment <= tile);
+        }
+        s.n = __builtin_amdgcn_readfirstlane(below) - 1;
+        if (s.n < 0) {
+            return s;
+        }
     }
-    s.n = __builtin_amdgcn_readfirstlane(below) - 1;
-    if (s.n < 0) {
-        return s;
-    }
-    s.request_begin = a.cu(s.n);
-    const int end = max(a.cu(s.n + 1), s.request_begin);
-    s.index = tile - s.request_begin / a.segment - s.n;
+    s.request_begin = __builtin_amdgcn_readfirstlane(a.cu(s.n));
+    const int end = __builtin_amdgcn_readfirstlane(max(a.cu(s.n + 1), s.request_begin));
     s.count = max((end - s.request_begin + a.segment - 1) / a.segment, 1);
-    if (s.index < 0 || s.index >= s.count) {
+    s.index = tile < whole ? tile - s.request_begin / a.segment : s.count - 1;
+    if (tile < whole && (s.index < 0 || s.index + 1 >= s.count)) {
         s.n = -1;
         return s;
     }
@@ -110,74 +121,150 @@ __device__ __forceinline__ uint32_t split(float &x, float &y) {
     return hi;
 }
 
+// Number of the scores of tokens 16 it .. with 32 y ..: those that can see any of them.
+__device__ __forceinline__ constexpr int unit(int it, int y) { return it < 2 ? it : 2 * it - 2 + y; }
+
 template <int D, bool OUTPUTS> struct Shared {
     char k[kChunk * D * 2];
     char v[kChunk * D * 2];
     char q[OUTPUTS ? kChunk * D * 2 : 16];
-    u32x4 scores[OUTPUTS ? 4 : 1][2][2][64];  // [16 tokens][32 earlier ones][part][lane]
+    u32x4 scores[OUTPUTS ? 6 : 1][2][64];  // [16 tokens and 32 up to them: unit()][part][lane]
     double sum[kChunk];                       // G in log2 units
     float late[kChunk];                       // e^(G_64 - G_j)
-    float early[kChunk];                      // e^G_i
-    int odd[kWaves];                          // some value is not finite
+    float early[kChunk];                      // scale e^G_i
+    int odd[kWaves<D>];                       // some value is not finite
 };
 
-// Tokens [segment.begin, segment.end) of one head, from the state in s (accumulators: columns 16 (wave VT + vt) + lane % 16,
-// rows 16 kt + 4 (lane / 16) + e). Returns the sum of the log decays (log2).
+// The lane, and what follows from it formed anew: kept from chunk to chunk, addresses in LDS do not all fit the registers.
+__device__ __forceinline__ int lane_here() {
+    int lane = static_cast<int>(__lane_id());
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// A sum of the values of this lane and those before it, over the wave.
+template <int CTRL, int ROWS> __device__ __forceinline__ double add_from(double x) {
+    const u32x2 w = __builtin_bit_cast(u32x2, x);
+    const u32x2 up = {static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w[0]), CTRL, ROWS, 0xf, false)),
+                      static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w[1]), CTRL, ROWS, 0xf, false))};
+    return x + __builtin_bit_cast(double, up);
+}
+__device__ __forceinline__ double prefix_sum(double x) {
+    x = add_from<0x111, 0xf>(x);  // one lane up within 16, then two, four and eight
+    x = add_from<0x112, 0xf>(x);
+    x = add_from<0x114, 0xf>(x);
+    x = add_from<0x118, 0xf>(x);
+    x = add_from<0x142, 0xa>(x);  // lane 15 to the second 16, lane 47 to the fourth
+    return add_from<0x143, 0xc>(x);  // lane 31 to the upper half
+}
+
+// Tokens [segment.begin, segment.end) of one head, from the state in s (accumulators: column 16 wave + lane % 16, rows
+// 16 kt + 4 (lane / 16) + e). Returns the sum of the log decays (log2).
+//
+// Two barriers a chunk: its rows are in LDS, and nobody reads them any more (the scores are there). What
+// comes after the second one, the scores' products with the values held in registers, overlaps with other waves'
+// staging of the next chunk, whose loads are in flight all the while.
 template <int D, bool OUTPUTS>
 __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> &sm, const Segment &seg, int head,
-                                       f32x4 (&s)[D / 16][D / 64], int64_t track_slot, int64_t track_at) {
-    constexpr int VT = D / 64, KT = D / 16, X = D / 32;
+                                       f32x4 (&s)[D / 16], int64_t track_slot, int track_at) {
+    constexpr int KT = D / 16, X = D / 32;
     constexpr int kRowChunks = D / 8;
-    constexpr int kLoads = D / 32;  // 16-byte loads a thread makes of 64 rows
-    constexpr int kStep = kThreads / kRowChunks;
-    const int tid = threadIdx.x, lane = tid & 63;
+    constexpr int kStep = kThreads<D> / kRowChunks;
+    constexpr int kLoads = kChunk / kStep;  // 16-byte loads a thread makes of 64 rows
+    static_assert(kLoads == 2);
+    const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, col = lane & 15;
     const int row = tid / kRowChunks, chunk = tid % kRowChunks;
-    const char *qb = static_cast<const char *>(a.q) + 2 * (head * a.q_stride_head) + chunk * 16;
-    const char *kb = static_cast<const char *>(a.k) + 2 * (head * a.k_stride_head) + chunk * 16;
-    const char *vb = static_cast<const char *>(a.v) + 2 * (head * a.v_stride_head) + chunk * 16;
-    u32x4 q[OUTPUTS ? kLoads : 1], k[kLoads], v[kLoads];
+    struct Rows {
+        const char *at;  // this thread's 16 bytes of its first row of the next chunk
+        int64_t token;   // bytes
+    };
+    auto rows_of = [&](const void *x, int64_t token, int64_t of_head) KDA_INLINE -> Rows {
+        return Rows{static_cast<const char *>(x) + 2 * (head * of_head + (seg.begin + row) * token) + chunk * 16, 2 * token};
+    };
+    Rows qr = rows_of(a.q, a.q_stride_token, a.q_stride_head);
+    Rows kr = rows_of(a.k, a.k_stride_token, a.k_stride_head);
+    Rows vr = rows_of(a.v, a.v_stride_token, a.v_stride_head);
+    u32x4 q[kLoads], k[kLoads], v[kLoads];
     float decay = 0.0f;
     double total = 0.0;
 
-    auto load = [&](int pos, int len) KDA_INLINE {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int64_t t = pos + min(row + i * kStep, len - 1);
-            if constexpr (OUTPUTS) {
-                q[i] = *reinterpret_cast<const u32x4 *>(qb + 2 * t * a.q_stride_token);
-            }
-            k[i] = *reinterpret_cast<const u32x4 *>(kb + 2 * t * a.k_stride_token);
-            v[i] = *reinterpret_cast<const u32x4 *>(vb + 2 * t * a.v_stride_token);
+    // The next chunk's rows: len tokens from pos, to which the pointers point; they go on by `step`.
+    auto load = [&](int pos, int len, int step) KDA_INLINE {
+        const int lane = lane_here();
+        const int row = (64 * wave + lane) / kRowChunks;
+        if (wave == 0) {
+            decay = a.g[(pos + min(lane, len - 1)) * a.g_stride_token + head * a.g_stride_head];
         }
-        decay = a.g[(pos + min(lane, len - 1)) * a.g_stride_token + head * a.g_stride_head];
+        auto of = [&](Rows &r, u32x4 (&x)[kLoads]) KDA_INLINE {
+            int64_t first = 0, second = kStep * r.token;
+            if (len < kChunk) {  // rows past the last stand for it
+                first = min(0, len - 1 - row) * r.token;
+                second = min(kStep, len - 1 - row) * r.token;
+            }
+            x[0] = *reinterpret_cast<const u32x4 *>(r.at + first);
+            x[1] = *reinterpret_cast<const u32x4 *>(r.at + second);
+            r.at += step * r.token;
+        };
+        if constexpr (OUTPUTS) {
+            of(qr, q);
+        }
+        of(kr, k);
+        of(vr, v);
     };
     int single = 0;  // tokens before this one go one at a time
     auto length = [&](int pos) KDA_INLINE -> int {
         const int len = pos < single ? 1 : min(kChunk, seg.end - pos);
-        return track_at > pos && track_at < pos + len ? static_cast<int>(track_at) - pos : len;
+        return track_at > pos && track_at < pos + len ? track_at - pos : len;
+    };
+    // A chunk's outputs are stored when the next one is in LDS, before the loads of the one after: whoever waits for
+    // those then does not wait for stores that have only begun.
+    u32x2 done[4];
+    int done_len = 0, done_step = 0;
+    const int64_t out_token = static_cast<int64_t>(a.num_heads) * D * 2;  // bytes
+    char *out = static_cast<char *>(a.out) + (seg.begin + (tid & 15)) * out_token + 2 * (head * D + 16 * wave + 4 * (tid >> 4 & 3));
+    auto store_done = [&]() KDA_INLINE {
+        if constexpr (OUTPUTS) {
+            const int col = lane_here() & 15;
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                if (16 * it + col < done_len) {
+                    *reinterpret_cast<u32x2 *>(out + 16 * it * out_token) = done[it];
+                }
+            }
+            out += done_step * out_token;
+            done_len = done_step = 0;
+        }
     };
 
     int pos = seg.begin, len = length(pos);
     if (pos < seg.end) {
-        load(pos, len);
+        load(pos, len, len);
     }
     while (pos < seg.end) {
+        const int lane = lane_here();
+        const int g = lane >> 4, col = lane & 15;
+        const int row = (64 * wave + lane) / kRowChunks, chunk = lane % kRowChunks;
         // ---- the chunk into LDS, its sums of decays
         uint32_t odd = 0;
+        if (wave == 0) {
+            const double sum = prefix_sum(lane < len ? kLog2e * static_cast<double>(decay < kSteepest ? kSteepest : decay) : 0.0);
+            const u32x2 w = __builtin_bit_cast(u32x2, sum);
+            const u32x2 last = {static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w[0]), 63)),
+                                static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w[1]), 63))};
+            sm.sum[lane] = sum;
+            sm.late[lane] = ex2(static_cast<float>(__builtin_bit_cast(double, last) - sum));
+            sm.early[lane] = ex2(static_cast<float>(sum)) * a.scale;
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int r = row + i * kStep;
-            if (r >= len) {
-                k[i] = v[i] = u32x4{0, 0, 0, 0};
+            if (len < kChunk && r >= len) {
+                q[i] = k[i] = v[i] = u32x4{0, 0, 0, 0};
             }
             *reinterpret_cast<u32x4 *>(sm.k + place<D>(r, chunk)) = k[i];
             *reinterpret_cast<u32x4 *>(sm.v + place<D>(r, chunk)) = v[i];
             if constexpr (OUTPUTS) {
-                if (r >= len) {
-                    q[i] = u32x4{0, 0, 0, 0};
-                }
                 // elements 4 u .. 4 u + 3 of each 32 go to place (u % 4, u / 4): a lane's eight of the
                 // contraction, 4 g .. and 16 + 4 g .., are then one read
                 const int c = chunk & ~3, u = 2 * (chunk & 3);
@@ -189,244 +276,199 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
                 }
             }
         }
-        if (wave == 0) {
-            double sum = lane < len ? static_cast<double>(decay < kSteepest ? kSteepest : decay) : 0.0;
-            sum *= kLog2e;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double up = __shfl_up(sum, d);
-                sum += lane >= d ? up : 0.0;
-            }
-            sm.sum[lane] = sum;
-            sm.late[lane] = ex2(static_cast<float>(__shfl(sum, 63) - sum));
-            sm.early[lane] = ex2(static_cast<float>(sum));
-        }
         if constexpr (OUTPUTS) {
-            const unsigned long long some = __ballot(odd != 0);
+            const bool some = __any(odd != 0);
             if (lane == 0) {
-                sm.odd[wave] = some != 0;
+                sm.odd[wave] = some;
             }
         }
         lds_barrier();
         if constexpr (OUTPUTS) {
             // An infinite or NaN value must not reach earlier tokens of its chunk, but in the product their score of 0
             // makes a NaN of it: such a chunk goes token by token.
-            if (len > 1 && (sm.odd[0] | sm.odd[1] | sm.odd[2] | sm.odd[3]) != 0) {
+            if (len > 1 && __any(sm.odd[lane % kWaves<D>] != 0)) {
                 single = pos + len;
+                qr.at -= len * qr.token;
+                kr.at -= len * kr.token;
+                vr.at -= len * vr.token;
                 len = 1;
-                load(pos, len);
+                load(pos, 1, 1);
                 lds_barrier();
                 continue;
             }
         }
+        store_done();
         const int next = pos + len, next_len = length(next);
         if (next < seg.end) {
-            load(next, next_len);
+            load(next, next_len, next_len);
         }
-        total += sm.sum[63];
-        const float all = ex2(static_cast<float>(sm.sum[63]));
+        const double last = sm.sum[kChunk - 1];
+        total += last;
+        const float all = ex2(static_cast<float>(last));
 
-        f32x4 o[VT][4];
-        u32x4 values[VT][2];
+        f32x4 o[4];
+        u32x4 values[2];
         if constexpr (OUTPUTS) {
-            // ---- scores of this wave's 16 tokens with those before them: lane: token 16 wave + col, earlier 16 jt + 4 g + e
-            f32x4 p[4];
-            const double mine = sm.sum[16 * wave + col];
+            // ---- scores of 16 tokens with 32 up to them: lane: token 16 it + col, earlier one 16 jt + 4 g + e
 #pragma unroll
-            for (int jt = 0; jt < 4; ++jt) {
-                p[jt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (jt > wave) {
+            for (int u = 0; u < 8 / kWaves<D>; ++u) {
+                const int it = (wave * (8 / kWaves<D>) + u) >> 1, y = (wave * (8 / kWaves<D>) + u) & 1;
+                if (y > it / 2) {
                     continue;
+                }
+                f32x4 p[2];
+                const double mine = sm.sum[16 * it + col];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    p[z] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
 #pragma unroll
                 for (int x = 0; x < X; ++x) {
-                    const char *kr = sm.k + (g & 1) * 8;
-                    const int r = 16 * jt + col;
-                    const u32x2 k0 = *reinterpret_cast<const u32x2 *>(kr + place<D>(r, 4 * x + (g >> 1)));
-                    const u32x2 k1 = *reinterpret_cast<const u32x2 *>(kr + place<D>(r, 4 * x + 2 + (g >> 1)));
-                    const u32x4 qx = *reinterpret_cast<const u32x4 *>(sm.q + place<D>(16 * wave + col, 4 * x + g));
-                    p[jt] = mfma16(u32x4{k0[0], k0[1], k1[0], k1[1]}, qx, p[jt]);
-                }
+                    const u32x4 right = *reinterpret_cast<const u32x4 *>(sm.q + place<D>(16 * it + col, 4 * x + g));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = 16 * jt + 4 * g + e;
-                    const float w = ex2(static_cast<float>(mine - sm.sum[j]));
-                    p[jt][e] = j <= 16 * wave + col ? p[jt][e] * w : 0.0f;
+                    for (int z = 0; z < 2; ++z) {
+                        const char *at = sm.k + (g & 1) * 8;
+                        const int r = 32 * y + 16 * z + col;
+                        const u32x2 k0 = *reinterpret_cast<const u32x2 *>(at + place<D>(r, 4 * x + (g >> 1)));
+                        const u32x2 k1 = *reinterpret_cast<const u32x2 *>(at + place<D>(r, 4 * x + 2 + (g >> 1)));
+                        p[z] = mfma16(u32x4{k0[0], k0[1], k1[0], k1[1]}, right, p[z]);
+                    }
                 }
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                if (2 * y > wave) {
-                    continue;
-                }
-                u32x4 part;
+                u32x4 hi, lo;
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
+                    float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        f32x4 &two = p[2 * y + (e >> 1)];
-                        float p0 = two[2 * (e & 1)], p1 = two[2 * (e & 1) + 1];
-                        part[e] = split(p0, p1);
-                        two[2 * (e & 1)] = p0;
-                        two[2 * (e & 1) + 1] = p1;
+                        const int j = 32 * y + 16 * z + 4 * g + e;
+                        w[e] = p[z][e] * (a.scale * ex2(static_cast<float>(mine - sm.sum[j])));
+                        asm volatile("" : "+v"(w[e]));  // formed in all lanes: no branch around it
+                        w[e] = j <= 16 * it + col ? w[e] : 0.0f;
                     }
-                    sm.scores[wave][y][z][lane] = part;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        hi[2 * z + e] = split(w[2 * e], w[2 * e + 1]);
+                        lo[2 * z + e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+                    }
                 }
+                sm.scores[unit(it, y)][0][lane] = hi;
+                sm.scores[unit(it, y)][1][lane] = lo;
             }
-            // ---- what the state gives, for all 64 tokens: rows 16 (wave VT + vt) + 4 g + e, token 16 it + col
+            // ---- what the state gives, for all 64 tokens: rows 16 wave + 4 g + e, token 16 it + col
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
-#pragma unroll
-                for (int vt = 0; vt < VT; ++vt) {
-                    o[vt][it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                }
+                o[it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
 #pragma unroll
             for (int x = 0; x < X; ++x) {
-                u32x4 hi[VT], lo[VT];
+                u32x4 hi, lo;
 #pragma unroll
-                for (int vt = 0; vt < VT; ++vt) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float s0 = s[2 * x + (e >> 1)][vt][2 * (e & 1)], s1 = s[2 * x + (e >> 1)][vt][2 * (e & 1) + 1];
-                        hi[vt][e] = split(s0, s1);
-                        lo[vt][e] = pack_bf16x2(s0, s1);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    float s0 = s[2 * x + (e >> 1)][2 * (e & 1)], s1 = s[2 * x + (e >> 1)][2 * (e & 1) + 1];
+                    hi[e] = split(s0, s1);
+                    lo[e] = pack_bf16x2(s0, s1);
                 }
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const u32x4 qx = *reinterpret_cast<const u32x4 *>(sm.q + place<D>(16 * it + col, 4 * x + g));
-#pragma unroll
-                    for (int vt = 0; vt < VT; ++vt) {
-                        o[vt][it] = mfma16(hi[vt], qx, o[vt][it]);
-                        o[vt][it] = mfma16(lo[vt], qx, o[vt][it]);
-                    }
+                for (int it = 0; it < 4; it += 2) {
+                    const u32x4 r0 = *reinterpret_cast<const u32x4 *>(sm.q + place<D>(16 * it + col, 4 * x + g));
+                    const u32x4 r1 = *reinterpret_cast<const u32x4 *>(sm.q + place<D>(16 * it + 16 + col, 4 * x + g));
+                    o[it] = mfma16(hi, r0, o[it]);
+                    o[it + 1] = mfma16(hi, r1, o[it + 1]);
+                    o[it] = mfma16(lo, r0, o[it]);
+                    o[it + 1] = mfma16(lo, r1, o[it + 1]);
                 }
             }
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
-                const float f = sm.early[16 * it + col];
-#pragma unroll
-                for (int vt = 0; vt < VT; ++vt) {
-                    o[vt][it] *= f;
-                }
-            }
-        }
-#pragma unroll
-        for (int vt = 0; vt < VT; ++vt) {
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                values[vt][y] = column<D>(sm.v, 32 * y, wave * VT + vt, lane);
-            }
-        }
-        if constexpr (OUTPUTS) {
-            lds_barrier();  // all scores are there
-#pragma unroll
-            for (int it = 0; it < 4; ++it) {
-#pragma unroll
-                for (int y = 0; y <= it / 2; ++y) {
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const u32x4 part = sm.scores[it][y][z][lane];
-#pragma unroll
-                        for (int vt = 0; vt < VT; ++vt) {
-                            o[vt][it] = mfma16(values[vt][y], part, o[vt][it]);
-                        }
-                    }
-                }
-                const int i = 16 * it + col;
-                if (i < len) {
-                    uint16_t *to = static_cast<uint16_t *>(a.out) +
-                                   (static_cast<int64_t>(pos + i) * a.num_heads + head) * D + 16 * wave * VT + 4 * g;
-#pragma unroll
-                    for (int vt = 0; vt < VT; ++vt) {
-                        const f32x4 y = o[vt][it] * a.scale;
-                        *reinterpret_cast<u32x2 *>(to + 16 * vt) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-                    }
-                }
+                o[it] *= sm.early[16 * it + col];
             }
         }
         // ---- the state
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-            for (int vt = 0; vt < VT; ++vt) {
-                s[kt][vt] *= all;
-            }
+            s[kt] *= all;
         }
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-            u32x4 part[VT][3];
+            values[y] = column<D>(sm.v, 32 * y, wave, lane);
+            u32x4 part[3];
             const f32x4 w0 = *reinterpret_cast<const f32x4 *>(sm.late + 32 * y + 4 * g);
             const f32x4 w1 = *reinterpret_cast<const f32x4 *>(sm.late + 32 * y + 16 + 4 * g);
 #pragma unroll
-            for (int vt = 0; vt < VT; ++vt) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t pair = values[vt][y][e];
-                    float x0 = low_bf16(pair) * (e < 2 ? w0[2 * e] : w1[2 * e - 4]);
-                    float x1 = high_bf16(pair) * (e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
-                    part[vt][0][e] = split(x0, x1);
-                    part[vt][1][e] = split(x0, x1);
-                    part[vt][2][e] = pack_bf16x2(x0, x1);
-                }
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t pair = values[y][e];
+                float x0 = low_bf16(pair) * (e < 2 ? w0[2 * e] : w1[2 * e - 4]);
+                float x1 = high_bf16(pair) * (e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
+                part[0][e] = split(x0, x1);
+                part[1][e] = split(x0, x1);
+                part[2][e] = pack_bf16x2(x0, x1);
             }
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const u32x4 keys = column<D>(sm.k, 32 * y, kt, lane);
+            for (int kt = 0; kt < KT; kt += 2) {
+                u32x4 keys[2];
 #pragma unroll
-                for (int vt = 0; vt < VT; ++vt) {
+                for (int z = 2; z >= 0; --z) {
 #pragma unroll
-                    for (int z = 2; z >= 0; --z) {
-                        s[kt][vt] = mfma16(keys, part[vt][z], s[kt][vt]);
+                    for (int i = 0; i < 2; ++i) {
+                        if (z == 2) {
+                            keys[i] = column<D>(sm.k, 32 * y, kt + i, lane);
+                        }
+                        s[kt + i] = mfma16(keys[i], part[z], s[kt + i]);
                     }
                 }
             }
         }
+        lds_barrier();  // all scores are there, all reads of the chunk's rows are done
         if constexpr (OUTPUTS) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+#pragma unroll
+                    for (int it = 2 * y; it < 4; ++it) {
+                        o[it] = mfma16(values[y], sm.scores[unit(it, y)][z][lane], o[it]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                done[it] = u32x2{pack_bf16x2(o[it][0], o[it][1]), pack_bf16x2(o[it][2], o[it][3])};
+            }
+            done_len = done_step = len;
             if (next == track_at) {
-                float *to = a.pool(track_slot, head) + (16 * wave * VT + col) * D + 4 * g;
+                float *to = a.pool(track_slot, head) + (16 * wave + col) * D + 4 * g;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-                    for (int vt = 0; vt < VT; ++vt) {
-                        *reinterpret_cast<f32x4 *>(to + 16 * vt * D + 16 * kt) = s[kt][vt];
-                    }
+                    *reinterpret_cast<f32x4 *>(to + 16 * kt) = s[kt];
                 }
             }
         }
         pos = next;
         len = next_len;
-        lds_barrier();  // before the next chunk is staged over this one
     }
+    store_done();
     return total;
 }
 
-template <int D> __global__ __launch_bounds__(kThreads, 2) void sums_kernel(const ChunkParams a) {
+template <int D> __global__ __launch_bounds__(kThreads<D>, 4) void sums_kernel(const ChunkParams a) {
     __shared__ __attribute__((aligned(16))) Shared<D, false> sm;
     const int head = blockIdx.x % a.num_heads;
-    const Segment seg = segment_of(a, blockIdx.x / a.num_heads);
-    if (seg.n < 0 || seg.index + 1 >= seg.count) {
+    const Segment seg = segment_of<kThreads<D>>(a, blockIdx.x / a.num_heads);
+    if (seg.n < 0) {
         return;
     }
-    f32x4 s[D / 16][D / 64];
+    f32x4 s[D / 16];
 #pragma unroll
     for (int kt = 0; kt < D / 16; ++kt) {
-#pragma unroll
-        for (int vt = 0; vt < D / 64; ++vt) {
-            s[kt][vt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const double total = walk<D, false>(a, sm, seg, head, s, 0, -1);
     const int64_t at = seg.slot * a.num_heads + head;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float *to = a.starts + at * (D * D) + (16 * wave * (D / 64) + (lane & 15)) * D + 4 * (lane >> 4);
+    float *to = a.starts + at * (D * D) + (16 * wave + (lane & 15)) * D + 4 * (lane >> 4);
 #pragma unroll
     for (int kt = 0; kt < D / 16; ++kt) {
-#pragma unroll
-        for (int vt = 0; vt < D / 64; ++vt) {
-            *reinterpret_cast<f32x4 *>(to + 16 * vt * D + 16 * kt) = s[kt][vt];
-        }
+        *reinterpret_cast<f32x4 *>(to + 16 * kt) = s[kt];
     }
     if (threadIdx.x == 0) {
         a.decays[at] = ex2(static_cast<float>(total));
@@ -434,7 +476,7 @@ template <int D> __global__ __launch_bounds__(kThreads, 2) void sums_kernel(cons
 }
 
 // A thread takes four elements of a state at a time through all of the request's segments.
-template <int D> __global__ __launch_bounds__(kThreads) void starts_kernel(const ChunkParams a, int parts) {
+template <int D> __global__ __launch_bounds__(kStartThreads) void starts_kernel(const ChunkParams a, int parts) {
     const int part = blockIdx.x % parts;
     const int pair = blockIdx.x / parts;
     const int n = pair / a.num_heads, head = pair - n * a.num_heads;
@@ -444,12 +486,12 @@ template <int D> __global__ __launch_bounds__(kThreads) void starts_kernel(const
         return;
     }
     const int64_t slot = a.slot(n), first = 2 * static_cast<int64_t>(begin) / a.segment;
-    for (int e = (part * kThreads + threadIdx.x) * 4; e < D * D; e += parts * kThreads * 4) {
+    for (int e = (part * kStartThreads + threadIdx.x) * 4; e < D * D; e += parts * kStartThreads * 4) {
         f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
         if (slot > 0) {
             s = *reinterpret_cast<const f32x4 *>(a.pool(slot, head) + e);
         }
-        constexpr int kAtOnce = 8;
+        constexpr int kAtOnce = 16;
         for (int i = 0; i < count; i += kAtOnce) {
             f32x4 sum[kAtOnce];
             float decay[kAtOnce];
@@ -470,52 +512,62 @@ template <int D> __global__ __launch_bounds__(kThreads) void starts_kernel(const
     }
 }
 
-template <int D> __global__ __launch_bounds__(kThreads, 2) void outputs_kernel(const ChunkParams a) {
+template <int D> __global__ __launch_bounds__(kThreads<D>, 4) void outputs_kernel(const ChunkParams a) {
     __shared__ __attribute__((aligned(16))) Shared<D, true> sm;
-    linear_zero_uncovered<D, uint16_t>(a, blockIdx.x, gridDim.x);
+    linear_zero_uncovered<D, uint16_t, kThreads<D>>(a, blockIdx.x, gridDim.x);
     const int head = blockIdx.x % a.num_heads;
-    const Segment seg = segment_of(a, blockIdx.x / a.num_heads);
+    const Segment seg = segment_of<kThreads<D>>(a, blockIdx.x / a.num_heads);
     if (seg.n < 0) {
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int at = (16 * wave * (D / 64) + (lane & 15)) * D + 4 * (lane >> 4);
-    const int64_t slot = a.slot(seg.n);
-    f32x4 s[D / 16][D / 64];
+    const int at = (16 * wave + (lane & 15)) * D + 4 * (lane >> 4);
+    const int64_t slot = uniform(a.slot(seg.n)), track_slot = uniform(a.track_slot(seg.n));
+    const int64_t track_len = track_slot > 0 ? a.track_len(seg.n) : -1;
+    f32x4 s[D / 16];
     const float *from = seg.count > 1 ? a.starts + (seg.slot * a.num_heads + head) * (D * D) : slot > 0 ? a.pool(slot, head) : nullptr;
 #pragma unroll
     for (int kt = 0; kt < D / 16; ++kt) {
+        s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (from != nullptr) {
 #pragma unroll
-        for (int vt = 0; vt < D / 64; ++vt) {
-            s[kt][vt] = from == nullptr ? f32x4{0.0f, 0.0f, 0.0f, 0.0f}
-                                        : *reinterpret_cast<const f32x4 *>(from + at + 16 * vt * D + 16 * kt);
+        for (int kt = 0; kt < D / 16; ++kt) {
+            s[kt] = *reinterpret_cast<const f32x4 *>(from + at + 16 * kt);
         }
     }
     auto store = [&](int64_t to_slot) KDA_INLINE {
         float *to = a.pool(to_slot, head) + at;
 #pragma unroll
         for (int kt = 0; kt < D / 16; ++kt) {
-#pragma unroll
-            for (int vt = 0; vt < D / 64; ++vt) {
-                *reinterpret_cast<f32x4 *>(to + 16 * vt * D + 16 * kt) = s[kt][vt];
-            }
+            *reinterpret_cast<f32x4 *>(to + 16 * kt) = s[kt];
         }
     };
-    const int64_t track_slot = a.track_slot(seg.n);
-    const int64_t track_len = track_slot > 0 ? a.track_len(seg.n) : -1;
     if (track_len == 0 && seg.index == 0) {
         store(track_slot);
     }
-    walk<D, true>(a, sm, seg, head, s, track_slot, track_len > 0 ? seg.request_begin + track_len : -1);
+    const bool here = track_len > seg.begin - seg.request_begin && track_len <= seg.end - seg.request_begin;
+    walk<D, true>(a, sm, seg, head, s, track_slot,
+                  __builtin_amdgcn_readfirstlane(here ? seg.request_begin + static_cast<int>(track_len) : -1));
     if (slot > 0 && seg.index + 1 == seg.count && seg.begin < seg.end) {
         store(slot);
     }
 }
 
-// Two workgroups a CU where all segments are whole.
+// A segment's tokens. As many workgroups as the card holds at once (two a CU of heads of 128, six of 64) where
+// segments are then long, at least as many as it has CUs elsewhere; not so short that the states between
+// them outweigh them, the less so the more requests and heads there are. Up to 320 tokens go as they are: 256 tokens
+// on 16 heads 27.6 us so, 30.0 in segments of 128 (320: 32.9 and 29.7). us, heads of 128, with segments of 128, 192 and 256:
+//   16001 tokens, 4 heads  62 65 55    5311, 16 heads  65 65 72    4096, 16  70 61 63    32768, 2  84 72 72
 int segment_of_call(const KdaLinearArgs &a) {
-    const int64_t per = (static_cast<int64_t>(a.num_tokens) * a.num_heads + 511) / 512;
-    return static_cast<int>(std::min<int64_t>(std::max<int64_t>((per + kChunk - 1) / kChunk, 2), 1 << 20) * kChunk);
+    const int64_t work = static_cast<int64_t>(a.num_tokens) * a.num_heads;
+    const int64_t pairs = static_cast<int64_t>(a.num_seqs) * a.num_heads;
+    int64_t tokens = work / (a.head_dim == 128 ? 512 : 1536);
+    if (a.head_dim == 128) {
+        tokens = std::max<int64_t>(tokens, std::min<int64_t>(work / 256, 256));
+    }
+    tokens = std::max<int64_t>(tokens, a.num_tokens <= 320 ? 320 : std::min<int64_t>(std::max<int64_t>(pairs, 128), 512));
+    return static_cast<int>(std::min<int64_t>((tokens + kChunk - 1) / kChunk, 1 << 20) * kChunk);
 }
 
 struct Plan {
@@ -536,17 +588,18 @@ Plan plan_of(const KdaLinearArgs &a) {
 }
 
 template <int D> int launch(const ChunkParams &a, const Plan &p, hipStream_t s) {
-    const int64_t blocks = (static_cast<int64_t>(a.num_tokens) / a.segment + a.num_seqs) * a.num_heads;
-    if (blocks > (INT64_C(1) << 24) - 1) {  // a grid counts its threads in 32 bits
+    const int64_t whole = static_cast<int64_t>(a.num_tokens) / a.segment * a.num_heads;
+    const int64_t blocks = whole + static_cast<int64_t>(a.num_seqs) * a.num_heads;
+    if (blocks * kThreads<D> > UINT32_MAX) {  // a grid counts its threads in 32 bits
         return KDA_ERR_TOO_LARGE;
     }
     if (p.slots > 0) {
-        sums_kernel<D><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a);
+        sums_kernel<D><<<static_cast<unsigned>(whole), kThreads<D>, 0, s>>>(a);
         const int64_t pairs = static_cast<int64_t>(a.num_seqs) * a.num_heads;
-        const int parts = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1024 / pairs, 1), D * D / (4 * kThreads)));
-        starts_kernel<D><<<static_cast<unsigned>(pairs * parts), kThreads, 0, s>>>(a, parts);
+        const int parts = static_cast<int>(std::min<int64_t>(std::max<int64_t>(4096 / pairs, 1), D * D / (4 * kStartThreads)));
+        starts_kernel<D><<<static_cast<unsigned>(pairs * parts), kStartThreads, 0, s>>>(a, parts);
     }
-    outputs_kernel<D><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a);
+    outputs_kernel<D><<<static_cast<unsigned>(blocks), kThreads<D>, 0, s>>>(a);
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 

@@ -10,9 +10,14 @@
 namespace kda {
 
 struct LinearParams : KdaLinearArgs {
-    // An entry of the metadata, whole.
+    // An entry of the metadata, whole: two words of an int64 one, the same word twice of an int32 one. Without a branch,
+    // so that the loads of several arrays are in flight together.
     __device__ __forceinline__ int64_t entry(const void *p, int n, int bit) const {
-        return (wide & bit) != 0 ? static_cast<const int64_t *>(p)[n] : static_cast<const int32_t *>(p)[n];
+        const int both = (wide & bit) != 0 ? 1 : 0;
+        const char *at = static_cast<const char *>(p) + (static_cast<uint64_t>(static_cast<uint32_t>(n)) << (2 + both));
+        const int32_t low = *reinterpret_cast<const int32_t *>(at);
+        const int32_t high = *reinterpret_cast<const int32_t *>(at + 4 * both);
+        return both != 0 ? static_cast<int64_t>(high) << 32 | static_cast<uint32_t>(low) : low;
     }
     // Token offsets cut to the tensors, whatever the metadata says.
     __device__ __forceinline__ int cu(int n) const {
@@ -31,15 +36,15 @@ struct LinearParams : KdaLinearArgs {
     }
 };
 
-// Tokens that no request covers: zeros, spread over a grid of 256 threads each.
-template <int D, typename T>
+// Tokens that no request covers: zeros, spread over a grid.
+template <int D, typename T, int THREADS>
 __device__ __forceinline__ void linear_zero_uncovered(const LinearParams &a, int64_t block, int64_t blocks) {
     const int64_t begin = a.cu(0), end = max(a.cu(a.num_seqs), a.cu(0));
     const int64_t count = begin + (a.num_tokens - end);
     const int64_t row = static_cast<int64_t>(a.num_heads) * D;
     for (int64_t i = block; i < count; i += blocks) {
         T *out = static_cast<T *>(a.out) + (i < begin ? i : end + (i - begin)) * row;
-        for (int64_t e = threadIdx.x; e < row; e += 256) {
+        for (int64_t e = threadIdx.x; e < row; e += THREADS) {
             out[e] = T(0);
         }
     }

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(const Linear
     constexpr int kRows = kThreads / kLanes * NP;     // rows of a workgroup
     constexpr int kTiles = D / kRows;                 // workgroups of a (request, head)
     static_assert(kTiles * kRows == D);
-    linear_zero_uncovered<D, T>(a, blockIdx.x, gridDim.x);
+    linear_zero_uncovered<D, T, kThreads>(a, blockIdx.x, gridDim.x);
     const int tile = blockIdx.x % kTiles;
     const int pair = blockIdx.x / kTiles;
     const int n = pair / a.num_heads;

@@ -480,8 +480,8 @@ template <int D> __global__ __launch_bounds__(kStartThreads) void starts_kernel(
     const int part = blockIdx.x % parts;
     const int pair = blockIdx.x / parts;
     const int n = pair / a.num_heads, head = pair - n * a.num_heads;
-    const int begin = a.cu(n), end = max(a.cu(n + 1), begin);
-    const int count = (end - begin + a.segment - 1) / a.segment;
+    const int begin = __builtin_amdgcn_readfirstlane(a.cu(n)), end = max(a.cu(n + 1), begin);
+    const int count = __builtin_amdgcn_readfirstlane((end - begin + a.segment - 1) / a.segment);
     if (count < 2) {
         return;
     }
@@ -494,17 +494,21 @@ template <int D> __global__ __launch_bounds__(kStartThreads) void starts_kernel(
         constexpr int kAtOnce = 16;
         for (int i = 0; i < count; i += kAtOnce) {
             f32x4 sum[kAtOnce];
-            float decay[kAtOnce];
+            float decay[kAtOnce];  // the last segment has neither
 #pragma unroll
             for (int x = 0; x < kAtOnce; ++x) {
-                const int64_t at = (first + min(i + x, count - 2)) * a.num_heads + head;
-                sum[x] = *reinterpret_cast<const f32x4 *>(a.starts + at * (D * D) + e);
-                decay[x] = a.decays[at];
+                if (i + x + 1 < count) {
+                    const int64_t at = (first + i + x) * a.num_heads + head;
+                    sum[x] = *reinterpret_cast<const f32x4 *>(a.starts + at * (D * D) + e);
+                    decay[x] = a.decays[at];
+                }
             }
 #pragma unroll
             for (int x = 0; x < kAtOnce; ++x) {
                 if (i + x < count) {
                     *reinterpret_cast<f32x4 *>(a.starts + ((first + i + x) * a.num_heads + head) * (D * D) + e) = s;
+                }
+                if (i + x + 1 < count) {
                     s = s * decay[x] + sum[x];
                 }
             }

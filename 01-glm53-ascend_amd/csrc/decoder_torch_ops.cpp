@@ -1,4 +1,4 @@
-// decoder_torch_ops.cpp -- torch operators of a decoder's norms and paged attention.
+// decoder_torch_ops.cpp -- torch operators of a decoder's norms, paged attention and sampling.
 //
 // The parts of a hybrid decoder that stand beside its KDA layers, in the same
 // operator namespace and manner as those: each op validates what its kernel indexes
@@ -298,6 +298,61 @@ at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const
     return out;
 }
 
+// ---------------------------------------------------------------------------
+// sample_tokens
+// ---------------------------------------------------------------------------
+
+std::tuple<at::Tensor, at::Tensor> sample_tokens(const at::Tensor &logits, const at::Tensor &uniforms,
+                                                 const std::optional<at::Tensor> &temperature,
+                                                 const std::optional<at::Tensor> &top_k,
+                                                 const std::optional<at::Tensor> &top_p,
+                                                 const std::optional<at::Tensor> &min_p) {
+    const char *op = "sample_tokens";
+    TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, op, " expects logits as [rows, vocab]");
+    TORCH_CHECK(bf16_or_fp32(logits), op, ": logits must be bf16 or fp32");
+    TORCH_CHECK(logits.size(1) == 1 || logits.stride(1) == 1, op, ": logits must be contiguous in the vocabulary");
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    TORCH_CHECK(vocab <= INT32_MAX - (1 << 16) && rows <= UINT32_MAX / 1024, op, " supports fewer than 2^22 rows of 2^31 - 2^16 logits");
+    const auto check = [&](const char *name, const at::Tensor &t) {
+        TORCH_CHECK(t.dim() == 1 && t.size(0) == rows && t.is_contiguous(), op, ": ", name,
+                    " must be contiguous with an entry per row of logits");
+        check_same_device(logits, name, t, "logits");
+    };
+    check("uniforms", uniforms);
+    TORCH_CHECK(uniforms.scalar_type() == at::kFloat, "uniforms must be fp32");
+    KdaSampleArgs a{};
+    for (const auto &[name, t, to] :
+         {std::tuple<const char *, const std::optional<at::Tensor> &, const float **>{"temperature", temperature, &a.temperature},
+          {"top_p", top_p, &a.top_p},
+          {"min_p", min_p, &a.min_p}}) {
+        if (t.has_value()) {
+            check(name, *t);
+            TORCH_CHECK(t->scalar_type() == at::kFloat, name, " must be fp32");
+            *to = t->data_ptr<float>();
+        }
+    }
+    if (top_k.has_value()) {
+        check("top_k", *top_k);
+        TORCH_CHECK(top_k->scalar_type() == at::kInt || top_k->scalar_type() == at::kLong, "top_k must be int32 or int64");
+        a.top_k = top_k->data_ptr();
+        a.top_k_int64 = top_k->scalar_type() == at::kLong ? 1 : 0;
+    }
+    check_on_gpu("logits", logits);
+    const c10::DeviceGuard device_guard(logits.device());
+    at::Tensor tokens = at::empty({rows}, logits.options().dtype(at::kLong));
+    at::Tensor logprobs = at::empty({rows}, logits.options().dtype(at::kFloat));
+    a.logits = logits.data_ptr();
+    a.logits_stride = logits.stride(0);
+    a.uniforms = uniforms.data_ptr<float>();
+    a.tokens = tokens.data_ptr<int64_t>();
+    a.logprobs = logprobs.data_ptr<float>();
+    a.rows = rows;
+    a.vocab = static_cast<int32_t>(vocab);
+    a.dtype = dtype_of(logits);
+    check_ok(kda_sample_launch(&a, stream_of(logits)), op);
+    return {tokens, logprobs};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(sgl_glm53_ascend, m) {
@@ -312,13 +367,17 @@ TORCH_LIBRARY_FRAGMENT(sgl_glm53_ascend, m) {
         "paged_attention(Tensor q, *, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor kv_lens, "
         "Tensor cu_seqlens, float scale, int max_query_len, int window=0, float logit_cap=0.0, "
         "Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor");
+    m.def(
+        "sample_tokens(Tensor logits, Tensor uniforms, *, Tensor? temperature=None, Tensor? top_k=None, "
+        "Tensor? top_p=None, Tensor? min_p=None) -> (Tensor, Tensor)");
 }
 
 #define DECODER_REGISTER_IMPLS(m)                    \
     m.impl("add_rms_norm", &add_rms_norm);           \
     m.impl("add_rms_norm_fp8", &add_rms_norm_fp8);   \
     m.impl("paged_kv_store", &paged_kv_store);       \
-    m.impl("paged_attention", &paged_attention)
+    m.impl("paged_attention", &paged_attention);     \
+    m.impl("sample_tokens", &sample_tokens)
 
 TORCH_LIBRARY_IMPL(sgl_glm53_ascend, CUDA, m) { DECODER_REGISTER_IMPLS(m); }
 

@@ -32,7 +32,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = os.environ.get("KDA_OFFLOAD_ARCH", "gfx950")
 
 HIP_SOURCES = ["kda_recurrent.hip", "kda_chunk.hip", "linear_recurrent.hip", "linear_chunk.hip", "rms_norm.hip",
-               "paged_store.hip", "paged_attention.hip"]
+               "paged_store.hip", "paged_attention.hip", "sample.hip"]
 ABI_SOURCES = ["kda_abi.cpp"]
 TORCH_SOURCES = ["kda_torch_ops.cpp", "linear_torch_ops.cpp", "decoder_torch_ops.cpp"]
 

@@ -1,4 +1,4 @@
-from .decoder import add_rms_norm, add_rms_norm_fp8, paged_attention, paged_kv_store
+from .decoder import add_rms_norm, add_rms_norm_fp8, paged_attention, paged_kv_store, sample_tokens
 from .kda import (
     kda_prepared_varlen_chunk,
     kda_prepared_varlen_recurrent,
@@ -26,4 +26,5 @@ __all__ = [
     "paged_attention",
     "paged_kv_store",
     "prepared_recurrent",
+    "sample_tokens",
 ]

@@ -2,9 +2,9 @@
 
 A model that interleaves KDA layers with full attention needs these beside
 ``ops.kda``: the residual RMS norm in front of every projection (with an 8-bit
-output where the projection is an 8-bit product), and for the full-attention
-layers a paged key/value cache, its writer and the attention that reads it. The
-reference package has no counterpart. Like the KDA operators they enqueue on the
+output where the projection is an 8-bit product), for the full-attention
+layers a paged key/value cache, its writer and the attention that reads it, and at its
+end the choice of a token. The reference package has no counterpart. Like the KDA operators they enqueue on the
 current stream, never synchronize the host and can be captured in a HIP graph.
 """
 
@@ -113,3 +113,29 @@ def paged_attention(
         cu_seqlens=cu_seqlens, scale=scale, max_query_len=max_query_len, window=window,
         logit_cap=logit_cap, k_scale=k_scale, v_scale=v_scale,
     )
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    *,
+    temperature: Optional[torch.Tensor] = None,
+    top_k: Optional[torch.Tensor] = None,
+    top_p: Optional[torch.Tensor] = None,
+    min_p: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A token drawn from every row of logits, and the log of its probability.
+
+    ``logits`` is bf16 or fp32 ``[rows, vocab]``, ``uniforms`` the fp32 random numbers in
+    [0, 1), one a row; so are the fp32 ``temperature``, ``top_p``, ``min_p`` and the int32 or int64 ``top_k``
+    (None: 1, 1, 0 and all). With the weights ``exp((l - max l) / temperature)``, kept are the
+    ``top_k`` largest (of equal ones the lowest indices; not above 0: all), of those in falling order each before
+    which less than ``top_p`` of their mass lies, of those the ones of at least ``min_p``
+    (the largest always is). The token is the first in the vocabulary's order at which the kept mass so far
+    exceeds ``uniform`` of the whole: the same for the same inputs, whatever else is in the batch.
+
+    A temperature that is not above 0 takes the first largest logit. -infinity and NaN are never
+    drawn; a row with nothing to draw gets -1 (and -infinity). Returns int64 tokens and fp32
+    log probabilities, ``[rows]`` each.
+    """
+    return _OPS.sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)

@@ -41,8 +41,8 @@
  * Beside the KDA entry points stand those of the other parts of a decoder that
  * interleaves KDA layers with others (no counterpart in the reference): linear
  * attention with a decay for each head (kda_linear_recurrent_launch,
- * kda_linear_chunk_launch), kda_rms_norm_launch, kda_paged_store_launch and
- * kda_paged_attention_launch.
+ * kda_linear_chunk_launch), kda_rms_norm_launch, kda_paged_store_launch,
+ * kda_paged_attention_launch, and kda_sample_launch for its answer.
  *
  * All launches are asynchronous on `stream` and never synchronize the host.
  * Every function returns a KdaStatus (0 = success).
@@ -371,6 +371,35 @@ typedef struct KdaRmsNormArgs {
 /* Pointers need their element's alignment only; rows of out and of the residual
  * must not overlap (stride >= width). */
 int kda_rms_norm_launch(const KdaRmsNormArgs *args, void *stream);
+
+/* A token drawn from every row of logits [rows, vocab], with the uniform number given for the row.
+ * With the weights w_i = exp((l_i - max l) / temperature), kept are
+ *   the top_k largest (of equal ones those of the lowest index),
+ *   of those, in falling order, each before which less than top_p of their mass lies,
+ *   of those the ones with w_i >= min_p (the largest always is);
+ * the token is the first in the vocabulary's order at which the kept mass so far exceeds
+ * uniform * (whole kept mass), its log probability the log of its share of that mass.
+ * A temperature that is not above 0 takes the first largest logit (log probability 0).
+ * -infinity and NaN are never drawn, infinite logits share the mass; a row with nothing to
+ * draw gets -1 and -infinity. Weights are formed in 64 bits and summed as multiples of 2^-s, s at most 51
+ * and as large as vocab * 2^s <= 2^62 allows. */
+typedef struct KdaSampleArgs {
+    const void *logits; /* [rows, vocab], bf16 or fp32 */
+    int64_t logits_stride; /* elements between rows */
+    const float *uniforms;    /* [rows], in [0, 1): outside it counts as its ends */
+    const float *temperature; /* [rows], or null: 1 */
+    const void *top_k;        /* [rows] int32 (or int64), not above 0: all; or null: all */
+    const float *top_p;       /* [rows], 1 and above (and NaN): all; or null: all */
+    const float *min_p;       /* [rows], or null: 0 */
+    int64_t *tokens;          /* [rows] */
+    float *logprobs;          /* [rows] */
+    int64_t rows;
+    int32_t vocab;
+    int32_t dtype; /* of the logits: KDA_BF16 or KDA_F32 */
+    int32_t top_k_int64;
+} KdaSampleArgs;
+
+int kda_sample_launch(const KdaSampleArgs *args, void *stream);
 
 /* A paged key/value cache: token `off` of page `p` and key head h are head_dim
  * contiguous elements at base + p * stride_page + off * stride_token + h * stride_head

@@ -59,7 +59,7 @@ struct Shared {
     u64 list[kList];
     u64 blocks[kMaxBlocks];
     u64 weights[kFew];
-    double powers[256];  // 2^{j / 256}
+    double powers[256];  // 2^{S + j / 256}
     u64 waves[kWaves];
     float tops[kWaves];
     int places[kWaves];
@@ -80,19 +80,23 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 __device__ __forceinline__ u64 rank_of(uint32_t key, uint32_t index) { return static_cast<u64>(key) << 32 | (0xffffffffu - index); }
 __device__ __forceinline__ uint32_t index_of(u64 rank) { return 0xffffffffu - static_cast<uint32_t>(rank); }
 
-__device__ __forceinline__ u64 up64(u64 x, int d) {
-    return static_cast<u64>(__shfl_up(static_cast<unsigned long long>(x), d));
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 add_from(u64 x) {
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(x >> 32), CTRL, ROWS, 0xf, false);
+    return x + (static_cast<u64>(high) << 32 | low);
 }
-
 // The sum of the values of this lane and those before it in the wave.
 __device__ __forceinline__ u64 wave_scan(u64 x) {
-    const int lane = static_cast<int>(__lane_id());
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 up = up64(x, d);
-        x += lane >= d ? up : 0;
-    }
-    return x;
+    x = add_from<0x111, 0xf>(x);  // one lane up within 16, then two, four and eight
+    x = add_from<0x112, 0xf>(x);
+    x = add_from<0x114, 0xf>(x);
+    x = add_from<0x118, 0xf>(x);
+    x = add_from<0x142, 0xa>(x);  // lane 15 to the second 16, lane 47 to the fourth
+    return add_from<0x143, 0xc>(x);  // lane 31 to the upper half
+}
+__device__ __forceinline__ u64 last_lane(u64 x) {
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(x), 63);
+    return static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), 63))) << 32 | low;
 }
 // ... of this thread and those before it, and the sum of all. By all threads.
 __device__ __forceinline__ u64 block_scan(Shared &sm, u64 x, u64 &total) {
@@ -132,23 +136,21 @@ __device__ __forceinline__ void sort(Shared &sm, int size) {
 }
 __device__ __forceinline__ int power_above(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
-// A row's logits; NaN counts as -infinity, and where the maximum is infinite all but it do.
+// A row's logits. Comparisons are written such that NaN fails them: it counts as -infinity.
 template <typename T> struct Row {
     static constexpr int E = 16 / sizeof(T);
     static constexpr int kGroup = 64 * E * kUnroll;  // elements that a wave loads at a time
     const T *at;
     int size;
-    float least, most;
 
     struct __attribute__((packed, aligned(sizeof(T)))) Raw {
         u32x4 w;
     };
-    __device__ __forceinline__ float value(float x) const {
-        x = x >= least ? x : -kInf;  // false for NaN
-        return fminf(x, most);
-    }
+    struct Group {
+        u32x4 w[kUnroll];
+    };
     // E logits from element `first`, beyond the row -infinity
-    __device__ __forceinline__ u32x4 raw(int first) const {
+    __device__ __forceinline__ u32x4 guarded(int64_t first) const {
         if (first + E <= size) {
             return reinterpret_cast<const Raw *>(at + first)->w;
         }
@@ -172,56 +174,79 @@ template <typename T> struct Row {
             return __uint_as_float((i & 1) != 0 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
         }
     }
-    // f(first index, E values) for the lane's loads of group `group`
-    template <class F> __device__ __forceinline__ void each(int group, F f) const {
-        const int64_t first = static_cast<int64_t>(group) * kGroup + static_cast<int>(__lane_id()) * E;
-        u32x4 w[kUnroll];
+    __device__ __forceinline__ Group load(int64_t group) const {
+        const int64_t begin = group * kGroup;
+        const int lane = static_cast<int>(__lane_id()) * E;
+        Group r;
+        if (begin + kGroup <= size) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t x = first + u * 64 * E;
-            w[u] = raw(static_cast<int>(x < size ? x : size));
+            for (int u = 0; u < kUnroll; ++u) {
+                r.w[u] = reinterpret_cast<const Raw *>(at + begin + u * 64 * E + lane)->w;
+            }
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+                for (int i = 0; i + 1 < kUnroll; ++i) {
+                    r.w[i] = r.w[i + 1];
+                }
+                r.w[kUnroll - 1] = guarded(begin + u * 64 * E + lane);
+            }
         }
-        // a loop, the loads handed down in it: unrolled, the passes' code would not fit the instruction cache
+        return r;
+    }
+    // f(index of the first, E logits) for the lane's loads of a group. A loop, the loads handed down in it: unrolled, the
+    // passes' code would not fit the instruction cache.
+    template <class F> __device__ __forceinline__ void each(int64_t group, Group r, F f) const {
+        const int first = static_cast<int>(group * kGroup) + static_cast<int>(__lane_id()) * E;
 #pragma unroll 1
         for (int u = 0; u < kUnroll; ++u) {
-            f(static_cast<int>(first + u * 64 * E), w[0]);
+            f(first + u * 64 * E, r.w[0]);
 #pragma unroll
             for (int i = 0; i + 1 < kUnroll; ++i) {
-                w[i] = w[i + 1];
+                r.w[i] = r.w[i + 1];
             }
         }
     }
 };
 
+enum Mode { kNumbers, kNucleus, kLeft };
+
 template <typename T> struct Sampler {
     const SampleParams &a;
     Shared &sm;
     Row<T> row;
-    float top;       // the largest logit
-    double scale;    // log2(e) / temperature
+    float top;            // the largest logit
+    double scale;         // 256 log2(e) / temperature
     float bin_scale;
-    float last;      // the last element in the order of the ranks that is not cut
+    float last;           // the last element in the order of the ranks that is not cut
     int last_index;
-    double least_weight;  // 0: none
+    double least_weight;  // min_p 2^S
+    float least;          // logits below it are cut or do not reach min_p (some others do neither)
 
     static constexpr int E = Row<T>::E;
+    static constexpr u64 kBias = 0x4330000000000000ull;  // the bits of 2^52
 
-    // log2 of a weight
+    // 256 log2 of a weight
     __device__ __forceinline__ double exponent(float x) const { return (static_cast<double>(x) - static_cast<double>(top)) * scale; }
-    // Of an element; `kept`: it reaches min_p.
-    __device__ __forceinline__ u64 weight(float x, bool &kept) const {
-        const double t = exponent(x) * 256.0;
+    // A weight times 2^S, not rounded; 0 where `in` does not hold.
+    __device__ __forceinline__ double scaled_weight(float x, bool in) const {
+        const double t = exponent(x);
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
-        const double k = fmax(t, -16384.0) + kMagic;   // 2^-64 at least
-        const int whole = static_cast<int>(static_cast<uint32_t>(__double_as_longlong(k)));
+        const double k = t + kMagic;
+        const int whole = __double2loint(k);
         const double r = t - (k - kMagic);
         constexpr double c1 = kLn2 / 256.0, c2 = c1 * c1 / 2.0, c3 = c2 * c1 / 3.0, c4 = c3 * c1 / 4.0;
         const double p = sm.powers[whole & 255] * fma(r, fma(r, fma(r, fma(r, c4, c3), c2), c1), 1.0);
-        kept = __builtin_amdgcn_ldexp(p, whole >> 8) >= least_weight;
-        constexpr double kTwo52 = 4503599627370496.0;
-        const double w = __builtin_amdgcn_ldexp(p, (whole >> 8) + a.shift) + kTwo52;
-        return t > -16384.0 ? static_cast<u64>(__double_as_longlong(w)) & 0xfffffffffffffull : 0;
+        const int high = __double2hiint(p) + static_cast<int>(static_cast<uint32_t>(whole & ~255) << 12);  // times 2^(whole / 256)
+        // below 2^-64 (and for NaN) 0; with a high word of 0 the number is far below 1, which is as good
+        return __hiloint2double(in && t > -16384.0 ? high : 0, __double2loint(p));
     }
+    // Such a number rounded to a whole one, plus kBias.
+    static __device__ __forceinline__ u64 biased(double w) {
+        return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0));
+    }
+    __device__ __forceinline__ u64 weight(float x) const { return biased(scaled_weight(x, true)) - kBias; }
     // Larger for smaller logits.
     __device__ __forceinline__ int bin(float x) const {
         return static_cast<int>(fminf((top - x) * bin_scale, static_cast<float>(kBins - 1)));
@@ -229,48 +254,146 @@ template <typename T> struct Sampler {
     __device__ __forceinline__ bool passes(float x, int index) const {
         return x > last || (x == last && index <= last_index);
     }
-    // f(index, value) for every element, group by group; after(block) when a block's are done
+    // Of an element that is left.
+    __device__ __forceinline__ u64 kept(int index, float x) const {
+        const double w = scaled_weight(x, passes(x, index));
+        return w >= least_weight ? biased(w) - kBias : 0;
+    }
+    // f(index of the first, E logits) for every load, group by group, the next group's loads in flight; after(block) when a
+    // block's are done.
     template <class F, class G> __device__ __forceinline__ void pass(F f, G after) const {
-        const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-        const int64_t per = static_cast<int64_t>(a.groups) * Row<T>::kGroup;
-        for (int block = wave; block * per < row.size; block += kWaves) {
-            for (int i = 0; i < a.groups && (static_cast<int64_t>(block) * a.groups + i) * Row<T>::kGroup < row.size; ++i) {
-                row.each(block * a.groups + i, [&](int first, u32x4 w) KDA_INLINE {
+        const int64_t groups = (row.size + Row<T>::kGroup - 1) / Row<T>::kGroup;
+        int block = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+        int64_t at = static_cast<int64_t>(block) * a.groups;
+        if (at >= groups) {
+            return;
+        }
+        typename Row<T>::Group now = row.load(at);
+        for (;;) {
+            int64_t next = at + 1;
+            const bool done = next >= groups || next == static_cast<int64_t>(block + 1) * a.groups;
+            if (done) {
+                next = static_cast<int64_t>(block + kWaves) * a.groups;
+            }
+            typename Row<T>::Group ahead = now;
+            if (next < groups) {
+                ahead = row.load(next);
+            }
+            row.each(at, now, f);
+            if (done) {
+                after(block);
+                block += kWaves;
+            }
+            if (next >= groups) {
+                break;
+            }
+            now = ahead;
+            at = next;
+        }
+    }
+    // f(index, x) for the elements for which test(x) holds, few in earnest
+    template <class Test, class F> __device__ __forceinline__ void pass_some(Test test, F f) const {
+        pass(
+            [&](int first, u32x4 w) KDA_INLINE {
+                bool some = false;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    some |= test(Row<T>::element(w, e));
+                }
+                if (__any(some)) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        f(first + e, row.value(Row<T>::element(w, e)));
-                        if (e % 4 == 3) {
-                            __builtin_amdgcn_sched_barrier(0);  // four at a time: all at once do not fit the registers
+                        const float x = Row<T>::element(w, e);
+                        if (test(x)) {
+                            f(first + e, x);
                         }
                     }
-                });
-            }
-            after(block);
-        }
+                }
+            },
+            [](int) {});
     }
     __device__ __forceinline__ int blocks() const {
         const int64_t per = static_cast<int64_t>(a.groups) * Row<T>::kGroup;
         return static_cast<int>((row.size + per - 1) / per);
     }
-    // The blocks' masses of w(index, value); their sum. By all threads.
-    template <class W> __device__ __forceinline__ u64 block_masses(W w) {
-        u64 mine = 0;
-        pass([&](int index, float x) KDA_INLINE { mine += w(index, x); },
-             [&](int block) KDA_INLINE {
-                 const u64 sum = wave_scan(mine);
-                 if (__lane_id() == 63) {
-                     sm.blocks[block] = sum;
-                 }
-                 mine = 0;
-             });
-        return all_blocks();
-    }
+    // The sum of the blocks' masses, once they are there. By all threads.
     __device__ __forceinline__ u64 all_blocks() {
         __syncthreads();
         u64 total;
         const int n = blocks(), i = 2 * static_cast<int>(threadIdx.x);
         block_scan(sm, (i < n ? sm.blocks[i] : 0) + (i + 1 < n ? sm.blocks[i + 1] : 0), total);
         return total;
+    }
+    __device__ __forceinline__ void block_done(int block, u64 &mine) {
+        const u64 sum = last_lane(wave_scan(mine));
+        if (__lane_id() == 0) {
+            sm.blocks[block] = sum;
+        }
+        mine = 0;
+    }
+    // The blocks' masses of what is left (kNucleus: and the bins' of all that pass; kNumbers: only the bins' numbers); their sum.
+    template <bool CUT> __device__ __forceinline__ u64 masses(Mode mode) {
+        u64 mine = 0;
+        pass(
+            [&](int first, u32x4 w) KDA_INLINE {
+                if (mode == kNumbers) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float x = Row<T>::element(w, e);
+                        if (x > -kInf) {
+                            atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[bin(x)]), 1ull);
+                        }
+                    }
+                    return;
+                }
+                if (mode == kLeft) {
+                    bool some = false;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        some |= Row<T>::element(w, e) >= least;
+                    }
+                    if (!__any(some)) {
+                        return;
+                    }
+                }
+#pragma unroll
+                for (int part = 0; part < E; part += 4) {
+                    u64 m[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = Row<T>::element(w, part + e);
+                        const double v = scaled_weight(x, CUT ? passes(x, first + part + e) : true);
+                        m[e] = biased(v);
+                        mine += v >= least_weight ? m[e] : kBias;
+                    }
+                    if (mode == kNucleus) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (!CUT || m[e] != kBias) {  // 0 is added to a bin sooner than looked for
+                                atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[bin(Row<T>::element(w, part + e))]),
+                                          static_cast<unsigned long long>(m[e] - kBias));
+                            }
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // four at a time: all at once do not fit the registers
+                }
+                mine -= E * kBias;
+            },
+            [&](int block) KDA_INLINE { block_done(block, mine); });
+        return all_blocks();
+    }
+    // The blocks' numbers of elements equal to x that pass; their sum.
+    __device__ __forceinline__ u64 numbers_of(float x) {
+        u64 mine = 0;
+        pass(
+            [&](int first, u32x4 w) KDA_INLINE {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    mine += Row<T>::element(w, e) == x && passes(x, first + e) ? 1 : 0;
+                }
+            },
+            [&](int block) KDA_INLINE { block_done(block, mine); });
+        return all_blocks();
     }
     // The first element in the vocabulary's order where the sum of w(index, value) reaches `target` (1 to the sum of
     // the blocks' masses), in every thread.
@@ -285,35 +408,39 @@ template <typename T> struct Sampler {
             sm.before = second ? sum - m1 : sum - m0 - m1;
         }
         __syncthreads();
-        if (threadIdx.x < 64) {
-            const int block = __builtin_amdgcn_readfirstlane(sm.count);
-            u64 before = sm.before;
-            bool done = false;
-            for (int g = 0; g < a.groups && !done && (static_cast<int64_t>(block) * a.groups + g) * Row<T>::kGroup < row.size; ++g) {
-                row.each(block * a.groups + g, [&](int first, u32x4 raw) KDA_INLINE {
-                    u64 m[E], mine = 0;
+        // a wave for each load of a group
+        const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+        const int64_t first_group = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(sm.count)) * a.groups;
+        u64 before = sm.before;
+        for (int64_t g = first_group; g < first_group + a.groups; ++g) {
+            u64 m[E], mine = 0;
+            const int64_t first = g * Row<T>::kGroup + (wave * 64 + static_cast<int>(__lane_id())) * E;
+            if (wave < kUnroll) {
+                const u32x4 raw = row.guarded(first);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        m[e] = w(first + e, row.value(Row<T>::element(raw, e)));
-                        mine += m[e];
+                for (int e = 0; e < E; ++e) {
+                    m[e] = w(static_cast<int>(first) + e, Row<T>::element(raw, e));
+                    mine += m[e];
+                    if (e % 4 == 3) {
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    u64 sum = before + wave_scan(mine);
-                    if (!done && __any(sum >= target)) {
-                        done = true;
-                        if (sum >= target && sum - mine < target) {
-                            sum -= mine;
+                }
+            }
+            u64 all;
+            u64 sum = before + block_scan(sm, mine, all);
+            if (sum >= target && sum - mine < target) {
+                sum -= mine;
 #pragma unroll
-                            for (int e = 0; e < E; ++e) {
-                                if (sum < target && sum + m[e] >= target) {
-                                    sm.found = static_cast<u64>(first + e);
-                                }
-                                sum += m[e];
-                            }
-                        }
+                for (int e = 0; e < E; ++e) {
+                    if (sum < target && sum + m[e] >= target) {
+                        sm.found = static_cast<u64>(first + e);
                     }
-                    before = static_cast<u64>(__shfl(static_cast<unsigned long long>(sum), 63));
-                });
+                    sum += m[e];
+                }
+            }
+            before += all;
+            if (before >= target) {
+                break;
             }
         }
         __syncthreads();
@@ -346,9 +473,9 @@ template <typename T> struct Sampler {
         }
         __syncthreads();
     }
-    // Appends to the list what `in` holds for, as far as it fits, and returns their number and the
+    // Appends to the list what test(x) and in(index, x) hold for, as far as it fits, and returns their number and the
     // least and largest key. By all threads.
-    template <class In> __device__ __forceinline__ int gather(In in, uint32_t &low, uint32_t &high) {
+    template <class Test, class In> __device__ __forceinline__ int gather(Test test, In in, uint32_t &low, uint32_t &high) {
         __syncthreads();
         if (threadIdx.x == 0) {
             sm.count = 0;
@@ -357,19 +484,17 @@ template <typename T> struct Sampler {
         }
         __syncthreads();
         uint32_t lo = 0xffffffffu, hi = 0;
-        pass(
-            [&](int index, float x) KDA_INLINE {
-                if (in(index, x)) {
-                    const uint32_t key = key_of(x);
-                    lo = min(lo, key);
-                    hi = max(hi, key);
-                    const int at = atomicAdd(&sm.count, 1);
-                    if (at < kList) {
-                        sm.list[at] = rank_of(key, static_cast<uint32_t>(index));
-                    }
+        pass_some(test, [&](int index, float x) KDA_INLINE {
+            if (in(index, x)) {
+                const uint32_t key = key_of(x);
+                lo = min(lo, key);
+                hi = max(hi, key);
+                const int at = atomicAdd(&sm.count, 1);
+                if (at < kList) {
+                    sm.list[at] = rank_of(key, static_cast<uint32_t>(index));
                 }
-            },
-            [](int) {});
+            }
+        });
         if (hi != 0) {
             atomicMin(&sm.low, lo);
             atomicMax(&sm.high, hi);
@@ -380,6 +505,10 @@ template <typename T> struct Sampler {
         const int n = __builtin_amdgcn_readfirstlane(sm.count);
         __syncthreads();
         return n;
+    }
+    __device__ __forceinline__ float logprob_of(int index, u64 mass) const {
+        const float x = Row<T>::element(row.guarded(index), 0);
+        return static_cast<float>((exponent(x) * (1.0 / 256.0) + a.shift) * kLn2 - log(static_cast<double>(mass)));
     }
     // Sorted, behind the entries zeros.
     __device__ __forceinline__ int sort_list(int n) {
@@ -394,10 +523,7 @@ template <typename T> struct Sampler {
     __device__ __forceinline__ void cut_behind(float x, int index) {
         last = x;
         last_index = index;
-    }
-    __device__ __forceinline__ u64 weight(float x) const {
-        bool reaches;
-        return weight(x, reaches);
+        least = fmaxf(least, x);
     }
     // Cuts behind the element at which the number (or mass) of the elements that pass, in the order of their ranks,
     // reaches `target`, which that of all does. The bins hold those of their elements.
@@ -406,42 +532,49 @@ template <typename T> struct Sampler {
         uint32_t at = static_cast<uint32_t>(border(target, before));
         uint32_t first = 0, last_key = 0, low, high;  // keys
         int shift = -1;                               // of the keys' bins, -1: bins by distance
+        // logits that bin `at` may hold, and some more
+        float from = -kInf, to = kInf;
+        if (bin_scale > 0.0f && bin_scale < 1e30f) {
+            const float slack = 1e-5f * fabsf(top);
+            from = at + 1 < kBins ? top - (static_cast<float>(at) + 2.0f) / bin_scale - slack : -kInf;
+            to = top - (static_cast<float>(at) - 1.0f) / bin_scale + slack;
+        }
         int n;
         for (;;) {
-            n = gather(
-                [&](int index, float x) KDA_INLINE {
-                    const uint32_t key = key_of(x);
-                    return passes(x, index) && (shift < 0 ? static_cast<uint32_t>(bin(x)) == at
-                                                          : key >= first && key <= last_key && (last_key - key) >> shift == at);
-                },
-                low, high);
+            n = gather([&](float x) KDA_INLINE { return x >= from && x <= to; },
+                       [&](int index, float x) KDA_INLINE {
+                           return x > -kInf && passes(x, index) && (shift < 0 ? static_cast<uint32_t>(bin(x)) == at
+                                                                              : (last_key - key_of(x)) >> shift == at);
+                       },
+                       low, high);
             if (n <= kList || low == high) {
                 break;
             }
             // more than fit: bins of their keys, the largest first
             first = low;
             last_key = high;
+            from = of_key(first);
+            to = of_key(last_key);
             shift = max(21 - __clz(high - low), 0);
             clear_bins();
-            pass(
-                [&](int index, float x) KDA_INLINE {
-                    const uint32_t key = key_of(x);
-                    if (passes(x, index) && key >= first && key <= last_key) {
-                        const u64 w = number ? 1 : weight(x);
-                        atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[(last_key - key) >> shift]), static_cast<unsigned long long>(w));
-                    }
-                },
-                [](int) {});
+            pass_some([&](float x) KDA_INLINE { return x >= from && x <= to; },
+                      [&](int index, float x) KDA_INLINE {
+                          if (passes(x, index)) {
+                              const u64 w = number ? 1 : weight(x);
+                              atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[(last_key - key_of(x)) >> shift]),
+                                        static_cast<unsigned long long>(w));
+                          }
+                      });
             at = static_cast<uint32_t>(border(target - before, more));
             before += more;
         }
         if (n > kList) {
             // all equal: so many of them in the vocabulary's order
-            const u64 each = number ? 1 : weight(of_key(low));
+            const float x = of_key(low);
+            const u64 each = number ? 1 : weight(x);
             const u64 count = (target - before + each - 1) / each;
-            const auto one = [&](int index, float x) KDA_INLINE -> u64 { return passes(x, index) && key_of(x) == low ? 1 : 0; };
-            block_masses(one);
-            cut_behind(of_key(low), locate(count, one));
+            numbers_of(x);
+            cut_behind(x, locate(count, [&](int index, float y) KDA_INLINE -> u64 { return y == x && passes(x, index) ? 1 : 0; }));
             return;
         }
         sort_list(n);
@@ -488,23 +621,34 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     const int64_t n = blockIdx.x;
     const float temperature = a.temperature != nullptr ? a.temperature[n] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
-    Row<T> row{static_cast<const T *>(a.logits) + n * a.logits_stride, a.vocab, -kInf, kInf};
-    Sampler<T> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0};
+    Row<T> row{static_cast<const T *>(a.logits) + n * a.logits_stride, a.vocab};
+    Sampler<T> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0, -kInf};
 
     // ---- the largest logit, and where it is first
     float top = -kInf;
     int place = 0;
     if (greedy) {
         s.pass(
-            [&](int index, float x) KDA_INLINE {
-                place = x > top ? index : place;
-                top = fmaxf(top, x);
+            [&](int first, u32x4 w) KDA_INLINE {
+#pragma unroll
+                for (int e = 0; e < s.E; ++e) {
+                    const float x = Row<T>::element(w, e);
+                    place = x > top ? first + e : place;
+                    top = fmaxf(top, x);
+                }
             },
             [](int) {});
     } else {
-        s.pass([&](int, float x) KDA_INLINE { top = fmaxf(top, x); }, [](int) {});
+        s.pass(
+            [&](int, u32x4 w) KDA_INLINE {
+#pragma unroll
+                for (int e = 0; e < s.E; ++e) {
+                    top = fmaxf(top, Row<T>::element(w, e));
+                }
+            },
+            [](int) {});
         if (tid < 256) {
-            sm.powers[tid] = exp2(tid * (1.0 / 256.0));
+            sm.powers[tid] = ldexp(exp2(tid * (1.0 / 256.0)), a.shift);
         }
     }
     const float mine = top;
@@ -535,16 +679,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         }
         return;
     }
-    if (top == kInf) {  // the infinite ones share the mass
-        s.row.least = kInf;
-        s.row.most = 0.0f;
-        top = 0.0f;
-    }
-    s.top = top;
-    s.scale = kLog2e / static_cast<double>(temperature);
-    s.bin_scale = static_cast<float>(static_cast<double>(kBins - 1) / (static_cast<double>(temperature) * kLn2 * (a.shift + 2)));
     const float min_p = a.min_p != nullptr ? a.min_p[n] : 0.0f;
-    s.least_weight = min_p > 0.0f ? static_cast<double>(fminf(min_p, 1.0f)) : 0.0;
     const float top_p = a.top_p != nullptr ? a.top_p[n] : 1.0f;
     const bool nucleus = top_p < 1.0f;
     const int64_t k = a.top_k == nullptr          ? 0
@@ -553,23 +688,45 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     const bool few_k = k > 0 && k < a.vocab;
     const float given = a.uniforms[n];
     const double u = given > 0.0f ? static_cast<double>(given) : 0.0;
+    if (top == kInf) {  // the infinite ones share the mass
+        u64 share = s.numbers_of(kInf);
+        share = few_k ? min(share, static_cast<u64>(k)) : share;
+        share = nucleus ? reaching(static_cast<double>(top_p), share) : share;
+        const int found = s.locate(exceeding(u, share), [](int, float x) KDA_INLINE -> u64 { return x == kInf ? 1 : 0; });
+        if (tid == 0) {
+            *token = found;
+            *logprob = static_cast<float>(-log(static_cast<double>(share)));
+        }
+        return;
+    }
+    s.top = top;
+    s.scale = 256.0 * kLog2e / static_cast<double>(temperature);
+    s.bin_scale = static_cast<float>(static_cast<double>(kBins - 1) / (static_cast<double>(temperature) * kLn2 * (a.shift + 2)));
+    if (min_p > 0.0f) {
+        const double p = static_cast<double>(fminf(min_p, 1.0f));
+        s.least_weight = ldexp(p, a.shift);
+        const double x = static_cast<double>(top) + log(p) * static_cast<double>(temperature);
+        s.least = static_cast<float>(x - 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + static_cast<double>(temperature)));
+    }
 
     if (a.vocab <= kFew || (few_k && k <= kFewK)) {
         // ---- candidates: what reaches the k-th largest of the threads' maxima
         uint32_t bound = 0;
         if (a.vocab > kFew) {
-            const uint32_t own = s.row.value(mine) > -kInf ? key_of(s.row.value(mine)) : 0;
+            const uint32_t own = mine > -kInf ? key_of(mine) : 0;
             for (uint32_t bit = 0x80000000u; bit >= (sizeof(T) == 4 ? 1u : 0x10000u); bit >>= 1) {
                 bound |= __syncthreads_count(own >= (bound | bit)) >= k ? bit : 0;
             }
         }
         uint32_t low, high;
-        const int count = s.gather([&](int, float x) KDA_INLINE { return x > -kInf && key_of(x) >= bound; }, low, high);
+        const float reached = bound != 0 ? of_key(bound) : -3.4028234663852886e38f;
+        const int count = s.gather([&](float x) KDA_INLINE { return x >= reached; }, [](int, float) { return true; }, low, high);
         if (count <= kFew) {
             s.sort_list(count);
             const u64 rank = tid < count ? sm.list[tid] : 0;
-            bool in = tid < count && (!few_k || tid < k), high_enough = false;
-            u64 w = in ? s.weight(of_key(static_cast<uint32_t>(rank >> 32)), high_enough) : 0;
+            bool in = tid < count && (!few_k || tid < k);
+            u64 w = in ? s.weight(of_key(static_cast<uint32_t>(rank >> 32))) : 0;
+            const bool high_enough = in && s.scaled_weight(of_key(static_cast<uint32_t>(rank >> 32)), true) >= s.least_weight;
             u64 total;
             u64 sum = block_scan(sm, w, total);
             if (nucleus) {
@@ -587,61 +744,37 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
             const u64 target = exceeding(u, total);
             if (sum >= target && sum - w < target) {
                 const int index = static_cast<int>(static_cast<uint32_t>(entry >> 32) ^ 0xffffffffu);
-                const float x = s.row.value(Row<T>::element(row.raw(index), 0));
                 *token = index;
-                *logprob = static_cast<float>((s.exponent(x) + a.shift) * kLn2 - log(static_cast<double>(total)));
+                *logprob = s.logprob_of(index, total);
             }
             return;
         }
     }
     // ---- top_k's cut (numbers in bins), the nucleus' (masses in bins), the blocks' masses of what is left
-    const auto kept = [&](int index, float x) KDA_INLINE -> u64 {
-        bool reaches;
-        const u64 w = s.weight(x, reaches);
-        return reaches && s.passes(x, index) ? w : 0;
-    };
-    enum { kNumbers, kNucleus, kLeft };
-    u64 mass;
-    for (int mode = few_k ? kNumbers : nucleus ? kNucleus : kLeft;;) {
-        if (mode != kLeft) {
-            s.clear_bins();
-        }
-        mass = s.block_masses([&](int index, float x) KDA_INLINE -> u64 {
-            if (mode == kNumbers) {
-                if (x > -kInf) {
-                    atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[s.bin(x)]), 1ull);
-                }
-                return 0;
-            }
-            bool reaches;
-            const u64 w = s.weight(x, reaches);
-            if (w == 0 || !s.passes(x, index)) {
-                return 0;
-            }
-            if (mode == kNucleus) {
-                atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[s.bin(x)]), static_cast<unsigned long long>(w));
-            }
-            return reaches ? w : 0;
-        });
-        if (mode == kLeft) {
-            break;
-        }
+    Mode mode = few_k ? kNumbers : nucleus ? kNucleus : kLeft;
+    if (mode != kLeft) {
+        s.clear_bins();
+    }
+    u64 mass = s.template masses<false>(mode);
+    while (mode != kLeft) {
         u64 all;
         block_scan(sm, sm.bins[2 * tid] + sm.bins[2 * tid + 1], all);
         const u64 target = mode == kNumbers ? static_cast<u64>(k) : reaching(static_cast<double>(top_p), all);
-        const bool cuts = mode == kNumbers ? target < all : target < mass;  // else min_p cuts what the nucleus would
-        if (cuts) {
+        if (mode == kNumbers ? target < all : target < mass) {
             s.cut(target, mode == kNumbers);
         } else if (mode == kNucleus) {
-            break;
+            break;  // min_p cuts what the nucleus would
         }
         mode = mode == kNumbers && nucleus ? kNucleus : kLeft;
+        if (mode == kNucleus) {
+            s.clear_bins();
+        }
+        mass = s.template masses<true>(mode);
     }
-    const int found = s.locate(exceeding(u, mass), kept);
+    const int found = s.locate(exceeding(u, mass), [&](int index, float x) KDA_INLINE -> u64 { return s.kept(index, x); });
     if (tid == 0) {
-        const float x = s.row.value(Row<T>::element(row.raw(found), 0));
         *token = found;
-        *logprob = static_cast<float>((s.exponent(x) + a.shift) * kLn2 - log(static_cast<double>(mass)));
+        *logprob = s.logprob_of(found, mass);
     }
 }
 

@@ -241,7 +241,8 @@ void paged_kv_store(const at::Tensor &k, const at::Tensor &v, at::Tensor &k_cach
 at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache,
                            const at::Tensor &page_table, const at::Tensor &kv_lens, const at::Tensor &cu_seqlens,
                            double scale, int64_t max_query_len, int64_t window, double logit_cap,
-                           const std::optional<at::Tensor> &k_scale, const std::optional<at::Tensor> &v_scale) {
+                           const std::optional<at::Tensor> &k_scale, const std::optional<at::Tensor> &v_scale,
+                           int64_t sink_tokens) {
     const char *op = "paged_attention";
     KdaPagedAttentionArgs a{};
     a.cache = cache_of(op, "q", q, k_cache, v_cache, k_scale, v_scale);
@@ -259,6 +260,7 @@ at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const
     TORCH_CHECK(N < INT32_MAX && page_table.size(1) <= INT32_MAX && max_query_len >= 0 && max_query_len <= INT32_MAX, op,
                 " supports at most 2^31-1 requests, pages and new tokens of a request");
     TORCH_CHECK(window >= 0 && window <= INT32_MAX, op, ": window must be 0 (all keys) or a number of keys, got ", window);
+    TORCH_CHECK(sink_tokens >= 0 && sink_tokens <= INT32_MAX, op, ": sink_tokens must be a number of keys, got ", sink_tokens);
     TORCH_CHECK(logit_cap == 0 || (logit_cap >= 1e-30 && logit_cap <= 1e30), op,
                 ": logit_cap must be 0 (none) or within 1e-30 and 1e30, got ", logit_cap);
     check_on_gpu("q", q);
@@ -293,7 +295,8 @@ at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const
     if (bytes > 0) {
         workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
     }
-    check_ok(kda_paged_attention_launch(&a, workspace.has_value() ? workspace->data_ptr() : nullptr, bytes, stream_of(q)),
+    check_ok(kda_paged_attention_launch_sinks(&a, static_cast<int32_t>(sink_tokens),
+                                              workspace.has_value() ? workspace->data_ptr() : nullptr, bytes, stream_of(q)),
              op);
     return out;
 }
@@ -366,7 +369,7 @@ TORCH_LIBRARY_FRAGMENT(sgl_glm53_ascend, m) {
     m.def(
         "paged_attention(Tensor q, *, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor kv_lens, "
         "Tensor cu_seqlens, float scale, int max_query_len, int window=0, float logit_cap=0.0, "
-        "Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor");
+        "Tensor? k_scale=None, Tensor? v_scale=None, int sink_tokens=0) -> Tensor");
     m.def(
         "sample_tokens(Tensor logits, Tensor uniforms, *, Tensor? temperature=None, Tensor? top_k=None, "
         "Tensor? top_p=None, Tensor? min_p=None) -> (Tensor, Tensor)");

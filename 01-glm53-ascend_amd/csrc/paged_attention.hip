@@ -196,6 +196,7 @@ __device__ __forceinline__ int page_of(int first, int last) { return last != 0 ?
 
 struct Params : KdaPagedAttentionArgs {
     int group;  // query heads a key head
+    int sinks;  // first keys that stay visible beside a window, 0 without one
 
     // Token ranges and lengths cut to the tensors, whatever the metadata says: int64 entries as they are, not
     // their low words.
@@ -221,6 +222,8 @@ struct Params : KdaPagedAttentionArgs {
         const int end = max(r.keys - r.tokens + i + 1, 0);
         return make_int2(window > 0 ? max(end - window, 0) : 0, end);
     }
+    // Whether a row with the window `see` sees a key (kernels without sinks look at the window alone)
+    __device__ __forceinline__ bool sees(int2 see, int key) const { return key < see.y && (key >= see.x || key < sinks); }
     // Request n's page table as a lane reads it: the entries' first words, or (`last`) the second ones of int64
     // entries, 0 for int32 ones. Looked up ahead by lanes that share an entry, one word each: one register a
     // lane, nothing waits for the load, and page_of puts them together.
@@ -423,13 +426,13 @@ __device__ __forceinline__ int tile_units(const Params &a, const Request &r, int
     if (a.window > 0) {
         const int64_t tokens = (rows + a.group - 2) / a.group + 1;  // that a tile may touch
         const int64_t span = a.window + tokens - 1;                 // keys that they see
-        const int64_t most = (span + kUnit - 2) / kUnit + 1;
+        const int64_t most = (span + kUnit - 2) / kUnit + 1 + (static_cast<int64_t>(a.sinks) + kUnit - 1) / kUnit;
         units = static_cast<int>(min(static_cast<int64_t>(units), most));
     }
     return max(units, 1);  // an item without keys still writes its zeros
 }
 
-template <int D, bool FP8, int NB>
+template <int D, bool FP8, int NB, bool SINKS>
 __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, const DecodeWs ws) {
     constexpr int kRows = 16 * NB;
     using R = Row<D, FP8>;
@@ -524,9 +527,14 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         const int rows = min(kRows, rows_all - row0);
         const int2 first = a.visible(req, row0 / a.group);
         const int2 last = a.visible(req, (row0 + rows - 1) / a.group);
-        const int unit0 = first.x / kUnit;
-        const int lo = max(first.x, (unit0 + part0) * kUnit);  // keys of this part: [lo, hi)
+        // the item's units: those of the sinks, then from the window's first on
+        const int sink_units = SINKS ? (min(a.sinks, last.y) + kUnit - 1) / kUnit : 0;
+        const int unit0 = max(first.x / kUnit, sink_units) - sink_units;
+        auto first_key_of = [&](int part) KDA_INLINE { return (SINKS && part < sink_units ? part : unit0 + part) * kUnit; };
+        // keys of this part: [lo, hi), of the sinks' units [0, sink_hi) too
+        const int lo = max(first.x, first_key_of(SINKS ? max(part0, sink_units) : part0));
         const int hi = min(last.y, (unit0 + part1) * kUnit);
+        const int sink_hi = SINKS ? min(last.y, min(part1, sink_units) * kUnit) : 0;
         const Scores sc = scores_of(a, head);
 
         // ---- queries: 16 rows a block as the right operand
@@ -547,8 +555,17 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         float m[NB], l[NB];
 
         // ---- this wave's blocks of 32 keys: key0 + 128 i
-        const int key0 = (unit0 + part0) * kUnit + wave * kBlock;
-        const int blocks = hi > key0 ? (hi - key0 + kUnit - 1) / kUnit : 0;
+        const int key0 = first_key_of(part0) + wave * kBlock;
+        int blocks = hi > key0 ? (hi - key0 + kUnit - 1) / kUnit : 0;
+        if constexpr (SINKS) {
+            const int before = sink_units - part0;  // blocks of the sinks; those behind the last key hold none
+            if (before > 0) {
+                const int from = first_key_of(sink_units) + wave * kBlock;
+                const int rest = part1 > sink_units && hi > from ? (hi - from + kUnit - 1) / kUnit : 0;
+                blocks = rest > 0 ? before + rest : sink_hi > key0 ? (sink_hi - key0 + kUnit - 1) / kUnit : 0;
+            }
+        }
+        auto block_key = [&](int i) KDA_INLINE { return SINKS ? first_key_of(part0 + i) + wave * kBlock : key0 + i * kUnit; };
         const char *kbase = static_cast<const char *>(a.cache.k) + ((head * a.cache.k_stride_head) << R::kShift);
         const char *vbase = static_cast<const char *>(a.cache.v) + ((head * a.cache.v_stride_head) << R::kShift);
         auto lookup = [&](int i) KDA_INLINE -> int {  // page of key lane % 32 of block i; any entry where it has none
@@ -556,7 +573,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
             if constexpr (NB > 1) {  // as in compute: the entry's word in no register of its own
                 asm volatile("" : "+v"(lane));
             }
-            const int key = key0 + i * kUnit + (lane & 31);
+            const int key = block_key(i) + (lane & 31);
             return a.page_words(n, lane >= 32).of(min(max(key, 0) / a.cache.page_size, a.max_pages - 1));
         };
         // keys of a block that every row of the tile sees: [seen0, seen1)
@@ -567,9 +584,14 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         auto rows_of = [&](int i, int word) KDA_INLINE -> Rows {
             const u32x2 words = __builtin_amdgcn_permlane32_swap(word, word, false, false);
             const int page = page_of(words[0], words[1]);
-            const int key = key0 + i * kUnit + (lane & 31);
+            const int key = block_key(i) + (lane & 31);
             const int off = key - key / a.cache.page_size * a.cache.page_size;
-            const bool real = key >= lo && key < hi && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.cache.num_pages);
+            bool real = key >= lo && key < hi;
+            if constexpr (SINKS) {
+                // in the sinks' units the keys that some row sees, behind them the window's
+                real = part0 + i < sink_units ? key < sink_hi && (key < a.sinks || key >= first.x) : real;
+            }
+            real &= static_cast<uint32_t>(page) < static_cast<uint32_t>(a.cache.num_pages);
             const char *kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
             const char *vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
             const char *zero = reinterpret_cast<const char *>(g_zero_row);
@@ -625,7 +647,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                 }
             }
             // a lane's scores: row `col`, keys 16 kt + 4 g + e
-            const int first_key = key0 + i * kUnit;
+            const int first_key = block_key(i);
             const float c = sc.cap > 0.0f ? 1.0f : sc.c;
             if (sc.cap > 0.0f) {
 #pragma unroll
@@ -633,7 +655,20 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                     s[e >> 3][e >> 2 & 1][e & 3] = capped(s[e >> 3][e >> 2 & 1][e & 3] * sc.in, sc.cap);
                 }
             }
-            if (first_key < seen0 || first_key + kBlock > seen1) {
+            if constexpr (SINKS) {
+                // every row sees the block: in its window, or as sinks
+                const bool all = (first_key >= last.x || first_key + kBlock <= a.sinks) && first_key + kBlock <= first.y;
+                if (!all) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int key = first_key + 4 * g + 16 * (e >> 2) + (e & 3);
+                            s[b][e >> 2][e & 3] = a.sees(see[b], key) ? s[b][e >> 2][e & 3] : kNegInf;
+                        }
+                    }
+                }
+            } else if (first_key < seen0 || first_key + kBlock > seen1) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int from = max(see[b].x, lo) - first_key - 4 * g, to = min(see[b].y, hi) - first_key - 4 * g;
@@ -723,10 +758,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
             }
         }
         if (again) {
-            each_not_finite<D, FP8>(a, n, head, lo, hi, [&](int key, const char *row) KDA_INLINE {
+            const auto add = [&](int key, const char *row) KDA_INLINE {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    if (key % kUnit / kBlock == wave && key >= see[b].x && key < see[b].y) {
+                    if (key % kUnit / kBlock == wave && (SINKS ? a.sees(see[b], key) : key >= see[b].x && key < see[b].y)) {
 #pragma unroll
                         for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
@@ -736,7 +771,13 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
                         }
                     }
                 }
-            });
+            };
+            if constexpr (SINKS) {
+                each_not_finite<D, FP8>(a, n, head, part0 * kUnit, sink_hi, add);
+            }
+            if (!SINKS || part1 > sink_units) {
+                each_not_finite<D, FP8>(a, n, head, lo, hi, add);
+            }
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -956,7 +997,7 @@ struct PrefillArgs {
     int tiles, splits;
 };
 
-template <int D, bool FP8, bool UNIFORM>
+template <int D, bool FP8, bool UNIFORM, bool SINKS>
 __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs args) {
     const Params &a = args.params;
     const int splits = args.splits;
@@ -1041,7 +1082,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     // ---- visible keys: of the tile in tiles of 64, of the wave, of each lane's rows
     const int2 see0 = a.visible(req, row0 / a.group);
     const int2 see1 = a.visible(req, (row0 + rows - 1) / a.group);
-    const int all0 = see0.x / kTile, all1 = (see1.y + kTile - 1) / kTile;
+    // With sinks the tiles are counted in the order of the walk: those of the sinks, then, `gap` further, the window's.
+    const int sink_tiles = SINKS ? (min(a.sinks, see1.y) + kTile - 1) / kTile : 0;
+    const int gap = SINKS ? max(see0.x / kTile, sink_tiles) - sink_tiles : 0;
+    const int sink_end = SINKS ? min(see0.x < sink_tiles * kTile ? see1.y : a.sinks, see1.y) : 0;  // of the keys in their tiles
+    const int all0 = SINKS ? 0 : see0.x / kTile, all1 = max((see1.y + kTile - 1) / kTile - gap, sink_tiles);
+    auto tile_key = [&](int t) KDA_INLINE { return (SINKS && t >= sink_tiles ? t + gap : t) * kTile; };
     const int share = max((all1 - all0 + splits - 1) / splits, kMinPart / kTile);
     const int t0 = all0 + split * share, t1 = min(all1, t0 + share);
     const int wrow0 = min(row0 + wave * 32, row0 + rows - 1);
@@ -1085,8 +1131,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     Group ahead;  // the walk's next
     int at = 0, off = 0;
     const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
-    auto begin_walk = [&]() KDA_INLINE {
-        ahead.key = t0 * kTile + wave * 16;
+    int left = 0;  // tiles of the sinks that are still ahead
+    auto begin_walk = [&](int key) KDA_INLINE {
+        ahead.key = key;
         if constexpr (UNIFORM) {
             at = ahead.key / a.cache.page_size;
             off = ahead.key - at * a.cache.page_size;
@@ -1115,6 +1162,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
             }
         }
         ahead.key += kTile;
+        if constexpr (SINKS) {
+            if (--left == 0) {
+                begin_walk(ahead.key + gap * kTile);
+            }
+        }
         return r;
     };
     // The entries have come: their pages, in every lane or (UNIFORM) in a scalar register. Done once, a turn before
@@ -1147,13 +1199,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     u32x4 kreg[FP8 ? kLoads : 1], vreg[FP8 ? kLoads : 1];
     auto load = [&](const Group &group, const char *base, int64_t page_bytes, int64_t in_page, int64_t token_bytes,
                     const uint32_t (&row)[kLoads], auto column, auto &reg, char *rows_at) KDA_INLINE {
+        // keys that the tile sees around the group
+        const bool of_sinks = SINKS && group.key < sink_tiles * kTile;
+        const int lo = of_sinks ? 0 : see0.x, hi = of_sinks ? sink_end : see1.y;
         if constexpr (UNIFORM) {
             const int page = group.page[0];
             const int key = group.key;
-            const bool any = static_cast<uint32_t>(page) < static_cast<uint32_t>(pool) && key < see1.y && key + 16 > see0.x;
+            const bool any = static_cast<uint32_t>(page) < static_cast<uint32_t>(pool) && key < hi && key + 16 > lo;
             uint32_t lane_at[kLoads];
             const char *first = zero;
-            if (any && key >= see0.x && key + 16 <= see1.y) {
+            if (any && key >= lo && key + 16 <= hi) {
                 first = base + page * page_bytes + in_page;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
@@ -1169,7 +1224,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 }
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int r = max(min(srow + i * R::kRows, see1.y - 1 - key), see0.x - key);
+                    const int r = max(min(srow + i * R::kRows, hi - 1 - key), lo - key);
                     lane_at[i] = static_cast<uint32_t>(r) * token + column(i) + (kLoads - 1 - i) * kKib;
                 }
             }
@@ -1187,7 +1242,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 const int key = group.key + srow + i * R::kRows;
                 const int page = group.page[i];
                 const int in = key - key / a.cache.page_size * a.cache.page_size;
-                const bool real = key >= see0.x && key < see1.y && static_cast<uint32_t>(page) < static_cast<uint32_t>(pool);
+                const bool real = key >= lo && key < hi && static_cast<uint32_t>(page) < static_cast<uint32_t>(pool);
                 const char *first = (real ? base + page * page_bytes + in * token_bytes : zero) + column(i);
                 if constexpr (FP8) {
                     reg[i] = load16(first);
@@ -1269,7 +1324,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 s[e] = capped(s[e] * sc.in, sc.cap);
             }
         }
-        if (!(key0 >= wsee1.x && key0 + 32 <= wsee0.y)) {  // some row of the wave does not see some key
+        if constexpr (SINKS) {
+            if (!((key0 >= wsee1.x || key0 + 32 <= a.sinks) && key0 + 32 <= wsee0.y)) {
+                const int from = see.x - key0 - 4 * half, to = see.y - key0 - 4 * half, sinks = a.sinks - key0 - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int k = 8 * (e >> 2) + (e & 3);
+                    s[e] = k < to && (k >= from || k < sinks) ? s[e] : kNegInf;
+                }
+            }
+        } else if (!(key0 >= wsee1.x && key0 + 32 <= wsee0.y)) {  // some row of the wave does not see some key
             const int from = see.x - key0 - 4 * half, to = see.y - key0 - 4 * half;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -1344,10 +1408,13 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
         }
         if (t0 < t1) {
             // tiles that the wave sees: [w0, w1)
-            const int w0 = active ? max(t0, wsee0.x / kTile) : t1, w1 = active ? min(t1, (wsee1.y + kTile - 1) / kTile) : t1;
+            // (with sinks: from the first on)
+            const int w0 = active ? (SINKS ? t0 : max(t0, wsee0.x / kTile)) : t1;
+            const int w1 = active ? min(t1, max((wsee1.y + kTile - 1) / kTile - gap, min(sink_tiles, (wsee1.y + kTile - 1) / kTile))) : t1;
             // In turn t V's buffer holds the keys 64 t .., K's the keys 64 t + 32 ..: the first 32 keys'
             // scores are formed before, from the second half of the other buffer.
-            begin_walk();
+            left = sink_tiles - t0;
+            begin_walk(tile_key(t0) + wave * 16);
             Group now = walk(), next = walk(), after = walk();
             now = looked_up(now);
             next = looked_up(next);
@@ -1368,7 +1435,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
             f32x16 even, odd;
             if (t0 == w0) {
                 products(1, 1, even);
-                finish(t0 * kTile, even);
+                finish(tile_key(t0), even);
             }
             lds_barrier();  // before the first turn stages over these keys
             auto turn = [&](int t, int parity) KDA_INLINE {
@@ -1380,12 +1447,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 after = walk();
                 if (t >= w0 && t < w1) {
                     step(parity, 0, even, odd);
-                    finish(t * kTile + 32, odd);
+                    finish(tile_key(t) + 32, odd);
                     step(parity, 1, odd, even);
-                    finish(t * kTile + kTile, even);
+                    finish(tile_key(t + 1), even);
                 } else if (t + 1 == w0) {
                     products(parity, 1, even);
-                    finish(t * kTile + kTile, even);
+                    finish(tile_key(t + 1), even);
                 }
                 write_k(parity ^ 1);
                 write_v(parity ^ 1);
@@ -1411,8 +1478,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     }
     if (!__syncthreads_and(fine)) {
         pass(std::true_type{});
-        each_not_finite<D, FP8>(arguments_again(args).params, n, head, max(t0 * kTile, wsee0.x), min(t1 * kTile, wsee1.y), [&](int key, const char *row) KDA_INLINE {
-            if (key >= see.x && key < see.y) {
+        const Params &again = arguments_again(args).params;
+        const auto add = [&](int key, const char *row) KDA_INLINE {
+            if (SINKS ? again.sees(see, key) : key >= see.x && key < see.y) {
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
@@ -1421,7 +1489,14 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                     }
                 }
             }
-        });
+        };
+        if constexpr (SINKS) {
+            each_not_finite<D, FP8>(again, n, head, t0 * kTile, min(min(t1, sink_tiles) * kTile, wsee1.y), add);
+        }
+        if (!SINKS || t1 > sink_tiles) {
+            const int from = tile_key(SINKS ? max(t0, sink_tiles) : t0);
+            each_not_finite<D, FP8>(again, n, head, max(from, wsee0.x), min((t1 + gap) * kTile, wsee1.y), add);
+        }
     }
 
     // ---- out, or this split's part: lane: row `col` of 32, columns 32 d + 8 (e / 4) + 4 half + e % 4
@@ -1646,7 +1721,11 @@ bool misaligned(const void *p, uintptr_t m) { return reinterpret_cast<uintptr_t>
 template <int D, bool FP8, int NB> void launch_decode(const Params &a, const Plan &p, char *ws, hipStream_t s) {
     const DecodeWs w{reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.ml_at),
                      reinterpret_cast<int4 *>(ws + p.desc_at)};
-    decode_kernel<D, FP8, NB><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
+    if (a.sinks > 0) {
+        decode_kernel<D, FP8, NB, true><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
+    } else {
+        decode_kernel<D, FP8, NB, false><<<kDecodeGroups, kThreads, 0, s>>>(a, w);
+    }
     if (p.join) {
         // Few items are cut into many parts: more workgroups an item then (one request of 32 K keys and one
         // key head: 26 us for 16 rows, 52 with 4 workgroups; 34 us for 32 rows, 95 with 4). Of many items most
@@ -1670,9 +1749,15 @@ template <int D, bool FP8> void launch_attention(const Params &a, const Plan &p,
     // rows (8192 tokens 540 us, chunks over 30 K keys 925 us; each row's page looked up: 720 and 1342)
     const auto near = [](int64_t stride) { return stride >= 0 && stride < (1 << 26); };
     if (a.cache.page_size % 16 == 0 && near(a.cache.k_stride_token) && near(a.cache.v_stride_token)) {
-        prefill_kernel<D, FP8, true><<<grid, kThreads, 0, s>>>(args);
+        if (a.sinks > 0) {
+            prefill_kernel<D, FP8, true, true><<<grid, kThreads, 0, s>>>(args);
+        } else {
+            prefill_kernel<D, FP8, true, false><<<grid, kThreads, 0, s>>>(args);
+        }
+    } else if (a.sinks > 0) {
+        prefill_kernel<D, FP8, false, true><<<grid, kThreads, 0, s>>>(args);
     } else {
-        prefill_kernel<D, FP8, false><<<grid, kThreads, 0, s>>>(args);
+        prefill_kernel<D, FP8, false, false><<<grid, kThreads, 0, s>>>(args);
     }
     if (p.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.num_heads;
@@ -1701,11 +1786,22 @@ extern "C" size_t kda_paged_attention_workspace_bytes(const KdaPagedAttentionArg
 
 extern "C" int kda_paged_attention_launch(const KdaPagedAttentionArgs *args, void *workspace, size_t workspace_bytes,
                                           void *stream) {
+    return kda_paged_attention_launch_sinks(args, 0, workspace, workspace_bytes, stream);
+}
+
+extern "C" int kda_paged_attention_launch_sinks(const KdaPagedAttentionArgs *args, int32_t sink_tokens, void *workspace,
+                                                size_t workspace_bytes, void *stream) {
     using namespace kda;
     if (const int rc = check(args); rc != KDA_OK) {
         return rc;
     }
-    Params a{*args, args->num_heads / args->cache.kv_heads};
+    if (sink_tokens < 0) {
+        return KDA_ERR_INVALID_ARGUMENT;
+    }
+    // Without a window every earlier key is visible; there are no more sinks than keys.
+    const int64_t keys = static_cast<int64_t>(args->max_pages) * args->cache.page_size;
+    const int sinks = args->window > 0 ? static_cast<int>(std::min<int64_t>(sink_tokens, keys)) : 0;
+    Params a{*args, args->num_heads / args->cache.kv_heads, sinks};
     if (a.num_tokens == 0) {
         return KDA_OK;
     }

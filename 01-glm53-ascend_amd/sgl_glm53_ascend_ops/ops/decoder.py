@@ -87,6 +87,7 @@ def paged_attention(
     scale: float,
     max_query_len: int,
     window: int = 0,
+    sink_tokens: int = 0,
     logit_cap: float = 0.0,
     k_scale: Optional[torch.Tensor] = None,
     v_scale: Optional[torch.Tensor] = None,
@@ -100,7 +101,9 @@ def paged_attention(
     One call serves decode steps, verify steps and prefill chunks alike, mixed too.
 
     ``window`` > 0 shows a token only the last ``window`` keys, its own among
-    them; ``logit_cap`` > 0 turns a score ``s`` into ``logit_cap * tanh(s /
+    them, and beside those the request's first ``sink_tokens`` keys (the sinks), so a token at position
+    ``p`` sees the keys ``j <= p`` with ``j > p - window or j < sink_tokens``; the pages in between are
+    not read. ``logit_cap`` > 0 turns a score ``s`` into ``logit_cap * tanh(s /
     logit_cap)``. ``k_scale, v_scale`` as in :func:`paged_kv_store`. A token that
     sees no key, or that no request covers, gets zeros; pages outside the pool
     read as zero keys and values. Scores, softmax and sums are fp32; the softmax
@@ -111,7 +114,7 @@ def paged_attention(
     return _OPS.paged_attention(
         q, k_cache=k_cache, v_cache=v_cache, page_table=page_table, kv_lens=kv_lens,
         cu_seqlens=cu_seqlens, scale=scale, max_query_len=max_query_len, window=window,
-        logit_cap=logit_cap, k_scale=k_scale, v_scale=v_scale,
+        logit_cap=logit_cap, k_scale=k_scale, v_scale=v_scale, sink_tokens=sink_tokens,
     )
 
 

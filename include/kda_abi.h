@@ -483,6 +483,12 @@ size_t kda_paged_attention_workspace_bytes(const KdaPagedAttentionArgs *args);
 int kda_paged_attention_launch(const KdaPagedAttentionArgs *args, void *workspace, size_t workspace_bytes,
                                void *stream);
 
+/* kda_paged_attention_launch with sinks: the request's first `sink_tokens` keys stay visible beside a
+ * window (no effect without one), so the token at position p sees the keys j <= p with
+ * j > p - window or j < sink_tokens. The workspace is the same. */
+int kda_paged_attention_launch_sinks(const KdaPagedAttentionArgs *args, int32_t sink_tokens, void *workspace,
+                                     size_t workspace_bytes, void *stream);
+
 /* Human-readable text of a KdaStatus. */
 const char *kda_status_string(int status);
 

@@ -421,12 +421,15 @@ template <int D, int NB> struct DecodeShared {
 };
 
 // Units of a tile of `rows` rows of a request: the most that any of its tiles has.
-__device__ __forceinline__ int tile_units(const Params &a, const Request &r, int rows) {
+template <bool SINKS> __device__ __forceinline__ int tile_units(const Params &a, const Request &r, int rows) {
     int units = (r.keys + kUnit - 1) / kUnit;
     if (a.window > 0) {
         const int64_t tokens = (rows + a.group - 2) / a.group + 1;  // that a tile may touch
         const int64_t span = a.window + tokens - 1;                 // keys that they see
-        const int64_t most = (span + kUnit - 2) / kUnit + 1 + (static_cast<int64_t>(a.sinks) + kUnit - 1) / kUnit;
+        int64_t most = (span + kUnit - 2) / kUnit + 1;
+        if constexpr (SINKS) {
+            most += (static_cast<int64_t>(a.sinks) + kUnit - 1) / kUnit;
+        }
         units = static_cast<int>(min(static_cast<int64_t>(units), most));
     }
     return max(units, 1);  // an item without keys still writes its zeros
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
     // ---- this workgroup's range of units
     const int per = (a.num_seqs + kThreads - 1) / kThreads;
     const int n0 = min(tid * per, a.num_seqs), n1 = min(n0 + per, a.num_seqs);
-    auto units_of = [&](const Request &r) { return (r.tokens * a.group + kRows - 1) / kRows * heads * tile_units(a, r, kRows); };
+    auto units_of = [&](const Request &r) { return (r.tokens * a.group + kRows - 1) / kRows * heads * tile_units<SINKS>(a, r, kRows); };
     int mine = 0;
     bool bad = false;  // token offsets that decrease: requests overlap, and their units may not fit 32 bits
     for (int n = n0; n < n1; ++n) {
@@ -510,7 +513,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
     for (int u = u0; u < u1;) {
         const int rows_all = req.tokens * a.group;
         const int tiles = (rows_all + kRows - 1) / kRows;
-        const int count = tile_units(a, req, kRows);
+        const int count = tile_units<SINKS>(a, req, kRows);
         if (u >= start + tiles * heads * count) {
             start += tiles * heads * count;
             n = next_request(a, n);
@@ -527,12 +530,15 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
         const int rows = min(kRows, rows_all - row0);
         const int2 first = a.visible(req, row0 / a.group);
         const int2 last = a.visible(req, (row0 + rows - 1) / a.group);
-        // the item's units: those of the sinks, then from the window's first on
-        const int sink_units = SINKS ? (min(a.sinks, last.y) + kUnit - 1) / kUnit : 0;
-        const int unit0 = max(first.x / kUnit, sink_units) - sink_units;
+        // the item's units: those of the sinks, then from the window's first on, which are unit0 ahead of their number
+        int sink_units = 0;
+        if constexpr (SINKS) {
+            sink_units = (min(a.sinks, last.y) + kUnit - 1) / kUnit;
+        }
+        const int unit0 = SINKS ? max(first.x / kUnit, sink_units) - sink_units : first.x / kUnit;
         auto first_key_of = [&](int part) KDA_INLINE { return (SINKS && part < sink_units ? part : unit0 + part) * kUnit; };
         // keys of this part: [lo, hi), of the sinks' units [0, sink_hi) too
-        const int lo = max(first.x, first_key_of(SINKS ? max(part0, sink_units) : part0));
+        const int lo = max(first.x, (unit0 + (SINKS ? max(part0, sink_units) : part0)) * kUnit);
         const int hi = min(last.y, (unit0 + part1) * kUnit);
         const int sink_hi = SINKS ? min(last.y, min(part1, sink_units) * kUnit) : 0;
         const Scores sc = scores_of(a, head);
@@ -586,12 +592,9 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
             const int page = page_of(words[0], words[1]);
             const int key = block_key(i) + (lane & 31);
             const int off = key - key / a.cache.page_size * a.cache.page_size;
-            bool real = key >= lo && key < hi;
-            if constexpr (SINKS) {
-                // in the sinks' units the keys that some row sees, behind them the window's
-                real = part0 + i < sink_units ? key < sink_hi && (key < a.sinks || key >= first.x) : real;
-            }
-            real &= static_cast<uint32_t>(page) < static_cast<uint32_t>(a.cache.num_pages);
+            // in the sinks' units the keys that some row sees, behind them the window's
+            const bool real = (SINKS && part0 + i < sink_units ? key < sink_hi && (key < a.sinks || key >= first.x) : key >= lo && key < hi) &&
+                              static_cast<uint32_t>(page) < static_cast<uint32_t>(a.cache.num_pages);
             const char *kp = kbase + ((page * a.cache.k_stride_page + off * a.cache.k_stride_token) << R::kShift);
             const char *vp = vbase + ((page * a.cache.v_stride_page + off * a.cache.v_stride_token) << R::kShift);
             const char *zero = reinterpret_cast<const char *>(g_zero_row);
@@ -758,7 +761,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const Params a, con
             }
         }
         if (again) {
-            const auto add = [&](int key, const char *row) KDA_INLINE {
+            auto add = [&](int key, const char *row) KDA_INLINE {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     if (key % kUnit / kBlock == wave && (SINKS ? a.sees(see[b], key) : key >= see[b].x && key < see[b].y)) {
@@ -1083,10 +1086,15 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     const int2 see0 = a.visible(req, row0 / a.group);
     const int2 see1 = a.visible(req, (row0 + rows - 1) / a.group);
     // With sinks the tiles are counted in the order of the walk: those of the sinks, then, `gap` further, the window's.
-    const int sink_tiles = SINKS ? (min(a.sinks, see1.y) + kTile - 1) / kTile : 0;
-    const int gap = SINKS ? max(see0.x / kTile, sink_tiles) - sink_tiles : 0;
-    const int sink_end = SINKS ? min(see0.x < sink_tiles * kTile ? see1.y : a.sinks, see1.y) : 0;  // of the keys in their tiles
-    const int all0 = SINKS ? 0 : see0.x / kTile, all1 = max((see1.y + kTile - 1) / kTile - gap, sink_tiles);
+    int sink_tiles = 0, gap = 0, sink_end = 0;
+    int all0 = see0.x / kTile, all1 = (see1.y + kTile - 1) / kTile;
+    if constexpr (SINKS) {
+        sink_tiles = (min(a.sinks, see1.y) + kTile - 1) / kTile;
+        gap = max(all0, sink_tiles) - sink_tiles;
+        sink_end = min(see0.x < sink_tiles * kTile ? see1.y : a.sinks, see1.y);  // of the keys in their tiles
+        all0 = 0;
+        all1 = max(all1 - gap, sink_tiles);
+    }
     auto tile_key = [&](int t) KDA_INLINE { return (SINKS && t >= sink_tiles ? t + gap : t) * kTile; };
     const int share = max((all1 - all0 + splits - 1) / splits, kMinPart / kTile);
     const int t0 = all0 + split * share, t1 = min(all1, t0 + share);
@@ -1131,14 +1139,20 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     Group ahead;  // the walk's next
     int at = 0, off = 0;
     const int step_at = kTile / a.cache.page_size, step_off = kTile - step_at * a.cache.page_size;
-    int left = 0;  // tiles of the sinks that are still ahead
-    auto begin_walk = [&](int key) KDA_INLINE {
-        ahead.key = key;
+    auto place_walk = [&]() KDA_INLINE {
         if constexpr (UNIFORM) {
             at = ahead.key / a.cache.page_size;
             off = ahead.key - at * a.cache.page_size;
             ahead.koff = off * ktoken;
             ahead.voff = off * vtoken;
+        }
+    };
+    int left = 0;  // tiles of the sinks that are still ahead
+    auto begin_walk = [&]() KDA_INLINE {
+        ahead.key = (SINKS ? tile_key(t0) : t0 * kTile) + wave * 16;
+        place_walk();
+        if constexpr (SINKS) {
+            left = sink_tiles - t0;
         }
     };
     auto walk = [&]() KDA_INLINE -> Group {
@@ -1164,7 +1178,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
         ahead.key += kTile;
         if constexpr (SINKS) {
             if (--left == 0) {
-                begin_walk(ahead.key + gap * kTile);
+                ahead.key += gap * kTile;
+                place_walk();
             }
         }
         return r;
@@ -1199,16 +1214,20 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     u32x4 kreg[FP8 ? kLoads : 1], vreg[FP8 ? kLoads : 1];
     auto load = [&](const Group &group, const char *base, int64_t page_bytes, int64_t in_page, int64_t token_bytes,
                     const uint32_t (&row)[kLoads], auto column, auto &reg, char *rows_at) KDA_INLINE {
-        // keys that the tile sees around the group
-        const bool of_sinks = SINKS && group.key < sink_tiles * kTile;
-        const int lo = of_sinks ? 0 : see0.x, hi = of_sinks ? sink_end : see1.y;
+        // keys that the tile sees around the group: with sinks [low, high), which in their tiles are not the window's
+        int low = 0, high = 0;
+        if constexpr (SINKS) {
+            const bool of_sinks = group.key < sink_tiles * kTile;
+            low = of_sinks ? 0 : see0.x;
+            high = of_sinks ? sink_end : see1.y;
+        }
         if constexpr (UNIFORM) {
             const int page = group.page[0];
             const int key = group.key;
-            const bool any = static_cast<uint32_t>(page) < static_cast<uint32_t>(pool) && key < hi && key + 16 > lo;
+            const bool any = static_cast<uint32_t>(page) < static_cast<uint32_t>(pool) && key < (SINKS ? high : see1.y) && key + 16 > (SINKS ? low : see0.x);
             uint32_t lane_at[kLoads];
             const char *first = zero;
-            if (any && key >= lo && key + 16 <= hi) {
+            if (any && key >= (SINKS ? low : see0.x) && key + 16 <= (SINKS ? high : see1.y)) {
                 first = base + page * page_bytes + in_page;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
@@ -1224,7 +1243,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 }
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int r = max(min(srow + i * R::kRows, hi - 1 - key), lo - key);
+                    const int r = max(min(srow + i * R::kRows, (SINKS ? high : see1.y) - 1 - key), (SINKS ? low : see0.x) - key);
                     lane_at[i] = static_cast<uint32_t>(r) * token + column(i) + (kLoads - 1 - i) * kKib;
                 }
             }
@@ -1242,7 +1261,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                 const int key = group.key + srow + i * R::kRows;
                 const int page = group.page[i];
                 const int in = key - key / a.cache.page_size * a.cache.page_size;
-                const bool real = key >= lo && key < hi && static_cast<uint32_t>(page) < static_cast<uint32_t>(pool);
+                const bool real = key >= (SINKS ? low : see0.x) && key < (SINKS ? high : see1.y) && static_cast<uint32_t>(page) < static_cast<uint32_t>(pool);
                 const char *first = (real ? base + page * page_bytes + in * token_bytes : zero) + column(i);
                 if constexpr (FP8) {
                     reg[i] = load16(first);
@@ -1410,11 +1429,14 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
             // tiles that the wave sees: [w0, w1)
             // (with sinks: from the first on)
             const int w0 = active ? (SINKS ? t0 : max(t0, wsee0.x / kTile)) : t1;
-            const int w1 = active ? min(t1, max((wsee1.y + kTile - 1) / kTile - gap, min(sink_tiles, (wsee1.y + kTile - 1) / kTile))) : t1;
+            int w1 = active ? min(t1, (wsee1.y + kTile - 1) / kTile) : t1;
+            if constexpr (SINKS) {
+                const int end = (wsee1.y + kTile - 1) / kTile;
+                w1 = active ? min(t1, max(end - gap, min(sink_tiles, end))) : t1;
+            }
             // In turn t V's buffer holds the keys 64 t .., K's the keys 64 t + 32 ..: the first 32 keys'
             // scores are formed before, from the second half of the other buffer.
-            left = sink_tiles - t0;
-            begin_walk(tile_key(t0) + wave * 16);
+            begin_walk();
             Group now = walk(), next = walk(), after = walk();
             now = looked_up(now);
             next = looked_up(next);
@@ -1449,10 +1471,10 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
                     step(parity, 0, even, odd);
                     finish(tile_key(t) + 32, odd);
                     step(parity, 1, odd, even);
-                    finish(tile_key(t + 1), even);
+                    finish(SINKS ? tile_key(t + 1) : t * kTile + kTile, even);
                 } else if (t + 1 == w0) {
                     products(parity, 1, even);
-                    finish(tile_key(t + 1), even);
+                    finish(SINKS ? tile_key(t + 1) : t * kTile + kTile, even);
                 }
                 write_k(parity ^ 1);
                 write_v(parity ^ 1);
@@ -1478,9 +1500,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
     }
     if (!__syncthreads_and(fine)) {
         pass(std::true_type{});
-        const Params &again = arguments_again(args).params;
         const auto add = [&](int key, const char *row) KDA_INLINE {
-            if (SINKS ? again.sees(see, key) : key >= see.x && key < see.y) {
+            if (SINKS ? a.sees(see, key) : key >= see.x && key < see.y) {
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
@@ -1491,11 +1512,13 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(const PrefillArgs 
             }
         };
         if constexpr (SINKS) {
-            each_not_finite<D, FP8>(again, n, head, t0 * kTile, min(min(t1, sink_tiles) * kTile, wsee1.y), add);
-        }
-        if (!SINKS || t1 > sink_tiles) {
-            const int from = tile_key(SINKS ? max(t0, sink_tiles) : t0);
-            each_not_finite<D, FP8>(again, n, head, max(from, wsee0.x), min((t1 + gap) * kTile, wsee1.y), add);
+            each_not_finite<D, FP8>(arguments_again(args).params, n, head, t0 * kTile, min(min(t1, sink_tiles) * kTile, wsee1.y), add);
+            if (t1 > sink_tiles) {
+                each_not_finite<D, FP8>(arguments_again(args).params, n, head, max(tile_key(max(t0, sink_tiles)), wsee0.x),
+                                        min((t1 + gap) * kTile, wsee1.y), add);
+            }
+        } else {
+            each_not_finite<D, FP8>(arguments_again(args).params, n, head, max(t0 * kTile, wsee0.x), min(t1 * kTile, wsee1.y), add);
         }
     }
 

@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from decoder_cases import assert_within
-from linear_cases import Linear, bounds
+from tests.decoder_cases import assert_within
+from tests.linear_cases import Linear, bounds
 
 pytestmark = pytest.mark.gpu
 

@@ -8,7 +8,7 @@ import random
 import pytest
 import torch
 
-import decoder_cases as C
+from tests import decoder_cases as C
 
 pytestmark = pytest.mark.gpu
 

@@ -1,15 +1,18 @@
-"""A hybrid decoder served with this package: KDA layers and paged full attention side by side.
+"""A hybrid decoder served with this package: KDA layers, linear attention and paged attention side by side.
 
-Every layer is: residual add and RMS norm in one call, projections, the mixer (KDA with its
-slot-indexed states, or attention over the paged cache that ``paged_kv_store`` has just
-written), a norm of the heads, the output projection. Prompts run as one ragged
+Every layer is: residual add and RMS norm in one call, projections, the mixer (KDA or linear
+attention with a decay for each head, with their slot-indexed states, or attention over the paged cache
+that ``paged_kv_store`` has just written), a norm of the heads, the output projection. The next token is
+drawn from the logits by ``sample_tokens``. Prompts run as one ragged
 prefill batch, then a decode step for all requests is captured in a HIP graph and
 replayed token by token; only the contents of its input tensors change in between.
 
 Weights are random: the example shows the calls and their bookkeeping.
 
     PYTHONPATH=01-glm53-ascend_amd python examples/hybrid_decoder.py [--fp8] [--tokens 32]
+    PYTHONPATH=01-glm53-ascend_amd python examples/hybrid_decoder.py --layers llal --window 256 --sinks 4 --temperature 0.8 --top-p 0.95
 
+The second decoder's layers all hold a bounded state, however long a request gets.
 ``--fp8`` keeps the cache in 8 bits and feeds the attention layers' first projection from
 ``add_rms_norm_fp8`` (8-bit weights, a scale per row and per output column).
 """
@@ -29,15 +32,20 @@ FP8 = torch.float8_e4m3fn
 @dataclass
 class Config:
     width: int = 1024
-    layers: str = "kkak"     # k: KDA, a: attention
-    kda_heads: int = 4       # of 128
+    layers: str = "kkak"     # k: KDA, l: linear attention, a: attention
+    kda_heads: int = 4       # of 128, of linear layers too
     heads: int = 8           # of the attention
     kv_heads: int = 2
     head_dim: int = 128
     vocab: int = 4096
     page_size: int = 64
     window: int = 0
+    sinks: int = 0           # first tokens that stay visible beside the window
     fp8: bool = False
+    temperature: float = 0.0  # 0: the likeliest token
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
 
 
 @dataclass
@@ -50,6 +58,7 @@ class Step:
     page_table: torch.Tensor    # [N, max_pages] int32
     state_slots: torch.Tensor   # [N] int32, > 0
     max_query_len: int
+    uniforms: torch.Tensor      # [N] fp32 in [0, 1): what the next tokens are drawn by
 
 
 class Pages:
@@ -78,6 +87,7 @@ class Pages:
             page_table=on(self.table, torch.int32),
             state_slots=on(torch.arange(1, len(new) + 1), torch.int32),
             max_query_len=max(new),
+            uniforms=on(torch.rand(len(new)), torch.float32),
         )
 
 
@@ -93,6 +103,9 @@ class HybridDecoder:
         self.embedding = torch.randn(cfg.vocab, cfg.width, device=device, generator=gen).bfloat16()
         self.head = weight(cfg.width, cfg.vocab)
         self.last_norm = one(cfg.width)
+        each = lambda x, dtype=torch.float32: torch.full((requests,), x, dtype=dtype, device=device)  # noqa: E731
+        self.sampling = dict(temperature=each(cfg.temperature), top_k=each(cfg.top_k, torch.int32), top_p=each(cfg.top_p),
+                             min_p=each(cfg.min_p))
         self.layers = []
         for kind in cfg.layers:
             layer = {"kind": kind, "norm": one(cfg.width)}
@@ -102,6 +115,14 @@ class HybridDecoder:
                     first=weight(cfg.width, 4 * H * K + H), last=weight(H * K, cfg.width), head_norm=one(K),
                     A_log=torch.rand(H, device=device, generator=gen), dt_bias=torch.zeros(H * K, device=device),
                     # slot 0 is the padding row; K contiguous
+                    state=torch.zeros(requests + 1, H, 128, K, device=device).transpose(2, 3),
+                )
+            elif kind == "l":
+                H, K = cfg.kda_heads, 128
+                layer.update(
+                    first=weight(cfg.width, 3 * H * K), last=weight(H * K, cfg.width), head_norm=one(K),
+                    # one decay a head, from a few tokens to hundreds
+                    g=-torch.pow(2.0, -8.0 * torch.arange(1, H + 1, device=device) / H),
                     state=torch.zeros(requests + 1, H, 128, K, device=device).transpose(2, 3),
                 )
             else:
@@ -137,6 +158,16 @@ class HybridDecoder:
             out = ops.kda_varlen_recurrent(**args)
         return ops.add_rms_norm(out, layer["head_norm"], EPS).reshape(T, H * K) @ layer["last"]
 
+    def linear(self, layer, x, residual, step):
+        cfg, T = self.cfg, x.shape[0]
+        H, K = cfg.kda_heads, 128
+        qkv = (ops.add_rms_norm(x, layer["norm"], EPS, residual=residual) @ layer["first"]).view(1, T, 3 * H, K)
+        q, k, v = (qkv[:, :, i * H:(i + 1) * H] for i in range(3))  # slices as they are
+        mix = ops.linear_varlen_chunk if step.max_query_len > 1 else ops.linear_varlen_recurrent
+        out = mix(q, k, v, layer["g"], initial_state_source=layer["state"], initial_state_indices=step.state_slots,
+                  cu_seqlens=step.cu_seqlens, scale=K ** -0.5)
+        return ops.add_rms_norm(out, layer["head_norm"], EPS).reshape(T, H * K) @ layer["last"]
+
     def attention(self, layer, x, residual, step):
         cfg, T = self.cfg, x.shape[0]
         H, KH, D = cfg.heads, cfg.kv_heads, cfg.head_dim
@@ -155,7 +186,7 @@ class HybridDecoder:
         out = ops.paged_attention(
             q, k_cache=layer["k_cache"], v_cache=layer["v_cache"], page_table=step.page_table, kv_lens=step.kv_lens,
             cu_seqlens=step.cu_seqlens, scale=D ** -0.5, max_query_len=step.max_query_len, window=cfg.window,
-            **layer["scales"],
+            sink_tokens=cfg.sinks, **layer["scales"],
         )
         return out.reshape(T, H * D) @ layer["last"]
 
@@ -163,14 +194,15 @@ class HybridDecoder:
         """The normed hidden states of the new tokens ``[T, width]``."""
         x = self.embedding[tokens]
         residual = torch.zeros_like(x, dtype=torch.float32)  # the sum of all layers, in 32 bits
+        mixers = {"k": self.kda, "l": self.linear, "a": self.attention}
         for layer in self.layers:
-            x = (self.kda if layer["kind"] == "k" else self.attention)(layer, x, residual, step)
+            x = mixers[layer["kind"]](layer, x, residual, step)
         return ops.add_rms_norm(x, self.last_norm, EPS, residual=residual)
 
     def next_tokens(self, tokens, step):
-        """The likeliest next token of every request."""
+        """The next token of every request, drawn from its logits."""
         last = self.hidden(tokens, step)[step.cu_seqlens[1:].long() - 1]
-        return (last @ self.head).argmax(-1)
+        return ops.sample_tokens(last @ self.head, step.uniforms, **self.sampling)[0]
 
 
 class DecodeGraph:
@@ -196,12 +228,13 @@ class DecodeGraph:
         self.tokens.copy_(tokens)
         self.step.kv_lens.copy_(step.kv_lens)
         self.step.slots.copy_(step.slots)
+        self.step.uniforms.copy_(step.uniforms)
         self.graph.replay()
         return self.next.clone()
 
 
 def generate(cfg, prompts, new_tokens, device="cuda"):
-    """Greedy continuations ``[requests, new_tokens]`` of token lists, and seconds a decode step."""
+    """Continuations ``[requests, new_tokens]`` of token lists, and seconds a decode step."""
     pages = Pages(cfg, len(prompts), max(map(len, prompts)) + new_tokens, device)
     model = HybridDecoder(cfg, len(prompts), pages.pages, device)
     tokens = torch.tensor([t for p in prompts for t in p], device=device)
@@ -222,12 +255,19 @@ def generate(cfg, prompts, new_tokens, device="cuda"):
 def main():
     parser = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     parser.add_argument("--fp8", action="store_true")
+    parser.add_argument("--layers", default=Config.layers, help="a letter each: k KDA, l linear attention, a attention")
     parser.add_argument("--window", type=int, default=0)
+    parser.add_argument("--sinks", type=int, default=0, help="first tokens that stay visible beside the window")
+    parser.add_argument("--temperature", type=float, default=0.0, help="0: the likeliest token")
+    parser.add_argument("--top-k", type=int, default=0)
+    parser.add_argument("--top-p", type=float, default=1.0)
+    parser.add_argument("--min-p", type=float, default=0.0)
     parser.add_argument("--requests", type=int, default=16)
     parser.add_argument("--tokens", type=int, default=32, help="new tokens of each request")
     args = parser.parse_args()
     torch.manual_seed(0)
-    cfg = Config(fp8=args.fp8, window=args.window)
+    cfg = Config(fp8=args.fp8, layers=args.layers, window=args.window, sinks=args.sinks, temperature=args.temperature,
+                 top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
     prompts = [torch.randint(cfg.vocab, (int(n),)).tolist() for n in torch.randint(1, 700, (args.requests,))]
     out, seconds = generate(cfg, prompts, args.tokens)
     print(f"{args.requests} requests, prompts of {min(map(len, prompts))} to {max(map(len, prompts))} tokens")

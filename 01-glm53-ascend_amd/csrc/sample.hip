@@ -66,6 +66,10 @@ struct Shared {
     int count;
     uint32_t low, high;  // keys
     u64 before, found;
+    // of patterns: their numbers lie in bins, their weights in list
+    uint32_t ties[kMaxBlocks];
+    u64 between;  // mass of the logits between the patterns of both signs
+    uint32_t between_count;
 };
 
 // A larger float has the larger key; both zeros have one.
@@ -210,6 +214,18 @@ template <typename T> struct Row {
     }
 };
 
+// The least sum that reaches the part p of a whole, 1 at least.
+__device__ __forceinline__ u64 reaching(double p, u64 whole) {
+    const double x = ceil(p * static_cast<double>(whole));
+    return x >= static_cast<double>(whole) ? whole : x > 1.0 ? static_cast<u64>(x) : 1;
+}
+// The least sum that exceeds the part u of a whole, the whole at most. (The 1 is added to a whole number: a double of this
+// size has no room for it.)
+__device__ __forceinline__ u64 exceeding(double u, u64 whole) {
+    const double x = u * static_cast<double>(whole);
+    return x >= static_cast<double>(whole) ? whole : min(static_cast<u64>(x) + 1, whole);
+}
+
 enum Mode { kNumbers, kNucleus, kLeft };
 
 template <typename T> struct Sampler {
@@ -222,7 +238,8 @@ template <typename T> struct Sampler {
     float last;           // the last element in the order of the ranks that is not cut
     int last_index;
     double least_weight;  // min_p 2^S
-    float least;          // logits below it are cut or do not reach min_p (some others do neither)
+    float floor;          // logits below it do not reach min_p (some others do not either)
+    float least;          // logits below it are cut or do not reach min_p
 
     static constexpr int E = Row<T>::E;
     static constexpr u64 kBias = 0x4330000000000000ull;  // the bits of 2^52
@@ -398,6 +415,11 @@ template <typename T> struct Sampler {
     // The first element in the vocabulary's order where the sum of w(index, value) reaches `target` (1 to the sum of
     // the blocks' masses), in every thread.
     template <class W> __device__ __forceinline__ int locate(u64 target, W w) {
+        u64 before;
+        return locate_in(block_of(target, before), before, target, w);
+    }
+    // The block in which the sum of the blocks' masses reaches `target`, and the sum before it, in every thread.
+    __device__ __forceinline__ int block_of(u64 target, u64 &before) {
         const int n = blocks(), i = 2 * static_cast<int>(threadIdx.x);
         const u64 m0 = i < n ? sm.blocks[i] : 0, m1 = i + 1 < n ? sm.blocks[i + 1] : 0;
         u64 total;
@@ -408,10 +430,15 @@ template <typename T> struct Sampler {
             sm.before = second ? sum - m1 : sum - m0 - m1;
         }
         __syncthreads();
+        const int found = __builtin_amdgcn_readfirstlane(sm.count);
+        before = sm.before;
+        __syncthreads();
+        return found;
+    }
+    template <class W> __device__ __forceinline__ int locate_in(int block, u64 before, u64 target, W w) {
         // a wave for each load of a group
         const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-        const int64_t first_group = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(sm.count)) * a.groups;
-        u64 before = sm.before;
+        const int64_t first_group = static_cast<int64_t>(block) * a.groups;
         for (int64_t g = first_group; g < first_group + a.groups; ++g) {
             u64 m[E], mine = 0;
             const int64_t first = g * Row<T>::kGroup + (wave * 64 + static_cast<int>(__lane_id())) * E;
@@ -508,7 +535,8 @@ template <typename T> struct Sampler {
     }
     __device__ __forceinline__ float logprob_of(int index, u64 mass) const {
         const float x = Row<T>::element(row.guarded(index), 0);
-        return static_cast<float>((exponent(x) * (1.0 / 256.0) + a.shift) * kLn2 - log(static_cast<double>(mass)));
+        // (the mass in units of the largest weight: a token that is left alone gets exactly 0)
+        return static_cast<float>(exponent(x) * (kLn2 / 256.0) - log(ldexp(static_cast<double>(mass), -a.shift)));
     }
     // Sorted, behind the entries zeros.
     __device__ __forceinline__ int sort_list(int n) {
@@ -523,8 +551,237 @@ template <typename T> struct Sampler {
     __device__ __forceinline__ void cut_behind(float x, int index) {
         last = x;
         last_index = index;
-        least = fmaxf(least, x);
+        least = fmaxf(floor, x);
     }
+    __device__ __forceinline__ void uncut() { cut_behind(-kInf, -1); }
+    // ---- bf16 logits have few values. Those of a row that have a weight lie within 16 powers of two of
+    // the largest magnitude among them, kPatterns patterns, in falling order: positive ones from the largest, negative
+    // ones to the largest magnitude. What lies between them, zeros too, is formed one by one.
+    static constexpr int kPatterns = 4096, kSide = kPatterns / 2;
+    static constexpr u64 kReaches = u64{1} << 63;  // of a weight in the list: not below min_p
+    int base;       // the least magnitude's pattern
+    u64 tie_limit;  // how many of those equal to `last` are left
+    __device__ __forceinline__ uint32_t *numbers() const { return reinterpret_cast<uint32_t *>(sm.bins); }
+    static __device__ __forceinline__ uint32_t pattern(u32x4 w, int e) { return (e & 1) != 0 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu; }
+    // The place of a pattern; one outside (as unsigned) kPatterns has a weight of 0 if its magnitude is not below base.
+    __device__ __forceinline__ bool placed(uint32_t p, int &place, bool &small) const {
+        const int m = static_cast<int>(p & 0x7fffu) - base;
+        place = m ^ ((p & 0x8000u) != 0 ? kSide : kSide - 1);
+        small = m < 0;
+        return static_cast<uint32_t>(m) < kSide;
+    }
+    __device__ __forceinline__ float value_at(int place) const {
+        const uint32_t m = static_cast<uint32_t>(place < kSide ? kSide - 1 - place : place - kSide) + base;
+        return __uint_as_float((m | (place < kSide ? 0u : 0x8000u)) << 16);
+    }
+    // Whether the row's logits are taken so; their weights into the list.
+    __device__ __forceinline__ bool tabulate() {
+        const float range = static_cast<float>(256.0 * (a.shift + 2.1) / scale);  // below it weights are 0
+        const float most = fmaxf(fabsf(top), fabsf(top - range));
+        const int exponent_of_most = __float_as_int(most) >> 23, exponent_of_top = __float_as_int(fabsf(top)) >> 23;
+        // (a very high temperature would put most logits between the patterns)
+        if (sizeof(T) != 2 || exponent_of_most < 17 || exponent_of_most > max(exponent_of_top, 130) + 4 || exponent_of_most > 254) {
+            return false;
+        }
+        base = (exponent_of_most - 15) << 7;
+        __syncthreads();  // the powers are there
+        for (int i = threadIdx.x; i < kPatterns; i += kThreads) {
+            const float x = value_at(i);
+            const double v = scaled_weight(fminf(x, top), true);
+            sm.list[i] = (biased(v) - kBias) | (v >= least_weight ? kReaches : 0);
+            numbers()[i] = 0;
+        }
+        if (threadIdx.x == 0) {
+            sm.between = 0;
+            sm.between_count = 0;
+        }
+        __syncthreads();
+        return true;
+    }
+    // Each pattern's number, and number and mass of what lies between.
+    __device__ __forceinline__ void count_patterns() {
+        pass(
+            [&](int, u32x4 w) KDA_INLINE {
+                bool some = false;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    int place;
+                    bool small;
+                    if (placed(pattern(w, e), place, small)) {
+                        atomicAdd(&numbers()[place], 1u);
+                    }
+                    some |= small;
+                }
+                if (__any(some)) {
+#pragma unroll 1
+                    for (int e = 0; e < E; ++e) {
+                        int place;
+                        bool small;
+                        placed(pattern(w, 0), place, small);
+                        if (small) {
+                            const u64 m = weight(Row<T>::element(w, 0));
+                            atomicAdd(&sm.between_count, m != 0 ? 1u : 0u);
+                            atomicAdd(reinterpret_cast<unsigned long long *>(&sm.between), static_cast<unsigned long long>(m));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = w[i] >> 16 | (i < 3 ? w[(i + 1) & 3] << 16 : 0u);
+                        }
+                    }
+                }
+            },
+            [](int) {});
+        __syncthreads();
+    }
+    // Cuts behind the k-th (0: does not) and behind the nucleus of what is left; false where a border lies between the patterns.
+    __device__ __forceinline__ bool cut_patterns(u64 k, bool nucleus, double top_p) {
+        const int first = 4 * static_cast<int>(threadIdx.x);
+        const bool behind = first >= kSide;
+        u64 n[4], all, total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            n[i] = numbers()[first + i];
+        }
+        u64 between_count = sm.between_count, between = sm.between;
+        tie_limit = ~u64{0};
+        // the place at which the sum of m reaches the target, into sm; false if that is between
+        const auto border_at = [&](const u64 (&m)[4], u64 middle, u64 target) KDA_INLINE -> bool {
+            u64 sum = m[0] + m[1] + m[2] + m[3];
+            sum = block_scan(sm, sum, all) - sum + (behind ? middle : 0);
+            if (threadIdx.x == 0) {
+                sm.count = -1;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (sum < target && sum + m[i] >= target) {
+                    sm.count = first + i;
+                    sm.before = sum;
+                }
+                sum += m[i];
+            }
+            __syncthreads();
+            return sm.count >= 0;
+        };
+        block_scan(sm, n[0] + n[1] + n[2] + n[3], total);
+        total += between_count;
+        if (k > 0 && k < total) {
+            if (!border_at(n, between_count, k)) {
+                return false;
+            }
+            const int at = sm.count;
+            tie_limit = k - sm.before;
+            cut_behind(value_at(at), 0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                n[i] = first + i < at ? n[i] : first + i == at ? tie_limit : 0;
+            }
+            between = at < kSide ? 0 : between;
+        }
+        if (nucleus) {
+            u64 m[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                m[i] = n[i] * (sm.list[first + i] & ~kReaches);
+            }
+            block_scan(sm, m[0] + m[1] + m[2] + m[3], total);
+            const u64 target = reaching(top_p, total + between);
+            if (!border_at(m, between, target)) {
+                return false;
+            }
+            const int at = sm.count;
+            const u64 each = sm.list[at] & ~kReaches;
+            tie_limit = (target - sm.before + each - 1) / each;
+            cut_behind(value_at(at), 0x7fffffff);
+        }
+        __syncthreads();
+        return true;
+    }
+    // The blocks' masses of what is left, as masses(); equal ones at the cut are counted by block, and those of the
+    // lowest indices added. `tie_block` gets the last block that holds any of those, `tie_count` their number in it.
+    __device__ __forceinline__ u64 pattern_masses(int &tie_block, u64 &tie_count) {
+        u64 mine = 0;
+        uint32_t ties = 0;
+        const bool cut = last > -kInf;
+        pass(
+            [&](int, u32x4 w) KDA_INLINE {
+                bool some = false, odd = false;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    some |= Row<T>::element(w, e) >= least;
+                }
+                if (!__any(some)) {
+                    return;
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = Row<T>::element(w, e);
+                    int place;
+                    bool small;
+                    const bool in = placed(pattern(w, e), place, small);
+                    odd |= small;
+                    const u64 m = in && x > last ? sm.list[place] : 0;
+                    mine += static_cast<int64_t>(m) < 0 ? m & ~kReaches : 0;
+                    ties += cut && x == last ? 1 : 0;
+                }
+                if (__any(odd)) {
+#pragma unroll 1
+                    for (int e = 0; e < E; ++e) {
+                        int place;
+                        bool small;
+                        placed(pattern(w, 0), place, small);
+                        const float x = Row<T>::element(w, 0);
+                        if (small && x > last) {
+                            const double v = scaled_weight(x, true);
+                            mine += v >= least_weight ? biased(v) - kBias : 0;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = w[i] >> 16 | (i < 3 ? w[(i + 1) & 3] << 16 : 0u);
+                        }
+                    }
+                }
+            },
+            [&](int block) KDA_INLINE {
+                const u64 number = last_lane(wave_scan(ties));
+                if (__lane_id() == 0) {
+                    sm.ties[block] = static_cast<uint32_t>(number);
+                }
+                ties = 0;
+                block_done(block, mine);
+            });
+        __syncthreads();
+        tie_block = 0x7fffffff;
+        tie_count = 0;
+        if (cut) {
+            const int n = blocks(), first = 2 * static_cast<int>(threadIdx.x);
+            const double v = scaled_weight(last, true);
+            const u64 each = v >= least_weight ? biased(v) - kBias : 0;
+            u64 t[2] = {first < n ? sm.ties[first] : 0u, first + 1 < n ? sm.ties[first + 1] : 0u}, all;
+            u64 before = block_scan(sm, t[0] + t[1], all) - t[0] - t[1];
+            if (threadIdx.x == 0) {
+                sm.count = 0x7fffffff;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const u64 left = before >= tie_limit ? 0 : min(t[i], tie_limit - before);
+                if (left > 0) {
+                    sm.blocks[first + i] += left * each;
+                }
+                if (before < tie_limit && before + t[i] >= tie_limit) {
+                    sm.count = first + i;
+                    sm.before = left;
+                }
+                before += t[i];
+            }
+            __syncthreads();
+            tie_block = sm.count;
+            tie_count = sm.before;
+        }
+        return all_blocks();
+    }
+
     // Cuts behind the element at which the number (or mass) of the elements that pass, in the order of their ranks,
     // reaches `target`, which that of all does. The bins hold those of their elements.
     __device__ __forceinline__ void cut(u64 target, bool number) {
@@ -602,18 +859,6 @@ template <typename T> struct Sampler {
     }
 };
 
-// The least sum that reaches the part p of a whole, 1 at least.
-__device__ __forceinline__ u64 reaching(double p, u64 whole) {
-    const double x = ceil(p * static_cast<double>(whole));
-    return x >= static_cast<double>(whole) ? whole : x > 1.0 ? static_cast<u64>(x) : 1;
-}
-// The least sum that exceeds the part u of a whole, the whole at most. (The 1 is added to a whole number: a double of this
-// size has no room for it.)
-__device__ __forceinline__ u64 exceeding(double u, u64 whole) {
-    const double x = u * static_cast<double>(whole);
-    return x >= static_cast<double>(whole) ? whole : min(static_cast<u64>(x) + 1, whole);
-}
-
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) {
     __shared__ Shared sm;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -622,7 +867,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     const float temperature = a.temperature != nullptr ? a.temperature[n] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
     Row<T> row{static_cast<const T *>(a.logits) + n * a.logits_stride, a.vocab};
-    Sampler<T> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0, -kInf};
+    Sampler<T> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0, -kInf, -kInf};
 
     // ---- the largest logit, and where it is first
     float top = -kInf;
@@ -706,7 +951,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         const double p = static_cast<double>(fminf(min_p, 1.0f));
         s.least_weight = ldexp(p, a.shift);
         const double x = static_cast<double>(top) + log(p) * static_cast<double>(temperature);
-        s.least = static_cast<float>(x - 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + static_cast<double>(temperature)));
+        s.floor = s.least = static_cast<float>(x - 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + static_cast<double>(temperature)));
     }
 
     if (a.vocab <= kFew || (few_k && k <= kFewK)) {
@@ -750,6 +995,40 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
             return;
         }
     }
+    const auto finish = [&](int found, u64 mass) KDA_INLINE {
+        if (tid == 0) {
+            *token = found;
+            *logprob = s.logprob_of(found, mass);
+        }
+    };
+    // ---- bf16: the patterns' numbers cut, then one pass for the blocks' masses
+    if constexpr (sizeof(T) == 2) {
+        if (s.tabulate()) {
+            bool cut = true;
+            if (few_k || nucleus) {
+                s.count_patterns();
+                cut = s.cut_patterns(few_k ? static_cast<u64>(k) : 0, nucleus, static_cast<double>(top_p));
+            }
+            if (cut) {
+                int tie_block;
+                u64 tie_count, before;
+                const u64 mass = s.pattern_masses(tie_block, tie_count);
+                const u64 target = exceeding(u, mass);
+                const int block = s.block_of(target, before);
+                // of equal elements at the cut: in blocks before the last that holds some all are left, behind it none
+                if (block == tie_block) {
+                    s.last_index = 0x7fffffff;
+                    const float x = s.last;
+                    s.last_index = s.locate_in(block, 0, tie_count, [&](int, float y) KDA_INLINE -> u64 { return y == x ? 1 : 0; });
+                } else {
+                    s.last_index = block < tie_block ? 0x7fffffff : -1;
+                }
+                finish(s.locate_in(block, before, target, [&](int index, float x) KDA_INLINE -> u64 { return s.kept(index, x); }), mass);
+                return;
+            }
+            s.uncut();
+        }
+    }
     // ---- top_k's cut (numbers in bins), the nucleus' (masses in bins), the blocks' masses of what is left
     Mode mode = few_k ? kNumbers : nucleus ? kNucleus : kLeft;
     if (mode != kLeft) {
@@ -771,11 +1050,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         }
         mass = s.template masses<true>(mode);
     }
-    const int found = s.locate(exceeding(u, mass), [&](int index, float x) KDA_INLINE -> u64 { return s.kept(index, x); });
-    if (tid == 0) {
-        *token = found;
-        *logprob = s.logprob_of(found, mass);
-    }
+    finish(s.locate(exceeding(u, mass), [&](int index, float x) KDA_INLINE -> u64 { return s.kept(index, x); }), mass);
 }
 
 }  // namespace

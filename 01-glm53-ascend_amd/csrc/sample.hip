@@ -13,6 +13,8 @@
 //   the maximum (and for T = 0 its first place, which is the answer);
 //   few candidates (top_k up to kFewK): the k-th largest of the threads' maxima is a bound that at least k elements
 //     reach, and hardly more do. Those go into LDS, are sorted, cut and drawn from there;
+//   bf16: the few values that such logits have are counted, top_k and top_p cut in their table, and one pass looks the
+//     weights up for the blocks' masses;
 //   else one pass forms the weights, their mass in kBins bins by distance from the maximum, and each
 //     block's mass. Where top_k or top_p cuts, the bin in which the border lies is gathered and sorted (bins of more
 //     elements than fit are divided again by their keys, equal elements by their index), and blocks' masses
@@ -37,8 +39,9 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = 16;
 constexpr int kBins = 2048;
-constexpr int kList = 4096;    // elements that are sorted
-constexpr int kFew = 1024;     // elements that are drawn from in LDS, one a thread
+constexpr int kList = 1024;    // elements that are sorted, one a thread
+constexpr int kFew = kList;    // elements that are drawn from in LDS
+constexpr int kPatterns = 4096;
 constexpr int kFewK = 512;
 constexpr int kMaxBlocks = 2048;
 constexpr int kUnroll = 4;     // 16-byte loads of a lane in flight together
@@ -55,18 +58,21 @@ struct SampleParams : KdaSampleArgs {
 };
 
 struct Shared {
-    u64 bins[kBins];
-    u64 list[kList];
+    u64 bins[kBins + 1];
+    union {
+        u64 list[kList];
+        u64 table[kPatterns + 2];  // weights of patterns, whose numbers lie in bins
+    };
     u64 blocks[kMaxBlocks];
     u64 weights[kFew];
     double powers[256];  // 2^{S + j / 256}
     u64 waves[kWaves];
     float tops[kWaves];
     int places[kWaves];
+    int ranks[256];
     int count;
     uint32_t low, high;  // keys
     u64 before, found;
-    // of patterns: their numbers lie in bins, their weights in list
     uint32_t ties[kMaxBlocks];
     u64 between;  // mass of the logits between the patterns of both signs
     uint32_t between_count;
@@ -98,48 +104,84 @@ __device__ __forceinline__ u64 wave_scan(u64 x) {
     x = add_from<0x142, 0xa>(x);  // lane 15 to the second 16, lane 47 to the fourth
     return add_from<0x143, 0xc>(x);  // lane 31 to the upper half
 }
-__device__ __forceinline__ u64 last_lane(u64 x) {
-    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(x), 63);
-    return static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), 63))) << 32 | low;
+__device__ __forceinline__ u64 lane_of(u64 x, int lane) {
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(x), lane);
+    return static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), lane))) << 32 | low;
 }
+__device__ __forceinline__ u64 last_lane(u64 x) { return lane_of(x, 63); }
 // ... of this thread and those before it, and the sum of all. By all threads.
 __device__ __forceinline__ u64 block_scan(Shared &sm, u64 x, u64 &total) {
-    const int lane = static_cast<int>(__lane_id()), wave = threadIdx.x >> 6;
+    const int lane = static_cast<int>(__lane_id()), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     x = wave_scan(x);
     __syncthreads();  // the last one's sums are read
     if (lane == 63) {
         sm.waves[wave] = x;
     }
     __syncthreads();
-    u64 before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        before += w < wave ? sm.waves[w] : 0;
-        total += sm.waves[w];
-    }
-    return x + before;
+    u64 sums = lane < kWaves ? sm.waves[lane] : 0;
+    sums = add_from<0x111, 0xf>(sums);
+    sums = add_from<0x112, 0xf>(sums);
+    sums = add_from<0x114, 0xf>(sums);
+    sums = add_from<0x118, 0xf>(sums);
+    total = lane_of(sums, kWaves - 1);
+    return wave > 0 ? x + lane_of(sums, wave - 1) : x;
 }
 
-// The list's first `size` (a power of two) entries in falling order. By all threads.
-__device__ __forceinline__ void sort(Shared &sm, int size) {
+// The list's first n entries (all different, but for zeros) in falling order. By all threads. Up to 256 by counting what is
+// larger, a quarter of the list a thread (60 entries 7000 cycles by steps of a sorting network, 1000 so); more by such a
+// network, an element a thread, where steps within a wave go through its lanes.
+__device__ __forceinline__ void sort(Shared &sm, int n) {
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (n <= 256) {
+        const int at = i & 255;
+        const u64 mine = at < n ? sm.list[at] : 0;
+        int larger = 0;
+        const int per = (n + 3) / 4, first = (i >> 8) * per;
+        for (int j = first; j < min(first + per, n); ++j) {
+            larger += sm.list[j] > mine ? 1 : 0;
+        }
+        if (i < 256) {
+            sm.ranks[i] = 0;
+        }
+        __syncthreads();
+        atomicAdd(&sm.ranks[at], larger);
+        __syncthreads();
+        const bool real = i < n && mine != 0;
+        const int rank = real ? sm.ranks[i] : 0;
+        if (i < 256) {
+            sm.list[i] = 0;
+        }
+        __syncthreads();
+        if (real) {
+            sm.list[rank] = mine;
+        }
+        __syncthreads();
+        return;
+    }
+    const int size = 1 << (32 - __clz(n - 1));
+    u64 x = i < n ? sm.list[i] : 0;
     for (int span = 2; span <= size; span <<= 1) {
         for (int step = span >> 1; step > 0; step >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                const u64 x = sm.list[a], y = sm.list[b];
-                if ((x < y) == ((a & span) == 0)) {
-                    sm.list[a] = y;
-                    sm.list[b] = x;
-                }
+            u64 y;
+            if (step >= 64) {
+                __syncthreads();
+                sm.list[i] = x;
+                __syncthreads();
+                y = sm.list[i ^ step];
+            } else if (__builtin_amdgcn_readfirstlane(i) >= size) {
+                break;  // a wave behind the list
+            } else {
+                y = static_cast<u64>(__shfl_xor(static_cast<unsigned long long>(x), step));
             }
+            const bool larger = ((i & step) == 0) == ((i & span) == 0);
+            x = (x < y) == larger ? y : x;
         }
     }
     __syncthreads();
+    sm.list[i] = x;
+    __syncthreads();
 }
-__device__ __forceinline__ int power_above(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
-
 // A row's logits. Comparisons are written such that NaN fails them: it counts as -infinity.
 template <typename T> struct Row {
     static constexpr int E = 16 / sizeof(T);
@@ -538,58 +580,49 @@ template <typename T> struct Sampler {
         // (the mass in units of the largest weight: a token that is left alone gets exactly 0)
         return static_cast<float>(exponent(x) * (kLn2 / 256.0) - log(ldexp(static_cast<double>(mass), -a.shift)));
     }
-    // Sorted, behind the entries zeros.
-    __device__ __forceinline__ int sort_list(int n) {
-        const int size = power_above(n);
-        for (int i = n + static_cast<int>(threadIdx.x); i < size; i += kThreads) {
-            sm.list[i] = 0;
-        }
-        sort(sm, size);
-        return size;
-    }
-
     __device__ __forceinline__ void cut_behind(float x, int index) {
         last = x;
         last_index = index;
         least = fmaxf(floor, x);
     }
     __device__ __forceinline__ void uncut() { cut_behind(-kInf, -1); }
+
     // ---- bf16 logits have few values. Those of a row that have a weight lie within 16 powers of two of
-    // the largest magnitude among them, kPatterns patterns, in falling order: positive ones from the largest, negative
-    // ones to the largest magnitude. What lies between them, zeros too, is formed one by one.
-    static constexpr int kPatterns = 4096, kSide = kPatterns / 2;
-    static constexpr u64 kReaches = u64{1} << 63;  // of a weight in the list: not below min_p
+    // the largest magnitude among them, kPatterns patterns. Their places are in falling order: positive ones 1 to kSide from the
+    // largest on, negative ones kSide + 1 to kPatterns to the largest magnitude; 0 and kPatterns + 1 are for all
+    // others, which have no weight, but those between the two sides (zeros too), which are formed one by one.
+    static constexpr int kSide = kPatterns / 2;
     int base;       // the least magnitude's pattern
     u64 tie_limit;  // how many of those equal to `last` are left
     __device__ __forceinline__ uint32_t *numbers() const { return reinterpret_cast<uint32_t *>(sm.bins); }
-    static __device__ __forceinline__ uint32_t pattern(u32x4 w, int e) { return (e & 1) != 0 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu; }
-    // The place of a pattern; one outside (as unsigned) kPatterns has a weight of 0 if its magnitude is not below base.
-    __device__ __forceinline__ bool placed(uint32_t p, int &place, bool &small) const {
-        const int m = static_cast<int>(p & 0x7fffu) - base;
-        place = m ^ ((p & 0x8000u) != 0 ? kSide : kSide - 1);
-        small = m < 0;
-        return static_cast<uint32_t>(m) < kSide;
+    // The place of a pattern; `under` is negative for one between the sides.
+    __device__ __forceinline__ int place_of(u32x4 w, int e, int &under) const {
+        const int word = static_cast<int>(w[e >> 1]);
+        const int sign = (e & 1) != 0 ? word >> 31 : __builtin_amdgcn_sbfe(word, 15, 1);
+        under = static_cast<int>(__builtin_amdgcn_ubfe(word, (e & 1) != 0 ? 16 : 0, 15)) - base;
+        return kSide + 1 + (static_cast<int>(min(static_cast<uint32_t>(under), static_cast<uint32_t>(kSide))) ^ ~sign);
     }
     __device__ __forceinline__ float value_at(int place) const {
-        const uint32_t m = static_cast<uint32_t>(place < kSide ? kSide - 1 - place : place - kSide) + base;
-        return __uint_as_float((m | (place < kSide ? 0u : 0x8000u)) << 16);
+        const uint32_t m = static_cast<uint32_t>(place <= kSide ? kSide - place : place - kSide - 1) + base;
+        return __uint_as_float((m | (place <= kSide ? 0u : 0x8000u)) << 16);
     }
-    // Whether the row's logits are taken so; their weights into the list.
+    // Whether the row's logits are taken so; their weights into the table.
     __device__ __forceinline__ bool tabulate() {
         const float range = static_cast<float>(256.0 * (a.shift + 2.1) / scale);  // below it weights are 0
         const float most = fmaxf(fabsf(top), fabsf(top - range));
         const int exponent_of_most = __float_as_int(most) >> 23, exponent_of_top = __float_as_int(fabsf(top)) >> 23;
-        // (a very high temperature would put most logits between the patterns)
+        // (a very high temperature would put most logits between the sides)
         if (sizeof(T) != 2 || exponent_of_most < 17 || exponent_of_most > max(exponent_of_top, 130) + 4 || exponent_of_most > 254) {
             return false;
         }
         base = (exponent_of_most - 15) << 7;
         __syncthreads();  // the powers are there
-        for (int i = threadIdx.x; i < kPatterns; i += kThreads) {
-            const float x = value_at(i);
-            const double v = scaled_weight(fminf(x, top), true);
-            sm.list[i] = (biased(v) - kBias) | (v >= least_weight ? kReaches : 0);
-            numbers()[i] = 0;
+        for (int i = threadIdx.x; i < kPatterns + 2; i += kThreads) {
+            const bool real = i > 0 && i <= kPatterns;
+            sm.table[i] = real ? weight(fminf(value_at(i), top)) : 0;
+            if (real) {
+                numbers()[i] = 0;
+            }
         }
         if (threadIdx.x == 0) {
             sm.between = 0;
@@ -598,56 +631,59 @@ template <typename T> struct Sampler {
         __syncthreads();
         return true;
     }
+    // f(x) for the logits between the sides among a lane's
+    template <class F> __device__ __forceinline__ void each_between(u32x4 w, F f) const {
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+            int under;
+            place_of(w, 0, under);
+            if (under < 0) {
+                f(Row<T>::element(w, 0));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = w[i] >> 16 | (i < 3 ? w[(i + 1) & 3] << 16 : 0u);
+            }
+        }
+    }
     // Each pattern's number, and number and mass of what lies between.
     __device__ __forceinline__ void count_patterns() {
         pass(
             [&](int, u32x4 w) KDA_INLINE {
-                bool some = false;
+                int some = 0;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    int place;
-                    bool small;
-                    if (placed(pattern(w, e), place, small)) {
+                    int under;
+                    const int place = place_of(w, e, under);
+                    if (static_cast<uint32_t>(under) < kSide) {
                         atomicAdd(&numbers()[place], 1u);
                     }
-                    some |= small;
+                    some |= under;
                 }
-                if (__any(some)) {
-#pragma unroll 1
-                    for (int e = 0; e < E; ++e) {
-                        int place;
-                        bool small;
-                        placed(pattern(w, 0), place, small);
-                        if (small) {
-                            const u64 m = weight(Row<T>::element(w, 0));
-                            atomicAdd(&sm.between_count, m != 0 ? 1u : 0u);
-                            atomicAdd(reinterpret_cast<unsigned long long *>(&sm.between), static_cast<unsigned long long>(m));
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[i] = w[i] >> 16 | (i < 3 ? w[(i + 1) & 3] << 16 : 0u);
-                        }
-                    }
+                if (__any(some < 0)) {
+                    each_between(w, [&](float x) KDA_INLINE {
+                        const u64 m = weight(x);
+                        atomicAdd(&sm.between_count, m != 0 ? 1u : 0u);
+                        atomicAdd(reinterpret_cast<unsigned long long *>(&sm.between), static_cast<unsigned long long>(m));
+                    });
                 }
             },
             [](int) {});
         __syncthreads();
     }
-    // Cuts behind the k-th (0: does not) and behind the nucleus of what is left; false where a border lies between the patterns.
+    // Cuts behind the k-th (0: does not) and behind the nucleus of what is left; false where a border lies between the sides.
     __device__ __forceinline__ bool cut_patterns(u64 k, bool nucleus, double top_p) {
-        const int first = 4 * static_cast<int>(threadIdx.x);
-        const bool behind = first >= kSide;
+        const int first = 4 * static_cast<int>(threadIdx.x) + 1;
         u64 n[4], all, total;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             n[i] = numbers()[first + i];
         }
-        u64 between_count = sm.between_count, between = sm.between;
-        tie_limit = ~u64{0};
-        // the place at which the sum of m reaches the target, into sm; false if that is between
+        u64 between = sm.between;
+        // the place at which the sum of m reaches the target, and the sum before it, into sm; false if that is between the sides
         const auto border_at = [&](const u64 (&m)[4], u64 middle, u64 target) KDA_INLINE -> bool {
             u64 sum = m[0] + m[1] + m[2] + m[3];
-            sum = block_scan(sm, sum, all) - sum + (behind ? middle : 0);
+            sum = block_scan(sm, sum, all) - sum + (first > kSide ? middle : 0);
             if (threadIdx.x == 0) {
                 sm.count = -1;
             }
@@ -664,9 +700,8 @@ template <typename T> struct Sampler {
             return sm.count >= 0;
         };
         block_scan(sm, n[0] + n[1] + n[2] + n[3], total);
-        total += between_count;
-        if (k > 0 && k < total) {
-            if (!border_at(n, between_count, k)) {
+        if (k > 0 && k < total + sm.between_count) {
+            if (!border_at(n, sm.between_count, k)) {
                 return false;
             }
             const int at = sm.count;
@@ -676,13 +711,13 @@ template <typename T> struct Sampler {
             for (int i = 0; i < 4; ++i) {
                 n[i] = first + i < at ? n[i] : first + i == at ? tie_limit : 0;
             }
-            between = at < kSide ? 0 : between;
+            between = at <= kSide ? 0 : between;
         }
         if (nucleus) {
             u64 m[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                m[i] = n[i] * (sm.list[first + i] & ~kReaches);
+                m[i] = n[i] * sm.table[first + i];
             }
             block_scan(sm, m[0] + m[1] + m[2] + m[3], total);
             const u64 target = reaching(top_p, total + between);
@@ -690,79 +725,83 @@ template <typename T> struct Sampler {
                 return false;
             }
             const int at = sm.count;
-            const u64 each = sm.list[at] & ~kReaches;
+            const u64 each = sm.table[at];
             tie_limit = (target - sm.before + each - 1) / each;
             cut_behind(value_at(at), 0x7fffffff);
         }
-        __syncthreads();
         return true;
+    }
+    // Takes out of the table what is cut or does not reach min_p, and what equals `last`.
+    __device__ __forceinline__ void cut_table() {
+        __syncthreads();
+        const u64 at_least = biased(least_weight) - kBias;
+        for (int i = threadIdx.x + 1; i <= kPatterns; i += kThreads) {
+            const float x = value_at(i);
+            const u64 m = sm.table[i];
+            // rounded weights decide where they differ from min_p's
+            if (!(x > last) || m < at_least || (m == at_least && !(scaled_weight(fminf(x, top), true) >= least_weight))) {
+                sm.table[i] = 0;
+            }
+        }
+        __syncthreads();
     }
     // The blocks' masses of what is left, as masses(); equal ones at the cut are counted by block, and those of the
     // lowest indices added. `tie_block` gets the last block that holds any of those, `tie_count` their number in it.
     __device__ __forceinline__ u64 pattern_masses(int &tie_block, u64 &tie_count) {
         u64 mine = 0;
         uint32_t ties = 0;
-        const bool cut = last > -kInf;
+        const bool cut = last > -kInf, few = least > -kInf;
         pass(
             [&](int, u32x4 w) KDA_INLINE {
-                bool some = false, odd = false;
+                if (few) {
+                    bool some = false;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    some |= Row<T>::element(w, e) >= least;
-                }
-                if (!__any(some)) {
-                    return;
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float x = Row<T>::element(w, e);
-                    int place;
-                    bool small;
-                    const bool in = placed(pattern(w, e), place, small);
-                    odd |= small;
-                    const u64 m = in && x > last ? sm.list[place] : 0;
-                    mine += static_cast<int64_t>(m) < 0 ? m & ~kReaches : 0;
-                    ties += cut && x == last ? 1 : 0;
-                }
-                if (__any(odd)) {
-#pragma unroll 1
                     for (int e = 0; e < E; ++e) {
-                        int place;
-                        bool small;
-                        placed(pattern(w, 0), place, small);
-                        const float x = Row<T>::element(w, 0);
-                        if (small && x > last) {
-                            const double v = scaled_weight(x, true);
-                            mine += v >= least_weight ? biased(v) - kBias : 0;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[i] = w[i] >> 16 | (i < 3 ? w[(i + 1) & 3] << 16 : 0u);
-                        }
+                        some |= Row<T>::element(w, e) >= least;
                     }
+                    if (!__any(some)) {
+                        return;
+                    }
+                }
+                int between = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    int under;
+                    mine += sm.table[place_of(w, e, under)];
+                    between |= under;
+                }
+                if (cut) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        ties += Row<T>::element(w, e) == last ? 1 : 0;
+                    }
+                }
+                if (__any(between < 0)) {
+                    each_between(w, [&](float x) KDA_INLINE {
+                        const double v = scaled_weight(x, x > last);
+                        mine += v >= least_weight ? biased(v) - kBias : 0;
+                    });
                 }
             },
             [&](int block) KDA_INLINE {
-                const u64 number = last_lane(wave_scan(ties));
-                if (__lane_id() == 0) {
-                    sm.ties[block] = static_cast<uint32_t>(number);
+                if (cut) {
+                    const u64 number = last_lane(wave_scan(ties));
+                    if (__lane_id() == 0) {
+                        sm.ties[block] = static_cast<uint32_t>(number);
+                    }
+                    ties = 0;
                 }
-                ties = 0;
                 block_done(block, mine);
             });
-        __syncthreads();
         tie_block = 0x7fffffff;
         tie_count = 0;
         if (cut) {
+            __syncthreads();
             const int n = blocks(), first = 2 * static_cast<int>(threadIdx.x);
             const double v = scaled_weight(last, true);
             const u64 each = v >= least_weight ? biased(v) - kBias : 0;
             u64 t[2] = {first < n ? sm.ties[first] : 0u, first + 1 < n ? sm.ties[first + 1] : 0u}, all;
             u64 before = block_scan(sm, t[0] + t[1], all) - t[0] - t[1];
-            if (threadIdx.x == 0) {
-                sm.count = 0x7fffffff;
-            }
-            __syncthreads();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const u64 left = before >= tie_limit ? 0 : min(t[i], tie_limit - before);
@@ -834,23 +873,13 @@ template <typename T> struct Sampler {
             cut_behind(x, locate(count, [&](int index, float y) KDA_INLINE -> u64 { return y == x && passes(x, index) ? 1 : 0; }));
             return;
         }
-        sort_list(n);
-        constexpr int kPer = kList / kThreads;
-        u64 mass[kPer], mine = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int x = static_cast<int>(threadIdx.x) * kPer + i;
-            mass[i] = x < n ? (number ? 1 : weight(of_key(static_cast<uint32_t>(sm.list[x] >> 32)))) : 0;
-            mine += mass[i];
-        }
+        sort(sm, n);
+        const int i = threadIdx.x;
+        const u64 mass = i < n ? (number ? 1 : weight(of_key(static_cast<uint32_t>(sm.list[i] >> 32)))) : 0;
         u64 total;
-        u64 sum = before + block_scan(sm, mine, total) - mine;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (sum < target && sum + mass[i] >= target) {
-                sm.found = sm.list[threadIdx.x * kPer + i];
-            }
-            sum += mass[i];
+        const u64 sum = before + block_scan(sm, mass, total);
+        if (sum >= target && sum - mass < target) {
+            sm.found = sm.list[i];
         }
         __syncthreads();
         const u64 rank = sm.found;
@@ -866,6 +895,16 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     const int64_t n = blockIdx.x;
     const float temperature = a.temperature != nullptr ? a.temperature[n] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
+    // (all of a row's numbers at once, before its logits)
+    const float min_p = a.min_p != nullptr ? a.min_p[n] : 0.0f;
+    const float top_p = a.top_p != nullptr ? a.top_p[n] : 1.0f;
+    const bool nucleus = top_p < 1.0f;
+    const int64_t k = a.top_k == nullptr          ? 0
+                      : (a.top_k_int64 != 0) ? static_cast<const int64_t *>(a.top_k)[n]
+                                             : static_cast<const int32_t *>(a.top_k)[n];
+    const bool few_k = k > 0 && k < a.vocab;
+    const float given = a.uniforms[n];
+    const double u = given > 0.0f ? static_cast<double>(given) : 0.0;
     Row<T> row{static_cast<const T *>(a.logits) + n * a.logits_stride, a.vocab};
     Sampler<T> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0, -kInf, -kInf};
 
@@ -924,15 +963,6 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         }
         return;
     }
-    const float min_p = a.min_p != nullptr ? a.min_p[n] : 0.0f;
-    const float top_p = a.top_p != nullptr ? a.top_p[n] : 1.0f;
-    const bool nucleus = top_p < 1.0f;
-    const int64_t k = a.top_k == nullptr          ? 0
-                      : (a.top_k_int64 != 0) ? static_cast<const int64_t *>(a.top_k)[n]
-                                             : static_cast<const int32_t *>(a.top_k)[n];
-    const bool few_k = k > 0 && k < a.vocab;
-    const float given = a.uniforms[n];
-    const double u = given > 0.0f ? static_cast<double>(given) : 0.0;
     if (top == kInf) {  // the infinite ones share the mass
         u64 share = s.numbers_of(kInf);
         share = few_k ? min(share, static_cast<u64>(k)) : share;
@@ -954,20 +984,31 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         s.floor = s.least = static_cast<float>(x - 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + static_cast<double>(temperature)));
     }
 
-    if (a.vocab <= kFew || (few_k && k <= kFewK)) {
-        // ---- candidates: what reaches the k-th largest of the threads' maxima
-        uint32_t bound = 0;
-        if (a.vocab > kFew) {
-            const uint32_t own = mine > -kInf ? key_of(mine) : 0;
-            for (uint32_t bit = 0x80000000u; bit >= (sizeof(T) == 4 ? 1u : 0x10000u); bit >>= 1) {
-                bound |= __syncthreads_count(own >= (bound | bit)) >= k ? bit : 0;
-            }
+    if (few_k && k <= kFewK && s.bin_scale > 1e-30f && s.bin_scale < 1e30f) {
+        // ---- candidates: what is in the bins up to that of the k-th largest of the threads' maxima. (The last bin's
+        // weights are 0.)
+        s.clear_bins();
+        const int own = mine > -kInf ? s.bin(mine) : kBins;
+        atomicAdd(reinterpret_cast<unsigned long long *>(&sm.bins[own]), 1ull);
+        __syncthreads();
+        u64 all;
+        const u64 m0 = sm.bins[2 * tid], m1 = sm.bins[2 * tid + 1];
+        const u64 below = block_scan(sm, m0 + m1, all) - m0 - m1;
+        if (tid == 0) {
+            sm.count = kBins - 1;
         }
+        __syncthreads();
+        if (below < static_cast<u64>(k) && below + m0 + m1 >= static_cast<u64>(k)) {
+            sm.count = below + m0 >= static_cast<u64>(k) ? 2 * tid : 2 * tid + 1;
+        }
+        __syncthreads();
+        const int bins = min(__builtin_amdgcn_readfirstlane(sm.count) + 1, kBins - 1);
         uint32_t low, high;
-        const float reached = bound != 0 ? of_key(bound) : -3.4028234663852886e38f;
-        const int count = s.gather([&](float x) KDA_INLINE { return x >= reached; }, [](int, float) { return true; }, low, high);
+        const float reached = top - (static_cast<float>(bins) + 1.0f) / s.bin_scale - 1e-5f * fabsf(top);
+        const int count = s.gather([&](float x) KDA_INLINE { return x >= reached; },
+                                   [&](int, float x) KDA_INLINE { return s.bin(x) < bins; }, low, high);
         if (count <= kFew) {
-            s.sort_list(count);
+            sort(sm, count);
             const u64 rank = tid < count ? sm.list[tid] : 0;
             bool in = tid < count && (!few_k || tid < k);
             u64 w = in ? s.weight(of_key(static_cast<uint32_t>(rank >> 32))) : 0;
@@ -982,7 +1023,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
             __syncthreads();  // everybody has their rank
             // in the vocabulary's order
             sm.list[tid] = w > 0 ? static_cast<u64>(index_of(rank) ^ 0xffffffffu) << 32 | static_cast<uint32_t>(tid) : 0;
-            sort(sm, power_above(count));
+            sort(sm, count);
             const u64 entry = sm.list[tid];
             w = tid < count && entry != 0 ? sm.weights[static_cast<uint32_t>(entry)] : 0;
             sum = block_scan(sm, w, total);
@@ -1010,6 +1051,9 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
                 cut = s.cut_patterns(few_k ? static_cast<u64>(k) : 0, nucleus, static_cast<double>(top_p));
             }
             if (cut) {
+                if (s.least > -kInf) {
+                    s.cut_table();
+                }
                 int tie_block;
                 u64 tie_count, before;
                 const u64 mass = s.pattern_masses(tie_block, tie_count);

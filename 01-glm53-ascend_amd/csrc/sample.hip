@@ -606,8 +606,24 @@ template <typename T> struct Sampler {
         const uint32_t m = static_cast<uint32_t>(place <= kSide ? kSide - place : place - kSide - 1) + base;
         return __uint_as_float((m | (place <= kSide ? 0u : 0x8000u)) << 16);
     }
-    // Whether the row's logits are taken so; their weights into the table.
-    __device__ __forceinline__ bool tabulate() {
+    // A window that fits most rows, of magnitudes from 2^-9 to below 2^7: patterns may be counted in it before the largest logit is
+    // known.
+    static constexpr int kUsualBase = 118 << 7;
+    static constexpr uint32_t kAside = kMaxBlocks;  // logits between the sides that are kept (in place of the blocks) until then
+    __device__ __forceinline__ void clear_patterns() {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kPatterns; i += kThreads) {
+            numbers()[i + 1] = 0;
+        }
+        if (threadIdx.x == 0) {
+            sm.between = 0;
+            sm.between_count = 0;
+        }
+        __syncthreads();
+    }
+    // Whether the row's logits are taken so; their weights into the table. `counted`: the patterns are, in the usual window; it is
+    // taken back where that does not do.
+    __device__ __forceinline__ bool tabulate(bool &counted) {
         const float range = static_cast<float>(256.0 * (a.shift + 2.1) / scale);  // below it weights are 0
         const float most = fmaxf(fabsf(top), fabsf(top - range));
         const int exponent_of_most = __float_as_int(most) >> 23, exponent_of_top = __float_as_int(fabsf(top)) >> 23;
@@ -615,21 +631,56 @@ template <typename T> struct Sampler {
         if (sizeof(T) != 2 || exponent_of_most < 17 || exponent_of_most > max(exponent_of_top, 130) + 4 || exponent_of_most > 254) {
             return false;
         }
-        base = (exponent_of_most - 15) << 7;
-        __syncthreads();  // the powers are there
-        for (int i = threadIdx.x; i < kPatterns + 2; i += kThreads) {
-            const bool real = i > 0 && i <= kPatterns;
-            sm.table[i] = real ? weight(fminf(value_at(i), top)) : 0;
-            if (real) {
-                numbers()[i] = 0;
-            }
+        counted = counted && exponent_of_most < 134 && sm.between_count <= kAside;
+        base = counted ? kUsualBase : (exponent_of_most - 15) << 7;
+        if (!counted) {
+            clear_patterns();
         }
-        if (threadIdx.x == 0) {
-            sm.between = 0;
-            sm.between_count = 0;
+        for (int i = threadIdx.x; i < kPatterns + 2; i += kThreads) {
+            sm.table[i] = i > 0 && i <= kPatterns ? weight(fminf(value_at(i), top)) : 0;
+        }
+        if (counted) {
+            u64 mine = 0;
+            const uint32_t *aside = reinterpret_cast<const uint32_t *>(sm.blocks);
+            for (uint32_t i = threadIdx.x; i < sm.between_count; i += kThreads) {
+                mine += weight(__uint_as_float(aside[i]));
+            }
+            u64 all;
+            block_scan(sm, mine, all);
+            if (threadIdx.x == 0) {
+                sm.between = all;
+            }
         }
         __syncthreads();
         return true;
+    }
+    // The patterns' numbers in the usual window, and the largest logit.
+    __device__ __forceinline__ void count_first(float &largest) {
+        base = kUsualBase;
+        clear_patterns();
+        pass(
+            [&](int, u32x4 w) KDA_INLINE {
+                int some = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    int under;
+                    const int place = place_of(w, e, under);
+                    if (static_cast<uint32_t>(under) < kSide) {
+                        atomicAdd(&numbers()[place], 1u);
+                    }
+                    some |= under;
+                    largest = fmaxf(largest, Row<T>::element(w, e));
+                }
+                if (__any(some < 0)) {
+                    each_between(w, [&](float x) KDA_INLINE {
+                        const uint32_t at = atomicAdd(&sm.between_count, 1u);
+                        if (at < kAside) {
+                            reinterpret_cast<uint32_t *>(sm.blocks)[at] = __float_as_uint(x);
+                        }
+                    });
+                }
+            },
+            [](int) {});
     }
     // f(x) for the logits between the sides among a lane's
     template <class F> __device__ __forceinline__ void each_between(u32x4 w, F f) const {
@@ -672,7 +723,8 @@ template <typename T> struct Sampler {
         __syncthreads();
     }
     // Cuts behind the k-th (0: does not) and behind the nucleus of what is left; false where a border lies between the sides.
-    __device__ __forceinline__ bool cut_patterns(u64 k, bool nucleus, double top_p) {
+    // `left`: about how many are left.
+    __device__ __forceinline__ bool cut_patterns(u64 k, bool nucleus, double top_p, u64 &left) {
         const int first = 4 * static_cast<int>(threadIdx.x) + 1;
         u64 n[4], all, total;
 #pragma unroll
@@ -700,7 +752,9 @@ template <typename T> struct Sampler {
             return sm.count >= 0;
         };
         block_scan(sm, n[0] + n[1] + n[2] + n[3], total);
+        left = total;
         if (k > 0 && k < total + sm.between_count) {
+            left = k;
             if (!border_at(n, sm.between_count, k)) {
                 return false;
             }
@@ -728,10 +782,16 @@ template <typename T> struct Sampler {
             const u64 each = sm.table[at];
             tie_limit = (target - sm.before + each - 1) / each;
             cut_behind(value_at(at), 0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                n[i] = first + i <= at ? n[i] : 0;
+            }
+            block_scan(sm, n[0] + n[1] + n[2] + n[3], left);
         }
         return true;
     }
-    // Takes out of the table what is cut or does not reach min_p, and what equals `last`.
+    // Takes out of the table what is cut or does not reach min_p; what equals `last` gets kTie: a lane's weights of a block
+    // stay below it, and their number above.
     __device__ __forceinline__ void cut_table() {
         __syncthreads();
         const u64 at_least = biased(least_weight) - kBias;
@@ -740,17 +800,19 @@ template <typename T> struct Sampler {
             const u64 m = sm.table[i];
             // rounded weights decide where they differ from min_p's
             if (!(x > last) || m < at_least || (m == at_least && !(scaled_weight(fminf(x, top), true) >= least_weight))) {
-                sm.table[i] = 0;
+                sm.table[i] = x == last ? kTie : 0;
             }
         }
         __syncthreads();
     }
+    static constexpr int kTieShift = 57;  // 32 elements of at most 2^51
+    static constexpr u64 kTie = u64{1} << kTieShift;
     // The blocks' masses of what is left, as masses(); equal ones at the cut are counted by block, and those of the
     // lowest indices added. `tie_block` gets the last block that holds any of those, `tie_count` their number in it.
-    __device__ __forceinline__ u64 pattern_masses(int &tie_block, u64 &tie_count) {
+    // `few`: most groups of loads hold nothing that is left.
+    __device__ __forceinline__ u64 pattern_masses(bool few, int &tie_block, u64 &tie_count) {
         u64 mine = 0;
-        uint32_t ties = 0;
-        const bool cut = last > -kInf, few = least > -kInf;
+        const bool cut = last > -kInf;
         pass(
             [&](int, u32x4 w) KDA_INLINE {
                 if (few) {
@@ -770,12 +832,6 @@ template <typename T> struct Sampler {
                     mine += sm.table[place_of(w, e, under)];
                     between |= under;
                 }
-                if (cut) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        ties += Row<T>::element(w, e) == last ? 1 : 0;
-                    }
-                }
                 if (__any(between < 0)) {
                     each_between(w, [&](float x) KDA_INLINE {
                         const double v = scaled_weight(x, x > last);
@@ -785,11 +841,11 @@ template <typename T> struct Sampler {
             },
             [&](int block) KDA_INLINE {
                 if (cut) {
-                    const u64 number = last_lane(wave_scan(ties));
+                    const u64 number = last_lane(wave_scan(mine >> kTieShift));
                     if (__lane_id() == 0) {
                         sm.ties[block] = static_cast<uint32_t>(number);
                     }
-                    ties = 0;
+                    mine &= kTie - 1;
                 }
                 block_done(block, mine);
             });
@@ -911,6 +967,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     // ---- the largest logit, and where it is first
     float top = -kInf;
     int place = 0;
+    bool counted = false;  // bf16 patterns
     if (greedy) {
         s.pass(
             [&](int first, u32x4 w) KDA_INLINE {
@@ -923,6 +980,12 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
             },
             [](int) {});
     } else {
+        if constexpr (sizeof(T) == 2) {
+            counted = a.groups == 1 && (few_k ? k > kFewK : nucleus);
+        }
+        if (counted) {
+            s.count_first(top);
+        } else {
         s.pass(
             [&](int, u32x4 w) KDA_INLINE {
 #pragma unroll
@@ -931,6 +994,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
                 }
             },
             [](int) {});
+        }
         if (tid < 256) {
             sm.powers[tid] = ldexp(exp2(tid * (1.0 / 256.0)), a.shift);
         }
@@ -1044,11 +1108,14 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     };
     // ---- bf16: the patterns' numbers cut, then one pass for the blocks' masses
     if constexpr (sizeof(T) == 2) {
-        if (s.tabulate()) {
+        if (a.groups == 1 && s.tabulate(counted)) {
             bool cut = true;
+            u64 left = 0;
             if (few_k || nucleus) {
-                s.count_patterns();
-                cut = s.cut_patterns(few_k ? static_cast<u64>(k) : 0, nucleus, static_cast<double>(top_p));
+                if (!counted) {
+                    s.count_patterns();
+                }
+                cut = s.cut_patterns(few_k ? static_cast<u64>(k) : 0, nucleus, static_cast<double>(top_p), left);
             }
             if (cut) {
                 if (s.least > -kInf) {
@@ -1056,7 +1123,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
                 }
                 int tie_block;
                 u64 tie_count, before;
-                const u64 mass = s.pattern_masses(tie_block, tie_count);
+                const u64 mass = s.pattern_masses(s.floor > -kInf || (s.last > -kInf && left < static_cast<u64>(a.vocab >> 8)), tie_block, tie_count);
                 const u64 target = exceeding(u, mass);
                 const int block = s.block_of(target, before);
                 // of equal elements at the cut: in blocks before the last that holds some all are left, behind it none

@@ -244,3 +244,44 @@ def test_another_stream_and_no_rows(ops):
     assert torch.equal(got, want)
     tokens, logprobs = ops.sample_tokens(x[:0], u[:0])
     assert tokens.shape == (0,) and logprobs.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["small", "large", "zeros", "mostly_zeros", "positive", "negative", "far", "masked"])
+def test_ranges_of_logits(ops, kind, dtype):
+    """Magnitudes around those that bf16 rows are counted in, zeros by the thousand at a border, rows of one sign, far from 0."""
+    V = 6000
+    logits, u, gen = draw(17, 6, V, torch.float32)
+    if kind == "small":
+        logits = logits * torch.tensor([1e-1, 1e-2, 1e-3, 1e-5, 1e-20, 1e-38])[:, None]
+    elif kind == "large":
+        logits = logits * torch.tensor([10.0, 30.0, 60.0, 1e3, 1e10, 1e37])[:, None]
+    elif kind == "zeros":
+        logits = torch.where(torch.rand(6, V, generator=gen) < 0.3, torch.tensor([0.0, -0.0])[torch.randint(2, (6, V), generator=gen)], logits)
+    elif kind == "mostly_zeros":
+        logits = torch.where(torch.rand(6, V, generator=gen) < 0.97, 0.0, logits)
+    elif kind == "positive":
+        logits = logits.abs() + torch.tensor([0.0, 0.01, 1.0, 8.0, 100.0, 1000.0])[:, None]
+    elif kind == "negative":
+        logits = -logits.abs() - torch.tensor([0.0, 0.01, 1.0, 8.0, 100.0, 1000.0])[:, None]
+    elif kind == "far":
+        logits = logits + torch.tensor([120.0, 128.0, -120.0, -128.0, 1e4, -1e4])[:, None]
+    else:  # all but a few masked, by -infinity or the lowest number
+        hidden = torch.rand(6, V, generator=gen) < torch.tensor([0.5, 0.9, 0.99, 0.999, 0.5, 0.99])[:, None]
+        logits = torch.where(hidden, torch.tensor([-INF, -INF, -INF, -INF, torch.finfo(dtype).min, -1e4])[:, None], logits)
+    logits = logits.to(dtype)
+    check(ops, logits, u)
+    check(ops, logits, u, t=[0.5, 1.0, 2.0, 0.1, 10.0, 200.0])
+    check(ops, logits, u, p=[0.3, 0.6, 0.9, 0.99, 0.5, 0.8])
+    check(ops, logits, u, p=[0.9, 0.5, 0.3, 0.7, 0.999, 0.95], t=[3.0, 0.7, 1.5, 20.0, 0.01, 5.0])
+    check(ops, logits, u, k=[600, 3000, 4000, 5999, 513, 2500], p=[0.9, 0.8, 0.7, 0.6, 0.99, 0.5])
+    check(ops, logits, u, k=[600, 3000, 4000, 5999, 20, 2500], floor=[0.1, 0.01, 0.3, 0.001, 0.5, 0.9])
+    check(ops, logits, u, p=[0.9] * 6, floor=[0.1, 0.01, 0.3, 0.001, 0.5, 0.9], t=[2.0] * 6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_vocabulary_of_millions(ops, dtype):
+    """More elements than a block of one group a wave holds."""
+    logits, u, _ = draw(18, 3, (1 << 22) + 4097, dtype, spread=1.5)
+    check(ops, logits, u, k=[0, 100, 2000000], p=[0.9, 0.8, 0.5], t=[1.0, 0.7, 2.0])
+    check(ops, logits, u, floor=[0.0, 0.01, 0.3])

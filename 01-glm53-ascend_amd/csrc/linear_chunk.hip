@@ -558,6 +558,9 @@ template <int D> __global__ __launch_bounds__(kThreads<D>, 4) void outputs_kerne
     }
 }
 
+constexpr int kMostChunks = 1 << 20;  // of a segment
+constexpr int kMostTokens = INT32_MAX - kMostChunks * kChunk;  // offsets a segment behind the last token stay in 32 bits
+
 // A segment's tokens. As many workgroups as the card holds at once (two a CU of heads of 128, six of 64) where
 // segments are then long, at least as many as it has CUs elsewhere; not so short that the states between
 // them outweigh them, the less so the more requests and heads there are. Up to 320 tokens go as they are: 256 tokens
@@ -571,7 +574,7 @@ int segment_of_call(const KdaLinearArgs &a) {
         tokens = std::max<int64_t>(tokens, std::min<int64_t>(work / 256, 256));
     }
     tokens = std::max<int64_t>(tokens, a.num_tokens <= 320 ? 320 : std::min<int64_t>(std::max<int64_t>(pairs, 128), 512));
-    return static_cast<int>(std::min<int64_t>((tokens + kChunk - 1) / kChunk, 1 << 20) * kChunk);
+    return static_cast<int>(std::min<int64_t>((tokens + kChunk - 1) / kChunk, kMostChunks) * kChunk);
 }
 
 struct Plan {
@@ -631,6 +634,9 @@ extern "C" int kda_linear_chunk_launch(const KdaLinearArgs *args, void *workspac
     }
     if (args->num_seqs == 0) {
         return args->num_tokens == 0 ? KDA_OK : KDA_ERR_INVALID_ARGUMENT;
+    }
+    if (args->num_tokens > kMostTokens) {
+        return KDA_ERR_TOO_LARGE;
     }
     const Plan p = plan_of(*args);
     if (p.bytes > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < p.bytes)) {

@@ -73,7 +73,7 @@ struct Shared {
     int count;
     uint32_t low, high;  // keys
     u64 before, found;
-    uint32_t ties[kMaxBlocks];
+    uint32_t ties[kMaxBlocks];  // numbers of elements that equal the last one left
     u64 between;  // mass of the logits between the patterns of both signs
     uint32_t between_count;
 };
@@ -986,14 +986,14 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         if (counted) {
             s.count_first(top);
         } else {
-        s.pass(
-            [&](int, u32x4 w) KDA_INLINE {
+            s.pass(
+                [&](int, u32x4 w) KDA_INLINE {
 #pragma unroll
-                for (int e = 0; e < s.E; ++e) {
-                    top = fmaxf(top, Row<T>::element(w, e));
-                }
-            },
-            [](int) {});
+                    for (int e = 0; e < s.E; ++e) {
+                        top = fmaxf(top, Row<T>::element(w, e));
+                    }
+                },
+                [](int) {});
         }
         if (tid < 256) {
             sm.powers[tid] = ldexp(exp2(tid * (1.0 / 256.0)), a.shift);
@@ -1101,6 +1101,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         }
     }
     const auto finish = [&](int found, u64 mass) KDA_INLINE {
+        found = min(static_cast<uint32_t>(found), static_cast<uint32_t>(a.vocab - 1));  // also if logits change between the passes
         if (tid == 0) {
             *token = found;
             *logprob = s.logprob_of(found, mass);

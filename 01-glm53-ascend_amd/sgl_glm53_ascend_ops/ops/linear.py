@@ -40,7 +40,8 @@ def linear_varlen_recurrent(
     ``q, k, v`` are ``[1, T, H, D]`` in bf16 or fp32 (slices of a fused projection work), D 64 or
     128; ``g`` is the fp32 log decay, ``[H]`` or ``[1, T, H]``. Request ``n`` has the tokens
     ``cu_seqlens[n]`` to ``cu_seqlens[n + 1]`` and the state ``initial_state_source[initial_state_indices[n]]``
-    (``[slots, H, K, V]``, K contiguous); requests of one call must not share a slot other than 0.
+    (``[slots, H, K, V]``, K contiguous). In one call a slot other than 0 is named once, as a state or as a tracked
+    prefix's.
 
     ``intermediate_state`` ``[requests, steps, H, K, V]`` receives the state after every token, and the
     pool is then left as it is. ``track_state_indices/lens``: the state after ``lens[n]`` tokens of request ``n``

@@ -282,7 +282,7 @@ int kda_chunk_launch_noalloc(const KdaChunkArgs *args, void *stream);
  * prefixes; a request with slot 0 starts from zeros and leaves no state. Metadata may be
  * int64 (`wide`), and int64 entries count whole: one beyond 32 bits is outside the pool or
  * past the tokens, not its low word. Every token of out is written, 0 where no request
- * covers it. Requests of one call must not share a slot other than 0 or a tracked one. */
+ * covers it. In one call a slot other than 0 is named once, as a state or as a tracked prefix's. */
 typedef struct KdaLinearArgs {
     const void *q; /* [tokens, heads, D], `dtype`, D contiguous; element strides of tokens and heads */
     const void *k;
@@ -335,7 +335,8 @@ size_t kda_linear_chunk_workspace_bytes(const KdaLinearArgs *args);
 /* In chunks of 64 tokens on the matrix cores: prompts. bf16 only, no checkpoints; alignment as
  * above. Log decays are at most 0 in earnest (positive ones work while exp(sum) stays finite over 64
  * tokens), down to -infinity; below -10000 they count as -10000, whose exponential is 0. An
- * infinite or NaN value reaches its own token and later ones of its request only.
+ * infinite or NaN value reaches its own token and later ones of its request only. At most 2^31 - 2^26 - 1
+ * tokens (KDA_ERR_TOO_LARGE).
  * `workspace`: 256-byte aligned device memory of the bytes above, no initialization needed. */
 int kda_linear_chunk_launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, void *stream);
 

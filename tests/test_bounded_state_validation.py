@@ -214,6 +214,12 @@ def test_linear_chunk_workspace(lib):
     assert size(head_dim=80, num_tokens=4000) == 0
 
 
+def test_linear_chunk_most_tokens(lib):
+    """Offsets a segment (2^26 tokens at most) behind the last token would pass 32 bits."""
+    for tokens in ((1 << 31) - 1, (1 << 31) - (1 << 26)):
+        assert lib.kda_linear_chunk_launch(_linear(num_tokens=tokens, num_heads=1), BASE, 1 << 60, None) == TOO_LARGE
+
+
 def test_sample_launch_refusals(lib):
     def status(**over):
         a = dict(logits=BASE, logits_stride=100, uniforms=BASE, tokens=BASE, logprobs=BASE, rows=2, vocab=100)

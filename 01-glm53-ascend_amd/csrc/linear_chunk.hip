@@ -41,6 +41,7 @@ constexpr int kChunk = 64;
 template <int D> constexpr int kWaves = D / 16;
 template <int D> constexpr int kThreads = 64 * kWaves<D>;
 constexpr int kStartThreads = 64;
+constexpr int kWaitMemory = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kSteepest = -1e4f;  // of a log decay: its exponential is 0 long before
 
@@ -293,6 +294,7 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
                 vr.at -= len * vr.token;
                 len = 1;
                 load(pos, 1, 1);
+                __builtin_amdgcn_s_waitcnt(kWaitMemory);  // or the compiler has everybody wait for loads where this path joins
                 lds_barrier();
                 continue;
             }

@@ -190,28 +190,31 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
     float decay = 0.0f;
     double total = 0.0;
 
-    // The next chunk's rows: len tokens from pos, to which the pointers point; they go on by `step`.
-    auto load = [&](int pos, int len, int step) KDA_INLINE {
-        const int lane = lane_here();
-        const int row = (64 * wave + lane) / kRowChunks;
+    // The next chunk's rows: len tokens, from the pointers on, which go on by as many. Their loads are spread over the
+    // chunk before: issued at once by all workgroups, they keep the waves waiting for their issue.
+    auto load_rows = [&](Rows &r, u32x4 (&x)[kLoads], int len) KDA_INLINE {
+        const int row = (64 * wave + lane_here()) / kRowChunks;
+        int64_t first = 0, second = kStep * r.token;
+        if (len < kChunk) {  // rows past the last stand for it
+            first = min(0, len - 1 - row) * r.token;
+            second = min(kStep, len - 1 - row) * r.token;
+        }
+        x[0] = *reinterpret_cast<const u32x4 *>(r.at + first);
+        x[1] = *reinterpret_cast<const u32x4 *>(r.at + second);
+        r.at += len * r.token;
+    };
+    auto load_decay = [&](int pos, int len) KDA_INLINE {
         if (wave == 0) {
-            decay = a.g[(pos + min(lane, len - 1)) * a.g_stride_token + head * a.g_stride_head];
+            decay = a.g[(pos + min(lane_here(), len - 1)) * a.g_stride_token + head * a.g_stride_head];
         }
-        auto of = [&](Rows &r, u32x4 (&x)[kLoads]) KDA_INLINE {
-            int64_t first = 0, second = kStep * r.token;
-            if (len < kChunk) {  // rows past the last stand for it
-                first = min(0, len - 1 - row) * r.token;
-                second = min(kStep, len - 1 - row) * r.token;
-            }
-            x[0] = *reinterpret_cast<const u32x4 *>(r.at + first);
-            x[1] = *reinterpret_cast<const u32x4 *>(r.at + second);
-            r.at += step * r.token;
-        };
+    };
+    auto load = [&](int pos, int len) KDA_INLINE {
+        load_decay(pos, len);
+        load_rows(kr, k, len);
+        load_rows(vr, v, len);
         if constexpr (OUTPUTS) {
-            of(qr, q);
+            load_rows(qr, q, len);
         }
-        of(kr, k);
-        of(vr, v);
     };
     int single = 0;  // tokens before this one go one at a time
     auto length = [&](int pos) KDA_INLINE -> int {
@@ -240,7 +243,7 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
 
     int pos = seg.begin, len = length(pos);
     if (pos < seg.end) {
-        load(pos, len, len);
+        load(pos, len);
     }
     while (pos < seg.end) {
         const int lane = lane_here();
@@ -293,7 +296,7 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
                 kr.at -= len * kr.token;
                 vr.at -= len * vr.token;
                 len = 1;
-                load(pos, 1, 1);
+                load(pos, 1);
                 __builtin_amdgcn_s_waitcnt(kWaitMemory);  // or the compiler has everybody wait for loads where this path joins
                 lds_barrier();
                 continue;
@@ -301,8 +304,10 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
         }
         store_done();
         const int next = pos + len, next_len = length(next);
-        if (next < seg.end) {
-            load(next, next_len, next_len);
+        const bool more = next < seg.end;
+        if (more) {
+            load_decay(next, next_len);
+            load_rows(kr, k, next_len);
         }
         const double last = sm.sum[kChunk - 1];
         total += last;
@@ -356,6 +361,9 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
                 sm.scores[unit(it, y)][0][lane] = hi;
                 sm.scores[unit(it, y)][1][lane] = lo;
             }
+            if (more) {
+                load_rows(vr, v, next_len);
+            }
             // ---- what the state gives, for all 64 tokens: rows 16 wave + 4 g + e, token 16 it + col
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
@@ -383,6 +391,13 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 o[it] *= sm.early[16 * it + col];
+            }
+        }
+        if (more) {
+            if constexpr (OUTPUTS) {
+                load_rows(qr, q, next_len);
+            } else {
+                load_rows(vr, v, next_len);
             }
         }
         // ---- the state

@@ -260,12 +260,18 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
             sm.late[lane] = ex2(static_cast<float>(__builtin_bit_cast(double, last) - sum));
             sm.early[lane] = ex2(static_cast<float>(sum)) * a.scale;
         }
+        if (len < kChunk) {
+            asm volatile("");  // stays a branch: selects would cost every chunk
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                if (row + i * kStep >= len) {
+                    q[i] = k[i] = v[i] = u32x4{0, 0, 0, 0};
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int r = row + i * kStep;
-            if (len < kChunk && r >= len) {
-                q[i] = k[i] = v[i] = u32x4{0, 0, 0, 0};
-            }
             *reinterpret_cast<u32x4 *>(sm.k + place<D>(r, chunk)) = k[i];
             *reinterpret_cast<u32x4 *>(sm.v + place<D>(r, chunk)) = v[i];
             if constexpr (OUTPUTS) {

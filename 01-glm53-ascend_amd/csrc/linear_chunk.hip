@@ -114,11 +114,18 @@ template <int D> __device__ __forceinline__ u32x4 column(const char *tile, int r
 __device__ __forceinline__ float low_bf16(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// x - (the pair's lower or upper), exact where that is x rounded; the other one times 0 stands for it, so what is not
+// finite spreads within the pair (two keys' parts or tokens of one column: one that is not finite spoils the sums of both)
+constexpr uint32_t kMinusLow = 0x0000bf80u, kMinusHigh = 0xbf800000u;
+__device__ __forceinline__ float minus(uint32_t pair, uint32_t which, float x) {
+    asm("" : "+s"(which));  // (the constant 0x0000bf80 would be encoded as the inline -1.0, whose halves are others here)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, which), x, false);
+}
 // x = hi + lo + rest, hi and lo in bf16
 __device__ __forceinline__ uint32_t split(float &x, float &y) {
     const uint32_t hi = pack_bf16x2(x, y);
-    x -= low_bf16(hi);
-    y -= high_bf16(hi);
+    x = minus(hi, kMinusLow, x);
+    y = minus(hi, kMinusHigh, y);
     return hi;
 }
 

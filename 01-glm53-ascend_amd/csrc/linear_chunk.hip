@@ -114,18 +114,17 @@ template <int D> __device__ __forceinline__ u32x4 column(const char *tile, int r
 __device__ __forceinline__ float low_bf16(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// x - (the pair's lower or upper), exact where that is x rounded; the other one times 0 stands for it, so what is not
-// finite spreads within the pair (two keys' parts or tokens of one column: one that is not finite spoils the sums of both)
-constexpr uint32_t kMinusLow = 0x0000bf80u, kMinusHigh = 0xbf800000u;
-__device__ __forceinline__ float minus(uint32_t pair, uint32_t which, float x) {
-    asm("" : "+s"(which));  // (the constant 0x0000bf80 would be encoded as the inline -1.0, whose halves are others here)
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, which), x, false);
+// x + the sum of a pair times two constants
+__device__ __forceinline__ float dot(uint32_t pair, uint32_t constants, float x) {
+    asm("" : "+s"(constants));  // (0x0000bf80 itself would be encoded as the inline -1.0, whose halves are others here)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, constants), x, false);
 }
-// x = hi + lo + rest, hi and lo in bf16
+// x = hi + lo + rest, hi and lo in bf16. What is not finite spreads within the pair: two keys' parts or tokens of one
+// column, where it spoils the sums of both.
 __device__ __forceinline__ uint32_t split(float &x, float &y) {
     const uint32_t hi = pack_bf16x2(x, y);
-    x = minus(hi, kMinusLow, x);
-    y = minus(hi, kMinusHigh, y);
+    x = dot(hi, 0x0000bf80u, x);  // x - hi's lower, exact
+    y = dot(hi, 0xbf800000u, y);
     return hi;
 }
 
@@ -257,7 +256,7 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
         const int g = lane >> 4, col = lane & 15;
         const int row = (64 * wave + lane) / kRowChunks, chunk = lane % kRowChunks;
         // ---- the chunk into LDS, its sums of decays
-        uint32_t odd = 0;
+        float odd = 0.0f;  // 0 times this thread's values: NaN if one is not finite
         if (wave == 0) {
             const double sum = prefix_sum(lane < len ? kLog2e * static_cast<double>(decay < kSteepest ? kSteepest : decay) : 0.0);
             const u32x2 w = __builtin_bit_cast(u32x2, sum);
@@ -289,12 +288,12 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
                 *reinterpret_cast<u32x2 *>(sm.q + place<D>(r, c + (u & 3) + 1) + (u >> 2) * 8) = u32x2{q[i][2], q[i][3]};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    odd |= ((v[i][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                    odd = dot(v[i][e], 0, odd);
                 }
             }
         }
         if constexpr (OUTPUTS) {
-            const bool some = __any(odd != 0);
+            const bool some = __any(odd != odd);
             if (lane == 0) {
                 sm.odd[wave] = some;
             }

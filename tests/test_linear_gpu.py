@@ -146,6 +146,23 @@ def test_what_is_not_finite_stays_behind_its_token(ops, chunk, which, value):
         assert not torch.isfinite(pool[held, head][:, 5]).any()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+def test_a_value_that_is_not_finite_is_found_anywhere(ops, dim, value):
+    """In every eighth of a row and row of a chunk: earlier tokens and other columns keep finite results."""
+    for token, column in [(0, 0), (1, 1), (2, 2), (17, 3), (31, dim // 2 + 4), (32, dim // 2 + 5), (62, dim - 2), (63, dim - 1)]:
+        case = Linear(9, lens=[64], heads=1, dim=dim)
+        case.v[0, token, 0, column] = value
+        out, pool, _ = run(ops, case, True)
+        fine = torch.ones(64, dim, dtype=torch.bool)
+        fine[token:, column] = False
+        assert torch.isfinite(out[0, :, 0].cpu()[fine]).all(), (token, column)
+        assert not torch.isfinite(out[0, token, 0, column]), (token, column)
+        state = pool[int(case.indices[0]), 0].cpu()
+        assert torch.isfinite(state[:, torch.arange(dim) != column]).all()
+        assert not torch.isfinite(state[:, column]).any()
+
+
 def test_forms_agree_and_calls_repeat(ops):
     """The chunk form is the same from call to call, and split calls continue each other's states."""
     case = Linear(7, lens=[600], heads=4, dim=128)

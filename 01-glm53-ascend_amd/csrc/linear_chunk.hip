@@ -19,8 +19,13 @@
 // LDS, serve both the outputs (left operand) and the update (right operand, times their decays). The
 // scores are formed once, by all waves for all, and go through LDS. q, k and v are exact in bf16; what is rounded
 // is split: scores and S into two parts (17 bits), the decayed values into three (25 bits, all of fp32: these errors
-// would stay in the state). The sums of log decays are formed in 64 bits, so that neighbours' differences are exact
-// behind a steep decay.
+// would stay in the state; two would do for 118 us instead of 128). The sums of log decays are formed in 64 bits, so that
+// neighbours' differences are exact behind a steep decay.
+//
+// Bound by the issue of vector and matrix instructions together, which splitting costs (outputs_kernel: half and 30% of the SIMDs'
+// cycles), and by HBM wherever all workgroups load at once. One MI355X: 8192 tokens of 32 heads of 128 in 126 to 134 us
+// (sums 37, starts 15, outputs 87: 4.6, 4.6 and 3.5 TB/s); 16001 of 4 heads in 51 us (15, 10, 31), of which a chunk is
+// 6 us of latency; 37 ragged requests of up to 2000, 16 heads of 64, in 141 to 155 us.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

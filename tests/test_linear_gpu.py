@@ -58,6 +58,12 @@ RECURRENT = [
     dict(lens=[9, 5, 1, 3], heads=2, dim=128, track=[4, 0, 1, 9], index64=True, zero_slots=(0,)),
     dict(lens=[33], heads=7, dim=64, gated=False, after=1),
     dict(lens=[1] * 300, heads=8, dim=128, gated=False, index64=True),
+    dict(lens=[1] * 9, heads=8, dim=128, fp32=True),
+    dict(lens=[2, 1, 0, 5] * 3, heads=8, dim=128, fp32=True, track=[1, 0, 0, 5] * 3),
+    dict(lens=[2, 1, 0, 5] * 3, heads=8, dim=128, zero_slots=(1,), track=[2, 0, 0, 3] * 3, after=1),
+    dict(lens=[3, 1] * 5, heads=8, dim=64, fp32=True, after=2),
+    dict(lens=[1] * 4, heads=16, dim=128),                                  # 63 and 64 states
+    dict(lens=[1] * 9, heads=7, dim=128),
 ]
 
 

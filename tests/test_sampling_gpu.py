@@ -107,6 +107,16 @@ def test_filters(ops, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [4000, 32001, 131072])
+def test_top_k_where_lists_fill(ops, vocab, dtype):
+    """Around the lengths at which candidates are sorted otherwise, or are not gathered at all."""
+    logits, u, gen = draw(vocab + 2, 8, vocab, dtype)
+    k = [190, 255, 256, 257, 319, 320, 321, 400]
+    check(ops, logits, u, k=k)
+    check(ops, logits, u, k=k[::-1], p=[0.9, 0.5, 0.99, 1.0, 0.7, 0.95, 0.2, 0.8], t=[0.5, 1.0, 2.0, 1.0, 3.0, 0.7, 1.0, 1.5])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_flat_rows_and_ties(ops, dtype):
     """Equal logits by the thousand: more than one list holds, cut by index; two values; steps."""
     V = 20000

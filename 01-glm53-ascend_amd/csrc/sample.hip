@@ -43,7 +43,6 @@ constexpr int kWaves = 16;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;    // elements that are sorted, one a thread
 constexpr int kFew = kList;    // elements that are drawn from in LDS
-constexpr int kPatterns = 4096;
 // top_k up to which candidates are looked for: with more, those of a bound grow past the list. us with them and without, top_k 64,
 // 200, 320 and 400: one row of 131072 in bf16 20 39, 28 42, 38 42, 49 44; of 32000 15 23, 21 23, 30 23, 39 23; 256 rows of 32000 in
 // fp32 18 30, 24 33, 34 34, 43 34 (with top_p too 18 48, 24 51, 34 52).
@@ -62,12 +61,19 @@ struct SampleParams : KdaSampleArgs {
     int groups;  // of kUnroll loads of a wave that make a block
 };
 
-struct Shared {
-    u64 bins[kBins + 1];
+// kPatterns: of bf16 logits, see Sampler
+template <int kPatterns> struct __attribute__((aligned(16))) Shared {
+    union {
+        u64 bins[kBins + 1];
+        uint32_t pattern_numbers[kPatterns + 5];
+    };
     union {
         u64 list[kList];
-        u64 table[kPatterns + 2];  // weights of patterns, whose numbers lie in bins
+        u64 pattern_weights[kPatterns + 3];
     };
+    // Of the patterns' places 0 to kPatterns + 1, with those from 1 on at multiples of 16 bytes.
+    __device__ __forceinline__ uint32_t *numbers() { return pattern_numbers + 3; }
+    __device__ __forceinline__ u64 *table() { return pattern_weights + 1; }
     u64 blocks[kMaxBlocks];
     u64 weights[kFew];
     double powers[256];  // 2^{S + j / 256}
@@ -115,7 +121,7 @@ __device__ __forceinline__ u64 lane_of(u64 x, int lane) {
 }
 __device__ __forceinline__ u64 last_lane(u64 x) { return lane_of(x, 63); }
 // ... of this thread and those before it, and the sum of all. By all threads.
-__device__ __forceinline__ u64 block_scan(Shared &sm, u64 x, u64 &total) {
+template <class S> __device__ __forceinline__ u64 block_scan(S &sm, u64 x, u64 &total) {
     const int lane = static_cast<int>(__lane_id()), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     x = wave_scan(x);
     __syncthreads();  // the last one's sums are read
@@ -135,7 +141,7 @@ __device__ __forceinline__ u64 block_scan(Shared &sm, u64 x, u64 &total) {
 // The list's first n entries (all different, but for zeros) in falling order. By all threads. Up to 256 by counting what is
 // larger, a quarter of the list a thread (60 entries 7000 cycles by steps of a sorting network, 1000 so); more by such a
 // network, an element a thread, where steps within a wave go through its lanes.
-__device__ __forceinline__ void sort(Shared &sm, int n) {
+template <class S> __device__ __forceinline__ void sort(S &sm, int n) {
     __syncthreads();
     const int i = threadIdx.x;
     if (n <= 256) {
@@ -275,9 +281,9 @@ __device__ __forceinline__ u64 exceeding(double u, u64 whole) {
 
 enum Mode { kNumbers, kNucleus, kLeft };
 
-template <typename T> struct Sampler {
+template <typename T, int kPatterns> struct Sampler {
     const SampleParams &a;
-    Shared &sm;
+    Shared<kPatterns> &sm;
     Row<T> row;
     float top;            // the largest logit
     double scale;         // 256 log2(e) / temperature
@@ -592,14 +598,13 @@ template <typename T> struct Sampler {
     }
     __device__ __forceinline__ void uncut() { cut_behind(-kInf, -1); }
 
-    // ---- bf16 logits have few values. Those of a row that have a weight lie within 16 powers of two of
+    // ---- bf16 logits have few values. Those of a row that have a weight lie within kOctaves powers of two of
     // the largest magnitude among them, kPatterns patterns. Their places are in falling order: positive ones 1 to kSide from the
     // largest on, negative ones kSide + 1 to kPatterns to the largest magnitude; 0 and kPatterns + 1 are for all
     // others, which have no weight, but those between the two sides (zeros too), which are formed one by one.
-    static constexpr int kSide = kPatterns / 2;
+    static constexpr int kSide = kPatterns / 2, kOctaves = kSide / 128;
     int base;       // the least magnitude's pattern
     u64 tie_limit;  // how many of those equal to `last` are left
-    __device__ __forceinline__ uint32_t *numbers() const { return reinterpret_cast<uint32_t *>(sm.bins); }
     // The place of a pattern; `under` is negative for one between the sides.
     __device__ __forceinline__ int place_of(u32x4 w, int e, int &under) const {
         const int word = static_cast<int>(w[e >> 1]);
@@ -611,14 +616,14 @@ template <typename T> struct Sampler {
         const uint32_t m = static_cast<uint32_t>(place <= kSide ? kSide - place : place - kSide - 1) + base;
         return __uint_as_float((m | (place <= kSide ? 0u : 0x8000u)) << 16);
     }
-    // A window that fits most rows, of magnitudes from 2^-9 to below 2^7: patterns may be counted in it before the largest logit is
+    // A window that fits most rows, of magnitudes below 2^7: patterns may be counted in it before the largest logit is
     // known.
-    static constexpr int kUsualBase = 118 << 7;
+    static constexpr int kUsualBase = (134 - kOctaves) << 7;
     static constexpr uint32_t kAside = kMaxBlocks;  // logits between the sides that are kept (in place of the blocks) until then
     __device__ __forceinline__ void clear_patterns() {
         __syncthreads();
         for (int i = threadIdx.x; i < kPatterns; i += kThreads) {
-            numbers()[i + 1] = 0;
+            sm.numbers()[i + 1] = 0;
         }
         if (threadIdx.x == 0) {
             sm.between = 0;
@@ -626,23 +631,26 @@ template <typename T> struct Sampler {
         }
         __syncthreads();
     }
-    // Whether the row's logits are taken so; their weights into the table. `counted`: the patterns are, in the usual window; it is
-    // taken back where that does not do.
-    __device__ __forceinline__ bool tabulate(bool &counted) {
+    // Whether the row's logits are taken so; their weights into the table, and their numbers if `cuts`. `counted`: these are
+    // there, in the usual window, which may not do.
+    __device__ __forceinline__ bool tabulate(bool counted, bool cuts) {
         const float range = static_cast<float>(256.0 * (a.shift + 2.1) / scale);  // below it weights are 0
         const float most = fmaxf(fabsf(top), fabsf(top - range));
         const int exponent_of_most = __float_as_int(most) >> 23, exponent_of_top = __float_as_int(fabsf(top)) >> 23;
         // (a very high temperature would put most logits between the sides)
-        if (sizeof(T) != 2 || exponent_of_most < 17 || exponent_of_most > max(exponent_of_top, 130) + 4 || exponent_of_most > 254) {
+        if (sizeof(T) != 2 || exponent_of_most <= kOctaves || exponent_of_most > max(exponent_of_top, 130) + kOctaves - 12 || exponent_of_most > 254) {
             return false;
         }
         counted = counted && exponent_of_most < 134 && sm.between_count <= kAside;
-        base = counted ? kUsualBase : (exponent_of_most - 15) << 7;
+        base = counted ? kUsualBase : (exponent_of_most - (kOctaves - 1)) << 7;
         if (!counted) {
             clear_patterns();
+            if (cuts) {
+                count_patterns();
+            }
         }
         for (int i = threadIdx.x; i < kPatterns + 2; i += kThreads) {
-            sm.table[i] = i > 0 && i <= kPatterns ? weight(fminf(value_at(i), top)) : 0;
+            sm.table()[i] = i > 0 && i <= kPatterns ? weight(fminf(value_at(i), top)) : 0;
         }
         if (counted) {
             u64 mine = 0;
@@ -671,7 +679,7 @@ template <typename T> struct Sampler {
                     int under;
                     const int place = place_of(w, e, under);
                     if (static_cast<uint32_t>(under) < kSide) {
-                        atomicAdd(&numbers()[place], 1u);
+                        atomicAdd(&sm.numbers()[place], 1u);
                     }
                     some |= under;
                     largest = fmaxf(largest, Row<T>::element(w, e));
@@ -712,7 +720,7 @@ template <typename T> struct Sampler {
                     int under;
                     const int place = place_of(w, e, under);
                     if (static_cast<uint32_t>(under) < kSide) {
-                        atomicAdd(&numbers()[place], 1u);
+                        atomicAdd(&sm.numbers()[place], 1u);
                     }
                     some |= under;
                 }
@@ -730,23 +738,36 @@ template <typename T> struct Sampler {
     // Cuts behind the k-th (0: does not) and behind the nucleus of what is left; false where a border lies between the sides.
     // `left`: about how many are left.
     __device__ __forceinline__ bool cut_patterns(u64 k, bool nucleus, double top_p, u64 &left) {
-        const int first = 4 * static_cast<int>(threadIdx.x) + 1;
-        u64 n[4], all, total;
+        constexpr int kEach = kPatterns / kThreads;
+        const int first = kEach * static_cast<int>(threadIdx.x) + 1;
+        u64 n[kEach], all, total;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            n[i] = numbers()[first + i];
+        for (int i = 0; i < kEach; i += 4) {  // 16 bytes at a time, or the lanes meet in few banks
+            const u32x4 four = *reinterpret_cast<const u32x4 *>(sm.numbers() + first + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                n[i + e] = four[e];
+            }
         }
         u64 between = sm.between;
+        const auto sum_of = [](const u64 (&m)[kEach]) KDA_INLINE -> u64 {
+            u64 sum = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                sum += m[i];
+            }
+            return sum;
+        };
         // the place at which the sum of m reaches the target, and the sum before it, into sm; false if that is between the sides
-        const auto border_at = [&](const u64 (&m)[4], u64 middle, u64 target) KDA_INLINE -> bool {
-            u64 sum = m[0] + m[1] + m[2] + m[3];
+        const auto border_at = [&](const u64 (&m)[kEach], u64 middle, u64 target) KDA_INLINE -> bool {
+            u64 sum = sum_of(m);
             sum = block_scan(sm, sum, all) - sum + (first > kSide ? middle : 0);
             if (threadIdx.x == 0) {
                 sm.count = -1;
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kEach; ++i) {
                 if (sum < target && sum + m[i] >= target) {
                     sm.count = first + i;
                     sm.before = sum;
@@ -756,7 +777,7 @@ template <typename T> struct Sampler {
             __syncthreads();
             return sm.count >= 0;
         };
-        block_scan(sm, n[0] + n[1] + n[2] + n[3], total);
+        block_scan(sm, sum_of(n), total);
         left = total;
         if (k > 0 && k < total + sm.between_count) {
             left = k;
@@ -767,31 +788,33 @@ template <typename T> struct Sampler {
             tie_limit = k - sm.before;
             cut_behind(value_at(at), 0x7fffffff);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kEach; ++i) {
                 n[i] = first + i < at ? n[i] : first + i == at ? tie_limit : 0;
             }
             between = at <= kSide ? 0 : between;
         }
         if (nucleus) {
-            u64 m[4];
+            u64 m[kEach];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                m[i] = n[i] * sm.table[first + i];
+            for (int i = 0; i < kEach; i += 2) {
+                const u32x4 two = *reinterpret_cast<const u32x4 *>(sm.table() + first + i);
+                m[i] = n[i] * (static_cast<u64>(two[1]) << 32 | two[0]);
+                m[i + 1] = n[i + 1] * (static_cast<u64>(two[3]) << 32 | two[2]);
             }
-            block_scan(sm, m[0] + m[1] + m[2] + m[3], total);
+            block_scan(sm, sum_of(m), total);
             const u64 target = reaching(top_p, total + between);
             if (!border_at(m, between, target)) {
                 return false;
             }
             const int at = sm.count;
-            const u64 each = sm.table[at];
+            const u64 each = sm.table()[at];
             tie_limit = (target - sm.before + each - 1) / each;
             cut_behind(value_at(at), 0x7fffffff);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kEach; ++i) {
                 n[i] = first + i <= at ? n[i] : 0;
             }
-            block_scan(sm, n[0] + n[1] + n[2] + n[3], left);
+            block_scan(sm, sum_of(n), left);
         }
         return true;
     }
@@ -802,10 +825,10 @@ template <typename T> struct Sampler {
         const u64 at_least = biased(least_weight) - kBias;
         for (int i = threadIdx.x + 1; i <= kPatterns; i += kThreads) {
             const float x = value_at(i);
-            const u64 m = sm.table[i];
+            const u64 m = sm.table()[i];
             // rounded weights decide where they differ from min_p's
             if (!(x > last) || m < at_least || (m == at_least && !(scaled_weight(fminf(x, top), true) >= least_weight))) {
-                sm.table[i] = x == last ? kTie : 0;
+                sm.table()[i] = x == last ? kTie : 0;
             }
         }
         __syncthreads();
@@ -834,7 +857,7 @@ template <typename T> struct Sampler {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     int under;
-                    mine += sm.table[place_of(w, e, under)];
+                    mine += sm.table()[place_of(w, e, under)];
                     between |= under;
                 }
                 if (__any(between < 0)) {
@@ -949,8 +972,8 @@ template <typename T> struct Sampler {
     }
 };
 
-template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) {
-    __shared__ Shared sm;
+template <typename T, int kPatterns> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) {
+    __shared__ Shared<kPatterns> sm;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t n = blockIdx.x;
@@ -967,7 +990,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     const float given = a.uniforms[n];
     const double u = given > 0.0f ? static_cast<double>(given) : 0.0;
     Row<T> row{static_cast<const T *>(a.logits) + n * a.logits_stride, a.vocab};
-    Sampler<T> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0, -kInf, -kInf};
+    Sampler<T, kPatterns> s{a, sm, row, 0.0f, 0.0, 0.0f, -kInf, -1, 0.0, -kInf, -kInf};
 
     // ---- the largest logit, and where it is first
     float top = -kInf;
@@ -1114,13 +1137,10 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     };
     // ---- bf16: the patterns' numbers cut, then one pass for the blocks' masses
     if constexpr (sizeof(T) == 2) {
-        if (a.groups == 1 && s.tabulate(counted)) {
+        if (a.groups == 1 && s.tabulate(counted, few_k || nucleus)) {
             bool cut = true;
             u64 left = 0;
             if (few_k || nucleus) {
-                if (!counted) {
-                    s.count_patterns();
-                }
                 cut = s.cut_patterns(few_k ? static_cast<u64>(k) : 0, nucleus, static_cast<double>(top_p), left);
             }
             if (cut) {
@@ -1209,10 +1229,15 @@ extern "C" int kda_sample_launch(const KdaSampleArgs *args, void *stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     const unsigned rows = static_cast<unsigned>(a.rows);
-    if (a.dtype == KDA_BF16) {
-        sample_kernel<uint16_t><<<rows, kThreads, 0, s>>>(a);
+    // Logits below the patterns (of 16 powers of two with 4096, 32 with 8192) are formed one by one, a few in 512, which costs long
+    // rows more than the larger table does. us with 4096 and 8192: 256 rows of 150000 with top_p and min_p 62.6 56.6, a row of 131072
+    // with top_k 2000 45 40; of 32000 23.4 24.0 (top_p 25.5 27.4), of 1000 13.8 15.1
+    if (a.dtype == KDA_F32) {
+        sample_kernel<float, 4096><<<rows, kThreads, 0, s>>>(a);
+    } else if (a.vocab <= 65536) {
+        sample_kernel<uint16_t, 4096><<<rows, kThreads, 0, s>>>(a);
     } else {
-        sample_kernel<float><<<rows, kThreads, 0, s>>>(a);
+        sample_kernel<uint16_t, 8192><<<rows, kThreads, 0, s>>>(a);
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }

@@ -21,9 +21,9 @@
 //     formed anew; the token's block is read once more.
 //
 // A row takes one CU, all of whose threads it has: the first pass is bound by what one CU can read, the later ones, which
-// read the caches, by LDS (bf16: a counter and a weight an element) or the vector instructions (fp32: 20 an element where
-// its weight is formed). One MI355X: a row of 131072 in bf16 with top_k 50 17 us, 256 rows of 150000 with every
-// filter 62 to 66 us, 37 rows of 32000 in fp32 18.5 us, of which 12 do not depend on the length (barriers, sorting, the launch).
+// read the caches, by the vector instructions (bf16: 13 an element for its counter and again for its weight; fp32: 20 where
+// its weight is formed). One MI355X: a row of 131072 in bf16 with top_k 50 17 us, 256 rows of 150000 with top_p and
+// min_p 57 us, 37 rows of 32000 in fp32 18.5 us, of which 12 do not depend on the length (barriers, sorting, the launch).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -21,9 +21,9 @@
 //     formed anew; the token's block is read once more.
 //
 // A row takes one CU, all of whose threads it has: the first pass is bound by what one CU can read, the later ones, which
-// read the caches, by the vector instructions (bf16: 13 an element for its counter and again for its weight; fp32: 20 where
-// its weight is formed). One MI355X: a row of 131072 in bf16 with top_k 50 17 us, 256 rows of 150000 with top_p and
-// min_p 57 us, 37 rows of 32000 in fp32 18.5 us, of which 12 do not depend on the length (barriers, sorting, the launch).
+// read the caches, by the vector instructions (bf16: about 10 an element for its counter and again for its weight; fp32: 20
+// where its weight is formed). One MI355X: a row of 131072 in bf16 with top_k 50 17 us, 256 rows of 150000 with top_p and
+// min_p 52 us, 37 rows of 32000 in fp32 18.5 us, of which 12 do not depend on the length (barriers, sorting, the launch).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -55,6 +55,8 @@ constexpr double kLn2 = 0.6931471805599453;
 
 typedef uint64_t u64;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
 
 struct SampleParams : KdaSampleArgs {
     int shift;   // S: weights are multiples of 2^-S
@@ -605,12 +607,13 @@ template <typename T, int kPatterns> struct Sampler {
     static constexpr int kSide = kPatterns / 2, kOctaves = kSide / 128;
     int base;       // the least magnitude's pattern
     u64 tie_limit;  // how many of those equal to `last` are left
-    // The place of a pattern; `under` is negative for one between the sides.
-    __device__ __forceinline__ int place_of(u32x4 w, int e, int &under) const {
-        const int word = static_cast<int>(w[e >> 1]);
-        const int sign = (e & 1) != 0 ? word >> 31 : __builtin_amdgcn_sbfe(word, 15, 1);
-        under = static_cast<int>(__builtin_amdgcn_ubfe(word, (e & 1) != 0 ? 16 : 0, 15)) - base;
-        return kSide + 1 + (static_cast<int>(min(static_cast<uint32_t>(under), static_cast<uint32_t>(kSide))) ^ ~sign);
+    // The places of a word's two patterns, 16 bits each (one at a time: 256 rows of 150000 57 us, 52 so); `magnitude` gets how
+    // far they are from the least one, 0x8000 and above for those between the sides.
+    __device__ __forceinline__ u16x2 places_of(uint32_t word, u16x2 &magnitude) const {
+        magnitude = __builtin_bit_cast(u16x2, word & 0x7fff7fffu) - static_cast<uint16_t>(base);
+        const u16x2 inside = __builtin_elementwise_min(magnitude, u16x2{kSide, kSide});
+        const uint32_t negative = __builtin_bit_cast(uint32_t, __builtin_bit_cast(s16x2, word) >> static_cast<int16_t>(15));
+        return __builtin_bit_cast(u16x2, __builtin_bit_cast(uint32_t, inside) ^ ~negative) + static_cast<uint16_t>(kSide + 1);
     }
     __device__ __forceinline__ float value_at(int place) const {
         const uint32_t m = static_cast<uint32_t>(place <= kSide ? kSide - place : place - kSide - 1) + base;
@@ -667,24 +670,35 @@ template <typename T, int kPatterns> struct Sampler {
         __syncthreads();
         return true;
     }
+    // Counts eight logits; the high bits of the result's halves tell whether some are between the sides.
+    __device__ __forceinline__ uint32_t count(u32x4 w) const {
+        uint32_t some = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u16x2 magnitude;
+            const u16x2 place = places_of(w[i], magnitude);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (magnitude[e] < kSide) {
+                    atomicAdd(&sm.numbers()[place[e]], 1u);
+                }
+            }
+            some |= __builtin_bit_cast(uint32_t, magnitude);
+        }
+        return some;
+    }
     // The patterns' numbers in the usual window, and the largest logit.
     __device__ __forceinline__ void count_first(float &largest) {
         base = kUsualBase;
         clear_patterns();
         pass(
             [&](int, u32x4 w) KDA_INLINE {
-                int some = 0;
+                const uint32_t some = count(w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    int under;
-                    const int place = place_of(w, e, under);
-                    if (static_cast<uint32_t>(under) < kSide) {
-                        atomicAdd(&sm.numbers()[place], 1u);
-                    }
-                    some |= under;
                     largest = fmaxf(largest, Row<T>::element(w, e));
                 }
-                if (__any(some < 0)) {
+                if (__any((some & 0x80008000u) != 0)) {
                     each_between(w, [&](float x) KDA_INLINE {
                         const uint32_t at = atomicAdd(&sm.between_count, 1u);
                         if (at < kAside) {
@@ -699,9 +713,7 @@ template <typename T, int kPatterns> struct Sampler {
     template <class F> __device__ __forceinline__ void each_between(u32x4 w, F f) const {
 #pragma unroll 1
         for (int e = 0; e < E; ++e) {
-            int under;
-            place_of(w, 0, under);
-            if (under < 0) {
+            if (static_cast<int>(w[0] & 0x7fffu) < base) {
                 f(Row<T>::element(w, 0));
             }
 #pragma unroll
@@ -714,17 +726,7 @@ template <typename T, int kPatterns> struct Sampler {
     __device__ __forceinline__ void count_patterns() {
         pass(
             [&](int, u32x4 w) KDA_INLINE {
-                int some = 0;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    int under;
-                    const int place = place_of(w, e, under);
-                    if (static_cast<uint32_t>(under) < kSide) {
-                        atomicAdd(&sm.numbers()[place], 1u);
-                    }
-                    some |= under;
-                }
-                if (__any(some < 0)) {
+                if (__any((count(w) & 0x80008000u) != 0)) {
                     each_between(w, [&](float x) KDA_INLINE {
                         const u64 m = weight(x);
                         atomicAdd(&sm.between_count, m != 0 ? 1u : 0u);
@@ -853,14 +855,16 @@ template <typename T, int kPatterns> struct Sampler {
                         return;
                     }
                 }
-                int between = 0;
+                uint32_t between = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    int under;
-                    mine += sm.table()[place_of(w, e, under)];
-                    between |= under;
+                for (int i = 0; i < 4; ++i) {
+                    u16x2 magnitude;
+                    const u16x2 place = places_of(w[i], magnitude);
+                    mine += sm.table()[place[0]];
+                    mine += sm.table()[place[1]];
+                    between |= __builtin_bit_cast(uint32_t, magnitude);
                 }
-                if (__any(between < 0)) {
+                if (__any((between & 0x80008000u) != 0)) {
                     each_between(w, [&](float x) KDA_INLINE {
                         const double v = scaled_weight(x, x > last);
                         mine += v >= least_weight ? biased(v) - kBias : 0;
@@ -1230,7 +1234,7 @@ extern "C" int kda_sample_launch(const KdaSampleArgs *args, void *stream) {
     (void)hipGetLastError();
     const unsigned rows = static_cast<unsigned>(a.rows);
     // Logits below the patterns (of 16 powers of two with 4096, 32 with 8192) are formed one by one, a few in 512, which costs long
-    // rows more than the larger table does. us with 4096 and 8192: 256 rows of 150000 with top_p and min_p 62.6 56.6, a row of 131072
+    // rows more than the larger table does. us with 4096 and 8192 (long rows take 7% less since places come two at a time): 256 rows of 150000 with top_p and min_p 62.6 56.6, a row of 131072
     // with top_k 2000 45 40; of 32000 23.4 24.0 (top_p 25.5 27.4), of 1000 13.8 15.1
     if (a.dtype == KDA_F32) {
         sample_kernel<float, 4096><<<rows, kThreads, 0, s>>>(a);

@@ -473,7 +473,8 @@ template <typename T, int kPatterns> struct Sampler {
         u64 before;
         return locate_in(block_of(target, before), before, target, w);
     }
-    // The block in which the sum of the blocks' masses reaches `target`, and the sum before it, in every thread.
+    // The block in which the sum of the blocks' masses reaches `target`, and the sum before it, in every thread; one of the
+    // row's blocks whatever the sums are.
     __device__ __forceinline__ int block_of(u64 target, u64 &before) {
         const int n = blocks(), i = 2 * static_cast<int>(threadIdx.x);
         const u64 m0 = i < n ? sm.blocks[i] : 0, m1 = i + 1 < n ? sm.blocks[i + 1] : 0;
@@ -485,10 +486,10 @@ template <typename T, int kPatterns> struct Sampler {
             sm.before = second ? sum - m1 : sum - m0 - m1;
         }
         __syncthreads();
-        const int found = __builtin_amdgcn_readfirstlane(sm.count);
+        const uint32_t found = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sm.count));
         before = sm.before;
         __syncthreads();
-        return found;
+        return static_cast<int>(min(found, static_cast<uint32_t>(n - 1)));
     }
     template <class W> __device__ __forceinline__ int locate_in(int block, u64 before, u64 target, W w) {
         // a wave for each load of a group
@@ -1076,7 +1077,8 @@ template <typename T, int kPatterns> __global__ __launch_bounds__(kThreads) void
     if (min_p > 0.0f) {
         const double p = static_cast<double>(fminf(min_p, 1.0f));
         s.least_weight = ldexp(p, a.shift);
-        const double x = static_cast<double>(top) + log(p) * static_cast<double>(temperature);
+        // (of p = 1 the logarithm is 0, which an infinite temperature would make NaN)
+        const double x = static_cast<double>(top) + (p < 1.0 ? log(p) * static_cast<double>(temperature) : 0.0);
         s.floor = s.least = static_cast<float>(x - 1e-6 * (fabs(x) + fabs(static_cast<double>(top)) + static_cast<double>(temperature)));
     }
 

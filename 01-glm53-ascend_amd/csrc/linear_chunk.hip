@@ -52,7 +52,7 @@ constexpr float kSteepest = -1e4f;  // of a log decay: its exponential is 0 long
 
 struct ChunkParams : LinearParams {
     float *starts;  // [slots][heads][D * D]: a segment's sum, then the state before it
-    float *decays;  // [slots][heads]: of a whole segment
+    float *decays;  // [slots][heads]: of a whole segment, see kept_decay
     int segment;    // tokens, a multiple of 64
 };
 
@@ -484,6 +484,25 @@ __device__ __forceinline__ double walk(const ChunkParams &a, Shared<D, OUTPUTS> 
     return total;
 }
 
+// A segment's decay from its log2, and its product with a state. Positive log decays may leave exp(sum) to fp32 over 64 tokens but
+// not over a segment, where a state (one of 0 above all) may still leave a finite product: such a decay is kept as minus its log2.
+__device__ __forceinline__ float kept_decay(double log2) {
+    const float decay = ex2(static_cast<float>(log2));
+    return decay < __builtin_inff() || !(log2 > 0.0) ? decay : -static_cast<float>(fmin(log2, 4096.0));
+}
+__device__ __forceinline__ f32x4 decayed(f32x4 s, float decay) {
+    if (decay < 0.0f) {
+        const float power = floorf(-decay);
+        s *= ex2(-decay - power);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s[e] = ldexpf(s[e], static_cast<int>(power));
+        }
+        return s;
+    }
+    return s * decay;
+}
+
 template <int D> __global__ __launch_bounds__(kThreads<D>, 4) void sums_kernel(const ChunkParams a) {
     __shared__ __attribute__((aligned(16))) Shared<D, false> sm;
     const int head = blockIdx.x % a.num_heads;
@@ -505,7 +524,7 @@ template <int D> __global__ __launch_bounds__(kThreads<D>, 4) void sums_kernel(c
         *reinterpret_cast<f32x4 *>(to + 16 * kt) = s[kt];
     }
     if (threadIdx.x == 0) {
-        a.decays[at] = ex2(static_cast<float>(total));
+        a.decays[at] = kept_decay(total);
     }
 }
 
@@ -536,6 +555,24 @@ template <int D> __global__ __launch_bounds__(kStartThreads) void starts_kernel(
                     sum[x] = *reinterpret_cast<const f32x4 *>(a.starts + at * (D * D) + e);
                     decay[x] = a.decays[at];
                 }
+            }
+            float least = 0.0f;
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+                least = i + x + 1 < count ? fminf(least, decay[x]) : least;
+            }
+            if (least < 0.0f) {  // one that fp32 does not hold: from memory again, one by one
+                for (int x = i; x < min(i + kAtOnce, count); ++x) {
+                    const int64_t at = (first + x) * a.num_heads + head;
+                    float *to = a.starts + at * (D * D) + e;
+                    f32x4 next = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (x + 1 < count) {
+                        next = decayed(s, a.decays[at]) + *reinterpret_cast<const f32x4 *>(to);
+                    }
+                    *reinterpret_cast<f32x4 *>(to) = s;
+                    s = next;
+                }
+                continue;
             }
 #pragma unroll
             for (int x = 0; x < kAtOnce; ++x) {

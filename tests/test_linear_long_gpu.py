@@ -1,4 +1,4 @@
-"""Linear attention in chunks: many segments, and how near states are to fp32."""
+"""Linear attention in chunks: many segments, decays that grow, and how near states are to fp32."""
 
 import pytest
 import torch
@@ -62,6 +62,19 @@ def check(ops, case, chunk=True):
 ], ids=range(8))
 def test_many_segments(ops, spec, dim):
     check(ops, Long(21, dim=dim, g_mean=-9.0, **spec))
+
+
+@pytest.mark.parametrize("chunk", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("begin", [0.0, 1e-12])
+def test_positive_decays_are_limited_by_64_tokens(ops, begin, dim, chunk):
+    """exp(sum) is past fp32 over a segment of 512 tokens, not over 64, and no state is near fp32's ends."""
+    case = Long(22, lens=[1200] + [1] * 255, heads=2, dim=dim)
+    case.g = torch.full_like(case.g, -0.2)
+    case.g[:, :512] = 0.2
+    case.v[:, :450] = 0
+    case.pool.mul_(begin)
+    check(ops, case, chunk)
 
 
 @pytest.mark.parametrize("dim", [64, 128])

@@ -34,17 +34,26 @@ template <typename T> __device__ __forceinline__ T narrowed(float x) {
     }
 }
 
+// N elements in one access, or in two of 16 bytes: what the tensors' rows are aligned to.
+template <typename T, int N> struct Vector {
+    static constexpr int kBytes = sizeof(T) * N < 16 ? sizeof(T) * N : 16;
+    typedef T type __attribute__((ext_vector_type(N), aligned(kBytes)));
+    static_assert(alignof(type) == kBytes);
+};
+
 template <typename T, int D, int NP> struct Token {
-    T q[4], k[4], v[NP];
+    alignas(16) T q[4];
+    alignas(16) T k[4];
+    alignas(16) T v[NP];
     float g;
     __device__ __forceinline__ void load(const LinearParams &a, int64_t t, int head, int c, int row) {
         const T *qp = static_cast<const T *>(a.q) + t * a.q_stride_token + head * a.q_stride_head + c;
         const T *kp = static_cast<const T *>(a.k) + t * a.k_stride_token + head * a.k_stride_head + c;
         const T *vp = static_cast<const T *>(a.v) + t * a.v_stride_token + head * a.v_stride_head + row;
-        typedef T four __attribute__((ext_vector_type(4)));
+        typedef typename Vector<T, 4>::type four;
         *reinterpret_cast<four *>(q) = *reinterpret_cast<const four *>(qp);
         *reinterpret_cast<four *>(k) = *reinterpret_cast<const four *>(kp);
-        typedef T some __attribute__((ext_vector_type(NP)));
+        typedef typename Vector<T, NP>::type some;
         *reinterpret_cast<some *>(v) = *reinterpret_cast<const some *>(vp);
         g = a.g[t * a.g_stride_token + head * a.g_stride_head];
     }
@@ -118,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(const Linear
             o[p] = group_sum<kLanes>(s[p].x * q[0] + s[p].y * q[1] + s[p].z * q[2] + s[p].w * q[3]) * a.scale;
         }
         if (kc == 0) {
-            typedef T some __attribute__((ext_vector_type(NP)));
+            typedef typename Vector<T, NP>::type some;
             some y;
 #pragma unroll
             for (int p = 0; p < NP; ++p) {

@@ -19,13 +19,14 @@
 // LDS, serve both the outputs (left operand) and the update (right operand, times their decays). The
 // scores are formed once, by all waves for all, and go through LDS. q, k and v are exact in bf16; what is rounded
 // is split: scores and S into two parts (17 bits), the decayed values into three (25 bits, all of fp32: these errors
-// would stay in the state; two would do for 118 us instead of 128). The sums of log decays are formed in 64 bits, so that
+// would stay in the state; two would do for 121 us instead of 129). The sums of log decays are formed in 64 bits, so that
 // neighbours' differences are exact behind a steep decay.
 //
-// Bound by the issue of vector and matrix instructions together, which splitting costs (outputs_kernel: half and 30% of the SIMDs'
-// cycles), and by HBM wherever all workgroups load at once. One MI355X: 8192 tokens of 32 heads of 128 in 126 to 134 us
-// (sums 37, starts 15, outputs 87: 4.6, 4.6 and 3.5 TB/s); 16001 of 4 heads in 51 us (15, 10, 31), of which a chunk is
-// 6 us of latency; 37 ragged requests of up to 2000, 16 heads of 64, in 141 to 155 us.
+// Bound by the issue of instructions, which splitting costs (each one taken out of outputs_kernel was worth its share; vector ones
+// take 49% of the SIMDs' cycles, matrix ones 30%, partly at once), and by HBM wherever all workgroups load at once. One MI355X,
+// by card: 8192 tokens of 32 heads of 128 in 126 to 138 us; 16001 of 4 heads in 53 us, of which a chunk is 6 us of latency;
+// 37 ragged requests of up to 2000, 16 heads of 64, in 141 to 155 us. Kernels traced one by one, which start and end apart and so
+// take longer together: sums 37, starts 15, outputs 87 us (4.6, 4.6 and 3.5 TB/s); 15, 11.5, 31; 31, 12, 105.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -632,11 +633,15 @@ template <int D> __global__ __launch_bounds__(kThreads<D>, 4) void outputs_kerne
 constexpr int kMostChunks = 1 << 20;  // of a segment
 constexpr int kMostTokens = INT32_MAX - kMostChunks * kChunk;  // offsets a segment behind the last token stay in 32 bits
 
-// A segment's tokens. As many workgroups as the card holds at once (two a CU of heads of 128, six of 64) where
-// segments are then long, at least as many as it has CUs elsewhere; not so short that the states between
+// A segment's tokens. As many workgroups as the card holds at once (of heads of 128, two a CU) where segments are then
+// long, at least as many as it has CUs elsewhere; not so short that the states between
 // them outweigh them, the less so the more requests and heads there are. Up to 320 tokens go as they are: 256 tokens
 // on 16 heads 27.6 us so, 30.0 in segments of 128 (320: 32.9 and 29.7). us, heads of 128, with segments of 128, 192 and 256:
 //   16001 tokens, 4 heads  62 65 55    5311, 16 heads  65 65 72    4096, 16  70 61 63    32768, 2  84 72 72
+// Of heads of 64 a CU holds four (124 registers, 38 KB of LDS), 1024 in all; 1536 leaves the last ones to a second round, which costs
+// single long requests, least where ragged ones fill it. us with work / 768, 1024, 1536 and 2048:
+//   16001 tokens, 16 heads  69 71 80 89    8192, 32 heads  67 66 74 81    37 of 1 to 2000, 16 heads  161 152 154 155
+//   8 of 2000 to 6000, 16 heads  125 119 123 121    100 of 100 to 1000, 8 heads  113 108 108 108
 int segment_of_call(const KdaLinearArgs &a) {
     const int64_t work = static_cast<int64_t>(a.num_tokens) * a.num_heads;
     const int64_t pairs = static_cast<int64_t>(a.num_seqs) * a.num_heads;

@@ -4,8 +4,8 @@
 //
 // Nothing mixes the columns of S, which are the contiguous rows of the pool: a lane holds four of
 // the K elements of NP rows, D / 4 lanes a row, and the state stays in its registers from the one load to the one
-// store. The only sum over lanes is the readout's. The update is formed as written, in fp32: the same
-// roundings as a loop over the tokens in fp32.
+// store. The only sum over lanes is the readout's. The update is formed as written, in fp32, one of its two
+// products and the sum in one rounding: none more than a loop over the tokens in fp32 has.
 //
 // Bound by HBM: a state is 4 D^2 bytes in and out for 5 D^2 operations a token. States are touched once a
 // call, so their loads and stores are marked as streams. One MI355X, heads of 128: one token of 256 requests, 32 heads, in

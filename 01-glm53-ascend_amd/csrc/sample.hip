@@ -21,9 +21,10 @@
 //     formed anew; the token's block is read once more.
 //
 // A row takes one CU, all of whose threads it has: the first pass is bound by what one CU can read, the later ones, which
-// read the caches, by the vector instructions (bf16: about 10 an element for its counter and again for its weight; fp32: 20
-// where its weight is formed). One MI355X: a row of 131072 in bf16 with top_k 50 17 us, 256 rows of 150000 with top_p and
-// min_p 52 us, 37 rows of 32000 in fp32 18.5 us, of which 12 do not depend on the length (barriers, sorting, the launch).
+// read the caches, by the vector instructions. Those of all passes, an element: 32 in bf16 (150000 with top_p and min_p), 59 in fp32
+// with a temperature alone and 129 with top_p (32000, a fixed part included), where weights are formed one by one. One MI355X: a row
+// of 131072 in bf16 with top_k 50 17 us, 256 rows of 150000 with top_p and min_p 52 us (257: 88 with top_p, a CU holds one
+// workgroup), 37 rows of 32000 in fp32 18.5 us, of which 12 do not depend on the length (barriers, sorting, the launch).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -43,9 +44,10 @@ constexpr int kWaves = 16;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;    // elements that are sorted, one a thread
 constexpr int kFew = kList;    // elements that are drawn from in LDS
-// top_k up to which candidates are looked for: with more, those of a bound grow past the list. us with them and without, top_k 64,
-// 200, 320 and 400: one row of 131072 in bf16 20 39, 28 42, 38 42, 49 44; of 32000 15 23, 21 23, 30 23, 39 23; 256 rows of 32000 in
-// fp32 18 30, 24 33, 34 34, 43 34 (with top_p too 18 48, 24 51, 34 52).
+// top_k up to which candidates are looked for: with more, sorting them costs more than the bins do. us with them and without, top_k
+// 64, 200, 320 and 400: one row of 131072 in bf16 20 34, 28 36, 38 37, 49 38 (with top_p too 20 39, 28 41, 38 41, 49 42); 256 rows of
+// 32000 in fp32 18 31, 24 33, 35 34, 43 35 (18 49, 24 52, 35 53, 43 53). One number for all rows: short ones in bf16 take less
+// without from 200 on (one row of 32000 15 23, 22 23, 31 23), long ones in fp32 with them for longer (131072: 22 53, 29 58, 40 63, 49 65).
 constexpr int kFewK = 320;
 constexpr int kMaxBlocks = 2048;
 constexpr int kUnroll = 4;     // 16-byte loads of a lane in flight together

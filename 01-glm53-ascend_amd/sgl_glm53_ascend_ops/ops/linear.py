@@ -69,9 +69,10 @@ def linear_varlen_chunk(
 ) -> torch.Tensor:
     """:func:`linear_varlen_recurrent` for prompts: 64 tokens at a time on the matrix cores, bf16 only.
 
-    Any lengths; log decays from 0 down to -infinity, exact for any steepness. The states are those of a loop
+    Any lengths; log decays from 0 down to -infinity, exact for any steepness (positive ones work while ``exp`` of
+    their sum over 64 tokens stays finite). The states are those of a loop
     in fp32 to within its own roundings. An infinite or NaN value reaches its own token and
-    later ones of its request only.
+    later ones of its request only; an infinite one may end as NaN where the recurrent form keeps it.
     """
     return _OPS.linear_varlen_chunk(
         q, k, v, g, initial_state_source=initial_state_source, initial_state_indices=initial_state_indices,

@@ -335,7 +335,8 @@ size_t kda_linear_chunk_workspace_bytes(const KdaLinearArgs *args);
 /* In chunks of 64 tokens on the matrix cores: prompts. bf16 only, no checkpoints; alignment as
  * above. Log decays are at most 0 in earnest (positive ones work while exp(sum) stays finite over 64
  * tokens), down to -infinity; below -10000 they count as -10000, whose exponential is 0. An
- * infinite or NaN value reaches its own token and later ones of its request only. At most 2^31 - 2^26 - 1
+ * infinite or NaN value reaches its own token and later ones of its request only; behind an infinite q, k, v or state
+ * there may be NaN where the recurrent form keeps the infinity. At most 2^31 - 2^26 - 1
  * tokens (KDA_ERR_TOO_LARGE).
  * `workspace`: 256-byte aligned device memory of the bytes above, no initialization needed. */
 int kda_linear_chunk_launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, void *stream);

@@ -81,8 +81,8 @@ def test_positive_decays_are_limited_by_64_tokens(ops, begin, dim, chunk):
 def test_states_are_those_of_fp32(ops, dim):
     """Token j alone has key element j: element j of the state is its value times its decay, no sum. Decays of up to a
     factor of two: an exponent is off by 2^-24 of at most 1 (2^-24 in the exponential), the exponential by 2^-23, its product by
-    2^-24, the three parts of that by 2^-27, and they are added up in fp32, 2^-23 each: less than 2^-20 together. Two
-    parts would be off by up to 2^-18."""
+    2^-24, the three parts of that by 2^-26, and they are added up in fp32, 2^-23 each: less than 2^-20 together. Two
+    parts would be off by up to 2^-17."""
     case = Linear(23, lens=[64], heads=2, dim=dim)
     case.k = torch.eye(64, dim)[None, :, None].expand(1, 64, 2, dim).contiguous().bfloat16()
     case.g = -torch.rand(case.g.shape, generator=torch.Generator().manual_seed(24)) * (0.69 / 64)
